@@ -377,6 +377,44 @@ int sharq_tp_reduce_rmsnorm_prepare_allgather(const void *partial_blocks, const 
                                               long long multicast_delta, float *scale_out, void *const *rank_state_ptrs,
                                               int rank, int world, int *error_flag, void *stream);
 
+/* ---- Decode step: a paged key/value cache, attention over it, and 4-bit weights with unquantised activations -------------
+ * (no counterpart in the reference, whose layers leave the cache and its attention to HuggingFace: model/qLlamaLayer.py:137-160).
+ *
+ * k and v are device arrays [pages][kv_heads][page_size][head_dim] of bf16 or, when k_scale and v_scale are given (float [kv_heads] on the
+ * device), of e4m3 values that stand for value * scale[head].  The strides (in elements, the same for both, multiples of 16 bytes) may
+ * order the first three dimensions in any way; head_dim elements are contiguous.  Token j of sequence s lies in slot j % page_size of
+ * page page_table[s * page_table_stride + j / page_size]; entries behind a sequence's last page are not read. */
+typedef struct sharq_paged_cache {
+  void *k, *v;
+  const int *page_table;
+  int64_t page_table_stride;
+  int64_t page_stride, head_stride, token_stride;
+  const float *k_scale, *v_scale;
+  int sequences, max_pages, pages, page_size, kv_heads, head_dim;
+} sharq_paged_cache;
+
+/* Rotary embedding (rotate-half) of the query and key heads of a merged qkv activation [rows, heads + 2 * kv_heads heads of head_dim]
+ * (bf16, row_stride elements between rows) with the rows positions[r] of cos and sin (bf16 [table_rows, head_dim]): the queries to
+ * q_out [rows, heads, head_dim], the keys to the cache (and to k_out [rows, kv_heads, head_dim] unless NULL), the values to the cache.
+ * Row r belongs to sequence sequences[r] (NULL: r) and has position positions[r] in it; no two rows may have the same place.  One
+ * rounding per result.  A row with a negative position is padding: zeros come out and the cache stays as it is.  A row whose position,
+ * sequence or page is outside its table or the cache gives NaN, leaves the cache as it is and stores 0x402 in *error_flag (may be NULL).
+ * head_dim a multiple of 16, at most 256. */
+int sharq_rope_append_paged(const void *qkv_bf16, int64_t row_stride, int rows, int heads, const void *cos_bf16, const void *sin_bf16,
+                            int table_rows, const int *positions, const int *sequences, const sharq_paged_cache *cache,
+                            void *q_out_bf16, void *k_out_bf16, int *error_flag, void *stream);
+
+/* Attention of one new token per sequence over the cache: out[s, h] = sum_j softmax_j(scale * q[s, h] . k[j]) v[j] over the first
+ * lengths[s] tokens of sequence s (the new one among them), query head h reading key/value head h / (heads / kv_heads).  q bf16 with
+ * q_row / q_head elements between sequences / heads (multiples of 8), out bf16 [sequences, heads, head_dim].  A sequence of length 0 gives
+ * zeros.  A length that is negative or more than the page table holds, or a page outside the cache, makes the rows of that sequence NaN and
+ * stores 0x402 in *error_flag (may be NULL).  head_dim 64 or 128; heads a multiple of kv_heads.  workspace:
+ * sharq_paged_attention_workspace_bytes(heads, kv_heads, head_dim) bytes of scratch, 16-byte aligned, not shared by calls that overlap. */
+size_t sharq_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
+int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int heads, const sharq_paged_cache *cache,
+                          const int *lengths, float scale, void *out_bf16, void *workspace, size_t workspace_bytes, int *error_flag,
+                          void *stream);
+
 /* Test/tuning hook: how many SM clock cycles a cross-GPU wait of the all-reduce and transition
  * kernels may take before the kernel gives up, stores its error code and returns (0 restores the
  * defaults of two to ten seconds).  Applies to launches made after the call. */

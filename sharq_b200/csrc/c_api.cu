@@ -8,6 +8,7 @@
 
 #include "allreduce.cuh"
 #include "common.cuh"
+#include "decode_ops.cuh"
 #include "decoder_ops.cuh"
 #include "gemm.cuh"
 #include "prepare.cuh"
@@ -38,6 +39,39 @@ inline cudaStream_t as_stream(void *s) { return static_cast<cudaStream_t>(s); }
   do {                           \
     if (!(cond)) return fail(__VA_ARGS__); \
   } while (0)
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The checks that all users of a paged cache share; strides become bytes.
+int paged_cache(const sharq_paged_cache *c, sharq::PagedCache *out, bool *fp8) {
+  SHARQ_REQUIRE(c && c->k && c->v && c->page_table, "null buffer");
+  SHARQ_REQUIRE((c->k_scale == nullptr) == (c->v_scale == nullptr), "k_scale and v_scale go together");
+  *fp8 = c->k_scale != nullptr;
+  const int64_t size = *fp8 ? 1 : 2;
+  SHARQ_REQUIRE(c->sequences > 0 && c->max_pages > 0 && c->pages > 0 && c->page_size > 0 && c->kv_heads > 0 && c->head_dim > 0,
+                "sequences, max_pages, pages, page_size, kv_heads and head_dim must be positive");
+  SHARQ_REQUIRE(c->page_table_stride >= c->max_pages || c->sequences == 1, "page_table_stride must cover max_pages");
+  SHARQ_REQUIRE(c->page_stride >= 0 && c->head_stride >= 0 && c->token_stride >= 0, "strides of the cache must not be negative");
+  SHARQ_REQUIRE(aligned16(c->k) && aligned16(c->v) && (c->page_stride * size) % 16 == 0 && (c->head_stride * size) % 16 == 0 &&
+                    (c->token_stride * size) % 16 == 0 && (c->head_dim * size) % 16 == 0,
+                "the cache and its strides must be multiples of 16 bytes");
+  out->k = static_cast<char *>(c->k);
+  out->v = static_cast<char *>(c->v);
+  out->page_table = c->page_table;
+  out->table_stride = c->page_table_stride;
+  out->page_stride = c->page_stride * size;
+  out->head_stride = c->head_stride * size;
+  out->token_stride = c->token_stride * size;
+  out->k_scale = c->k_scale;
+  out->v_scale = c->v_scale;
+  out->seqs = c->sequences;
+  out->max_pages = c->max_pages;
+  out->pages = c->pages;
+  out->page_size = c->page_size;
+  out->kv_heads = c->kv_heads;
+  out->head_dim = c->head_dim;
+  return 0;
+}
 
 }  // namespace
 
@@ -732,6 +766,49 @@ int sharq_linear_gemm_swiglu(const void *a_comp, const void *e, const void *sfa_
   g.amax_bits = static_cast<unsigned int *>(amax_bits);
   g.error_flag = error_flag;
   return check_cuda(sharq::run_gemm_swiglu(g, as_stream(stream)), "linear_gemm_swiglu");
+}
+
+int sharq_rope_append_paged(const void *qkv_bf16, int64_t row_stride, int rows, int heads, const void *cos_bf16, const void *sin_bf16,
+                            int table_rows, const int *positions, const int *sequences, const sharq_paged_cache *cache,
+                            void *q_out_bf16, void *k_out_bf16, int *error_flag, void *stream) {
+  sharq::PagedCache c;
+  bool fp8 = false;
+  if (paged_cache(cache, &c, &fp8)) return 1;
+  SHARQ_REQUIRE(qkv_bf16 && cos_bf16 && sin_bf16 && positions && q_out_bf16, "null buffer");
+  SHARQ_REQUIRE(rows >= 0 && heads > 0 && table_rows > 0, "rows must be >= 0, heads and table_rows positive");
+  SHARQ_REQUIRE(c.head_dim % 16 == 0 && c.head_dim <= 256, "head_dim must be a multiple of 16, at most 256, got %d", c.head_dim);
+  SHARQ_REQUIRE((int64_t)heads + 2 * (int64_t)c.kv_heads <= 65536, "at most 65536 heads in a row");
+  SHARQ_REQUIRE(row_stride >= ((int64_t)heads + 2 * (int64_t)c.kv_heads) * c.head_dim && row_stride % 8 == 0,
+                "row_stride must cover all heads and be a multiple of 8");
+  SHARQ_REQUIRE(aligned16(qkv_bf16) && aligned16(cos_bf16) && aligned16(sin_bf16) && aligned16(q_out_bf16) && aligned16(k_out_bf16),
+                "buffers must be 16-byte aligned");
+  return check_cuda(sharq::run_rope_append_paged(qkv_bf16, row_stride, rows, heads, cos_bf16, sin_bf16, table_rows, positions, sequences,
+                                                 c, fp8, q_out_bf16, k_out_bf16, error_flag, as_stream(stream)),
+                    "rope_append_paged");
+}
+
+size_t sharq_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
+  if (heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+  return sharq::paged_attention_workspace_bytes(heads, kv_heads, head_dim);
+}
+
+int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int heads, const sharq_paged_cache *cache,
+                          const int *lengths, float scale, void *out_bf16, void *workspace, size_t workspace_bytes, int *error_flag,
+                          void *stream) {
+  sharq::PagedCache c;
+  bool fp8 = false;
+  if (paged_cache(cache, &c, &fp8)) return 1;
+  SHARQ_REQUIRE(q_bf16 && lengths && out_bf16 && workspace, "null buffer");
+  SHARQ_REQUIRE(c.head_dim == 64 || c.head_dim == 128, "head_dim must be 64 or 128, got %d", c.head_dim);
+  SHARQ_REQUIRE(heads > 0 && heads % c.kv_heads == 0, "heads must be a positive multiple of kv_heads");
+  SHARQ_REQUIRE((int64_t)c.seqs * heads <= 0x7fffffff, "too many sequences");
+  SHARQ_REQUIRE(q_row >= 0 && q_head >= 0 && q_row % 8 == 0 && q_head % 8 == 0, "the strides of q must be multiples of 8");
+  SHARQ_REQUIRE(aligned16(q_bf16) && aligned16(out_bf16) && aligned16(workspace), "buffers must be 16-byte aligned");
+  const size_t need = sharq::paged_attention_workspace_bytes(heads, c.kv_heads, c.head_dim);
+  SHARQ_REQUIRE(workspace_bytes >= need, "workspace too small: need %zu bytes", need);
+  return check_cuda(sharq::run_paged_attention(q_bf16, q_row, q_head, heads, c, fp8, lengths, scale, out_bf16, workspace, error_flag,
+                                               as_stream(stream)),
+                    "paged_attention");
 }
 
 }  // extern "C"

@@ -1,0 +1,183 @@
+// Rotary embedding of a merged qkv activation on its way into a paged key/value cache, for prompts and for single tokens.
+//
+// Row r of qkv holds the query, key and value heads of one token, which has position p = positions[r] of sequence s (r itself, or
+// sequences[r]).  Per query and key head, with the halves (x1, x2):
+//     out1 = x1 cos1 - x2 sin1,   out2 = x2 cos2 + x1 sin2         (rows p of the tables)
+// The queries go to q_out [rows, heads, D], the keys to slot p % page_size of page page_table[s][p / page_size] of the key cache (and to
+// k_out), the values to the same place of the value cache.  The tables and the activation are bf16, so every product is exact in float
+// and a sum is rounded once to float, whichever way it is contracted; it is rounded once more, to bf16 or, divided by the head's scale, to
+// e4m3 (saturating at +-448).
+//
+// Bound by HBM for prompts (2 bytes in and 2 out per element, the tables come from L2) and by latency for single tokens.
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include <cstdint>
+
+#include "decode_ops.cuh"
+#include "sm100_ptx.cuh"
+
+namespace sharq {
+
+namespace {
+
+__device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t *>(&v);
+}
+
+__device__ __forceinline__ void unpack8(const uint4 &w, float (&f)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[2 * j] = lo_f(u[j]), f[2 * j + 1] = hi_f(u[j]);
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7]));
+}
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+
+// eight neighbouring elements of a head into the cache
+template <bool kFp8>
+__device__ __forceinline__ void store8(char *at, const float (&f)[8], float scale) {
+  if (kFp8) {
+    float q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(f[j], scale);
+    *reinterpret_cast<uint2 *>(at) = make_uint2(e4m3x4(q[0], q[1], q[2], q[3]), e4m3x4(q[4], q[5], q[6], q[7]));
+  } else {
+    *reinterpret_cast<uint4 *>(at) = pack8(f);
+  }
+}
+
+struct AppendArgs {
+  const __nv_bfloat16 *qkv, *cos_t, *sin_t;
+  long long row_stride;
+  const int *positions, *sequences;
+  __nv_bfloat16 *q_out, *k_out;
+  int *error_flag;
+  int rows, heads, table_rows, rows_per_cta;
+};
+
+// A thread takes 8 elements of the first half of a head and their 8 partners of the second half; a row's threads are those of one CTA
+// (several rows share one while a row has few).
+template <bool kFp8>
+__global__ void __launch_bounds__(512) rope_append_kernel(AppendArgs a, PagedCache c) {
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  const int half = c.head_dim >> 1;
+  const unsigned vecs = (unsigned)half >> 3;
+  const unsigned per_row = (unsigned)(a.heads + 2 * c.kv_heads) * vecs;
+  unsigned i = threadIdx.x, row = blockIdx.x;
+  if (a.rows_per_cta > 1) {
+    const unsigned in_cta = i / per_row;
+    i -= in_cta * per_row;
+    row = row * a.rows_per_cta + in_cta;
+    if (in_cta >= (unsigned)a.rows_per_cta) return;
+  }
+  if (row >= (unsigned)a.rows) return;
+  const int position = a.positions[row];
+  const int seq = a.sequences != nullptr ? a.sequences[row] : (int)row;
+  const bool padding = position < 0;
+  bool good = !padding && position < a.table_rows && position < paged_capacity(c) && seq >= 0 && seq < c.seqs;
+  int page = 0;
+  if (good) {
+    page = c.page_table[seq * c.table_stride + position / c.page_size];
+    good = page >= 0 && page < c.pages;
+  }
+  if (!good && !padding && i == 0 && a.error_flag != nullptr) atomicExch(a.error_flag, kBadCacheIndex);
+  const long long slot = page * c.page_stride + (position % c.page_size) * c.token_stride;
+  const size_t table = (size_t)position * c.head_dim;
+  for (; i < per_row; i += blockDim.x) {
+    const int head = (int)(i / vecs), v = (int)(i % vecs);
+    const int kv = head - a.heads;  // key head, or kv_heads + value head
+    float x1[8], x2[8];
+    if (good) {
+      const __nv_bfloat16 *x = a.qkv + row * a.row_stride + (size_t)head * c.head_dim + v * 8;
+      unpack8(*reinterpret_cast<const uint4 *>(x), x1);
+      unpack8(*reinterpret_cast<const uint4 *>(x + half), x2);
+      if (kv < c.kv_heads) {
+        float c1[8], c2[8], s1[8], s2[8];
+        unpack8(*reinterpret_cast<const uint4 *>(a.cos_t + table + v * 8), c1);
+        unpack8(*reinterpret_cast<const uint4 *>(a.cos_t + table + v * 8 + half), c2);
+        unpack8(*reinterpret_cast<const uint4 *>(a.sin_t + table + v * 8), s1);
+        unpack8(*reinterpret_cast<const uint4 *>(a.sin_t + table + v * 8 + half), s2);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float o1 = __fadd_rn(__fmul_rn(x1[j], c1[j]), -__fmul_rn(x2[j], s1[j]));
+          x2[j] = __fadd_rn(__fmul_rn(x2[j], c2[j]), __fmul_rn(x1[j], s2[j]));
+          x1[j] = o1;
+        }
+      }
+    } else {
+      // a padding row gives zeros, a row without a place NaN; neither touches the cache
+      const float fill = padding ? 0.0f : __int_as_float(0x7fffffff);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x1[j] = x2[j] = fill;
+    }
+    if (kv < c.kv_heads) {
+      __nv_bfloat16 *out = nullptr;
+      if (kv < 0)
+        out = a.q_out + ((size_t)row * a.heads + head) * c.head_dim + v * 8;
+      else if (a.k_out != nullptr)
+        out = a.k_out + ((size_t)row * c.kv_heads + kv) * c.head_dim + v * 8;
+      if (out != nullptr) {
+        *reinterpret_cast<uint4 *>(out) = pack8(x1);
+        *reinterpret_cast<uint4 *>(out + half) = pack8(x2);
+      }
+    }
+    if (kv >= 0 && good) {
+      const bool value = kv >= c.kv_heads;
+      const int h = value ? kv - c.kv_heads : kv;
+      const int size = kFp8 ? 1 : 2;
+      char *at = (value ? c.v : c.k) + slot + h * c.head_stride + v * 8 * size;
+      const float scale = kFp8 ? (value ? c.v_scale : c.k_scale)[h] : 1.0f;
+      store8<kFp8>(at, x1, scale);
+      store8<kFp8>(at + half * size, x2, scale);
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t run_rope_append_paged(const void *qkv, long long row_stride, int rows, int heads, const void *cos_t, const void *sin_t,
+                                  int table_rows, const int *positions, const int *sequences, const PagedCache &cache, bool fp8,
+                                  void *q_out, void *k_out, int *error_flag, cudaStream_t stream) {
+  if (rows <= 0) return cudaSuccess;
+  const long long per_row = (long long)(heads + 2 * cache.kv_heads) * (cache.head_dim / 16);
+  AppendArgs a;
+  a.qkv = static_cast<const __nv_bfloat16 *>(qkv);
+  a.cos_t = static_cast<const __nv_bfloat16 *>(cos_t);
+  a.sin_t = static_cast<const __nv_bfloat16 *>(sin_t);
+  a.row_stride = row_stride;
+  a.positions = positions;
+  a.sequences = sequences;
+  a.q_out = static_cast<__nv_bfloat16 *>(q_out);
+  a.k_out = static_cast<__nv_bfloat16 *>(k_out);
+  a.error_flag = error_flag;
+  a.rows = rows;
+  a.heads = heads;
+  a.table_rows = table_rows;
+  a.rows_per_cta = per_row < 64 ? (int)(128 / per_row) : 1;
+  const int threads = per_row > 512 ? 512 : (int)((a.rows_per_cta * per_row + 31) / 32 * 32);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)((rows + a.rows_per_cta - 1) / a.rows_per_cta));
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fp8 ? rope_append_kernel<true> : rope_append_kernel<false>, a, cache);
+}
+
+}  // namespace sharq

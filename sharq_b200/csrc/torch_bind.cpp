@@ -11,6 +11,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <optional>
 #include <stdexcept>
@@ -392,6 +394,132 @@ void rope_inplace(const Tensor &qkv, int64_t heads, int64_t head_dim, const Tens
                            ptr(sin), stream_of(qkv)));
 }
 
+// A paged key/value cache as the C ABI takes it (include/sharq_b200.h): k and v [pages, kv_heads, page_size, head_dim].
+sharq_paged_cache cache_of(const Tensor &k, const Tensor &v, const Tensor &table, const std::optional<Tensor> &k_scale,
+                           const std::optional<Tensor> &v_scale, const at::Device &dev) {
+  need(k.is_cuda() && v.is_cuda() && k.device() == dev && v.device() == dev, "k_cache and v_cache must be CUDA tensors on the device of the input");
+  need(k.dim() == 4 && k.sizes() == v.sizes() && k.strides() == v.strides() && k.scalar_type() == v.scalar_type(),
+       "k_cache and v_cache must be shaped [pages, kv_heads, page_size, head_dim], alike in shape, strides and type");
+  const bool fp8 = k.scalar_type() == at::kFloat8_e4m3fn;
+  need(fp8 || k.scalar_type() == at::kBFloat16, "k_cache and v_cache must be torch.bfloat16 or torch.float8_e4m3fn");
+  need(k.numel() > 0 && k.stride(3) == 1, "the cache must have pages, and the elements of a head must be contiguous");
+  // no two elements at one address: every stride reaches over the dimensions with smaller ones
+  std::vector<int> order;
+  for (int d = 0; d < 3; ++d)
+    if (k.size(d) > 1) order.push_back(d);
+  std::sort(order.begin(), order.end(), [&](int a, int b) { return k.stride(a) < k.stride(b); });
+  int64_t reach = k.size(3);
+  for (int d : order) {
+    need(k.stride(d) >= reach, "elements of the cache must not overlap");
+    reach = k.stride(d) * k.size(d);
+  }
+  for (int d = 0; d < 3; ++d) need(k.size(d) <= INT32_MAX, "a dimension of the cache is too large");
+  need(table.is_cuda() && table.device() == dev && table.scalar_type() == at::kInt && table.dim() == 2 &&
+           (table.size(1) <= 1 || table.stride(1) == 1),
+       "page_table must be a CUDA int32 matrix [sequences, pages] with unit column stride on the device of the input");
+  need(table.numel() > 0 && table.size(0) <= INT32_MAX && table.size(1) <= INT32_MAX, "page_table must not be empty");
+  need(table.size(0) == 1 || table.stride(0) >= table.size(1), "rows of page_table must not overlap");
+  const std::optional<Tensor> *scales[2] = {&k_scale, &v_scale};
+  for (const auto *s : scales) {
+    need(s->has_value() == fp8, "k_scale and v_scale are given for a torch.float8_e4m3fn cache and for no other");
+    if (fp8)
+      need(is_plain(**s, at::kFloat) && (*s)->device() == dev && (*s)->dim() == 1 && (*s)->size(0) == k.size(1),
+           "k_scale and v_scale must be contiguous CUDA float32 vectors with one entry per key/value head");
+  }
+  sharq_paged_cache c = {};
+  c.k = ptr(k);
+  c.v = ptr(v);
+  c.page_table = static_cast<const int *>(ptr(table));
+  c.page_table_stride = table.size(0) > 1 ? table.stride(0) : table.size(1);
+  // a dimension of one element has no stride to speak of
+  c.page_stride = k.size(0) > 1 ? k.stride(0) : 0;
+  c.head_stride = k.size(1) > 1 ? k.stride(1) : 0;
+  c.token_stride = k.size(2) > 1 ? k.stride(2) : 0;
+  if (fp8) {
+    c.k_scale = static_cast<const float *>(ptr(*k_scale));
+    c.v_scale = static_cast<const float *>(ptr(*v_scale));
+  }
+  c.sequences = (int)table.size(0);
+  c.max_pages = (int)table.size(1);
+  c.pages = (int)k.size(0);
+  c.page_size = (int)k.size(2);
+  c.kv_heads = (int)k.size(1);
+  c.head_dim = (int)k.size(3);
+  return c;
+}
+
+int *flag_of(const Tensor &flag) { return static_cast<int *>(ptr(flag)); }
+
+void check_indices(const Tensor &t, int64_t n, const at::Device &dev, const char *name) {
+  if (!(is_plain(t, at::kInt) && t.device() == dev && t.dim() == 1 && t.size(0) == n))
+    fail(std::string(name) + " must be a contiguous CUDA int32 vector with " + std::to_string(n) + " entries on the device of the input");
+}
+
+// -> (q [rows, heads, head_dim], k [rows, kv_heads, head_dim] or an empty tensor)
+std::vector<Tensor> rope_append_paged(const Tensor &qkv, int64_t heads, int64_t kv_heads, int64_t head_dim, const Tensor &cos,
+                                      const Tensor &sin, const Tensor &positions, const Tensor &table, const Tensor &k_cache,
+                                      const Tensor &v_cache, const std::optional<Tensor> &sequences,
+                                      const std::optional<Tensor> &k_scale, const std::optional<Tensor> &v_scale, bool return_k,
+                                      const Tensor &flag) {
+  need(qkv.is_cuda() && qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 2 && qkv.stride(1) == 1,
+       "qkv must be a CUDA bfloat16 matrix with unit column stride");
+  const at::Device dev = qkv.device();
+  const int64_t rows = qkv.size(0);
+  need(heads > 0 && kv_heads > 0 && head_dim > 0 && heads <= 65536 && kv_heads <= 65536 && head_dim <= 256,
+       "heads and kv_heads must be in [1, 65536], head_dim in [1, 256]");
+  need((heads + 2 * kv_heads) * head_dim <= qkv.size(1), "(heads + 2 * kv_heads) * head_dim exceeds the row width");
+  const Tensor *tables[2] = {&cos, &sin};
+  for (int i = 0; i < 2; ++i)
+    if (!(is_plain(*tables[i], at::kBFloat16) && tables[i]->device() == dev && tables[i]->dim() == 2 && tables[i]->size(0) > 0 &&
+          tables[i]->sizes() == cos.sizes() && tables[i]->size(1) == head_dim))
+      fail(std::string(i == 0 ? "cos" : "sin") + " must be a contiguous CUDA bfloat16 tensor shaped [positions, head_dim]");
+  need(rows <= INT32_MAX && cos.size(0) <= INT32_MAX, "too many rows");
+  const sharq_paged_cache c = cache_of(k_cache, v_cache, table, k_scale, v_scale, dev);
+  need(c.kv_heads == kv_heads && c.head_dim == head_dim, "the cache must have kv_heads heads of head_dim elements");
+  check_indices(positions, rows, dev, "positions");
+  if (sequences)
+    check_indices(*sequences, rows, dev, "sequences");
+  else
+    need(rows <= c.sequences, "page_table must have a row for every row of qkv when sequences is not given");
+  c10::cuda::OptionalCUDAGuard guard(dev);
+  Tensor q = empty_like_on(qkv, {rows, heads, head_dim}, at::kBFloat16);
+  Tensor k = empty_like_on(qkv, {return_k ? rows : 0, kv_heads, head_dim}, at::kBFloat16);
+  if (rows > 0)
+    check(sharq_rope_append_paged(ptr(qkv), rows > 1 ? qkv.stride(0) : qkv.size(1) / 8 * 8, (int)rows, (int)heads, ptr(cos), ptr(sin),
+                                  (int)cos.size(0), static_cast<const int *>(ptr(positions)),
+                                  sequences ? static_cast<const int *>(ptr(*sequences)) : nullptr, &c, ptr(q), return_k ? ptr(k) : nullptr,
+                                  flag_of(flag), stream_of(qkv)));
+  return {q, k};
+}
+
+Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &table, const Tensor &lengths,
+                       const std::optional<double> &scale, const std::optional<Tensor> &k_scale, const std::optional<Tensor> &v_scale,
+                       const std::optional<Tensor> &out, const Tensor &flag) {
+  need(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.stride(2) == 1,
+       "q must be a CUDA bfloat16 tensor shaped [sequences, heads, head_dim] whose heads are contiguous");
+  const at::Device dev = q.device();
+  const sharq_paged_cache c = cache_of(k_cache, v_cache, table, k_scale, v_scale, dev);
+  const int64_t seqs = q.size(0), heads = q.size(1), d = q.size(2);
+  need(table.size(0) >= seqs, "page_table must have a row for every row of q");
+  need(d == c.head_dim && heads > 0 && heads % c.kv_heads == 0,
+       "q must have head_dim elements per head and a multiple of the cache's heads");
+  check_indices(lengths, seqs, dev, "lengths");
+  if (out)
+    need(is_plain(*out, at::kBFloat16) && out->device() == dev && out->sizes() == q.sizes(),
+         "out must be a contiguous CUDA bfloat16 tensor shaped like q");
+  c10::cuda::OptionalCUDAGuard guard(dev);
+  Tensor o = out ? *out : empty_like_on(q, {seqs, heads, d}, at::kBFloat16);
+  if (seqs == 0) return o;
+  sharq_paged_cache used = c;
+  used.sequences = (int)seqs;
+  const int64_t ws_bytes = (int64_t)sharq_paged_attention_workspace_bytes((int)heads, c.kv_heads, (int)d);
+  Tensor ws = empty_like_on(q, {ws_bytes}, at::kByte);
+  check(sharq_paged_attention(ptr(q), seqs > 1 ? q.stride(0) : 0, heads > 1 ? q.stride(1) : 0, (int)heads, &used,
+                              static_cast<const int *>(ptr(lengths)), (float)(scale ? *scale : 1.0 / std::sqrt((double)d)), ptr(o), ptr(ws),
+                              (size_t)ws_bytes, flag_of(flag), stream_of(q)));
+  return o;
+}
+
 // The GIL is released while a call allocates and launches (a launch waits when the queue of the GPU is full).
 template <typename... Args>
 auto as_tuple(std::vector<Tensor> (*fn)(Args...)) {
@@ -424,6 +552,8 @@ PYBIND11_MODULE(sharq_native, m) {
   m.def("scaled_quantize", as_tuple(&scaled_quantize));
   m.def("linear_gemm_swiglu", as_tuple(&linear_gemm_swiglu));
   m.def("absmax_prepare", as_tuple(&absmax_prepare));
+  m.def("rope_append_paged", as_tuple(&rope_append_paged));
+  m.def("paged_attention", &paged_attention, nogil());
   m.def("rope_inplace", &rope_inplace, nogil());
   m.def("linear_gemm", &linear_gemm, nogil());
   m.def("linear_forward", &linear_forward, nogil());

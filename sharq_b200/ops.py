@@ -29,6 +29,7 @@ _ERROR_FLAGS: dict[int, torch.Tensor] = {}
 _NO_FLAG = torch.zeros(1, dtype=torch.int32, device="cpu")
 _PREPARE_TIMEOUTS_SEEN = 0
 _BAD_EXPERT = 0x401  # kPlanBadExpert of csrc/decoder_ops.cu
+_BAD_CACHE_INDEX = 0x402  # kBadCacheIndex of csrc/decode_ops.cuh
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -57,7 +58,8 @@ def _error_flag(device: torch.device) -> torch.Tensor:
 
 def check_device_errors(device=None) -> None:
     """Synchronising check of the kernels' bounded waits, the GEMM / all-reduce error flag of each device and the grid
-    barrier of the one-launch prepare, and of the expert ids that a mixture-of-experts plan was given."""
+    barrier of the one-launch prepare, of the expert ids that a mixture-of-experts plan was given, and of the positions, lengths and
+    pages that the paged cache was used with."""
     global _PREPARE_TIMEOUTS_SEEN
     if torch.cuda.is_available() and torch.cuda.is_initialized():
         torch.cuda.synchronize()
@@ -73,6 +75,9 @@ def check_device_errors(device=None) -> None:
             flag.zero_()
             if code == _BAD_EXPERT:
                 raise RuntimeError(f"sharq_b200 moe_plan: an expert id was outside [0, experts) on cuda:{idx}")
+            if code == _BAD_CACHE_INDEX:
+                raise RuntimeError("sharq_b200 paged cache: a position, length, sequence or page was outside the cache or its tables "
+                                   f"on cuda:{idx}")
             raise RuntimeError(f"sharq_b200 GEMM kernel reported a timed-out wait (code {code}) on cuda:{idx}")
 
 
@@ -190,6 +195,35 @@ def rope_inplace_(qkv: torch.Tensor, heads: int, head_dim: int, cos: torch.Tenso
     Equals `x * cos + rotate_half(x) * sin` of the ATen ops, head by head."""
     _lib.native().rope_inplace(qkv, heads, head_dim, cos, sin, seq_len)
     return qkv
+
+
+def rope_append_paged(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: int, cos: torch.Tensor, sin: torch.Tensor,
+                      positions: torch.Tensor, page_table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      sequences: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
+                      v_scale: Optional[torch.Tensor] = None, return_k: bool = False):
+    """Rotary embedding of the query and key heads of a merged qkv activation [rows, >= (heads + 2 * kv_heads) * head_dim]
+    (bf16), with keys and values appended to a paged cache -> q [rows, heads, head_dim], or (q, k [rows, kv_heads, head_dim])
+    with return_k.  Row r is the token at position positions[r] (int32) of sequence sequences[r] (int32, default r); cos and sin
+    bf16 [positions, head_dim].  k_cache / v_cache [pages, kv_heads, page_size, head_dim] (any order of the first three
+    dimensions), bf16 or, with k_scale and v_scale (float32 [kv_heads]), float8_e4m3fn values of x / scale; the token lies in slot
+    p % page_size of page page_table[sequence, p // page_size] (int32).  float32 arithmetic, one rounding per result.  A negative
+    position is padding (zeros, nothing appended); a place outside the tables or the cache gives NaN, appends nothing and is reported by
+    check_device_errors.  No two rows may have the same place."""
+    q, k = _lib.native().rope_append_paged(qkv, heads, kv_heads, head_dim, cos, sin, positions, page_table, k_cache, v_cache,
+                                           sequences, k_scale, v_scale, return_k, _error_flag(qkv.device))
+    return (q, k) if return_k else q
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                    scale: Optional[float] = None, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per sequence over a paged cache (see rope_append_paged for its layout): q bf16
+    [sequences, heads, head_dim] (heads contiguous, other strides multiples of 8), head_dim 64 or 128, heads a multiple of the cache's
+    -> bf16 [sequences, heads, head_dim], the softmax of scale * q . k (default head_dim ** -0.5) over the first lengths[s] (int32) tokens
+    of every sequence, the new one among them, applied to the values.  Length 0 gives zeros.  A length beyond the page table or a page
+    outside the cache makes that sequence's rows NaN and is reported by check_device_errors.  A sequence may stand in several
+    rows with lengths of their own (drafted tokens).  The same bits from call to call."""
+    return _lib.native().paged_attention(q, k_cache, v_cache, page_table, lengths, scale, k_scale, v_scale, out, _error_flag(q.device))
 
 
 def scatter_add_scaled_(out: torch.Tensor, y: torch.Tensor, rows: torch.Tensor, w: torch.Tensor) -> torch.Tensor:

@@ -1,0 +1,295 @@
+"""Rotary embedding with the append to a paged cache, and attention over it, against their definitions in 64 bits."""
+import pytest
+import torch
+
+from tests import paged_util as P
+
+pytestmark = pytest.mark.gpu
+
+
+def _append(ops, qkv, heads, kv, dim, cos, sin, positions, table, cache, **kw):
+    k, v, ks, vs = cache
+    return ops.rope_append_paged(qkv, heads, kv, dim, cos, sin, positions, table, k, v, k_scale=ks, v_scale=vs, **kw)
+
+
+@pytest.mark.parametrize("order", ["hnd", "nhd"])
+@pytest.mark.parametrize("fp8", [False, True])
+# one row; a decode batch; ragged prompts of sequences in any order; rows that share a CTA; rows of more vectors than a CTA has threads
+@pytest.mark.parametrize("rows,heads,kv,dim,page", [(1, 32, 8, 128, 16), (37, 28, 4, 128, 24), (300, 4, 1, 64, 8), (5, 1, 1, 16, 1),
+                                                    (3, 70, 5, 128, 32), (9, 8, 2, 256, 7)])
+def test_append(rows, heads, kv, dim, page, fp8, order):
+    from sharq_b200 import ops
+
+    g = torch.Generator().manual_seed(rows + dim)
+    seqs = max(1, rows // 3)
+    # sequences of several rows, at scattered positions of their own
+    per = torch.full((seqs,), rows // seqs)
+    per[:rows % seqs] += 1
+    reach = [int(n) + 11 + 3 * i for i, n in enumerate(per)]
+    sequences = torch.cat([torch.full((int(n),), i) for i, n in enumerate(per)])
+    positions = torch.cat([torch.randperm(r, generator=g)[:int(n)] for r, n in zip(reach, per)])
+    mixed = torch.randperm(rows, generator=g)
+    sequences, positions = (t[mixed].to(torch.int32).cuda() for t in (sequences, positions))
+    table, pages = P.make_table(reach, page, 2, seed=rows)
+    cache = P.make_cache(pages, kv, page, dim, fp8, 3, order)
+    before = [c.clone() for c in cache[:2]]
+    qkv = torch.randn(rows, (heads + 2 * kv) * dim + 24, generator=g).to(torch.bfloat16).cuda()[:, :(heads + 2 * kv) * dim + 8]
+    cos, sin = P.rope_tables(max(reach), dim)
+    q, k = _append(ops, qkv, heads, kv, dim, cos, sin, positions, table, cache, sequences=sequences, return_k=True)
+    ops.check_device_errors()
+    want_q, want_k, want_v = P.rotated64(qkv, heads, kv, dim, cos, sin, positions)
+    # products of bf16 values are exact in float; the sum is rounded to float (2^-24) and to bf16 (2^-8)
+    for got, want in ((q, want_q), (k, want_k)):
+        assert bool(((got.double() - want).abs() <= 2.0 ** -8 * (1 + 2.0 ** -15) * want.abs()).all())
+    pages_at = table[sequences.long(), (positions // page).long()].long()
+    slots = (positions % page).long()
+    for c, was, want, scale in zip(cache[:2], before, (want_k, want_v), cache[2:]):
+        got = c[pages_at, :, slots]
+        if fp8:
+            # what a float division and one conversion give, to the bit; and within half a step (2^-4, or 2^-10 of the subnormal ones)
+            exact = (want / scale.double()[:, None]).clamp(-448, 448)
+            plain = (want.float() / scale[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+            assert torch.equal(got.view(torch.uint8), plain.view(torch.uint8))
+            assert bool(((got.double() - exact).abs() <= 2.0 ** -4 * (1 + 2.0 ** -15) * exact.abs() + 2.0 ** -10).all())
+        else:
+            assert bool(((got.double() - want).abs() <= 2.0 ** -8 * (1 + 2.0 ** -15) * want.abs()).all())
+        # every other place is as it was
+        was[pages_at, :, slots] = got
+        assert torch.equal(c.contiguous().view(torch.uint8), was.contiguous().view(torch.uint8))
+    # without the keys, and (one row per sequence) without a list of sequences
+    only = _append(ops, qkv, heads, kv, dim, cos, sin, positions, table, cache, sequences=sequences)
+    assert torch.equal(only, q)
+
+
+def test_append_of_rows_without_sequences_equals_listed_ones():
+    from sharq_b200 import ops
+
+    table, pages = P.make_table([40, 3, 17], 16, 1, 5)
+    cos, sin = P.rope_tables(64, 128)
+    qkv = torch.randn(3, 48 * 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    positions = torch.tensor([39, 2, 16], dtype=torch.int32).cuda()
+    a, b = (P.make_cache(pages, 8, 16, 128, False, 3) for _ in range(2))
+    qa = _append(ops, qkv, 32, 8, 128, cos, sin, positions, table, a)
+    qb = _append(ops, qkv, 32, 8, 128, cos, sin, positions, table, b, sequences=torch.arange(3, dtype=torch.int32).cuda())
+    assert torch.equal(qa, qb) and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_append_leaves_out_padding_and_reports_bad_places():
+    from sharq_b200 import ops
+
+    page, kv, dim, heads = 8, 2, 64, 4
+    table, pages = P.make_table([16, 16, 16], page, 1, 5)
+    table[2, 0] = pages  # one behind the last page
+    cos, sin = P.rope_tables(64, dim)
+    qkv = torch.randn(7, (heads + 2 * kv) * dim, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    #            padding, good, beyond the table of pages, bad page, bad sequences, beyond the tables of angles
+    sequences = torch.tensor([0, 1, 1, 2, 3, -1, 0], dtype=torch.int32).cuda()
+    positions = torch.tensor([-1, 15, 16, 3, 0, 0, 64], dtype=torch.int32).cuda()
+    cache = P.make_cache(pages, kv, page, dim, False, 3)
+    before = [c.clone() for c in cache[:2]]
+    q, k = _append(ops, qkv, heads, kv, dim, cos, sin, positions, table, cache, sequences=sequences, return_k=True)
+    with pytest.raises(RuntimeError, match="paged cache"):
+        ops.check_device_errors()
+    ops.check_device_errors()  # reported once
+    assert bool((q[0] == 0).all()) and bool((k[0] == 0).all())
+    assert bool(torch.isfinite(q[1]).all())
+    assert bool(q[2:].isnan().all()) and bool(k[2:].isnan().all())
+    for c, was in zip(cache[:2], before):
+        was[table[1, 1], :, 7] = c[table[1, 1], :, 7]
+        assert torch.equal(c, was)
+
+
+SHAPES = [  # sequences' lengths, heads, kv_heads, dim, page size
+    ([1], 32, 8, 128, 16),
+    ([0], 4, 2, 128, 16),
+    ([2, 0, 1, 63, 64, 65], 8, 8, 64, 16),
+    ([97], 32, 8, 128, 16),
+    ([15, 16, 17, 31, 32, 33, 0, 129], 28, 4, 128, 24),
+    ([5000], 4, 1, 128, 64),
+    ([777, 3, 2048, 1500], 16, 1, 128, 128),   # 16 query heads of one key/value head
+    ([100, 900], 24, 1, 64, 7),                # 24: two pieces
+    ([40, 41], 36, 2, 128, 1),                 # 18: two pieces, pages of one token
+    ([300] * 40, 9, 3, 128, 32),               # many equal sequences
+    ([3000, 1] + [0] * 5 + [64] * 70, 10, 2, 64, 256),
+]
+
+
+@pytest.mark.parametrize("order", ["hnd", "nhd"])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("lengths,heads,kv,dim,page", SHAPES)
+def test_attention(lengths, heads, kv, dim, page, fp8, order):
+    from sharq_b200 import ops
+
+    table, pages = P.make_table(lengths, page, 2, seed=len(lengths))
+    k, v, ks, vs = P.make_cache(pages, kv, page, dim, fp8, 7, order)
+    g = torch.Generator().manual_seed(11)
+    # rows of a merged activation: the heads of a row are contiguous, the rows are not
+    merged = (2 * torch.randn(len(lengths), (heads + 2 * kv) * dim, generator=g)).to(torch.bfloat16).cuda()
+    q = merged[:, :heads * dim].view(len(lengths), heads, dim)
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    got = ops.paged_attention(q, k, v, table, n, k_scale=ks, v_scale=vs)
+    ops.check_device_errors()
+    out, size, reach = P.attention64(q, P.values64(k, ks), P.values64(v, vs), table, lengths)
+    bound = P.attention_bound(out, size, reach, dim, max(lengths), fp8)
+    assert bool(((got.double() - out).abs() <= bound).all()), float(((got.double() - out).abs() / bound).max())
+    assert bool((got[torch.tensor(lengths) == 0] == 0).all())
+    # the same bits again, into a given tensor
+    again = torch.full_like(got, 7.0)
+    assert ops.paged_attention(q, k, v, table, n, k_scale=ks, v_scale=vs, out=again) is not None
+    assert torch.equal(again, got)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_ignores_what_lies_behind_a_sequence(dim, fp8):
+    """NaN and infinities in slots behind the length and in pages of nobody, bad entries behind the last page."""
+    from sharq_b200 import ops
+
+    lengths, page = [5, 40, 0, 33], 16
+    table, pages = P.make_table(lengths, page, 3, 1, unused=2 ** 30)
+    k, v, ks, vs = P.make_cache(pages, 2, page, dim, fp8, 7)
+    used = torch.zeros(pages, page, dtype=torch.bool)
+    for i, n in enumerate(lengths):
+        for j in range(n):
+            used[int(table[i, j // page]), j % page] = True
+    used = used.cuda()
+    q = torch.randn(4, 6, dim, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    clean = ops.paged_attention(q, k, v, table, n, k_scale=ks, v_scale=vs)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        dirty = [torch.where(used[:, None, :, None], c.float(), bad).to(c.dtype) for c in (k, v)]
+        assert torch.equal(ops.paged_attention(q, *dirty, table, n, k_scale=ks, v_scale=vs), clean)
+    ops.check_device_errors()
+
+
+def test_attention_reports_bad_lengths_and_pages():
+    from sharq_b200 import ops
+
+    page, dim = 16, 128
+    for fp8 in (False, True):
+        table, pages = P.make_table([64, 64, 64, 64, 64], page, 1, 1)
+        k, v, ks, vs = P.make_cache(pages, 2, page, dim, fp8, 7)
+        q = torch.randn(5, 8, dim, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+        good = ops.paged_attention(q, k, v, table, torch.full((5,), 64, dtype=torch.int32).cuda(), k_scale=ks, v_scale=vs)
+        ops.check_device_errors()
+        table[3, 2] = -1
+        table[4, 3] = pages
+        n = torch.tensor([64, -1, 65, 64, 64], dtype=torch.int32).cuda()
+        got = ops.paged_attention(q, k, v, table, n, k_scale=ks, v_scale=vs)
+        with pytest.raises(RuntimeError, match="paged cache"):
+            ops.check_device_errors()
+        assert torch.equal(got[0], good[0]) and bool(got[1:].isnan().all())
+        n[4] = 48  # the bad page lies behind the last one in use
+        got = ops.paged_attention(q, k, v, table, n, k_scale=ks, v_scale=vs)
+        assert bool(torch.isfinite(got[4]).all())
+        with pytest.raises(RuntimeError, match="paged cache"):
+            ops.check_device_errors()
+
+
+def test_attention_of_extreme_scores():
+    """Scores far apart, equal, -inf through values of the cache, and a scale that is negative or zero."""
+    from sharq_b200 import ops
+
+    lengths, page, dim = [50, 200], 16, 128
+    table, pages = P.make_table(lengths, page, 1, 1)
+    for fp8 in (False, True):
+        k, v, ks, vs = P.make_cache(pages, 1, page, dim, fp8, 7)
+        q = (30 * torch.randn(2, 4, dim, generator=torch.Generator().manual_seed(2))).to(torch.bfloat16).cuda()
+        q[1, 0] = 0
+        q[1, 1] *= 2.0 ** -100
+        n = torch.tensor(lengths, dtype=torch.int32).cuda()
+        for scale in (None, 0.0, -0.5, 1.0):
+            got = ops.paged_attention(q, k, v, table, n, scale=scale, k_scale=ks, v_scale=vs)
+            out, size, reach = P.attention64(q, P.values64(k, ks), P.values64(v, vs), table, lengths, scale)
+            bound = P.attention_bound(out, size, reach, dim, 200, fp8)
+            assert bool(((got.double() - out).abs() <= bound).all()), (fp8, scale)
+    # an infinite key: a score of -inf drops its token, one of +inf or NaN makes the row NaN
+    k, v, _, _ = P.make_cache(pages, 1, page, dim, False, 7)
+    at = (table[0, 0].item(), 0, 3)
+    k[at][0] = float("inf")
+    q = q.abs()
+    q[0, 1, 0] = -1
+    got = ops.paged_attention(q, k, v, table, n)
+    out, size, reach = P.attention64(q, P.values64(k, None), P.values64(v, None), table, lengths)
+    assert bool(got[0, 0].isnan().all()) and bool(torch.isfinite(got[0, 1]).all())
+    k[at][0] = 0
+    k[at][1:] = -30000  # in its place a score that is as good as -inf: its probability is 0 either way
+    q[0, 1, 0] = 1
+    lo = ops.paged_attention(q, k, v, table, n)[0, 1]
+    out, size, reach = P.attention64(q, P.values64(k, None), P.values64(v, None), table, lengths)
+    assert bool(((lo.double() - out[0, 1]).abs() <= P.attention_bound(out, size, reach, dim, 200, False)[0, 1]).all())
+
+
+def test_attention_far_into_a_large_cache():
+    """Offsets beyond 2^31 elements and 2^32 bytes."""
+    from sharq_b200 import ops
+
+    kv, page, dim = 8, 128, 128
+    pages = 2 ** 32 // (kv * page * dim * 2) + 3
+    k = torch.zeros(pages, kv, page, dim, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    last = pages - 1
+    g = torch.Generator().manual_seed(2)
+    cos, sin = P.rope_tables(256, dim)
+    table = torch.tensor([[last, last - 1]], dtype=torch.int32).cuda()
+    qkv = torch.randn(200, (16 + 2 * kv) * dim, generator=g).to(torch.bfloat16).cuda()
+    positions = torch.arange(200, dtype=torch.int32).cuda()
+    q = ops.rope_append_paged(qkv, 16, kv, dim, cos, sin, positions, table, k, v, sequences=torch.zeros(200, dtype=torch.int32).cuda())
+    got = ops.paged_attention(q[-1:], k, v, table, torch.tensor([200], dtype=torch.int32).cuda())
+    ops.check_device_errors()
+    assert not bool(k[:last - 1].any())
+    small = torch.tensor([[0, 1]], dtype=torch.int32).cuda()
+    want, size, reach = P.attention64(q[-1:], *(P.values64(c[[last, last - 1]], None) for c in (k, v)), small, [200])
+    assert bool(((got.double() - want).abs() <= P.attention_bound(want, size, reach, dim, 200, False)).all())
+
+
+def test_refusals():
+    from sharq_b200 import ops
+
+    table, pages = P.make_table([40, 30], 16, 1, 5)
+    k, v, _, _ = P.make_cache(pages, 2, 16, 128, False, 3)
+    k8, v8, ks, vs = P.make_cache(pages, 2, 16, 128, True, 3)
+    cos, sin = P.rope_tables(64, 128)
+    q = torch.zeros(2, 4, 128, dtype=torch.bfloat16).cuda()
+    n = torch.tensor([1, 2], dtype=torch.int32).cuda()
+    qkv = torch.zeros(2, 8 * 128, dtype=torch.bfloat16).cuda()
+
+    def attend(match, *args, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            ops.paged_attention(*args, **kw)
+
+    attend("CUDA bfloat16", q.float(), k, v, table, n)
+    attend("multiple of the cache's heads", q[:, :3], k, v, table, n)
+    attend("head_dim", q[..., :64].contiguous(), k, v, table, n)
+    attend("heads are contiguous", q.transpose(1, 2), k, v, table, n)
+    attend("k_scale", q, k8, v8, table, n)
+    attend("k_scale", q, k, v, table, n, k_scale=ks, v_scale=vs)
+    attend("k_scale", q, k8, v8, table, n, k_scale=ks[:1], v_scale=vs)
+    attend("alike", q, k, v8, table, n)
+    attend("alike", q, k, v[1:], table, n)
+    attend("bfloat16 or torch.float8_e4m3fn", q, k.half(), v.half(), table, n)
+    attend("overlap", q, k[:1].expand(pages, -1, -1, -1), v[:1].expand(pages, -1, -1, -1), table, n)
+    attend("int32", q, k, v, table.long(), n)
+    attend("int32", q, k, v, table, n.long())
+    attend("row for every row", q, k, v, table[:1], n)
+    attend("page_table must not be empty", q, k, v, table[:, :0], n)
+    attend("out must be", q, k, v, table, n, out=torch.empty_like(q).float())
+    attend("head_dim must be 64 or 128", q[..., :32].contiguous(), k[..., :32].contiguous(), v[..., :32].contiguous(), table, n)
+    attend("multiples of 8", torch.zeros(2, 4 * 128 + 4, dtype=torch.bfloat16).cuda()[:, 4:].view(2, 4, 128), k, v, table, n)
+
+    def append(match, *args, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            ops.rope_append_paged(*args, **kw)
+
+    append("unit column stride", qkv.t(), 4, 2, 128, cos, sin, n, table, k, v)
+    append("exceeds the row width", qkv[:, :-8], 4, 2, 128, cos, sin, n, table, k, v)
+    append("cos must be", qkv, 4, 2, 128, cos.float(), sin, n, table, k, v)
+    append("sin must be", qkv, 4, 2, 128, cos, sin[:-1], n, table, k, v)
+    append("positions must be", qkv, 4, 2, 128, cos, sin, n.long(), table, k, v)
+    append("sequences must be", qkv, 4, 2, 128, cos, sin, n, table, k, v, sequences=n[:1])
+    append("row for every row", qkv, 4, 2, 128, cos, sin, n, table[:1], k, v)
+    append("kv_heads heads", qkv, 6, 1, 128, cos, sin, n, table, k, v)
+    append("16-byte aligned", torch.zeros(2, 8 * 128 + 8, dtype=torch.bfloat16).cuda()[:, 4:], 4, 2, 128, cos, sin, n, table, k, v)
+    # nothing to do
+    assert ops.paged_attention(q[:0], k, v, table, n[:0]).shape == (0, 4, 128)
+    assert ops.rope_append_paged(qkv[:0], 4, 2, 128, cos, sin, n[:0], table, k, v).shape == (0, 4, 128)
