@@ -415,6 +415,13 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
                           const int *lengths, float scale, void *out_bf16, void *workspace, size_t workspace_bytes, int *error_flag,
                           void *stream);
 
+/* Product of m (1 to 16) unquantised bf16 rows (x_row elements between them, a multiple of 8) with a 4-bit weight:
+ * y[m, n] = bf16(scale * scale_dev[0] * sum_k x[m, k] * W[n, k] + bias[n]), W = payload qw [n, k/2] times the dense scale factors sfw_dense, as
+ * sharq_quantize_w32_shared and sharq_quantize_nvfp4 make them.  scale_dev (float on the device) and bias (bf16 [n]) may be NULL.  Float
+ * sums, one rounding.  k % 64 == 0; x, qw and sfw_dense 16-byte aligned. */
+int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, int k, const void *qw, const void *sfw_dense,
+                             const float *scale_dev, float scale, const void *bias_bf16, void *y_bf16, void *stream);
+
 /* Test/tuning hook: how many SM clock cycles a cross-GPU wait of the all-reduce and transition
  * kernels may take before the kernel gives up, stores its error code and returns (0 restores the
  * defaults of two to ten seconds).  Applies to launches made after the call. */

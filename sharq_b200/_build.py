@@ -23,7 +23,8 @@ BIND_TAG_PATH = LIB_DIR / "sharq_native.tag"  # what the binding was built again
 BIND_SOURCE = CSRC / "torch_bind.cpp"
 HEADER = PKG.parent / "include" / "sharq_b200.h"
 SOURCES = ["prepare.cu", "prepare_static.cu", "sp_transition.cu", "quant.cu", "gemm.cu", "allreduce.cu", "decoder_ops.cu",
-           "paged_cache.cu", "paged_attention.cu", "c_api.cu"]
+           "paged_cache.cu", "paged_attention.cu", "weight_only.cu",
+           "c_api.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

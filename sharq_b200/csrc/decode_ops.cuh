@@ -33,4 +33,9 @@ size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
 cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head, int heads, const PagedCache &cache, bool fp8,
                                 const int *lengths, float scale, void *out, void *workspace, int *error_flag, cudaStream_t stream);
 
+// y[m, n] = bf16(scale * x . W^T + bias), m rows (1..16) of bf16 against a 4-bit weight with dense scale factors, k % 64 == 0.
+constexpr int kWeightOnlyMaxRows = 16;
+cudaError_t run_weight_only(const void *x, long long x_row, int m, int n, int k, const void *qw, const void *sf, const float *scale_dev,
+                            float scale, const void *bias, void *y, cudaStream_t stream);
+
 }  // namespace sharq

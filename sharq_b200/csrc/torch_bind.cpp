@@ -520,6 +520,32 @@ Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_c
   return o;
 }
 
+Tensor weight_only_linear(const Tensor &x, const Tensor &qw, const Tensor &sf, const std::optional<Tensor> &scale_t, double scale,
+                          const std::optional<Tensor> &bias, const std::optional<Tensor> &out) {
+  need(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1),
+       "x must be a CUDA bfloat16 matrix with unit column stride");
+  const at::Device dev = x.device();
+  const int64_t m = x.size(0), k = x.size(1);
+  need(qw.is_cuda() && qw.dim() == 2 && qw.size(0) > 0 && qw.size(0) <= INT32_MAX && k <= INT32_MAX, "qw must be a CUDA matrix [N, K/2]");
+  const int64_t n = qw.size(0);
+  if (qw.size(1) * 2 != k) fail("qw must have K/2 = " + std::to_string(k / 2) + " columns, got " + std::to_string(qw.size(1)));
+  if (k == 0 || k % 64 != 0) fail("weight_only_linear requires K to be a multiple of 64, got " + std::to_string(k));
+  if (m > 16) fail("weight_only_linear takes at most 16 rows, got " + std::to_string(m));
+  const Tensor *held[2] = {&qw, &sf};
+  for (int i = 0; i < 2; ++i)
+    if (!(is_plain(*held[i], at::kByte) && held[i]->device() == dev && held[i]->numel() == (i == 0 ? n * (k / 2) : sf_bytes(n, k))))
+      fail(std::string(i == 0 ? "qw" : "sfw_dense") + " must be a contiguous CUDA uint8 tensor of " +
+           std::to_string(i == 0 ? n * (k / 2) : sf_bytes(n, k)) + " bytes on the device of x");
+  check_bias(bias, n, dev);
+  const float *scale_dev = scale_t ? scale_ptr(*scale_t, dev, "weight_scale") : nullptr;
+  c10::cuda::OptionalCUDAGuard guard(dev);
+  Tensor y = output(x, m, n, out);
+  if (m == 0) return y;
+  check(sharq_weight_only_linear(ptr(x), x.stride(0), (int)m, (int)n, (int)k, ptr(qw), ptr(sf), scale_dev, (float)scale,
+                                 bias ? ptr(*bias) : nullptr, ptr(y), stream_of(x)));
+  return y;
+}
+
 // The GIL is released while a call allocates and launches (a launch waits when the queue of the GPU is full).
 template <typename... Args>
 auto as_tuple(std::vector<Tensor> (*fn)(Args...)) {
@@ -554,6 +580,7 @@ PYBIND11_MODULE(sharq_native, m) {
   m.def("absmax_prepare", as_tuple(&absmax_prepare));
   m.def("rope_append_paged", as_tuple(&rope_append_paged));
   m.def("paged_attention", &paged_attention, nogil());
+  m.def("weight_only_linear", &weight_only_linear, nogil());
   m.def("rope_inplace", &rope_inplace, nogil());
   m.def("linear_gemm", &linear_gemm, nogil());
   m.def("linear_forward", &linear_forward, nogil());

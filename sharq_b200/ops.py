@@ -543,6 +543,16 @@ def sharq_linear_forward(x: torch.Tensor, qw: torch.Tensor, sfw_sparse: torch.Te
     return _lib.native().linear_forward(x, qw, sfw_sparse, sfw_dense, weight_scale, bias, _error_flag(x.device), _split_k())
 
 
+def weight_only_linear(x: torch.Tensor, qw: torch.Tensor, sfw_dense: torch.Tensor, weight_scale, bias: Optional[torch.Tensor] = None,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bf16(weight_scale * x . W^T + bias) of at most 16 unquantised bf16 rows [M, K] (unit column stride) with a 4-bit weight: qw [N, K/2]
+    and its dense scale factors, as quantize_w32_shared and quantize_w_nvfp4 make them, K % 64 == 0.  weight_scale: python float or
+    1-element CUDA float32 tensor.  float32 sums, one rounding.  One launch, and no quantisation of the activation: for decode
+    steps of few tokens, which read the weight once either way."""
+    scale_t = weight_scale if isinstance(weight_scale, torch.Tensor) else None
+    return _lib.native().weight_only_linear(x, qw, sfw_dense, scale_t, 1.0 if scale_t is not None else float(weight_scale), bias, out)
+
+
 # --------------------------------------------------------------------------- grouped (mixture-of-experts) launches
 
 def _check_grouped(x: torch.Tensor, unit_group: torch.Tensor, groups: int, name: str):

@@ -226,5 +226,17 @@ class QLinearLayer(nn.Module):
             return y.reshape(bsz, q_len, -1)
         return y.reshape(q_len, -1)
 
+    @without_grad
+    def forward_weight_only(self, x: torch.Tensor) -> torch.Tensor:
+        """The layer on an unquantised activation [..., in_features] of at most 16 rows: the 4-bit weight is the only quantised
+        operand, one launch (ops.weight_only_linear).  For decode steps of few tokens, which read the weight once either way."""
+        x2 = x.reshape(-1, x.shape[-1]).to(torch.bfloat16)
+        sf = self.scale_w_dense if self.quant_type == "SHARQ" else self.scale_w
+        bias = self.bias
+        folded = bias if (bias is not None and bias.dtype == torch.bfloat16 and bias.dim() == 1 and bias.is_contiguous()
+                          and bias.numel() == self.out_features) else None
+        y = ops.weight_only_linear(x2, self.weight_q, sf, self.weight_scale_host, bias=folded)
+        return (y if folded is bias else y + bias).reshape(*x.shape[:-1], -1)
+
 
 QLINEAR_METHODS = {name: vars(QLinearLayer)[name] for name in ("prepare_input", "prepare_input_swiglu", "apply_prepared")}

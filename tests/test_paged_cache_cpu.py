@@ -84,3 +84,27 @@ def test_ops_refuse_cpu_tensors():
         ops.paged_attention(torch.zeros(1, 4, 128, dtype=torch.bfloat16), k, k, table, n)
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.rope_append_paged(torch.zeros(1, 1024, dtype=torch.bfloat16), 4, 2, 128, k[0, 0], k[0, 0], n, table, k, k)
+
+
+def test_weight_only_arguments_that_are_refused():
+    from sharq_b200 import _lib, ops
+
+    L = _lib.lib()
+    one, odd = ctypes.c_void_p(256), ctypes.c_void_p(264)
+
+    def refuse(message, x=one, x_row=256, m=2, n=128, k=256, qw=one):
+        assert L.sharq_weight_only_linear(x, x_row, m, n, k, qw, one, None, 1.0, None, one, None) != 0
+        assert message in L.sharq_last_error()
+
+    refuse(b"null buffer", x=None)
+    refuse(b"1 to 16 rows", m=0)
+    refuse(b"1 to 16 rows", m=17)
+    refuse(b"N must be", n=0)
+    refuse(b"N must be", n=65535 * 128 + 1)
+    refuse(b"multiple of 64", k=96)
+    refuse(b"must not overlap", x_row=128)
+    refuse(b"must not overlap", x_row=260)
+    refuse(b"16-byte aligned", qw=odd)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.weight_only_linear(torch.zeros(1, 64, dtype=torch.bfloat16), torch.zeros(4, 32, dtype=torch.uint8),
+                               torch.zeros(512, dtype=torch.uint8), 1.0)
