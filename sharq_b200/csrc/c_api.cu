@@ -800,8 +800,10 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
   if (paged_cache(cache, &c, &fp8)) return 1;
   SHARQ_REQUIRE(q_bf16 && lengths && out_bf16 && workspace, "null buffer");
   SHARQ_REQUIRE(c.head_dim == 64 || c.head_dim == 128, "head_dim must be 64 or 128, got %d", c.head_dim);
-  SHARQ_REQUIRE(heads > 0 && heads % c.kv_heads == 0, "heads must be a positive multiple of kv_heads");
-  SHARQ_REQUIRE((int64_t)c.seqs * heads <= 0x7fffffff, "too many sequences");
+  SHARQ_REQUIRE(heads > 0 && heads % c.kv_heads == 0 && heads <= 65536, "heads must be a positive multiple of kv_heads, at most 65536");
+  SHARQ_REQUIRE((int64_t)c.seqs * heads <= 0x7fffffff &&
+                    (int64_t)c.seqs * (sharq::paged_capacity(c) / 16 + 4) <= 0x7fffffff,
+                "too many sequences, or a page table for too many tokens");
   SHARQ_REQUIRE(q_row >= 0 && q_head >= 0 && q_row % 8 == 0 && q_head % 8 == 0, "the strides of q must be multiples of 8");
   SHARQ_REQUIRE(aligned16(q_bf16) && aligned16(out_bf16) && aligned16(workspace), "buffers must be 16-byte aligned");
   const size_t need = sharq::paged_attention_workspace_bytes(heads, c.kv_heads, c.head_dim);

@@ -9,6 +9,8 @@ namespace sharq {
 
 constexpr int kBadCacheIndex = 0x402;  // error code: a position, length, sequence or page outside the cache or its tables
 
+constexpr int kAttentionTimeout = 0x403;  // error code: a wait for a copy ran out
+
 // A position of a sequence in the cache; also what the kernels check before every access.
 struct PagedCache {
   char *k, *v;

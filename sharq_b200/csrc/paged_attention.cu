@@ -2,25 +2,36 @@
 //
 //   out[b, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q[b, h] . k_j - max),   j < lengths[b]
 //
-// One pass over the cache with a running maximum and sum.  A query group (the query heads that share a key/value head) is the 16-row operand of
-// mma.sync.m16n8k16, in chunks of 16 heads; a warp streams tiles of keys and values through a ring of its own in shared memory (cp.async,
-// no barrier between the warps of a CTA), multiplies, and keeps maximum, sum and the output rows in float registers.  The work is
-// bound by reading the cache: 4 flop per byte and query head of the group, far below what even this tensor path gives, and a legacy MMA
-// takes its operands from registers in the layout in which ldmatrix delivers cache rows, without a trip through tensor memory.
+// One pass over the cache with a running maximum and sum.  The work is bound by reading the cache: 4 flop per byte and query head of a group (the query
+// heads that share a key/value head), far below what even mma.sync gives, and a legacy MMA takes its operands from registers in the
+// layout in which ldmatrix delivers cache rows, without a trip through tensor memory.  Tokens (for the scores) and elements of a head (for the
+// output) are the 16-row operand, the group's query heads the 8 columns, in chunks of up to 16 heads: S^T = K Q^T and O^T = V^T P^T.  The scores'
+// accumulator is [token][head]; movmatrix turns the probabilities, packed to 16 bits, into the operand of the second product.
 //
-// The tiles of all sequences and heads are one list, and every CTA takes an equal stretch of it, whatever the lengths: a CTA joins the
-// warps' parts of each (sequence, head) in shared memory and writes the finished row, or, where the stretch begins or ends inside a
-// (sequence, head), a float part with its maximum and sum; a second kernel, which starts early and waits, joins those parts in the
-// order of the list.  So the result does not depend on timing.
+// A warp streams tiles of keys and values through a ring of its own in shared memory: tensor-map copies counted on the stage's barrier,
+// in the 128-byte swizzle in which eight rows lie in different banks.  (The first form copied 16 bytes per lane with cp.async, and had queries as the
+// 16-row operand: 655 instructions per tile of 16 tokens, 107 us for 131072 tokens of 8 heads, bound by their latency.)
+//
+// The tiles of all sequences and heads are one list, and every warp takes an equal stretch of it, whatever the lengths; each (sequence, head) counts
+// kItemCost tiles more, for its queries and its result.  A warp writes the finished rows of a (sequence, head) that lies within its stretch, and
+// leaves a float part with its maximum and sum of one that does not (two at most, at the ends).  When its warps are done, a CTA joins
+// their parts in shared memory, and a second kernel, which starts early and waits, those of different CTAs, both in the order of the list: the
+// result does not depend on timing.  (With warps that met at the end of every (sequence, head) 64 sequences of 10 to 300 tokens took 33 us; without the
+// join of a CTA's own parts the second kernel had four times as many, 17 us for 131072 tokens of 8 heads.)
+//
+// The maximum is raised only when a score exceeds it by more than kLazy (then probabilities stay below 2^kLazy, and the sum and the output
+// are relative to the same value): raising it costs shuffles and a pass over the output.
 //
 // e4m3 caches go through f16: their values are exact in it, queries are scaled to it by a power of two per head (a value below 2^-39 of its
-// head's largest is lost), and probabilities carry a factor of 2^10, so that those down to 2^-24 of the largest keep f16's full precision.  For bf16
+// head's largest is lost), and probabilities carry a factor of 2^10, so that those down to 2^-24 of the maximum keep f16's full precision.  For bf16
 // caches the probabilities are rounded to bf16 for the product with the values (half a unit in the 8th bit, as the output itself); their sum is
 // taken before that rounding, in float.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <mutex>
 
 #include "decode_ops.cuh"
 #include "sm100_ptx.cuh"
@@ -31,22 +42,10 @@ namespace {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-constexpr int kAttnStages = 3;
-constexpr uint32_t kNaNWord = 0x7FFF7FFFu;  // NaN as two bf16 and as four e4m3
 constexpr float kF16Lift = 10.0f;
+constexpr int kItemCost = 2;
+constexpr int kStretchLeast = 6;
 
-__device__ __forceinline__ void cp_async16(uint32_t smem, const void *gmem, bool valid) {
-  const int bytes = valid ? 16 : 0;  // 0: nothing is read, zeros are written
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kPending>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
-}
-__device__ __forceinline__ void st_shared16(uint32_t smem, uint32_t w) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem), "r"(w) : "memory");
-}
 __device__ __forceinline__ uint4 ld_shared16(uint32_t smem) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem) : "memory");
@@ -69,6 +68,11 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t smem)
                : "r"(smem)
                : "memory");
 }
+__device__ __forceinline__ uint32_t movmatrix(uint32_t w) {  // transpose of an 8 x 8 matrix of 16-bit elements, two per lane
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+  return r;
+}
 
 template <bool kF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -87,7 +91,6 @@ __device__ __forceinline__ float exp2_approx(float x) {  // 2 units in the last 
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<uint32_t *>(&v);
@@ -107,47 +110,62 @@ __device__ __forceinline__ uint32_t e4m3_hi(uint32_t w) {
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(w));
   return r;
 }
+// tokens of a cache [page][head][half][token][128 bytes]
+__device__ __forceinline__ void copy_tokens(uint32_t dst, const CUtensorMap *m, int token, int half, int head, int page, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(m), "r"(ptx::smem_u32(bar)), "r"(0), "r"(token), "r"(half), "r"(head), "r"(page)
+      : "memory");
+}
 
 struct AttnArgs {
   const __nv_bfloat16 *q;
   long long q_row, q_head;
   const int *lengths;
   __nv_bfloat16 *out;
-  float *parts;  // [2 * gridDim.x][kRows][D] unnormalised rows, then their [maximum, sum]
-  int *splits;   // [gridDim.x][2]: (sequence, head chunk) whose last tile lies in a later CTA and how many CTAs follow; 0 followers: none
+  float *parts;  // [2 * CTAs][D][kCols] unnormalised columns, then [2 * CTAs][kCols] of their [maximum, sum]
+  int *splits;   // [CTAs][2]: (sequence, head chunk) that begins in this CTA and goes on in the next ones, and in how many; 0: none
   int seqs, heads, group, chunks;  // chunks: pieces of 16 query heads of a group
+  int box_shift;                   // log2 of the tokens of a copy: the largest power of two, at most a tile, that divides the page size
+  double per_stretches, per_items; // 1 / (stretches of the list), 1 / (items of a sequence)
+  int page_shift;                  // log2 of the page size, -1 if it is no power of two
   float scale_log2;                // scale * log2(e)
   int *error_flag;
 };
 
-// Sizes that follow from the head and the type of the cache.  A tile holds 8 KB of keys and values (4 KB for e4m3 heads of 64).
+// Sizes that follow from the head and the type of the cache.  Rows lie 128 bytes apart: a row of 256 bytes in two halves, one of 64 bytes (e4m3 heads of
+// 64) with zeros behind it, which the copy fills in.  A tile holds 8 KB.
 template <int D, bool kFp8>
 struct Tile {
   static constexpr int kSize = kFp8 ? 1 : 2;
-  static constexpr int kTokens = D == 128 && !kFp8 ? 16 : 32;
-  static constexpr int kChunks = D * kSize / 16;                // 16-byte pieces of a row
-  static constexpr int kBytes = kTokens * D * kSize;            // of keys, or of values
+  static constexpr int kHalves = D * kSize > 128 ? 2 : 1;
+  static constexpr int kTokens = 32 / kHalves;
+  static constexpr int kHalf = kTokens * 128;
+  static constexpr int kBytes = kHalf * kHalves;  // of keys, or of values
   static constexpr int kStage = 2 * kBytes;
-  static constexpr int kLoads = kTokens * kChunks / 32;         // per lane, for the keys and for the values
-  // byte of piece `c` of row `r`: pieces are permuted so that the 8 rows of an ldmatrix, or the rows and pieces that a quarter of a warp
-  // reads at once from an e4m3 tile, lie in different banks
-  static __device__ __forceinline__ uint32_t at(int r, int c) {
-    if (!kFp8) return (uint32_t)(r * kChunks + (c ^ (r & 7))) * 16;
-    const int f = (r & 6) ^ ((r & 1) << 2);
-    if (kChunks == 8) return (uint32_t)(r * 8 + (c ^ f)) * 16;
-    return (uint32_t)((r >> 1) * 8 + ((((r & 1) << 2) | c) ^ (r & 6))) * 16;
-  }
 };
+static_assert(Tile<128, false>::kStage == 8192 && Tile<64, true>::kStage == 8192, "a stage is a multiple of the swizzle's 1024 bytes");
 
-template <int D, int kRows>
-constexpr int join_floats() {
-  return kAttnWarps * 8 * (D + 4) + kAttnWarps * 16 * 2;  // eight rows at a time, and maximum and sum of all
-}
-
-template <int D, bool kFp8, int kRows>
-constexpr int attn_smem_bytes() {
-  return kAttnWarps * kAttnStages * Tile<D, kFp8>::kStage + join_floats<D, kRows>() * 4;
-}
+// What a warp leaves of an item that does not lie within its stretch.
+struct Part {
+  int item;  // seq * items + item, -1: nothing
+  int begins, tiles_left;
+};
+// Shared memory of a CTA: the rings (the swizzle wants 1024 bytes), then the part at the beginning of every warp's stretch (the one at the end goes
+// to the warp's ring, which is free by then), two parts' maxima and sums per warp, their descriptions, barriers and the flag of a wait that ran out.
+template <int D, bool kFp8, int kCols>
+struct Layout {
+  static constexpr int kStages = kCols == 8 ? 3 : 2;  // two CTAs in an SM's memory
+  static constexpr int kRing = kStages * Tile<D, kFp8>::kStage;
+  static constexpr int kPart = D * kCols * 4;
+  static constexpr int kParts = kAttnWarps * kRing;
+  static constexpr int kMl = kParts + kAttnWarps * kPart;
+  static constexpr int kInfo = kMl + 2 * kAttnWarps * kCols * 8;
+  static constexpr int kBars = kInfo + (2 * kAttnWarps * (int)sizeof(Part) + 7) / 8 * 8;
+  static constexpr int kFlag = kBars + kAttnWarps * kStages * 8;
+  static constexpr int kTotal = kFlag + 8;
+  static_assert(kPart <= kRing && kTotal <= 115712, "a part fits a ring, two CTAs an SM");
+};
 
 // A length as the kernel uses it: one that the page table cannot hold counts as an empty sequence whose rows come out as NaN.
 struct Length {
@@ -164,149 +182,219 @@ __device__ __forceinline__ int tiles_of(int tokens) {  // an empty sequence has 
   return tokens <= kTokens ? 1 : (tokens - 1) / kTokens + 1;
 }
 
-// kRows: rows of the 16-row operand that hold query heads (8 or 16)
-template <int D, bool kFp8, int kRows>
-__global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(AttnArgs a, PagedCache c) {
+// n / d for n < 2^52 with the reciprocal of d at hand (an integer division by a variable takes some hundred cycles)
+__device__ __forceinline__ long long divide(long long n, long long d, double reciprocal) {
+  long long q = (long long)((double)n * reciprocal);
+  const long long r = n - q * d;
+  if (r < 0)
+    --q;
+  else if (r >= d)
+    ++q;
+  return q;
+}
+
+// Where a warp stands in its stretch: tiles [tile, end) of an item are its own.  An item is kItemCost + its tiles long in the list, of which `skip` lie
+// in earlier stretches; `left`: how much of the stretch remains from there on.
+struct Place {
+  int seq, head, chunk, skip, left, tokens, tile, end;
+};
+template <int kTokens>
+__device__ __forceinline__ void enter(Place &p, const AttnArgs &a, const PagedCache &c) {
+  p.tokens = length_of(a, c, p.seq).tokens;
+  p.tile = max(0, p.skip - kItemCost);
+  p.end = (int)min((long long)tiles_of<kTokens>(p.tokens), (long long)p.skip + p.left - kItemCost);
+}
+template <int kTokens>
+__device__ __forceinline__ void leave(Place &p, const AttnArgs &a, const PagedCache &c) {
+  const long long rest = (long long)kItemCost + tiles_of<kTokens>(p.tokens) - p.skip;
+  p.left = rest >= p.left ? 0 : p.left - (int)rest;
+  if (p.left == 0) return;
+  p.skip = 0;
+  if (++p.chunk == a.chunks) {
+    p.chunk = 0;
+    ++p.head;
+  }
+  if (p.head == c.kv_heads) {
+    p.head = 0;
+    ++p.seq;
+    enter<kTokens>(p, a, c);
+  } else {  // the same sequence's tokens
+    p.tile = 0;
+    p.end = (int)min((long long)tiles_of<kTokens>(p.tokens), (long long)p.left - kItemCost);
+  }
+}
+
+// kCols: columns for query heads (8 or 16)
+template <int D, bool kFp8, int kCols>
+__global__ void __launch_bounds__(kAttnThreads, 2)
+    paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                           const __grid_constant__ AttnArgs a, const __grid_constant__ PagedCache c) {
   using T = Tile<D, kFp8>;
-  constexpr int kTokens = T::kTokens;
-  extern __shared__ __align__(128) unsigned char smem[];
+  using L = Layout<D, kFp8, kCols>;
+  constexpr int kTokens = T::kTokens, kN = kCols / 8, kStages = L::kStages;
+  constexpr float kLazy = kFp8 ? 4.0f : 8.0f;  // f16: 2^(10 + 4) at most
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t ring = ptx::smem_u32(smem) + warp * L::kRing;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars) + warp * kStages;
+  volatile int *gave_up = reinterpret_cast<volatile int *>(smem + L::kFlag);
+  Part *info = reinterpret_cast<Part *>(smem + L::kInfo);
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) ptx::mbar_init(bars + i, 1);
+    ptx::fence_barrier_init();
+    ptx::tma_prefetch_desc(&map_k);
+    ptx::tma_prefetch_desc(&map_v);
+  }
+  if (threadIdx.x == 0) *gave_up = 0;
+  if (threadIdx.x < 2 * kAttnWarps) info[threadIdx.x].item = -1;
+  __syncthreads();
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = ptx::smem_u32(smem) + warp * kAttnStages * T::kStage;
-  float *join_o = reinterpret_cast<float *>(smem + kAttnWarps * kAttnStages * T::kStage);
-  float *join_ml = join_o + kAttnWarps * 8 * (D + 4);
   const int items = c.kv_heads * a.chunks;  // (head, chunk) pairs of a sequence
 
-  // this CTA's stretch [u0, u1) of the list of tiles
-  long long total = 0;
-  for (int b = lane; b < a.seqs; b += 32) total += tiles_of<kTokens>(length_of(a, c, b).tokens);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-  total *= items;
-  long long per = (total + gridDim.x - 1) / gridDim.x;
-  if (per < kAttnWarps) per = kAttnWarps;
-  const long long u0 = blockIdx.x * per, u1 = min(u0 + per, total);
+  // this warp's stretch [u0, u1) of the list, in tiles
+  const int stretch = blockIdx.x * kAttnWarps + warp, stretches = gridDim.x * kAttnWarps;
+  unsigned per_head = 0;  // less than 2^31: the launcher checks
+#pragma unroll 4
+  for (int b = lane; b < a.seqs; b += 32) per_head += kItemCost + tiles_of<kTokens>(length_of(a, c, b).tokens);
+  per_head = __reduce_add_sync(0xffffffffu, per_head);
+  const long long total = (long long)per_head * items;
+  long long per = divide(total + stretches - 1, stretches, a.per_stretches);
+  if (per < kStretchLeast) per = kStretchLeast;
+  const long long u0 = stretch * per, u1 = min(u0 + per, total);
   if (threadIdx.x == 0) a.splits[2 * blockIdx.x + 1] = 0;
-  if (u0 >= u1) return;
-  int seq = 0, item = 0, first = 0;  // sequence, (head, chunk) and tile at u0
-  {
-    long long before = 0;
+  Place at = {0, 0, 0, 0, u0 < u1 ? (int)min(u1 - u0, 0x7fffffffLL) : 0, 0, 0, 0};
+  if (u0 < u1) {
+    unsigned before = 0;
+    const unsigned u_head = (unsigned)divide(u0, items, a.per_items);  // u0 in units of a head: sequence s begins at items times what lies before it
     for (int b0 = 0; b0 < a.seqs; b0 += 32) {
       const int b = b0 + lane;
-      long long n = b < a.seqs ? (long long)items * tiles_of<kTokens>(length_of(a, c, b).tokens) : 0;
+      const unsigned n_units = b < a.seqs ? kItemCost + tiles_of<kTokens>(length_of(a, c, b).tokens) : 0;
+      unsigned n = n_units;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, n, off);
+        const unsigned up = __shfl_up_sync(0xffffffffu, n, off);
         if (lane >= off) n += up;
       }
-      const unsigned over = __ballot_sync(0xffffffffu, before + n > u0);
+      const unsigned over = __ballot_sync(0xffffffffu, before + n > u_head);
       if (over != 0) {
-        const int at = __ffs(over) - 1;
-        const long long upto = __shfl_sync(0xffffffffu, n, at > 0 ? at - 1 : 0);
-        seq = b0 + at;
-        const long long rest = u0 - before - (at > 0 ? upto : 0);
-        const int n_tiles = tiles_of<kTokens>(length_of(a, c, seq).tokens);
-        item = (int)(rest / n_tiles);
-        first = (int)(rest % n_tiles);
+        const int in = __ffs(over) - 1;
+        const unsigned units = __shfl_sync(0xffffffffu, n_units, in), upto = before + __shfl_sync(0xffffffffu, n, in) - units;
+        const long long rest = u0 - (long long)upto * items;
+        at.seq = b0 + in;
+        const int item = (int)divide(rest, units, (double)__frcp_rn((float)units));  // less than 2^16 items: one off at most
+        at.skip = (int)(rest - (long long)item * units);
+        at.head = a.chunks == 1 ? item : item / a.chunks;
+        at.chunk = item - at.head * a.chunks;
         break;
       }
       before += __shfl_sync(0xffffffffu, n, 31);
     }
+    enter<kTokens>(at, a, c);
   }
 
-  // the next tile that this warp loads: tile `p_tile` < p_end of (p_seq, p_item), with p_left tiles of the stretch from p_tile's item on
-  int p_seq = seq, p_item = item, p_tile = first + warp, p_tokens = length_of(a, c, seq).tokens;
-  long long p_left = u1 - u0;
-  int p_end = (int)min((long long)tiles_of<kTokens>(p_tokens), first + p_left);
-  int p_first = first;
-  int p_page = 0;  // lane j: page of the tile's token j
-  auto settle = [&]() {  // moves on to the next item with a tile for this warp, and looks up the tile's pages
-    while (p_tile >= p_end && p_left > 0) {
-      p_left -= p_end - p_first;
-      if (p_left <= 0) break;
-      if (++p_item == items) {
-        p_item = 0;
-        ++p_seq;
-        p_tokens = length_of(a, c, p_seq).tokens;
-      }
-      p_first = 0;
-      p_tile = warp;
-      p_end = (int)min((long long)tiles_of<kTokens>(p_tokens), p_left);
+  Place next = at;  // of the tile that is loaded next
+  const int box = 1 << a.box_shift, boxes = kTokens >> a.box_shift;  // pieces of `box` tokens of a page that a tile consists of
+  int held_seq = -1, held_first = 0, held_page = 0;  // lane j: page of piece held_first + j of sequence held_seq
+  auto settle = [&]() {  // moves on to the next item with a tile for this warp
+    bool entered = false;
+    while (next.tile >= next.end && next.left > 0) {
+      leave<kTokens>(next, a, c);
+      entered = true;
     }
-    const int token = p_tile * kTokens + lane;
-    p_page = p_left > 0 && lane < kTokens && token < p_tokens ? c.page_table[p_seq * c.table_stride + token / c.page_size] : 0;
+    if (entered && next.left > 0) {  // its queries on their way to the SM
+      const int rows = min(16, a.group - next.chunk * 16);
+      constexpr int kLines = D * 2 / 128;
+      if (lane < rows * kLines)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(a.q + next.seq * a.q_row + (next.head * a.group + next.chunk * 16 + lane / kLines) * a.q_head +
+                                                      lane % kLines * 64));
+    }
   };
-  int put = 0;  // stage that is filled next
+  int put = 0;              // stage that is filled next
+  unsigned bad_stages = 0;  // stages with a piece of no page
   auto load = [&]() {
-    if (p_left > 0) {
+    if (next.left > 0) {
       const uint32_t stage = ring + put * T::kStage;
-      const int token0 = p_tile * kTokens, row0 = lane / T::kChunks, piece = lane % T::kChunks;
-      const long long in_page = (p_item / a.chunks) * c.head_stride + piece * 16;
-      const int slot0 = (token0 + lane) % c.page_size;  // lane j: slot of token j
-#pragma unroll
-      for (int i = 0; i < T::kLoads; ++i) {
-        const int row = row0 + i * (32 / T::kChunks);
-        const int page = __shfl_sync(0xffffffffu, p_page, row), slot = __shfl_sync(0xffffffffu, slot0, row);
-        const bool live = token0 + row < p_tokens;
-        const bool bad = live && (unsigned)page >= (unsigned)c.pages;
-        const long long from = bad || !live ? 0 : page * c.page_stride + slot * c.token_stride + in_page;
-        const uint32_t to = stage + T::at(row, piece);
-        if (bad) {
-          st_shared16(to, kNaNWord);
-          if (a.error_flag != nullptr) atomicExch(a.error_flag, kBadCacheIndex);
-        } else {
-          cp_async16(to, c.k + from, live);
-        }
-        cp_async16(to + T::kBytes, c.v + from, live && !bad);
+      const int live = next.tokens - next.tile * kTokens;  // tokens from this tile on
+      const int pieces = live <= 0 ? 0 : min(boxes, (live + box - 1) >> a.box_shift);
+      const int piece0 = next.tile * boxes;
+      if (next.seq != held_seq || piece0 < held_first || piece0 + boxes > held_first + 32) {
+        held_seq = next.seq;
+        held_first = piece0;
+        const int token = (piece0 + lane) << a.box_shift;
+        held_page = 0;
+        if (token < next.tokens) held_page = c.page_table[next.seq * c.table_stride + (a.page_shift >= 0 ? token >> a.page_shift : token / c.page_size)];
       }
-      p_tile += kAttnWarps;
+      bool any_bad = false;
+      const bool chosen = ptx::elect_one();
+      if (chosen) ptx::mbar_arrive_expect_tx(bars + put, (pieces << a.box_shift) * 256 * T::kHalves);
+      for (int i = 0; i < pieces; ++i) {
+        int page = __shfl_sync(0xffffffffu, held_page, piece0 + i - held_first);
+        const int token = (piece0 + i) << a.box_shift;
+        const int slot = a.page_shift >= 0 ? token & (c.page_size - 1) : token % c.page_size;
+        if ((unsigned)page >= (unsigned)c.pages) {
+          any_bad = true;
+          page = c.pages;  // one behind the last: zeros are filled in
+        }
+        if (chosen) {
+          const uint32_t to = stage + (i << a.box_shift) * 128;
+          copy_tokens(to, &map_k, slot, 0, next.head, page, bars + put);
+          copy_tokens(to + T::kBytes, &map_v, slot, 0, next.head, page, bars + put);
+          if (T::kHalves == 2 && boxes > 1) {  // a whole tile's halves are one copy
+            copy_tokens(to + T::kHalf, &map_k, slot, 1, next.head, page, bars + put);
+            copy_tokens(to + T::kBytes + T::kHalf, &map_v, slot, 1, next.head, page, bars + put);
+          }
+        }
+      }
+      bad_stages = (bad_stages & ~(1u << put)) | (any_bad ? 1u << put : 0);
+      ++next.tile;
+      put = put + 1 == kStages ? 0 : put + 1;
+      settle();
     }
-    cp_async_commit();
-    put = put + 1 == kAttnStages ? 0 : put + 1;
-    settle();
   };
   settle();
-  for (int i = 0; i < kAttnStages - 1; ++i) load();
+  for (int i = 0; i < kStages - 1; ++i) load();
 
-  int take = 0;  // stage that is used next
-  long long left = u1 - u0;
-  while (left > 0) {
-    const Length len = length_of(a, c, seq);
-    const int n_tiles = tiles_of<kTokens>(len.tokens);
-    const int last = (int)min((long long)n_tiles, first + left);
-    const int kv = item / a.chunks, chunk = item % a.chunks;
-    const int rows = min(16, a.group - chunk * 16);  // query heads of the chunk
+  // Rows of a tile that a lane reads.  bf16: an ldmatrix takes 8 rows x 16 bytes per 8 lanes; lane & 7 is the row in the swizzle.
+  // keys: matrices (tokens 0-7 | 8-15) x (16-byte piece 2k | 2k + 1), values: pieces first, as the transposed operand wants them
+  const uint32_t k_lane = ((lane & 7) + ((lane >> 3) & 1) * 8) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_lane = ((lane & 7) + (lane >> 4) * 8) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+  // e4m3: lane (g, t) holds token row (g >> 1) + 4 (g & 1) of eight, so that the rows and pieces that a quarter of a warp reads at once lie in
+  // different banks; of the values it reads piece (g >> 1) + 4 (g & 1) of the tokens of slots 2t and 2t + 1, the rows t and t + 4
+  const int g_mixed = (g >> 1) | ((g & 1) << 2);
+  const int my_token = kFp8 ? g_mixed : g;
+
+  int take = 0;         // stage that is used next
+  unsigned phases = 0;  // parity of every stage's barrier
+  for (; at.left > 0; leave<kTokens>(at, a, c)) {
+    if (at.tile >= at.end) continue;
+    const int kv = at.head, chunk = at.chunk;
+    const int cols = min(16, a.group - chunk * 16);  // query heads of the chunk
     const int head0 = kv * a.group + chunk * 16;
+    const bool begins = at.tile == 0;
 
-    // queries: rows g and g + 8 of the operand, zeros behind the group's heads
-    uint32_t qa[D / 16][4];
-    float sl[2] = {a.scale_log2, a.scale_log2};
-    if (!kFp8) {
+    // queries: columns 8 n + g, zeros behind the group's heads
+    uint32_t qb[kN][D / 16][2];
+    float sl[kN][2];  // of columns 8 n + 2 t and the next one
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = g + 8 * h;
-        const __nv_bfloat16 *q = a.q + seq * a.q_row + (head0 + row) * a.q_head + 2 * t;
+    for (int n = 0; n < kN; ++n) {
+      const bool live = 8 * n + g < cols;
+      const __nv_bfloat16 *q = a.q + at.seq * a.q_row + (head0 + 8 * n + g) * a.q_head;
+      if (!kFp8) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const bool live = h < kRows / 8 && row < rows;
-          qa[k][h] = live ? *reinterpret_cast<const uint32_t *>(q + 16 * k) : 0;
-          qa[k][h + 2] = live ? *reinterpret_cast<const uint32_t *>(q + 16 * k + 8) : 0;
+          qb[n][k][0] = live ? *reinterpret_cast<const uint32_t *>(q + 2 * t + 16 * k) : 0;
+          qb[n][k][1] = live ? *reinterpret_cast<const uint32_t *>(q + 2 * t + 16 * k + 8) : 0;
         }
-      }
-    } else {
-      // step k of a span of 64 elements takes the elements 16 t + 4 (k % 4) + {0, 1, 2, 3} of the span from lane t, as the keys do
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = g + 8 * h;
-        const bool live = h < kRows / 8 && row < rows;
-        const __nv_bfloat16 *q = a.q + seq * a.q_row + (head0 + row) * a.q_head + 16 * t;
+        sl[n][0] = sl[n][1] = a.scale_log2;
+      } else {
+        // step k of a span of 64 elements takes the elements 16 t + 4 (k % 4) + {0, 1, 2, 3} of the span from lane t, as the keys do
         uint32_t top = 0;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint2 w = live ? *reinterpret_cast<const uint2 *>(q + (k / 4) * 64 + (k % 4) * 4) : make_uint2(0, 0);
-          qa[k][h] = w.x;
-          qa[k][h + 2] = w.y;
+          const uint2 w = live ? *reinterpret_cast<const uint2 *>(q + 16 * t + (k / 4) * 64 + (k % 4) * 4) : make_uint2(0, 0);
+          qb[n][k][0] = w.x;
+          qb[n][k][1] = w.y;
           top = __vmaxu2(top, __vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu));
         }
         top = max(top & 0xFFFFu, top >> 16);
@@ -317,248 +405,430 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(AttnAr
         // in two factors, each a normal float
         const int s1 = shift / 2, s2 = shift - s1;
         const float f1 = __int_as_float((127 + s1) << 23), f2 = __int_as_float((127 + s2) << 23);
-        sl[h] = a.scale_log2 * c.k_scale[kv] * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23);
+        const float back = a.scale_log2 * c.k_scale[kv] * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23);
+        sl[n][0] = __shfl_sync(0xffffffffu, back, 8 * t);  // lane of column 2 t
+        sl[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
+        for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-          for (int j = 0; j < 4; j += 2) {
-            const uint32_t w = qa[k][h + j];
-            qa[k][h + j] = pack_f16(__uint_as_float(w << 16) * f1 * f2, __uint_as_float(w & 0xFFFF0000u) * f1 * f2);
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t w = qb[n][k][j];
+            qb[n][k][j] = pack_f16(__uint_as_float(w << 16) * f1 * f2, __uint_as_float(w & 0xFFFF0000u) * f1 * f2);
           }
-        }
       }
     }
 
-    float o[D / 8][4];
+    float o[D / 16][kN][4];  // rows of 16 elements of the head; columns as in sl
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+    for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-    // maximum (of the scores, in units of log 2) and sum of rows g and g + 8
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][n][j] = 0.0f;
+    // maximum (in units of log 2, the same in all lanes of a column) and this lane's share of the sum
+    float m[kN][2], l[kN][2];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
 
-    for (int tile = first + warp; tile < last; tile += kAttnWarps) {
+    for (int tile = at.tile; tile < at.end; ++tile) {
       load();
-      cp_async_wait<kAttnStages - 1>();
-      __syncwarp();
       const uint32_t keys = ring + take * T::kStage, values = keys + T::kBytes;
+      bool poison = (bad_stages >> take) & 1;
+      if (!ptx::mbar_wait(bars + take, (phases >> take) & 1, gave_up)) {
+        *gave_up = 1;
+        poison = true;
+        if (a.error_flag != nullptr) atomicExch(a.error_flag, kAttentionTimeout);
+      }
+      __syncwarp();
+      phases ^= 1u << take;
+      const int live = at.tokens - tile * kTokens;  // tokens from this tile on
 
-      float s[kTokens / 8][4];
+      float s[kTokens / 16][kN][4], s2[kTokens / 16][kN][4];  // [token][column], in two sums: a product waits for the one before it
 #pragma unroll
-      for (int n = 0; n < kTokens / 8; ++n)
+      for (int b = 0; b < kTokens / 16; ++b)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
-      if (!kFp8) {
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
-        for (int n = 0; n < kTokens / 16; ++n)
+          for (int j = 0; j < 4; ++j) s[b][n][j] = s2[b][n][j] = 0.0f;
+#pragma unroll
+      for (int b = 0; b < kTokens / 16; ++b) {
+        if (!kFp8) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            uint32_t b[4];
-            ldmatrix4(b, keys + T::at(n * 16 + (lane >> 4) * 8 + (lane & 7), 2 * k + ((lane >> 3) & 1)));
-            mma16816<kFp8>(s[2 * n], qa[k], b[0], b[1]);
-            mma16816<kFp8>(s[2 * n + 1], qa[k], b[2], b[3]);
-          }
-      } else {
+            uint32_t w[4];
+            ldmatrix4(w, (keys + b * 2048 + k_lane + (k / 4) * T::kHalf) ^ ((k % 4) * 32));
 #pragma unroll
-        for (int n = 0; n < kTokens / 8; ++n)
+            for (int n = 0; n < kN; ++n) mma16816<kFp8>(k % 2 == 0 ? s[b][n] : s2[b][n], w, qb[n][k][0], qb[n][k][1]);
+          }
+        } else {
 #pragma unroll
           for (int span = 0; span < D / 64; ++span) {
-            const uint4 w = ld_shared16(keys + T::at(n * 8 + g, span * 4 + t));
-            mma16816<kFp8>(s[n], qa[span * 4 + 0], e4m3_lo(w.x), e4m3_hi(w.x));
-            mma16816<kFp8>(s[n], qa[span * 4 + 1], e4m3_lo(w.y), e4m3_hi(w.y));
-            mma16816<kFp8>(s[n], qa[span * 4 + 2], e4m3_lo(w.z), e4m3_hi(w.z));
-            mma16816<kFp8>(s[n], qa[span * 4 + 3], e4m3_lo(w.w), e4m3_hi(w.w));
-          }
-      }
-
+            const uint32_t row = keys + (b * 16 + my_token) * 128 + ((uint32_t)((span * 4 + t) ^ my_token) << 4);
+            const uint4 lo = ld_shared16(row), hi = ld_shared16(row + 8 * 128);
+            const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-      for (int n = 0; n < kTokens / 8; ++n)
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t w[4] = {e4m3_lo(wl[j]), e4m3_lo(wh[j]), e4m3_hi(wl[j]), e4m3_hi(wh[j])};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][j] *= sl[j >> 1];
-      const int live = len.tokens - tile * kTokens;  // tokens of the tile
-      if (live < kTokens) {
-#pragma unroll
-        for (int n = 0; n < kTokens / 8; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (n * 8 + 2 * t + (j & 1) >= live) s[n][j] = -INFINITY;
-      }
-      float top[2] = {m[0], m[1]};
-#pragma unroll
-      for (int h = 0; h < kRows / 8; ++h) {
-#pragma unroll
-        for (int n = 0; n < kTokens / 8; ++n) top[h] = fmaxf(top[h], fmaxf(s[n][2 * h], s[n][2 * h + 1]));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-      }
-      if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
-#pragma unroll
-        for (int h = 0; h < kRows / 8; ++h) {
-          const float f = top[h] > m[h] ? exp2_approx(m[h] - top[h]) : 1.0f;  // m = -inf: 0, and nothing to keep
-          m[h] = top[h];
-          l[h] *= f;
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            o[i][2 * h] *= f;
-            o[i][2 * h + 1] *= f;
+              for (int n = 0; n < kN; ++n) mma16816<kFp8>(j % 2 == 0 ? s[b][n] : s2[b][n], w, qb[n][span * 4 + j][0], qb[n][span * 4 + j][1]);
+            }
           }
         }
       }
-      uint32_t p[kTokens / 8][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (h >= kRows / 8) {
+      for (int b = 0; b < kTokens / 16; ++b)
 #pragma unroll
-          for (int n = 0; n < kTokens / 8; ++n) p[n][h] = 0;
-          continue;
-        }
-        // a row with no finite score so far has maximum -inf: its probabilities are 0, not exp(-inf + inf)
-        const float base = (m[h] == -INFINITY ? 0.0f : m[h]) - (kFp8 ? kF16Lift : 0.0f);
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
-        for (int n = 0; n < kTokens / 8; ++n) {
-          const float p0 = exp2_approx(s[n][2 * h] - base), p1 = exp2_approx(s[n][2 * h + 1] - base);
-          l[h] += p0 + p1;
-          p[n][h] = kFp8 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
-        }
+          for (int j = 0; j < 4; ++j) s[b][n][j] = (s[b][n][j] + s2[b][n][j]) * sl[n][j & 1];
+      if (live < kTokens || poison) {
+#pragma unroll
+        for (int b = 0; b < kTokens / 16; ++b)
+#pragma unroll
+          for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (b * 16 + (j >> 1) * 8 + my_token >= live) s[b][n][j] = -INFINITY;
+              if (poison) s[b][n][j] = __int_as_float(0x7fffffff);
+            }
+        // values behind the sequence: whatever the page or an earlier tile left there must not meet a probability of 0
+        for (int i = max(live, 0) * 8 + lane; i < kTokens * 8; i += 32)
+#pragma unroll
+          for (int half = 0; half < T::kHalves; ++half)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(values + half * T::kHalf + i * 16), "r"(0) : "memory");
+        ptx::fence_proxy_async();  // a later copy into this stage comes behind these stores
+        __syncwarp();
       }
-
+      bool raise = false;
 #pragma unroll
-      for (int k = 0; k < kTokens / 16; ++k) {
-        const uint32_t pa[4] = {p[2 * k][0], p[2 * k][1], p[2 * k + 1][0], p[2 * k + 1][1]};
+      for (int b = 0; b < kTokens / 16; ++b)
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) raise |= s[b][n][j] > m[n][j & 1] + kLazy;
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float top = m[n][j];
+#pragma unroll
+            for (int b = 0; b < kTokens / 16; ++b) top = fmaxf(top, fmaxf(s[b][n][j], s[b][n][j + 2]));
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            const float f = top > m[n][j] ? exp2_approx(m[n][j] - top) : 1.0f;  // from -inf: 0, and nothing to keep
+            m[n][j] = top;
+            l[n][j] *= f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              o[i][n][j] *= f;
+              o[i][n][j + 2] *= f;
+            }
+          }
+      }
+      // a column with no finite score so far has maximum -inf: its probabilities are 0, not exp(-inf + inf)
+      float base[kN][2];
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) base[n][j] = (m[n][j] == -INFINITY ? 0.0f : m[n][j]) - (kFp8 ? kF16Lift : 0.0f);
+#pragma unroll
+      for (int b = 0; b < kTokens / 16; ++b) {
+        uint32_t pb[kN][2];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          float p[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            p[j] = exp2_approx(s[b][n][j] - base[n][j & 1]);
+            l[n][j & 1] += p[j];
+          }
+          pb[n][0] = movmatrix(kFp8 ? pack_f16(p[0], p[1]) : pack_bf16(p[0], p[1]));
+          pb[n][1] = movmatrix(kFp8 ? pack_f16(p[2], p[3]) : pack_bf16(p[2], p[3]));
+        }
         if (!kFp8) {
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
-            uint32_t b[4];
-            ldmatrix4_trans(b, values + T::at(k * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), 2 * i + (lane >> 4)));
-            mma16816<kFp8>(o[2 * i], pa, b[0], b[1]);
-            mma16816<kFp8>(o[2 * i + 1], pa, b[2], b[3]);
+            uint32_t w[4];
+            ldmatrix4_trans(w, (values + b * 2048 + v_lane + (i / 4) * T::kHalf) ^ ((i % 4) * 32));
+#pragma unroll
+            for (int n = 0; n < kN; ++n) mma16816<kFp8>(o[i][n], w, pb[n][0], pb[n][1]);
           }
         } else {
-          // lane (g, t) takes the elements g * (D / 8) + i of four tokens; column g of output tile i is element g * (D / 8) + i
+          // lane (g, t) takes D / 8 neighbouring elements of four tokens: rows g and g + 8 of tile i are its elements 2 i and 2 i + 1
           constexpr int kWords = D / 32;
-          uint32_t w[4][kWords];
+          uint32_t w[4][4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int row = k * 16 + 2 * t + (j & 1) + (j >> 1) * 8;
+            const int in_eight = t + (j & 1) * 4;
+            const uint32_t row = values + (b * 16 + (j >> 1) * 8 + in_eight) * 128;
             if (D == 128) {
-              const uint4 v = ld_shared16(values + T::at(row, g));
-              w[j][0] = v.x, w[j][1] = v.y, w[j][kWords - 2] = v.z, w[j][kWords - 1] = v.w;
+              const uint4 v = ld_shared16(row + ((uint32_t)(g_mixed ^ in_eight) << 4));
+              w[j][0] = v.x, w[j][1] = v.y, w[j][2] = v.z, w[j][3] = v.w;
             } else {
-              const uint2 v = ld_shared8(values + T::at(row, g >> 1) + (g & 1) * 8);
+              const uint2 v = ld_shared8(row + ((uint32_t)((g >> 1) ^ in_eight) << 4) + (g & 1) * 8);
               w[j][0] = v.x, w[j][1] = v.y;
             }
           }
 #pragma unroll
           for (int i = 0; i < kWords; ++i) {
+            // elements 4 i .. 4 i + 3 of the tokens of slots 2t and 2t + 1, and of 2t + 8 and 2t + 9
             const uint32_t a0 = __byte_perm(w[0][i], w[1][i], 0x5140), a1 = __byte_perm(w[0][i], w[1][i], 0x7362);
             const uint32_t b0 = __byte_perm(w[2][i], w[3][i], 0x5140), b1 = __byte_perm(w[2][i], w[3][i], 0x7362);
-            mma16816<kFp8>(o[4 * i + 0], pa, e4m3_lo(a0), e4m3_lo(b0));
-            mma16816<kFp8>(o[4 * i + 1], pa, e4m3_hi(a0), e4m3_hi(b0));
-            mma16816<kFp8>(o[4 * i + 2], pa, e4m3_lo(a1), e4m3_lo(b1));
-            mma16816<kFp8>(o[4 * i + 3], pa, e4m3_hi(a1), e4m3_hi(b1));
+            const uint32_t even[4] = {e4m3_lo(a0), e4m3_hi(a0), e4m3_lo(b0), e4m3_hi(b0)};
+            const uint32_t odd[4] = {e4m3_lo(a1), e4m3_hi(a1), e4m3_lo(b1), e4m3_hi(b1)};
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+              mma16816<kFp8>(o[2 * i][n], even, pb[n][0], pb[n][1]);
+              mma16816<kFp8>(o[2 * i + 1][n], odd, pb[n][0], pb[n][1]);
+            }
           }
         }
       }
+      if (poison && lane == 0 && a.error_flag != nullptr) atomicCAS(a.error_flag, 0, kBadCacheIndex);
       __syncwarp();  // the stage may be filled again
-      take = take + 1 == kAttnStages ? 0 : take + 1;
+      take = take + 1 == kStages ? 0 : take + 1;
     }
 
-    // join the warps' parts
 #pragma unroll
-    for (int h = 0; h < kRows / 8; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    }
-    const bool whole = first == 0 && last == n_tiles;
-    // the part of an item that began in an earlier CTA goes to this CTA's first place, of one that goes on in a later CTA to the second
-    const long long place = 2LL * blockIdx.x + (first == 0 ? 1 : 0);
-    float *part = a.parts + place * kRows * D;
-    float *part_ml = a.parts + 2LL * gridDim.x * kRows * D + place * kRows * 2;
+    for (int n = 0; n < kN; ++n)
 #pragma unroll
-    for (int h = 0; h < kRows / 8; ++h) {
-      __syncthreads();  // the space is free
-      if (t == 0) {
-        join_ml[(warp * 8 + g) * 2] = m[h];
-        join_ml[(warp * 8 + g) * 2 + 1] = l[h];
-      }
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        float *to = join_o + (warp * 8 + g) * (D + 4);
-        if (!kFp8) {
-          *reinterpret_cast<float2 *>(to + 8 * i + 2 * t) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
-        } else {
-          to[2 * t * (D / 8) + i] = o[i][2 * h];
-          to[(2 * t + 1) * (D / 8) + i] = o[i][2 * h + 1];
-        }
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < 8 * D; i += kAttnThreads) {
-        const int row = i / D, d = i % D;
-        if (8 * h + row >= rows) break;
-        float top = -INFINITY;
+        for (int off = 4; off < 32; off <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], off);
+    const int n_tiles = tiles_of<kTokens>(at.tokens);
+    if (begins && at.end == n_tiles) {
+      const int raw = a.lengths[at.seq];
+      const bool bad = raw < 0 || raw > paged_capacity(c);
+      if (bad && lane == 0 && a.error_flag != nullptr) atomicCAS(a.error_flag, 0, kBadCacheIndex);
+      __nv_bfloat16 *out = a.out + ((long long)at.seq * a.heads + head0) * D;
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, join_ml[(w * 8 + row) * 2]);
-        float sum = 0.0f, acc = 0.0f;
+      for (int n = 0; n < kN; ++n) {
+        float f[2];
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w) {
-          const float mw = join_ml[(w * 8 + row) * 2];
-          const float f = mw == top ? 1.0f : exp2_approx(mw - top);  // also where all are -inf
-          sum += join_ml[(w * 8 + row) * 2 + 1] * f;
-          acc += join_o[(w * 8 + row) * (D + 4) + d] * f;
-        }
-        if (whole) {
-          float y = len.tokens == 0 ? 0.0f : acc / sum * (kFp8 ? c.v_scale[kv] : 1.0f);
-          if (len.bad) y = __int_as_float(0x7fffffff);
-          a.out[((long long)seq * a.heads + head0 + 8 * h + row) * D + d] = __float2bfloat16_rn(y);
-        } else {
-          part[(8 * h + row) * D + d] = acc;
-          if (d == 0) {
-            part_ml[(8 * h + row) * 2] = top;
-            part_ml[(8 * h + row) * 2 + 1] = sum;
+        for (int j = 0; j < 2; ++j) f[j] = (kFp8 ? c.v_scale[kv] : 1.0f) / l[n][j];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          float y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            y[j] = raw == 0 ? 0.0f : o[i][n][j] * f[j & 1];
+            if (bad) y[j] = __int_as_float(0x7fffffff);
+          }
+          if (!kFp8) {
+            // [element][column] to [column][element]
+            const uint32_t w0 = movmatrix(pack_bf16(y[0], y[1])), w1 = movmatrix(pack_bf16(y[2], y[3]));
+            if (8 * n + g < cols) {
+              *reinterpret_cast<uint32_t *>(out + (8 * n + g) * D + 16 * i + 2 * t) = w0;
+              *reinterpret_cast<uint32_t *>(out + (8 * n + g) * D + 16 * i + 8 + 2 * t) = w1;
+            }
+          } else {
+            __nv_bfloat16 *to = out + (8 * n + 2 * t) * D + (D == 128 ? g_mixed : g) * (D / 8) + 2 * i;
+            if (8 * n + 2 * t < cols) *reinterpret_cast<uint32_t *>(to) = pack_bf16(y[0], y[2]);
+            if (8 * n + 2 * t + 1 < cols) *reinterpret_cast<uint32_t *>(to + D) = pack_bf16(y[1], y[3]);
           }
         }
       }
-    }
-    if (threadIdx.x == 0) {
-      if (len.bad && a.error_flag != nullptr) atomicExch(a.error_flag, kBadCacheIndex);
-      if (first == 0 && !whole) {  // goes on in the next CTAs
-        a.splits[2 * blockIdx.x] = seq * items + item;
-        a.splits[2 * blockIdx.x + 1] = (int)((n_tiles - last + per - 1) / per);
+    } else {
+      // [element][column], with the maxima and sums beside it
+      const int slot = 2 * warp + (begins ? 1 : 0);
+      float *part = reinterpret_cast<float *>(begins ? smem + warp * L::kRing : smem + L::kParts + warp * L::kPart);
+      float *part_ml = reinterpret_cast<float *>(smem + L::kMl) + slot * kCols * 2;
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        if (g == 0) *reinterpret_cast<float4 *>(part_ml + (8 * n + 2 * t) * 2) = make_float4(m[n][0], l[n][0], m[n][1], l[n][1]);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const int d0 = kFp8 ? (D == 128 ? g_mixed : g) * (D / 8) + 2 * i : 16 * i + g, d1 = kFp8 ? d0 + 1 : d0 + 8;
+          *reinterpret_cast<float2 *>(part + d0 * kCols + 8 * n + 2 * t) = make_float2(o[i][n][0], o[i][n][1]);
+          *reinterpret_cast<float2 *>(part + d1 * kCols + 8 * n + 2 * t) = make_float2(o[i][n][2], o[i][n][3]);
+        }
       }
-    }
-    left -= last - first;
-    first = 0;
-    if (++item == items) {
-      item = 0;
-      ++seq;
+      if (lane == 0) info[slot] = {at.seq * items + at.head * a.chunks + at.chunk, begins, n_tiles - at.end};
     }
   }
-  cp_async_wait<0>();
+
+  // Join this CTA's parts: neighbouring ones of the same item.
+  __syncthreads();
+  constexpr int kVecs = D * kCols / 4 / kAttnThreads;  // a thread's float4s of a part; its columns are the same in all of them
+  static_assert(kVecs >= 1 && kAttnThreads * 4 % kCols == 0, "every thread has a share of a part");
+  const int col0 = threadIdx.x * 4 % kCols;
+  float top[4], sum[4];
+  float4 acc[kVecs];
+  Part run = {-1, 0, 0};  // the item whose parts are being joined
+  for (int i = 0; i <= 2 * kAttnWarps; ++i) {
+    const Part now = i < 2 * kAttnWarps ? info[i] : Part{-2, 0, 0};
+    if (now.item == -1) continue;
+    if (run.item >= 0 && now.item != run.item) {
+      if (run.begins && run.tiles_left == 0) {
+        const int seq = run.item / items, pair = run.item - seq * items, kv = pair / a.chunks, chunk = pair % a.chunks;
+        const int cols = min(16, a.group - chunk * 16);
+        __nv_bfloat16 *out = a.out + ((long long)seq * a.heads + kv * a.group + chunk * 16 + col0) * D;
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = (kFp8 ? c.v_scale[kv] : 1.0f) / sum[j];
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          const int d = (v * kAttnThreads + threadIdx.x) * 4 / kCols;
+          const float y[4] = {acc[v].x, acc[v].y, acc[v].z, acc[v].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (col0 + j < cols) out[j * D + d] = __float2bfloat16_rn(y[j] * f[j]);
+        }
+      } else {
+        // the part of an item that began in an earlier CTA goes to this CTA's first place, of one that goes on in a later one to the second
+        const long long place = 2LL * blockIdx.x + (run.begins ? 1 : 0);
+        float4 *part = reinterpret_cast<float4 *>(a.parts + place * D * kCols);
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) part[v * kAttnThreads + threadIdx.x] = acc[v];
+        float4 *ml = reinterpret_cast<float4 *>(a.parts + 2LL * gridDim.x * D * kCols + (place * kCols + col0) * 2);
+        if (threadIdx.x * 4 < kCols) {
+          ml[0] = make_float4(top[0], sum[0], top[1], sum[1]);
+          ml[1] = make_float4(top[2], sum[2], top[3], sum[3]);
+        }
+        if (run.begins && threadIdx.x == 0) {
+          a.splits[2 * blockIdx.x] = run.item;
+          a.splits[2 * blockIdx.x + 1] = (int)((run.tiles_left + kAttnWarps * per - 1) / (kAttnWarps * per));
+        }
+      }
+    }
+    if (now.item < 0) break;
+    const float4 *of_ml = reinterpret_cast<const float4 *>(smem + L::kMl + (i * kCols + col0) * 8);
+    const float4 p = of_ml[0], q = of_ml[1];
+    const float of[4] = {p.x, p.z, q.x, q.z}, s[4] = {p.y, p.w, q.y, q.w};
+    const float4 *x = reinterpret_cast<const float4 *>((i & 1) != 0 ? smem + (i >> 1) * L::kRing : smem + L::kParts + (i >> 1) * L::kPart);
+    if (now.item != run.item) {
+      run = now;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top[j] = of[j], sum[j] = s[j];
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) acc[v] = x[v * kAttnThreads + threadIdx.x];
+    } else {
+      run.tiles_left = now.tiles_left;
+      float f[4], f_old[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float high = fmaxf(top[j], of[j]);
+        f_old[j] = top[j] == high ? 1.0f : exp2_approx(top[j] - high);  // also where both are -inf
+        f[j] = of[j] == high ? 1.0f : exp2_approx(of[j] - high);
+        top[j] = high;
+        sum[j] = sum[j] * f_old[j] + s[j] * f[j];
+      }
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const float4 w = x[v * kAttnThreads + threadIdx.x];
+        acc[v].x = acc[v].x * f_old[0] + w.x * f[0];
+        acc[v].y = acc[v].y * f_old[1] + w.y * f[1];
+        acc[v].z = acc[v].z * f_old[2] + w.z * f[2];
+        acc[v].w = acc[v].w * f_old[3] + w.w * f[3];
+      }
+    }
+  }
 }
 
-// The row blockIdx.y of the item that begins in CTA blockIdx.x of the kernel above and goes on in the next ones.
-template <int D, int kRows, bool kFp8>
-__global__ void __launch_bounds__(D) paged_attention_join_kernel(AttnArgs a, PagedCache c, int ctas) {
+// Joins the parts of the items that begin in one of eight CTAs of the kernel above and go on: elements 32 blockIdx.y .. + 31 of all columns.  A warp takes an item, or, where
+// one of them has many parts, all warps take the parts of one item after the other in turn, and their sums meet in shared memory.  The
+// maximum over an item's parts comes first, so that the parts are independent of each other.
+constexpr int kJoinWarps = 8;
+constexpr int kJoinMany = 8;
+
+template <int D, int kCols, bool kFp8>
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_attention_join_kernel(const __grid_constant__ AttnArgs a,
+                                                                               const __grid_constant__ PagedCache c, int ctas) {
+  constexpr int kVecs = kCols / 4;  // a lane's float4s of an element slice [32][kCols]; a lane's columns are the same in all of them
+  __shared__ float4 accs[kJoinWarps][kVecs][32], sums[kJoinWarps][32];
+  __shared__ float tops[kJoinWarps][kCols];
   ptx::grid_dependency_wait();
-  const int followers = a.splits[2 * blockIdx.x + 1];
-  if (followers == 0) return;
-  const int at = a.splits[2 * blockIdx.x], items = c.kv_heads * a.chunks;
-  const int seq = at / items, kv = at % items / a.chunks, chunk = at % items % a.chunks, row = blockIdx.y;
-  if (row >= min(16, a.group - chunk * 16)) return;
-  const float *ml = a.parts + 2LL * ctas * kRows * D;
-  // part 0: the second place of this CTA, part i: the first place of the i-th CTA behind it
-  auto place = [&](int i) { return i == 0 ? 2LL * blockIdx.x + 1 : 2LL * (blockIdx.x + i); };
-  float top = -INFINITY;
-  for (int i = 0; i <= followers; ++i) top = fmaxf(top, ml[(place(i) * kRows + row) * 2]);
-  float sum = 0.0f, acc = 0.0f;
-  for (int i = 0; i <= followers; ++i) {
-    const float mi = ml[(place(i) * kRows + row) * 2];
-    const float f = mi == top ? 1.0f : exp2_approx(mi - top);
-    sum += ml[(place(i) * kRows + row) * 2 + 1] * f;
-    acc += a.parts[(place(i) * kRows + row) * D + threadIdx.x] * f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, items = c.kv_heads * a.chunks;
+  const int base = blockIdx.x * kJoinWarps;
+  const int of_lane = lane < kJoinWarps && base + lane < ctas ? a.splits[2 * (base + lane) + 1] : 0;
+  const unsigned any = __ballot_sync(0xffffffffu, of_lane > 0);
+  if (any == 0) return;
+  const bool many = __any_sync(0xffffffffu, of_lane > kJoinMany);
+  const float *ml = a.parts + 2LL * ctas * D * kCols;
+  const int col0 = lane * 4 % kCols;
+  // part 0 of the item that begins in CTA `begin`: its second place; part i: the first place of the i-th CTA behind it
+  auto place = [&](int begin, int i) { return 2LL * (begin + i) + (i == 0 ? 1 : 0); };
+
+  unsigned todo = many ? any : any & (1u << warp);
+  while (todo != 0) {
+    const int which = __ffs(todo) - 1, begin = base + which;
+    todo &= todo - 1;
+    const int followers = __shfl_sync(0xffffffffu, of_lane, which);
+    const int at = a.splits[2 * begin];
+    const int from = many ? warp : 0, step = many ? kJoinWarps : 1;
+    // maximum of column lane % kCols, the parts dealt over the lanes and warps
+    float top = -INFINITY;
+    for (int i = (many ? warp * (32 / kCols) : 0) + lane / kCols; i <= followers; i += step * (32 / kCols))
+      top = fmaxf(top, ml[(place(begin, i) * kCols + lane % kCols) * 2]);
+#pragma unroll
+    for (int off = kCols; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if (many) {
+      __syncthreads();  // the space is free
+      if (lane < kCols) tops[warp][lane] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w][lane % kCols]);
+    }
+    float tops4[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) tops4[j] = __shfl_sync(0xffffffffu, top, col0 + j);
+
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, acc[kVecs][4];
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[v][j] = 0.0f;
+#pragma unroll 4
+    for (int i = from; i <= followers; i += step) {
+      const long long where = place(begin, i);
+      const float4 *of_ml = reinterpret_cast<const float4 *>(ml + (where * kCols + col0) * 2);
+      const float4 p = of_ml[0], q = of_ml[1];
+      const float m[4] = {p.x, p.z, q.x, q.z}, l[4] = {p.y, p.w, q.y, q.w};
+      float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[j] = m[j] == tops4[j] ? 1.0f : exp2_approx(m[j] - tops4[j]);  // also where all are -inf
+        sum[j] += l[j] * f[j];
+      }
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const float4 w = reinterpret_cast<const float4 *>(a.parts + (where * D + 32 * blockIdx.y) * kCols)[v * 32 + lane];
+        acc[v][0] += w.x * f[0];
+        acc[v][1] += w.y * f[1];
+        acc[v][2] += w.z * f[2];
+        acc[v][3] += w.w * f[3];
+      }
+    }
+    if (many) {
+      sums[warp][lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) accs[warp][v][lane] = make_float4(acc[v][0], acc[v][1], acc[v][2], acc[v][3]);
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int w = 1; w < kJoinWarps; ++w) {
+          const float4 s = sums[w][lane];
+          sum[0] += s.x, sum[1] += s.y, sum[2] += s.z, sum[3] += s.w;
+#pragma unroll
+          for (int v = 0; v < kVecs; ++v) {
+            const float4 x = accs[w][v][lane];
+            acc[v][0] += x.x, acc[v][1] += x.y, acc[v][2] += x.z, acc[v][3] += x.w;
+          }
+        }
+      }
+    }
+    if (!many || warp == 0) {
+      const int seq = at / items, kv = at % items / a.chunks, chunk = at % items % a.chunks, cols = min(16, a.group - chunk * 16);
+      __nv_bfloat16 *out = a.out + ((long long)seq * a.heads + kv * a.group + chunk * 16 + col0) * D + 32 * blockIdx.y;
+      const float scale = kFp8 ? c.v_scale[kv] : 1.0f;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col0 + j < cols) out[j * D + (v * 128 + lane * 4) / kCols] = __float2bfloat16_rn(acc[v][j] / sum[j] * scale);
+    }
   }
-  const float y = acc / sum * (kFp8 ? c.v_scale[kv] : 1.0f);
-  a.out[((long long)seq * a.heads + kv * a.group + chunk * 16 + row) * D + threadIdx.x] = __float2bfloat16_rn(y);
 }
 
 int attn_sm_count() {
@@ -569,10 +839,50 @@ int attn_sm_count() {
   return sms[dev];
 }
 
-template <int D, bool kFp8, int kRows>
-cudaError_t launch(const AttnArgs &a, const PagedCache &c, int ctas, cudaStream_t stream) {
-  constexpr int kSmem = attn_smem_bytes<D, kFp8, kRows>();
-  const auto kernel = paged_attention_kernel<D, kFp8, kRows>;
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                              CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void *ptr = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(ptr);
+  });
+  return fn;
+}
+
+// The cache as [page][head][half][token][bytes of a half], copied `box` tokens of one half or of all `halves` at a time.
+bool encode(CUtensorMap *map, char *base, const PagedCache &c, int size, int box, int halves) {
+  const EncodeFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t row = (cuuint64_t)c.head_dim * size, in_half = row < 128 ? row : 128;
+  const cuuint64_t dims[5] = {in_half, (cuuint64_t)c.page_size, row / in_half, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
+  // a dimension of one element is never stepped along
+  const cuuint64_t strides[4] = {c.token_stride > 0 ? (cuuint64_t)c.token_stride : row, 128, c.head_stride > 0 ? (cuuint64_t)c.head_stride : row,
+                                 c.page_stride > 0 ? (cuuint64_t)c.page_stride : row};
+  const cuuint32_t sizes[5] = {128, (cuuint32_t)box, (cuuint32_t)halves, 1, 1}, steps[5] = {1, 1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, base, dims, strides, sizes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool kFp8, int kCols>
+cudaError_t launch(AttnArgs a, const PagedCache &c, int ctas, cudaStream_t stream) {
+  using T = Tile<D, kFp8>;
+  constexpr int kSmem = Layout<D, kFp8, kCols>::kTotal;
+  const auto kernel = paged_attention_kernel<D, kFp8, kCols>;
+  int box = c.page_size & -c.page_size;
+  if (box > T::kTokens) box = T::kTokens;
+  a.box_shift = __builtin_ctz((unsigned)box);
+  a.per_stretches = 1.0 / (kAttnWarps * ctas);
+  a.per_items = 1.0 / (c.kv_heads * a.chunks);
+  a.page_shift = (c.page_size & (c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)c.page_size) : -1;
+  const int halves = box == T::kTokens ? T::kHalves : 1;
+  CUtensorMap map_k, map_v;
+  if (!encode(&map_k, c.k, c, T::kSize, box, halves) || !encode(&map_v, c.v, c, T::kSize, box, halves)) return cudaErrorInvalidValue;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
@@ -585,12 +895,12 @@ cudaError_t launch(const AttnArgs &a, const PagedCache &c, int ctas, cudaStream_
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  err = cudaLaunchKernelEx(&cfg, kernel, a, c);
+  err = cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, a, c);
   if (err != cudaSuccess) return err;
-  cfg.gridDim = dim3((unsigned)ctas, (unsigned)(a.group < 16 ? a.group : 16));
-  cfg.blockDim = dim3(D);
+  cfg.gridDim = dim3((unsigned)((ctas + kJoinWarps - 1) / kJoinWarps), D / 32);
+  cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<D, kRows, kFp8>, a, c, ctas);
+  return cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<D, kCols, kFp8>, a, c, ctas);
 }
 
 int attn_ctas() { return 2 * attn_sm_count(); }
@@ -598,13 +908,13 @@ int attn_ctas() { return 2 * attn_sm_count(); }
 }  // namespace
 
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
-  const size_t rows = heads / kv_heads <= 8 ? 8 : 16, places = 2 * (size_t)attn_ctas();
-  return places * rows * (head_dim + 2) * sizeof(float) + places * sizeof(int);
+  const size_t cols = heads / kv_heads <= 8 ? 8 : 16, places = 2 * (size_t)attn_ctas();
+  return places * cols * (head_dim + 2) * sizeof(float) + places * sizeof(int);
 }
 
 cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head, int heads, const PagedCache &cache, bool fp8,
                                 const int *lengths, float scale, void *out, void *workspace, int *error_flag, cudaStream_t stream) {
-  const int ctas = attn_ctas(), group = heads / cache.kv_heads, rows = group <= 8 ? 8 : 16, d = cache.head_dim;
+  const int ctas = attn_ctas(), group = heads / cache.kv_heads, cols = group <= 8 ? 8 : 16, d = cache.head_dim;
   AttnArgs a;
   a.q = static_cast<const __nv_bfloat16 *>(q);
   a.q_row = q_row;
@@ -612,15 +922,15 @@ cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head
   a.lengths = lengths;
   a.out = static_cast<__nv_bfloat16 *>(out);
   a.parts = static_cast<float *>(workspace);
-  a.splits = reinterpret_cast<int *>(a.parts + 2LL * ctas * rows * (d + 2));
+  a.splits = reinterpret_cast<int *>(a.parts + 2LL * ctas * cols * (d + 2));
   a.seqs = cache.seqs;
   a.heads = heads;
   a.group = group;
   a.chunks = (group + 15) / 16;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.error_flag = error_flag;
-#define SHARQ_ATTN(D, FP8, ROWS) \
-  if (d == D && fp8 == FP8 && rows == ROWS) return launch<D, FP8, ROWS>(a, cache, ctas, stream);
+#define SHARQ_ATTN(D, FP8, COLS) \
+  if (d == D && fp8 == FP8 && cols == COLS) return launch<D, FP8, COLS>(a, cache, ctas, stream);
   SHARQ_ATTN(128, false, 8)
   SHARQ_ATTN(128, false, 16)
   SHARQ_ATTN(128, true, 8)

@@ -30,6 +30,7 @@ _NO_FLAG = torch.zeros(1, dtype=torch.int32, device="cpu")
 _PREPARE_TIMEOUTS_SEEN = 0
 _BAD_EXPERT = 0x401  # kPlanBadExpert of csrc/decoder_ops.cu
 _BAD_CACHE_INDEX = 0x402  # kBadCacheIndex of csrc/decode_ops.cuh
+_ATTENTION_TIMEOUT = 0x403  # kAttentionTimeout of csrc/decode_ops.cuh
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -78,6 +79,8 @@ def check_device_errors(device=None) -> None:
             if code == _BAD_CACHE_INDEX:
                 raise RuntimeError("sharq_b200 paged cache: a position, length, sequence or page was outside the cache or its tables "
                                    f"on cuda:{idx}")
+            if code == _ATTENTION_TIMEOUT:
+                raise RuntimeError(f"sharq_b200 paged_attention: a wait for a copy ran out on cuda:{idx}; outputs are undefined")
             raise RuntimeError(f"sharq_b200 GEMM kernel reported a timed-out wait (code {code}) on cuda:{idx}")
 
 
