@@ -802,7 +802,7 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
   SHARQ_REQUIRE(c.head_dim == 64 || c.head_dim == 128, "head_dim must be 64 or 128, got %d", c.head_dim);
   SHARQ_REQUIRE(heads > 0 && heads % c.kv_heads == 0 && heads <= 65536, "heads must be a positive multiple of kv_heads, at most 65536");
   SHARQ_REQUIRE((int64_t)c.seqs * heads <= 0x7fffffff &&
-                    (int64_t)c.seqs * (sharq::paged_capacity(c) / 16 + 4) <= 0x7fffffff,
+                    (int64_t)c.seqs * (sharq::paged_capacity(c) / 16 + 4) <= 0x70000000 / (c.kv_heads * (int64_t)((heads / c.kv_heads + 15) / 16)),
                 "too many sequences, or a page table for too many tokens");
   SHARQ_REQUIRE(q_row >= 0 && q_head >= 0 && q_row % 8 == 0 && q_head % 8 == 0, "the strides of q must be multiples of 8");
   SHARQ_REQUIRE(aligned16(q_bf16) && aligned16(out_bf16) && aligned16(workspace), "buffers must be 16-byte aligned");

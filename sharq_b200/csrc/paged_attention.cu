@@ -44,7 +44,10 @@ constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
 constexpr float kF16Lift = 10.0f;
 constexpr int kItemCost = 2;
-constexpr int kStretchLeast = 6;
+constexpr int kStretchLeast = 4;
+constexpr int kAttnClusterMost = 8;
+constexpr int kDirectTiles = 3;  // tiles of a warp that a cluster is sized for, and for which it is taken at most
+constexpr int kDirectMost = 16;
 
 __device__ __forceinline__ uint4 ld_shared16(uint32_t smem) {
   uint4 v;
@@ -124,10 +127,10 @@ struct AttnArgs {
   const int *lengths;
   __nv_bfloat16 *out;
   float *parts;  // [2 * CTAs][D][kCols] unnormalised columns, then [2 * CTAs][kCols] of their [maximum, sum]
-  int *splits;   // [CTAs][2]: (sequence, head chunk) that begins in this CTA and goes on in the next ones, and in how many; 0: none
   int seqs, heads, group, chunks;  // chunks: pieces of 16 query heads of a group
   int box_shift;                   // log2 of the tokens of a copy: the largest power of two, at most a tile, that divides the page size
-  double per_stretches, per_items; // 1 / (stretches of the list), 1 / (items of a sequence)
+  int stretch_shift;               // direct form: log2 of the warps of a cluster
+  unsigned stretches_magic, items_magic;  // list: for divide() by the stretches and by the items of a sequence
   int page_shift;                  // log2 of the page size, -1 if it is no power of two
   float scale_log2;                // scale * log2(e)
   int *error_flag;
@@ -147,21 +150,21 @@ struct Tile {
 static_assert(Tile<128, false>::kStage == 8192 && Tile<64, true>::kStage == 8192, "a stage is a multiple of the swizzle's 1024 bytes");
 
 // What a warp leaves of an item that does not lie within its stretch.
-struct Part {
-  int item;  // seq * items + item, -1: nothing
+struct __align__(16) Part {
+  int seq, item;  // item: head and chunk, -1: nothing
   int begins, tiles_left;
 };
 // Shared memory of a CTA: the rings (the swizzle wants 1024 bytes), then the part at the beginning of every warp's stretch (the one at the end goes
 // to the warp's ring, which is free by then), two parts' maxima and sums per warp, their descriptions, barriers and the flag of a wait that ran out.
 template <int D, bool kFp8, int kCols>
 struct Layout {
-  static constexpr int kStages = kCols == 8 ? 3 : 2;  // two CTAs in an SM's memory
+  static constexpr int kStages = 2;
   static constexpr int kRing = kStages * Tile<D, kFp8>::kStage;
   static constexpr int kPart = D * kCols * 4;
   static constexpr int kParts = kAttnWarps * kRing;
   static constexpr int kMl = kParts + kAttnWarps * kPart;
   static constexpr int kInfo = kMl + 2 * kAttnWarps * kCols * 8;
-  static constexpr int kBars = kInfo + (2 * kAttnWarps * (int)sizeof(Part) + 7) / 8 * 8;
+  static constexpr int kBars = kInfo + 2 * kAttnWarps * (int)sizeof(Part);
   static constexpr int kFlag = kBars + kAttnWarps * kStages * 8;
   static constexpr int kTotal = kFlag + 8;
   static_assert(kPart <= kRing && kTotal <= 115712, "a part fits a ring, two CTAs an SM");
@@ -182,15 +185,10 @@ __device__ __forceinline__ int tiles_of(int tokens) {  // an empty sequence has 
   return tokens <= kTokens ? 1 : (tokens - 1) / kTokens + 1;
 }
 
-// n / d for n < 2^52 with the reciprocal of d at hand (an integer division by a variable takes some hundred cycles)
-__device__ __forceinline__ long long divide(long long n, long long d, double reciprocal) {
-  long long q = (long long)((double)n * reciprocal);
-  const long long r = n - q * d;
-  if (r < 0)
-    --q;
-  else if (r >= d)
-    ++q;
-  return q;
+// n / d for n < 2^31 with ceil(2^32 / d) at hand (an integer division by a variable takes some hundred cycles): at most one too high
+__device__ __forceinline__ int divide(int n, int d, unsigned magic) {
+  const int q = d == 1 ? n : (int)__umulhi((unsigned)n, magic);
+  return q * d > n ? q - 1 : q;
 }
 
 // Where a warp stands in its stretch: tiles [tile, end) of an item are its own.  An item is kItemCost + its tiles long in the list, of which `skip` lie
@@ -202,12 +200,11 @@ template <int kTokens>
 __device__ __forceinline__ void enter(Place &p, const AttnArgs &a, const PagedCache &c) {
   p.tokens = length_of(a, c, p.seq).tokens;
   p.tile = max(0, p.skip - kItemCost);
-  p.end = (int)min((long long)tiles_of<kTokens>(p.tokens), (long long)p.skip + p.left - kItemCost);
+  p.end = min(tiles_of<kTokens>(p.tokens), p.skip + p.left - kItemCost);
 }
 template <int kTokens>
 __device__ __forceinline__ void leave(Place &p, const AttnArgs &a, const PagedCache &c) {
-  const long long rest = (long long)kItemCost + tiles_of<kTokens>(p.tokens) - p.skip;
-  p.left = rest >= p.left ? 0 : p.left - (int)rest;
+  p.left = max(0, p.left - (kItemCost + tiles_of<kTokens>(p.tokens) - p.skip));
   if (p.left == 0) return;
   p.skip = 0;
   if (++p.chunk == a.chunks) {
@@ -220,12 +217,58 @@ __device__ __forceinline__ void leave(Place &p, const AttnArgs &a, const PagedCa
     enter<kTokens>(p, a, c);
   } else {  // the same sequence's tokens
     p.tile = 0;
-    p.end = (int)min((long long)tiles_of<kTokens>(p.tokens), (long long)p.left - kItemCost);
+    p.end = min(tiles_of<kTokens>(p.tokens), p.left - kItemCost);
   }
 }
 
-// kCols: columns for query heads (8 or 16)
-template <int D, bool kFp8, int kCols>
+// The list of all tiles, its length and the part of it that a warp takes: less than 2^31, the launcher checks.
+struct List {
+  int total, per;
+};
+template <int kTokens>
+__device__ __forceinline__ List list_of(const AttnArgs &a, const PagedCache &c, int items, int stretches, int lane) {
+  int per_head = 0;
+#pragma unroll 4
+  for (int b = lane; b < a.seqs; b += 32) per_head += kItemCost + tiles_of<kTokens>(length_of(a, c, b).tokens);
+  const int total = __reduce_add_sync(0xffffffffu, per_head) * items;
+  return {total, max(kStretchLeast, divide(total + stretches - 1, stretches, a.stretches_magic))};
+}
+// the item that unit u of the list belongs to, and what of it lies before u -> the item's length
+template <int kTokens>
+__device__ __forceinline__ int locate(Place &at, int u, const AttnArgs &a, const PagedCache &c, int items, int lane) {
+  int before = 0;
+  const int u_head = divide(u, items, a.items_magic);  // in units of a head: a sequence begins at items times what lies before it
+  for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+    const int b = b0 + lane;
+    const int n_units = b < a.seqs ? kItemCost + tiles_of<kTokens>(length_of(a, c, b).tokens) : 0;
+    int n = n_units;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, n, off);
+      if (lane >= off) n += up;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, before + n > u_head);
+    if (over != 0) {
+      const int in = __ffs(over) - 1;
+      const int units = __shfl_sync(0xffffffffu, n_units, in), rest = u - (before + __shfl_sync(0xffffffffu, n, in) - units) * items;
+      // less than 2^16 items, so the float quotient is one off at most
+      int item = (int)__fdividef((float)rest, (float)units);
+      if (item * units > rest) --item;
+      if (rest - item * units >= units) ++item;
+      at.seq = b0 + in;
+      at.skip = rest - item * units;
+      at.head = a.chunks == 1 ? item : item / a.chunks;
+      at.chunk = item - at.head * a.chunks;
+      return units;
+    }
+    before += __shfl_sync(0xffffffffu, n, 31);
+  }
+  return 0;
+}
+
+// kCols: columns for query heads (8 or 16).  kDirect: a cluster per (sequence, head chunk), blockIdx = (rank, head chunk, sequence), whose warps take equal
+// stretches of its tiles and whose CTAs join their parts through distributed shared memory; nothing is left for a second launch.
+template <int D, bool kFp8, int kCols, bool kDirect>
 __global__ void __launch_bounds__(kAttnThreads, 2)
     paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const __grid_constant__ AttnArgs a, const __grid_constant__ PagedCache c) {
@@ -248,49 +291,30 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   if (threadIdx.x == 0) *gave_up = 0;
   if (threadIdx.x < 2 * kAttnWarps) info[threadIdx.x].item = -1;
   __syncthreads();
-  ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();  // behind the wait: the second kernel reads the lengths ahead of its own
   const int items = c.kv_heads * a.chunks;  // (head, chunk) pairs of a sequence
 
-  // this warp's stretch [u0, u1) of the list, in tiles
+  // this warp's stretch of the list of tiles
   const int stretch = blockIdx.x * kAttnWarps + warp, stretches = gridDim.x * kAttnWarps;
-  unsigned per_head = 0;  // less than 2^31: the launcher checks
-#pragma unroll 4
-  for (int b = lane; b < a.seqs; b += 32) per_head += kItemCost + tiles_of<kTokens>(length_of(a, c, b).tokens);
-  per_head = __reduce_add_sync(0xffffffffu, per_head);
-  const long long total = (long long)per_head * items;
-  long long per = divide(total + stretches - 1, stretches, a.per_stretches);
-  if (per < kStretchLeast) per = kStretchLeast;
-  const long long u0 = stretch * per, u1 = min(u0 + per, total);
-  if (threadIdx.x == 0) a.splits[2 * blockIdx.x + 1] = 0;
-  Place at = {0, 0, 0, 0, u0 < u1 ? (int)min(u1 - u0, 0x7fffffffLL) : 0, 0, 0, 0};
-  if (u0 < u1) {
-    unsigned before = 0;
-    const unsigned u_head = (unsigned)divide(u0, items, a.per_items);  // u0 in units of a head: sequence s begins at items times what lies before it
-    for (int b0 = 0; b0 < a.seqs; b0 += 32) {
-      const int b = b0 + lane;
-      const unsigned n_units = b < a.seqs ? kItemCost + tiles_of<kTokens>(length_of(a, c, b).tokens) : 0;
-      unsigned n = n_units;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const unsigned up = __shfl_up_sync(0xffffffffu, n, off);
-        if (lane >= off) n += up;
-      }
-      const unsigned over = __ballot_sync(0xffffffffu, before + n > u_head);
-      if (over != 0) {
-        const int in = __ffs(over) - 1;
-        const unsigned units = __shfl_sync(0xffffffffu, n_units, in), upto = before + __shfl_sync(0xffffffffu, n, in) - units;
-        const long long rest = u0 - (long long)upto * items;
-        at.seq = b0 + in;
-        const int item = (int)divide(rest, units, (double)__frcp_rn((float)units));  // less than 2^16 items: one off at most
-        at.skip = (int)(rest - (long long)item * units);
-        at.head = a.chunks == 1 ? item : item / a.chunks;
-        at.chunk = item - at.head * a.chunks;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, n, 31);
+  Place at = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (kDirect) {
+    at.seq = blockIdx.z;
+    at.head = a.chunks == 1 ? blockIdx.y : blockIdx.y / a.chunks;
+    at.chunk = blockIdx.y - at.head * a.chunks;
+    at.tokens = length_of(a, c, at.seq).tokens;
+    const int n_tiles = tiles_of<kTokens>(at.tokens), each = (n_tiles + stretches - 1) >> a.stretch_shift;
+    at.tile = stretch * each;
+    at.end = min(n_tiles, at.tile + each);
+    at.left = 1;  // this item and no other
+  } else {
+    const List list = list_of<kTokens>(a, c, items, stretches, lane);
+    const int u0 = stretch * list.per;  // stretches * per: total and a little more
+    at.left = max(0, min(list.per, list.total - u0));
+    if (at.left > 0) {
+      locate<kTokens>(at, u0, a, c, items, lane);
+      enter<kTokens>(at, a, c);
     }
-    enter<kTokens>(at, a, c);
   }
 
   Place next = at;  // of the tile that is loaded next
@@ -400,12 +424,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         top = max(top & 0xFFFFu, top >> 16);
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the largest value to [2^14, 2^15); a row with infinities or NaN as it is
-        const int e = (int)(top >> 7), shift = e == 255 ? 0 : 141 - max(e, 1);
-        // in two factors, each a normal float
-        const int s1 = shift / 2, s2 = shift - s1;
-        const float f1 = __int_as_float((127 + s1) << 23), f2 = __int_as_float((127 + s2) << 23);
-        const float back = a.scale_log2 * c.k_scale[kv] * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23);
+        // the largest value to [2^14, 2^15), or up by 2^126; a row with infinities or NaN as it is
+        const int e = (int)(top >> 7), shift = e == 255 ? 0 : min(126, 141 - max(e, 1));
+        const float up = __int_as_float((127 + shift) << 23), back = a.scale_log2 * c.k_scale[kv] * __int_as_float((127 - shift) << 23);
         sl[n][0] = __shfl_sync(0xffffffffu, back, 8 * t);  // lane of column 2 t
         sl[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
 #pragma unroll
@@ -413,7 +434,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint32_t w = qb[n][k][j];
-            qb[n][k][j] = pack_f16(__uint_as_float(w << 16) * f1 * f2, __uint_as_float(w & 0xFFFF0000u) * f1 * f2);
+            qb[n][k][j] = pack_f16(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xFFFF0000u) * up);
           }
       }
     }
@@ -606,7 +627,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       for (int n = 0; n < kN; ++n) {
         float f[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) f[j] = (kFp8 ? c.v_scale[kv] : 1.0f) / l[n][j];
+        for (int j = 0; j < 2; ++j) f[j] = __fdividef(kFp8 ? c.v_scale[kv] : 1.0f, l[n][j]);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           float y[4];
@@ -644,190 +665,300 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           *reinterpret_cast<float2 *>(part + d1 * kCols + 8 * n + 2 * t) = make_float2(o[i][n][2], o[i][n][3]);
         }
       }
-      if (lane == 0) info[slot] = {at.seq * items + at.head * a.chunks + at.chunk, begins, n_tiles - at.end};
+      if (lane == 0) info[slot] = {at.seq, at.head << 16 | at.chunk, begins, n_tiles - at.end};
     }
   }
 
-  // Join this CTA's parts: neighbouring ones of the same item.
+  if (kDirect && tiles_of<kTokens>(at.tokens) == 1) return;  // one warp of the cluster has done it all
   __syncthreads();
   constexpr int kVecs = D * kCols / 4 / kAttnThreads;  // a thread's float4s of a part; its columns are the same in all of them
   static_assert(kVecs >= 1 && kAttnThreads * 4 % kCols == 0, "every thread has a share of a part");
   const int col0 = threadIdx.x * 4 % kCols;
   float top[4], sum[4];
   float4 acc[kVecs];
-  Part run = {-1, 0, 0};  // the item whose parts are being joined
-  for (int i = 0; i <= 2 * kAttnWarps; ++i) {
-    const Part now = i < 2 * kAttnWarps ? info[i] : Part{-2, 0, 0};
-    if (now.item == -1) continue;
-    if (run.item >= 0 && now.item != run.item) {
-      if (run.begins && run.tiles_left == 0) {
-        const int seq = run.item / items, pair = run.item - seq * items, kv = pair / a.chunks, chunk = pair % a.chunks;
-        const int cols = min(16, a.group - chunk * 16);
-        __nv_bfloat16 *out = a.out + ((long long)seq * a.heads + kv * a.group + chunk * 16 + col0) * D;
-        float f[4];
+  auto clear = [&]() {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = (kFp8 ? c.v_scale[kv] : 1.0f) / sum[j];
+    for (int j = 0; j < 4; ++j) top[j] = -INFINITY, sum[j] = 0.0f;
 #pragma unroll
-        for (int v = 0; v < kVecs; ++v) {
-          const int d = (v * kAttnThreads + threadIdx.x) * 4 / kCols;
-          const float y[4] = {acc[v].x, acc[v].y, acc[v].z, acc[v].w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (col0 + j < cols) out[j * D + d] = __float2bfloat16_rn(y[j] * f[j]);
-        }
-      } else {
-        // the part of an item that began in an earlier CTA goes to this CTA's first place, of one that goes on in a later one to the second
-        const long long place = 2LL * blockIdx.x + (run.begins ? 1 : 0);
-        float4 *part = reinterpret_cast<float4 *>(a.parts + place * D * kCols);
-#pragma unroll
-        for (int v = 0; v < kVecs; ++v) part[v * kAttnThreads + threadIdx.x] = acc[v];
-        float4 *ml = reinterpret_cast<float4 *>(a.parts + 2LL * gridDim.x * D * kCols + (place * kCols + col0) * 2);
-        if (threadIdx.x * 4 < kCols) {
-          ml[0] = make_float4(top[0], sum[0], top[1], sum[1]);
-          ml[1] = make_float4(top[2], sum[2], top[3], sum[3]);
-        }
-        if (run.begins && threadIdx.x == 0) {
-          a.splits[2 * blockIdx.x] = run.item;
-          a.splits[2 * blockIdx.x + 1] = (int)((run.tiles_left + kAttnWarps * per - 1) / (kAttnWarps * per));
-        }
-      }
-    }
-    if (now.item < 0) break;
+    for (int v = 0; v < kVecs; ++v) acc[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  };
+  auto merge = [&](int i) {  // one of the CTA's parts
     const float4 *of_ml = reinterpret_cast<const float4 *>(smem + L::kMl + (i * kCols + col0) * 8);
     const float4 p = of_ml[0], q = of_ml[1];
     const float of[4] = {p.x, p.z, q.x, q.z}, s[4] = {p.y, p.w, q.y, q.w};
     const float4 *x = reinterpret_cast<const float4 *>((i & 1) != 0 ? smem + (i >> 1) * L::kRing : smem + L::kParts + (i >> 1) * L::kPart);
-    if (now.item != run.item) {
-      run = now;
+    float f[4], f_old[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) top[j] = of[j], sum[j] = s[j];
+    for (int j = 0; j < 4; ++j) {
+      const float high = fmaxf(top[j], of[j]);
+      f_old[j] = top[j] == high ? 1.0f : exp2_approx(top[j] - high);  // also where both are -inf
+      f[j] = of[j] == high ? 1.0f : exp2_approx(of[j] - high);
+      top[j] = high;
+      sum[j] = sum[j] * f_old[j] + s[j] * f[j];
+    }
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) acc[v] = x[v * kAttnThreads + threadIdx.x];
-    } else {
-      run.tiles_left = now.tiles_left;
-      float f[4], f_old[4];
+    for (int v = 0; v < kVecs; ++v) {
+      const float4 w = x[v * kAttnThreads + threadIdx.x];
+      acc[v].x = acc[v].x * f_old[0] + w.x * f[0];
+      acc[v].y = acc[v].y * f_old[1] + w.y * f[1];
+      acc[v].z = acc[v].z * f_old[2] + w.z * f[2];
+      acc[v].w = acc[v].w * f_old[3] + w.w * f[3];
+    }
+  };
+  auto write = [&](int seq, int head, int chunk, int vec, const float4 &of) {  // finished elements
+    const int cols = min(16, a.group - chunk * 16), d = vec * 4 / kCols;
+    __nv_bfloat16 *out = a.out + ((long long)seq * a.heads + head * a.group + chunk * 16 + col0) * D + d;
+    const float y[4] = {of.x, of.y, of.z, of.w}, scale = kFp8 ? c.v_scale[head] : 1.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float high = fmaxf(top[j], of[j]);
-        f_old[j] = top[j] == high ? 1.0f : exp2_approx(top[j] - high);  // also where both are -inf
-        f[j] = of[j] == high ? 1.0f : exp2_approx(of[j] - high);
-        top[j] = high;
-        sum[j] = sum[j] * f_old[j] + s[j] * f[j];
+    for (int j = 0; j < 4; ++j)
+      if (col0 + j < cols) out[j * D] = __float2bfloat16_rn(y[j] * __fdividef(scale, sum[j]));
+  };
+
+  if (kDirect) {
+    clear();
+    for (int i = 0; i < 2 * kAttnWarps; ++i)
+      if (info[i].item >= 0) merge(i);
+    if (gridDim.x == 1) {
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) write(at.seq, at.head, at.chunk, v * kAttnThreads + threadIdx.x, acc[v]);
+      return;
+    }
+    __syncthreads();  // the warps' parts have been read: the CTA's takes their place
+    float4 *mine = reinterpret_cast<float4 *>(smem), *mine_ml = reinterpret_cast<float4 *>(smem + L::kMl);
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) mine[v * kAttnThreads + threadIdx.x] = acc[v];
+    if (threadIdx.x * 4 < kCols) {
+      mine_ml[threadIdx.x * 2] = make_float4(top[0], sum[0], top[1], sum[1]);
+      mine_ml[threadIdx.x * 2 + 1] = make_float4(top[2], sum[2], top[3], sum[3]);
+    }
+    ptx::cluster_sync();
+    // the CTAs take turns at 128 of the part's float4s, and sum in rank order
+    for (int vec = blockIdx.x * kAttnThreads + threadIdx.x; vec < kVecs * kAttnThreads; vec += gridDim.x * kAttnThreads) {
+      float4 p[kAttnClusterMost], q[kAttnClusterMost], x[kAttnClusterMost];
+#pragma unroll
+      for (int r = 0; r < kAttnClusterMost; ++r)
+        if (r < (int)gridDim.x) {
+          p[r] = ptx::ld_cluster_f32x4(ptx::smem_u32(mine_ml + col0 / 2), r);
+          q[r] = ptx::ld_cluster_f32x4(ptx::smem_u32(mine_ml + col0 / 2 + 1), r);
+          x[r] = ptx::ld_cluster_f32x4(ptx::smem_u32(mine + vec), r);
+        } else {
+          p[r] = q[r] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+          x[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+      clear();
+#pragma unroll
+      for (int r = 0; r < kAttnClusterMost; ++r) {
+        top[0] = fmaxf(top[0], p[r].x), top[1] = fmaxf(top[1], p[r].z);
+        top[2] = fmaxf(top[2], q[r].x), top[3] = fmaxf(top[3], q[r].z);
       }
+      float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) {
-        const float4 w = x[v * kAttnThreads + threadIdx.x];
-        acc[v].x = acc[v].x * f_old[0] + w.x * f[0];
-        acc[v].y = acc[v].y * f_old[1] + w.y * f[1];
-        acc[v].z = acc[v].z * f_old[2] + w.z * f[2];
-        acc[v].w = acc[v].w * f_old[3] + w.w * f[3];
+      for (int r = 0; r < kAttnClusterMost; ++r) {
+        const float of[4] = {p[r].x, p[r].z, q[r].x, q[r].z}, s[4] = {p[r].y, p[r].w, q[r].y, q[r].w};
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[j] = of[j] == top[j] ? 1.0f : exp2_approx(of[j] - top[j]);
+          sum[j] += s[j] * f[j];
+        }
+        y.x += x[r].x * f[0];
+        y.y += x[r].y * f[1];
+        y.z += x[r].z * f[2];
+        y.w += x[r].w * f[3];
+      }
+      write(at.seq, at.head, at.chunk, vec, y);
+    }
+    __syncwarp();
+    ptx::cluster_sync();  // a CTA's memory is read until here
+    return;
+  }
+
+  Part run = {0, -1, 0, 0};  // the item whose parts are being joined: neighbouring ones
+  const Part of_lane = info[lane % (2 * kAttnWarps)];
+  unsigned places = __ballot_sync(0xffffffffu, lane < 2 * kAttnWarps && of_lane.item >= 0);
+  while (true) {
+    const int i = __ffs(places) - 1;  // -1: no more
+    const int from = max(i, 0);
+    const Part now = {__shfl_sync(0xffffffffu, of_lane.seq, from), i < 0 ? -2 : __shfl_sync(0xffffffffu, of_lane.item, from),
+                      __shfl_sync(0xffffffffu, of_lane.begins, from), __shfl_sync(0xffffffffu, of_lane.tiles_left, from)};
+    places &= places - 1;
+    const bool same = now.item == run.item && now.seq == run.seq;
+    if (run.item >= 0 && !same) {
+      if (run.begins && run.tiles_left == 0) {
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) write(run.seq, run.item >> 16, run.item & 0xFFFF, v * kAttnThreads + threadIdx.x, acc[v]);
+      } else {
+        // the part of an item that began in an earlier CTA goes to this CTA's first place, of one that goes on in a later one to the second
+        const int place = 2 * blockIdx.x + (run.begins ? 1 : 0);
+        float4 *part = reinterpret_cast<float4 *>(a.parts + place * D * kCols);
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) part[v * kAttnThreads + threadIdx.x] = acc[v];
+        float4 *ml = reinterpret_cast<float4 *>(a.parts + 2 * gridDim.x * D * kCols + (place * kCols + col0) * 2);
+        if (threadIdx.x * 4 < kCols) {
+          ml[0] = make_float4(top[0], sum[0], top[1], sum[1]);
+          ml[1] = make_float4(top[2], sum[2], top[3], sum[3]);
+        }
       }
     }
+    if (now.item < 0) break;
+    if (!same) {
+      clear();
+      run = now;
+    }
+    run.tiles_left = now.tiles_left;
+    merge(i);
   }
 }
 
-// Joins the parts of the items that begin in one of eight CTAs of the kernel above and go on: elements 32 blockIdx.y .. + 31 of all columns.  A warp takes an item, or, where
-// one of them has many parts, all warps take the parts of one item after the other in turn, and their sums meet in shared memory.  The
-// maximum over an item's parts comes first, so that the parts are independent of each other.
+// Joins the parts of the items that begin in one of eight CTAs of the kernel above and go on: a quarter of the floats [element][column].  A
+// warp takes an item, or, where one of them has many parts, all warps take the parts of one item after the other in turn, and their sums meet in
+// shared memory.  Which items these are follows from the lengths, which are read while the kernel above runs: it lets this one start
+// behind its own wait, so what precedes them both is done.
 constexpr int kJoinWarps = 8;
-constexpr int kJoinMany = 8;
+constexpr int kJoinSlices = 4;
+constexpr int kJoinBatch = 4;  // parts whose loads are in flight together; more would take registers that the kernel above still holds
+constexpr int kJoinAlone = 8;  // parts that one warp joins
 
 template <int D, int kCols, bool kFp8>
 __global__ void __launch_bounds__(32 * kJoinWarps) paged_attention_join_kernel(const __grid_constant__ AttnArgs a,
                                                                                const __grid_constant__ PagedCache c, int ctas) {
-  constexpr int kVecs = kCols / 4;  // a lane's float4s of an element slice [32][kCols]; a lane's columns are the same in all of them
-  __shared__ float4 accs[kJoinWarps][kVecs][32], sums[kJoinWarps][32];
-  __shared__ float tops[kJoinWarps][kCols];
-  ptx::grid_dependency_wait();
+  constexpr int kTokens = Tile<D, kFp8>::kTokens, kVecs = D * kCols / (128 * kJoinSlices);  // float4s of a lane
+  __shared__ float4 accs[kJoinWarps][kVecs][32], sums[kJoinWarps][32], tops[kJoinWarps][32];
+  __shared__ int4 items_of[kJoinWarps];  // sequence, head, chunk, parts (0: nothing begins in that CTA and goes on)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, items = c.kv_heads * a.chunks;
   const int base = blockIdx.x * kJoinWarps;
-  const int of_lane = lane < kJoinWarps && base + lane < ctas ? a.splits[2 * (base + lane) + 1] : 0;
-  const unsigned any = __ballot_sync(0xffffffffu, of_lane > 0);
-  if (any == 0) return;
-  const bool many = __any_sync(0xffffffffu, of_lane > kJoinMany);
-  const float *ml = a.parts + 2LL * ctas * D * kCols;
-  const int col0 = lane * 4 % kCols;
-  // part 0 of the item that begins in CTA `begin`: its second place; part i: the first place of the i-th CTA behind it
-  auto place = [&](int begin, int i) { return 2LL * (begin + i) + (i == 0 ? 1 : 0); };
-
-  unsigned todo = many ? any : any & (1u << warp);
-  while (todo != 0) {
-    const int which = __ffs(todo) - 1, begin = base + which;
-    todo &= todo - 1;
-    const int followers = __shfl_sync(0xffffffffu, of_lane, which);
-    const int at = a.splits[2 * begin];
-    const int from = many ? warp : 0, step = many ? kJoinWarps : 1;
-    // maximum of column lane % kCols, the parts dealt over the lanes and warps
-    float top = -INFINITY;
-    for (int i = (many ? warp * (32 / kCols) : 0) + lane / kCols; i <= followers; i += step * (32 / kCols))
-      top = fmaxf(top, ml[(place(begin, i) * kCols + lane % kCols) * 2]);
-#pragma unroll
-    for (int off = kCols; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    if (many) {
-      __syncthreads();  // the space is free
-      if (lane < kCols) tops[warp][lane] = top;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w][lane % kCols]);
+  {
+    const List list = list_of<kTokens>(a, c, items, kAttnWarps * ctas, lane);
+    const int span = list.per * kAttnWarps, from = (base + warp) * span, to = from + span;
+    Place at = {0, 0, 0, 0, 0, 0, 0, 0};
+    int parts = 0;
+    if (base + warp < ctas && to < list.total) {
+      const int units = locate<kTokens>(at, to, a, c, items, lane), first = to - at.skip + kItemCost;  // unit of the item's first tile
+      if (at.skip > 0 && first >= from && first < to) parts = 2 + (units - at.skip - 1) / span;
     }
-    float tops4[4];
+    if (lane == 0) items_of[warp] = make_int4(at.seq, at.head, at.chunk, parts);
+  }
+  __syncthreads();
+  int most = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) tops4[j] = __shfl_sync(0xffffffffu, top, col0 + j);
+  for (int i = 0; i < kJoinWarps; ++i) most = max(most, items_of[i].w);
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  if (most == 0) return;
+  const bool many = most > kJoinAlone;
+  const int vec = blockIdx.y * kVecs * 32 + lane, col0 = lane * 4 % kCols;
+  const float4 *ml = reinterpret_cast<const float4 *>(a.parts + 2LL * ctas * D * kCols);
+  const float4 *data = reinterpret_cast<const float4 *>(a.parts);
 
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, acc[kVecs][4];
-#pragma unroll
-    for (int v = 0; v < kVecs; ++v)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[v][j] = 0.0f;
-#pragma unroll 4
-    for (int i = from; i <= followers; i += step) {
-      const long long where = place(begin, i);
-      const float4 *of_ml = reinterpret_cast<const float4 *>(ml + (where * kCols + col0) * 2);
-      const float4 p = of_ml[0], q = of_ml[1];
-      const float m[4] = {p.x, p.z, q.x, q.z}, l[4] = {p.y, p.w, q.y, q.w};
-      float f[4];
+#pragma unroll 1
+  for (int which = many ? 0 : warp; which < (many ? kJoinWarps : warp + 1); ++which) {
+    const int4 item = items_of[which];
+    if (item.w == 0) continue;
+    float top[4], sum[4], acc[kVecs][4];
+    auto clear = [&]() {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f[j] = m[j] == tops4[j] ? 1.0f : exp2_approx(m[j] - tops4[j]);  // also where all are -inf
-        sum[j] += l[j] * f[j];
+        sum[j] = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) acc[v][j] = 0.0f;
+      }
+    };
+    clear();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top[j] = -INFINITY;
+    const int step = many ? kJoinWarps : 1;
+    for (int i0 = many ? warp : 0; i0 < item.w; i0 += step * kJoinBatch) {
+      float4 p[kJoinBatch], q[kJoinBatch], x[kJoinBatch][kVecs];
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) {
+        const int i = i0 + k * step;
+        if (i < item.w) {
+          // part 0 lies in the second place of the item's first CTA, part i in the first place of the i-th CTA behind it
+          const long long place = 2LL * (base + which + i) + (i == 0 ? 1 : 0);
+          p[k] = ml[(place * kCols + col0) / 2];
+          q[k] = ml[(place * kCols + col0) / 2 + 1];
+#pragma unroll
+          for (int v = 0; v < kVecs; ++v) x[k][v] = data[place * (D * kCols / 4) + vec + v * 32];
+        } else {
+          p[k] = q[k] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+#pragma unroll
+          for (int v = 0; v < kVecs; ++v) x[k][v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+      }
+      float high[4] = {top[0], top[1], top[2], top[3]};
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) {
+        high[0] = fmaxf(high[0], p[k].x), high[1] = fmaxf(high[1], p[k].z);
+        high[2] = fmaxf(high[2], q[k].x), high[3] = fmaxf(high[3], q[k].z);
       }
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) {
-        const float4 w = reinterpret_cast<const float4 *>(a.parts + (where * D + 32 * blockIdx.y) * kCols)[v * 32 + lane];
-        acc[v][0] += w.x * f[0];
-        acc[v][1] += w.y * f[1];
-        acc[v][2] += w.z * f[2];
-        acc[v][3] += w.w * f[3];
+      for (int j = 0; j < 4; ++j) {
+        const float f = top[j] == high[j] ? 1.0f : exp2_approx(top[j] - high[j]);  // also where both are -inf
+        sum[j] *= f;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) acc[v][j] *= f;
+        top[j] = high[j];
+      }
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) {
+        const float of[4] = {p[k].x, p[k].z, q[k].x, q[k].z}, s[4] = {p[k].y, p[k].w, q[k].y, q[k].w};
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[j] = of[j] == top[j] ? 1.0f : exp2_approx(of[j] - top[j]);
+          sum[j] += s[j] * f[j];
+        }
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          acc[v][0] += x[k][v].x * f[0];
+          acc[v][1] += x[k][v].y * f[1];
+          acc[v][2] += x[k][v].z * f[2];
+          acc[v][3] += x[k][v].w * f[3];
+        }
       }
     }
     if (many) {
+      __syncthreads();  // the space is free
+      tops[warp][lane] = make_float4(top[0], top[1], top[2], top[3]);
       sums[warp][lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
 #pragma unroll
       for (int v = 0; v < kVecs; ++v) accs[warp][v][lane] = make_float4(acc[v][0], acc[v][1], acc[v][2], acc[v][3]);
       __syncthreads();
-      if (warp == 0) {
+      if (warp != 0) continue;
 #pragma unroll
-        for (int w = 1; w < kJoinWarps; ++w) {
-          const float4 s = sums[w][lane];
-          sum[0] += s.x, sum[1] += s.y, sum[2] += s.z, sum[3] += s.w;
+      for (int w = 1; w < kJoinWarps; ++w) {
+        const float4 h = tops[w][lane];
+        top[0] = fmaxf(top[0], h.x), top[1] = fmaxf(top[1], h.y), top[2] = fmaxf(top[2], h.z), top[3] = fmaxf(top[3], h.w);
+      }
+      clear();
 #pragma unroll
-          for (int v = 0; v < kVecs; ++v) {
-            const float4 x = accs[w][v][lane];
-            acc[v][0] += x.x, acc[v][1] += x.y, acc[v][2] += x.z, acc[v][3] += x.w;
-          }
+      for (int w = 0; w < kJoinWarps; ++w) {
+        const float4 h = tops[w][lane], s = sums[w][lane];
+        const float of[4] = {h.x, h.y, h.z, h.w}, l[4] = {s.x, s.y, s.z, s.w};
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[j] = of[j] == top[j] ? 1.0f : exp2_approx(of[j] - top[j]);
+          sum[j] += l[j] * f[j];
+        }
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          const float4 x = accs[w][v][lane];
+          acc[v][0] += x.x * f[0];
+          acc[v][1] += x.y * f[1];
+          acc[v][2] += x.z * f[2];
+          acc[v][3] += x.w * f[3];
         }
       }
     }
-    if (!many || warp == 0) {
-      const int seq = at / items, kv = at % items / a.chunks, chunk = at % items % a.chunks, cols = min(16, a.group - chunk * 16);
-      __nv_bfloat16 *out = a.out + ((long long)seq * a.heads + kv * a.group + chunk * 16 + col0) * D + 32 * blockIdx.y;
-      const float scale = kFp8 ? c.v_scale[kv] : 1.0f;
+    const int cols = min(16, a.group - item.z * 16);
+    __nv_bfloat16 *out = a.out + ((long long)item.x * a.heads + item.y * a.group + item.z * 16 + col0) * D;
+    const float scale = kFp8 ? c.v_scale[item.y] : 1.0f;
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v)
+    for (int v = 0; v < kVecs; ++v)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col0 + j < cols) out[j * D + (v * 128 + lane * 4) / kCols] = __float2bfloat16_rn(acc[v][j] / sum[j] * scale);
-    }
+      for (int j = 0; j < 4; ++j)
+        if (col0 + j < cols) out[j * D + (vec + v * 32) * 4 / kCols] = __float2bfloat16_rn(acc[v][j] * __fdividef(scale, sum[j]));
   }
 }
 
@@ -869,35 +1000,60 @@ bool encode(CUtensorMap *map, char *base, const PagedCache &c, int size, int box
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+unsigned magic_of(int d) { return (unsigned)(((1ULL << 32) + d - 1) / d); }  // for divide(), which does not use it for 1
+
+// CTAs of the direct form's clusters, 0 for the list of tiles.
+int direct_splits(int seqs, int items, int most_tiles, int ctas) {
+  const long long pairs = (long long)seqs * items;
+  int splits = 1;
+  while (splits < kAttnClusterMost && splits * kAttnWarps * kDirectTiles < most_tiles && pairs * splits * 2 <= ctas) splits *= 2;
+  if (items > 65535 || seqs > 65535) return 0;
+  return (pairs * splits <= ctas || splits == 1) && most_tiles <= splits * kAttnWarps * kDirectMost ? splits : 0;
+}
+
 template <int D, bool kFp8, int kCols>
 cudaError_t launch(AttnArgs a, const PagedCache &c, int ctas, cudaStream_t stream) {
   using T = Tile<D, kFp8>;
   constexpr int kSmem = Layout<D, kFp8, kCols>::kTotal;
-  const auto kernel = paged_attention_kernel<D, kFp8, kCols>;
   int box = c.page_size & -c.page_size;
   if (box > T::kTokens) box = T::kTokens;
   a.box_shift = __builtin_ctz((unsigned)box);
-  a.per_stretches = 1.0 / (kAttnWarps * ctas);
-  a.per_items = 1.0 / (c.kv_heads * a.chunks);
+  a.stretches_magic = magic_of(kAttnWarps * ctas);
+  a.items_magic = magic_of(c.kv_heads * a.chunks);
   a.page_shift = (c.page_size & (c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)c.page_size) : -1;
   const int halves = box == T::kTokens ? T::kHalves : 1;
   CUtensorMap map_k, map_v;
   if (!encode(&map_k, c.k, c, T::kSize, box, halves) || !encode(&map_v, c.v, c, T::kSize, box, halves)) return cudaErrorInvalidValue;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(kAttnThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  const int items = c.kv_heads * a.chunks;
+  const int splits = direct_splits(a.seqs, items, (paged_capacity(c) + T::kTokens - 1) / T::kTokens, ctas);
+  if (splits > 0) {
+    const auto kernel = paged_attention_kernel<D, kFp8, kCols, true>;
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (err != cudaSuccess) return err;
+    a.stretch_shift = __builtin_ctz((unsigned)(splits * kAttnWarps));
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)splits;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    if (splits > 1) cfg.numAttrs = 2;
+    cfg.gridDim = dim3((unsigned)splits, (unsigned)items, (unsigned)a.seqs);
+    return cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, a, c);
+  }
+  const auto kernel = paged_attention_kernel<D, kFp8, kCols, false>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (err != cudaSuccess) return err;
+  cfg.gridDim = dim3((unsigned)ctas);
   err = cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, a, c);
   if (err != cudaSuccess) return err;
-  cfg.gridDim = dim3((unsigned)((ctas + kJoinWarps - 1) / kJoinWarps), D / 32);
+  cfg.gridDim = dim3((unsigned)((ctas + kJoinWarps - 1) / kJoinWarps), kJoinSlices);
   cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<D, kCols, kFp8>, a, c, ctas);
@@ -909,7 +1065,7 @@ int attn_ctas() { return 2 * attn_sm_count(); }
 
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
   const size_t cols = heads / kv_heads <= 8 ? 8 : 16, places = 2 * (size_t)attn_ctas();
-  return places * cols * (head_dim + 2) * sizeof(float) + places * sizeof(int);
+  return places * cols * (head_dim + 2) * sizeof(float);
 }
 
 cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head, int heads, const PagedCache &cache, bool fp8,
@@ -922,7 +1078,6 @@ cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head
   a.lengths = lengths;
   a.out = static_cast<__nv_bfloat16 *>(out);
   a.parts = static_cast<float *>(workspace);
-  a.splits = reinterpret_cast<int *>(a.parts + 2LL * ctas * cols * (d + 2));
   a.seqs = cache.seqs;
   a.heads = heads;
   a.group = group;
