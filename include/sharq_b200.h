@@ -408,7 +408,7 @@ int sharq_rope_append_paged(const void *qkv_bf16, int64_t row_stride, int rows, 
  * lengths[s] tokens of sequence s (the new one among them), query head h reading key/value head h / (heads / kv_heads).  q bf16 with
  * q_row / q_head elements between sequences / heads (multiples of 8), out bf16 [sequences, heads, head_dim].  A sequence of length 0 gives
  * zeros.  A length that is negative or more than the page table holds, or a page outside the cache, makes the rows of that sequence NaN and
- * stores 0x402 in *error_flag (may be NULL).  head_dim 64 or 128; heads a multiple of kv_heads.  workspace:
+ * stores 0x402 in *error_flag (may be NULL; 0x403: a wait ran out).  head_dim 64 or 128; heads a multiple of kv_heads.  workspace:
  * sharq_paged_attention_workspace_bytes(heads, kv_heads, head_dim) bytes of scratch, 16-byte aligned, not shared by calls that overlap. */
 size_t sharq_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
 int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int heads, const sharq_paged_cache *cache,
@@ -418,9 +418,9 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
 /* Product of m (1 to 16) unquantised bf16 rows (x_row elements between them, a multiple of 8) with a 4-bit weight:
  * y[m, n] = bf16(scale * scale_dev[0] * sum_k x[m, k] * W[n, k] + bias[n]), W = payload qw [n, k/2] times the dense scale factors sfw_dense, as
  * sharq_quantize_w32_shared and sharq_quantize_nvfp4 make them.  scale_dev (float on the device) and bias (bf16 [n]) may be NULL.  Float
- * sums, one rounding.  k % 64 == 0; x, qw and sfw_dense 16-byte aligned. */
+ * sums, one rounding.  k % 64 == 0; x, qw and sfw_dense 16-byte aligned.  A wait that ran out stores 0x404 in *error_flag (may be NULL). */
 int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, int k, const void *qw, const void *sfw_dense,
-                             const float *scale_dev, float scale, const void *bias_bf16, void *y_bf16, void *stream);
+                             const float *scale_dev, float scale, const void *bias_bf16, void *y_bf16, int *error_flag, void *stream);
 
 /* Test/tuning hook: how many SM clock cycles a cross-GPU wait of the all-reduce and transition
  * kernels may take before the kernel gives up, stores its error code and returns (0 restores the

@@ -814,14 +814,15 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
 }
 
 int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, int k, const void *qw, const void *sfw_dense,
-                             const float *scale_dev, float scale, const void *bias_bf16, void *y_bf16, void *stream) {
+                             const float *scale_dev, float scale, const void *bias_bf16, void *y_bf16, int *error_flag, void *stream) {
   SHARQ_REQUIRE(x_bf16 && qw && sfw_dense && y_bf16, "null buffer");
   SHARQ_REQUIRE(m >= 1 && m <= sharq::kWeightOnlyMaxRows, "weight_only_linear takes 1 to %d rows, got %d", sharq::kWeightOnlyMaxRows, m);
   SHARQ_REQUIRE(n > 0 && n <= 65535 * 128, "N must be in [1, %d], got %d", 65535 * 128, n);
   SHARQ_REQUIRE(k > 0 && k % 64 == 0, "weight_only_linear requires K to be a multiple of 64, got %d", k);
   SHARQ_REQUIRE(m == 1 || (x_row >= k && x_row % 8 == 0), "the rows of x must not overlap and be a multiple of 8 elements apart");
   SHARQ_REQUIRE(aligned16(x_bf16) && aligned16(qw) && aligned16(sfw_dense), "x, qw and sfw_dense must be 16-byte aligned");
-  return check_cuda(sharq::run_weight_only(x_bf16, x_row, m, n, k, qw, sfw_dense, scale_dev, scale, bias_bf16, y_bf16, as_stream(stream)),
+  return check_cuda(sharq::run_weight_only(x_bf16, x_row, m, n, k, qw, sfw_dense, scale_dev, scale, bias_bf16, y_bf16, error_flag,
+                                           as_stream(stream)),
                     "weight_only_linear");
 }
 

@@ -10,6 +10,7 @@ namespace sharq {
 constexpr int kBadCacheIndex = 0x402;  // error code: a position, length, sequence or page outside the cache or its tables
 
 constexpr int kAttentionTimeout = 0x403;  // error code: a wait for a copy ran out
+constexpr int kWeightOnlyTimeout = 0x404;
 
 // A position of a sequence in the cache; also what the kernels check before every access.
 struct PagedCache {
@@ -38,6 +39,6 @@ cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head
 // y[m, n] = bf16(scale * x . W^T + bias), m rows (1..16) of bf16 against a 4-bit weight with dense scale factors, k % 64 == 0.
 constexpr int kWeightOnlyMaxRows = 16;
 cudaError_t run_weight_only(const void *x, long long x_row, int m, int n, int k, const void *qw, const void *sf, const float *scale_dev,
-                            float scale, const void *bias, void *y, cudaStream_t stream);
+                            float scale, const void *bias, void *y, int *error_flag, cudaStream_t stream);
 
 }  // namespace sharq

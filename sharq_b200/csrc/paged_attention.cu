@@ -31,10 +31,10 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
-#include <mutex>
 
 #include "decode_ops.cuh"
 #include "sm100_ptx.cuh"
+#include "tensor_map.cuh"
 
 namespace sharq {
 
@@ -970,34 +970,15 @@ int attn_sm_count() {
   return sms[dev];
 }
 
-using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                              CUtensorMapFloatOOBfill);
-
-EncodeFn encode_fn() {
-  static EncodeFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void *ptr = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeFn>(ptr);
-  });
-  return fn;
-}
-
 // The cache as [page][head][half][token][bytes of a half], copied `box` tokens of one half or of all `halves` at a time.
 bool encode(CUtensorMap *map, char *base, const PagedCache &c, int size, int box, int halves) {
-  const EncodeFn fn = encode_fn();
-  if (fn == nullptr) return false;
   const cuuint64_t row = (cuuint64_t)c.head_dim * size, in_half = row < 128 ? row : 128;
   const cuuint64_t dims[5] = {in_half, (cuuint64_t)c.page_size, row / in_half, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
   // a dimension of one element is never stepped along
   const cuuint64_t strides[4] = {c.token_stride > 0 ? (cuuint64_t)c.token_stride : row, 128, c.head_stride > 0 ? (cuuint64_t)c.head_stride : row,
                                  c.page_stride > 0 ? (cuuint64_t)c.page_stride : row};
-  const cuuint32_t sizes[5] = {128, (cuuint32_t)box, (cuuint32_t)halves, 1, 1}, steps[5] = {1, 1, 1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, base, dims, strides, sizes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t sizes[5] = {128, (cuuint32_t)box, (cuuint32_t)halves, 1, 1};
+  return make_tensor_map(map, 5, base, dims, strides, sizes, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 unsigned magic_of(int d) { return (unsigned)(((1ULL << 32) + d - 1) / d); }  // for divide(), which does not use it for 1

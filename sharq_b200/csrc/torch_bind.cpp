@@ -521,7 +521,7 @@ Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_c
 }
 
 Tensor weight_only_linear(const Tensor &x, const Tensor &qw, const Tensor &sf, const std::optional<Tensor> &scale_t, double scale,
-                          const std::optional<Tensor> &bias, const std::optional<Tensor> &out) {
+                          const std::optional<Tensor> &bias, const std::optional<Tensor> &out, const Tensor &flag) {
   need(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1),
        "x must be a CUDA bfloat16 matrix with unit column stride");
   const at::Device dev = x.device();
@@ -542,7 +542,7 @@ Tensor weight_only_linear(const Tensor &x, const Tensor &qw, const Tensor &sf, c
   Tensor y = output(x, m, n, out);
   if (m == 0) return y;
   check(sharq_weight_only_linear(ptr(x), x.stride(0), (int)m, (int)n, (int)k, ptr(qw), ptr(sf), scale_dev, (float)scale,
-                                 bias ? ptr(*bias) : nullptr, ptr(y), stream_of(x)));
+                                 bias ? ptr(*bias) : nullptr, ptr(y), flag_of(flag), stream_of(x)));
   return y;
 }
 

@@ -4,44 +4,55 @@
 //
 // on the payload and the dense scale factors that a quantised linear holds.  Reading the weight (9/16 byte per element) is what it costs.
 // At that rate an SM gets some 42 elements per clock, so the instructions per element count: a pair of codes is one conversion to f16 (exact), its
-// scale one packed product (exact: 2 x 4 significant bits, between 2^-10 and 2688), and mma.sync.m16n8k16 with the 16 rows of weight as
-// the large operand does the rest, 1.3 instructions per element in all.  The k positions of an instruction may stand for any elements
-// as long as both operands agree, so lane (g, t) takes 32 neighbouring elements of a row, 16 bytes, straight from where it copied them.
+// scale one packed product (exact: 2 x 4 significant bits, between 2^-10 and 2688), and mma.sync.m16n8k16 with 16 rows of weight as
+// the large operand does the rest.  The k positions of an instruction may stand for any elements as long as both operands agree, so
+// lane (g, t) takes 32 neighbouring elements of a row, 16 bytes, straight from where it copied them.
 //
-// The activation goes to f16 as well, 128 elements of a row at a time, scaled by the power of two that takes their largest to [2^14, 2^15):
-// exact but for elements below 2^-39 of it.  Sums are float: the tensor core's over 128 elements, then one float accumulator.
-//
-// A CTA takes 128 rows of the weight (a tile of scale factors) and a stretch of K; its warps stream their parts through rings of their own
-// (cp.async).  Where the row tiles do not fill the GPU, K is dealt over the CTAs of a cluster of up to 8, whose float parts meet in
-// distributed shared memory and are summed in rank order: the same bits from call to call, no scratch and no second launch.
+// A warp keeps 256 elements of K of the activation in registers, as f16 operands, and streams that slice of the weight's rows past them, 16 rows at a
+// time, through a ring of its own (tensor-map copies; cp.async needs a pass of the load unit for every row of every copy, half of its time).  f16 is reached by scaling 128 elements of a row by
+// the power of two that takes their largest to [2^14, 2^15): exact but for elements below 2^-39 of it.  Sums are float.  A CTA's 16 warps cover
+// 4096 elements of K (or fewer, and several rows at a time), the CTAs of a cluster the rest; the clusters take equal shares of the rows.  The
+// warps' float sums of some rows meet in shared memory, those of CTAs in distributed shared memory, each added up in a fixed order: the same bits from
+// call to call, no scratch and no second launch.  (With tiles of 128 rows per CTA and the activation in shared memory, 323 instead of SOME
+// instructions per 16 rows x 256 and uneven shares: 28672 x 4096 with one row 19.8 us, with 16 rows 38.)
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "decode_ops.cuh"
 #include "sm100_ptx.cuh"
+#include "tensor_map.cuh"
 
 namespace sharq {
 
 namespace {
 
-constexpr int kWoWarps = 8;  // four of 32 rows each, times two over K
+constexpr int kWoWarps = 16;
 constexpr int kWoThreads = 32 * kWoWarps;
-constexpr int kWoStages = 4;
-constexpr int kWoStage = 5 * 512;  // 128 elements of 32 rows and their scale factors, 16 bytes per lane and piece
-constexpr int kWoXBytes = 24576;
-constexpr int kWoPitch = 132;  // floats between the columns of a float part [columns][128 rows]
-constexpr int kWoXScales = 96 * 8;  // one per block of 128 elements and column: at most 96 blocks of one row at a time
-constexpr int kWoSmem = kWoWarps * kWoStages * kWoStage + kWoXBytes + kWoXScales * 4;
+constexpr int kWoSlice = 256;               // elements of K of a warp
+constexpr int kWoStages = 2;
+constexpr int kWoCodes = 32 * 128, kWoScales = 4 * 128;  // 32 rows x 256 codes; 8 rows x 16 bytes of scale factors for each of 4 x 64 elements
+constexpr int kWoRing = kWoStages * (kWoCodes + kWoScales);
+constexpr int kWoParts = 70144;             // bytes for the warps' float sums: of all of a CTA's tiles, or of two chunks of them
+constexpr int kWoSums = 6144;               // for a CTA's float sums of a chunk, twice
+constexpr int kWoXWarp = 8 * 512;            // of a warp's slice of 8 rows on its way to the registers
+constexpr int kWoClusterMost = 8;
+constexpr int kWoFactors = kWoWarps * kWoRing + kWoParts + 2 * kWoSums;
+constexpr int kWoBars = kWoFactors + kWoWarps * 64;  // the barriers behind it all, and the flag of a wait that ran out
+constexpr int kWoSmem = kWoBars + kWoWarps * kWoStages * 8 + 8;
+static_assert(kWoSmem <= 232448 && kWoWarps * kWoXWarp <= kWoParts, "what a CTA can have");
 
-__device__ __forceinline__ void wo_cp_async16(uint32_t smem, const void *gmem, bool valid) {
-  const int bytes = valid ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ uint4 wo_lds16(uint32_t smem) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint16_t wo_lds2(uint32_t smem) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(smem) : "memory");
   return v;
 }
 // eight e2m1 codes -> four pairs of f16
@@ -57,14 +68,19 @@ __device__ __forceinline__ void e2m1_to_f16(uint32_t w, uint32_t (&h)[4]) {
       : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
       : "r"(w));
 }
-__device__ __forceinline__ uint32_t e4m3x2_to_f16(uint32_t w) {
+__device__ __forceinline__ __half2 e4m3x2_to_f16(uint16_t w) {
   uint32_t r;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
-  return r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(w));
+  return *reinterpret_cast<const __half2 *>(&r);
 }
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, __half2 b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), b);
   return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ void mma_f16_from0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -76,197 +92,306 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float f) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// a float of CTA `rank`'s shared memory (addr: this CTA's address of the same variable); not volatile, so that loads go out together
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, int rank) {
+  uint32_t remote;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
+  return v;
+}
+
+__device__ __forceinline__ void copy_2d(uint32_t dst, const CUtensorMap *m, int c0, int c1, uint64_t *bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(m),
+               "r"(ptx::smem_u32(bar)), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void copy_3d(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, uint64_t *bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(m),
+               "r"(ptx::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+
 struct WeightOnlyArgs {
   const __nv_bfloat16 *x;
   long long x_row;
-  const unsigned char *qw, *sf;
+  int *error_flag;
   const float *scale_dev;
   const __nv_bfloat16 *bias;
   __nv_bfloat16 *y;
   float scale;
-  int m, n, k, splits;
+  int m, n, k;
+  int slices;       // warps of a CTA along K
+  int row_groups;   // warps of a CTA along the rows
+  int passes;       // times that a cluster goes along K for all of it
+  int cluster;      // CTAs
+  int tiles;        // of 16 rows, of the whole weight
+  int per_cluster;  // tiles
+  int chunk;        // tiles whose sums are joined at a time
+  int parts_at, parts_bytes;  // of the space of kWoParts bytes, for the warps' sums; they are all of it unless the activation is read more than once
+  unsigned per_tile_magic[2]; // ceil(2^32 / (16 rows)) of the first and second eight rows
 };
 
-// kTiles: 8-row tiles of the activation (1 or 2).  blockIdx.x: stretch of K, rank in the cluster; blockIdx.y: 128 rows of the weight.
-template <int kTiles>
-__global__ void __launch_bounds__(kWoThreads, 2) weight_only_kernel(WeightOnlyArgs a) {
-  extern __shared__ __align__(128) unsigned char smem[];
-  ptx::grid_launch_dependents();
-  ptx::grid_dependency_wait();
+// Tile j: rows 32 i + 8 c + g of a block of 128, i = 2 h and 2 h + 1, with c = j / 2 % 4 and h = j % 2: the scale factors of a pair of tiles, for
+// 64 elements of K, are 16 neighbouring bytes per g.  Pairs are copied together; a share of the rows may begin or end within one.
+__device__ __forceinline__ int tile_row(int j) { return (j >> 3) * 128 + (j & 1) * 64 + ((j >> 1) & 3) * 8; }
+
+// blockIdx.x: CTA of the cluster, blockIdx.y: cluster, blockIdx.z: eight rows of the activation.
+__global__ void __launch_bounds__(kWoThreads, 1)
+    weight_only_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_sf, const __grid_constant__ WeightOnlyArgs a) {
+  extern __shared__ __align__(1024) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int row_warp = warp & 3, k_warp = warp >> 2;
-  const uint32_t ring = ptx::smem_u32(smem) + warp * kWoStages * kWoStage + lane * 16;
-  unsigned char *xs = smem + kWoWarps * kWoStages * kWoStage;
-  float *x_scale = reinterpret_cast<float *>(xs + kWoXBytes);
-  const uint32_t xs_addr = ptx::smem_u32(xs);
+  const int row_first = blockIdx.z * 8, m = min(8, a.m - row_first);
+  const uint32_t codes = ptx::smem_u32(smem) + warp * kWoStages * kWoCodes;  // on 1024 bytes, for the swizzle
+  const uint32_t scales = ptx::smem_u32(smem) + kWoWarps * kWoStages * kWoCodes + warp * kWoStages * kWoScales;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kWoBars) + warp * kWoStages;
+  volatile int *gave_up = reinterpret_cast<volatile int *>(smem + kWoBars + kWoWarps * kWoStages * 8);
+  if (threadIdx.x == 0) *gave_up = 0;
+  if (lane == 0) {
+    for (int i = 0; i < kWoStages; ++i) ptx::mbar_init(bars + i, 1);
+    ptx::fence_barrier_init();
+    ptx::tma_prefetch_desc(&map_w);
+    ptx::tma_prefetch_desc(&map_sf);
+  }
+  unsigned char *space = smem + kWoWarps * kWoRing;
+  float *parts = reinterpret_cast<float *>(space + a.parts_at), *sums = reinterpret_cast<float *>(space + kWoParts);
+  int row_group = 0, slice_in = warp;
+  while (slice_in >= a.slices) slice_in -= a.slices, ++row_group;
+  const bool works = row_group < a.row_groups;
+  const int j0 = blockIdx.y * a.per_cluster, j1 = min(j0 + a.per_cluster, a.tiles);
+  const int k_first = (blockIdx.x * a.slices + slice_in) * kWoSlice, k_pass = a.cluster * a.slices * kWoSlice;
 
-  // this CTA's blocks of 128 elements of K
-  const int blocks = (a.k + 127) / 128;
-  const int b0 = (int)((long long)blocks * blockIdx.x / a.splits), b1 = (int)((long long)blocks * (blockIdx.x + 1) / a.splits);
+  // The pairs of this warp in order: those of its row group, pass by pass within a chunk of tiles whose sums are joined together.
+  int l_chunk = j0, l_pass = 0, l_pair = (j0 >> 1) + row_group, l_end = min(j0 + a.chunk, j1), put = 0, k0 = k_first;
+  if (!works || 2 * l_pair >= l_end) l_chunk = j1;  // fewer pairs than row groups
+  __syncthreads();
+  const bool chosen = ptx::elect_one();
+  if (l_chunk < j1 && chosen) {
+    // the first rows into L2, where they may be as old as they like: ahead of the wait for the kernels before
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) ptx::tma_prefetch_l2_2d(&map_w, k0 / 2, tile_row(2 * l_pair) + 32 * i);
+  }
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
 
-  // rows 32 i + 8 row_warp + g of the tile, i = 0..3: their scale factors for 64 elements are 16 neighbouring bytes
-  const int row0 = blockIdx.y * 128 + 8 * row_warp + g;
-  const long long row_bytes = a.k / 2;
-  const unsigned char *w0 = a.qw + row0 * row_bytes + t * 16;
-  const unsigned char *s0 = a.sf + (long long)blockIdx.y * (a.k / 64) * 512 + (t >> 1) * 512 + (8 * row_warp + g) * 16;
-  int next = b0 + k_warp, put = 0;
   auto load = [&]() {
-    if (next < b1) {
-      const uint32_t to = ring + put * kWoStage;
-      const bool in_k = next * 128 + 32 * t < a.k;  // K may end in the middle of a block
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool valid = in_k && row0 + 32 * i < a.n;
-        wo_cp_async16(to + i * 512, valid ? w0 + 32 * i * row_bytes + next * 64LL : a.qw, valid);
+    if (l_chunk < j1) {
+      if (chosen) {
+        // rows and elements that are not there come as zeros
+        const int from = 2 * l_pair < l_chunk ? 2 : 0, to = 2 * l_pair + 1 < l_end ? 4 : 2, row = tile_row(2 * l_pair);
+        ptx::mbar_arrive_expect_tx(bars + put, (to - from) * 1024 + kWoScales);
+        for (int i = from; i < to; ++i) copy_2d(codes + put * kWoCodes + i * 1024, &map_w, k0 / 2, row + 32 * i, bars + put);
+        copy_3d(scales + put * kWoScales, &map_sf, (l_pair & 3) * 128, k0 / 64, l_pair >> 2, bars + put);
       }
-      wo_cp_async16(to + 4 * 512, in_k ? s0 + next * 1024LL : a.sf, in_k);
-      next += 2;
+      l_pair += a.row_groups;
+      if (2 * l_pair >= l_end) {
+        if (++l_pass == a.passes) {
+          l_pass = 0;
+          l_chunk += a.chunk;
+          l_end = min(l_chunk + a.chunk, j1);
+          while (l_chunk < j1 && 2 * ((l_chunk >> 1) + row_group) >= l_end) {  // no pair of this row group in the chunk
+            l_chunk += a.chunk;
+            l_end = min(l_chunk + a.chunk, j1);
+          }
+        }
+        l_pair = (l_chunk >> 1) + row_group;
+        k0 = k_first + l_pass * k_pass;
+      }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    put = put + 1 == kWoStages ? 0 : put + 1;
+    put ^= 1;
   };
-  for (int i = 0; i < kWoStages - 1; ++i) load();
+  static_assert(kWoStages == 2, "stages in turn");
 
-  float acc[2][kTiles][4];
+  // the weight's scale goes into the factors of the activation's blocks, so that a sum is in the result's range on its way
+  const float scale_of = a.scale_dev != nullptr ? *a.scale_dev : 1.0f;
+  uint4 x[2][4];
+  // The slice's 512 bytes of a row, 16 per lane; as f16 through shared memory to the lanes that multiply them.  Piece c of row r lies at
+  // c ^ (c / 8 % 2 + 2 (r % 2)): the four pieces of eight lanes that read at once are in different banks.
+  unsigned char *x_space = space + warp * kWoXWarp;
+  float *factors = reinterpret_cast<float *>(smem + kWoFactors) + warp * 16;  // [block of 128 elements][column]: what its sum is multiplied by
+  uint4 raw[2][4];  // of eight rows at a time
+  auto load_x = [&](int from_k) {
+    const bool in_k = works && from_k + lane * 8 < a.k;
+    const __nv_bfloat16 *from = a.x + row_first * a.x_row + from_k + lane * 8;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int half = 0; half < 2; ++half) {
+      if (4 * half >= m) break;
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
-  // the weight's scale goes into the blocks' factors, so that a sum is in the result's range on its way
-  const float scale = a.scale_dev != nullptr ? *a.scale_dev * a.scale : a.scale;
-  const int room = min(96, kWoXBytes / (256 * a.m)) & ~1;  // blocks of the activation that are held at a time
-  int take = 0;
-  for (int c0 = b0; c0 < b1; c0 += room) {
-    const int c1 = min(b1, c0 + room);
-    if (c0 != b0) __syncthreads();
-    // the activation's blocks as f16, in the order in which lanes read them: [block][word of a lane's 16 bytes][row][t], 16 bytes each
-    const int half_warp = threadIdx.x >> 4, sub = threadIdx.x & 15;
-    for (int i = half_warp; i < (c1 - c0) * a.m; i += kWoThreads / 16) {
-      const int block = i / a.m, row = i % a.m, e0 = (c0 + block) * 128 + sub * 8;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (e0 < a.k) v = *reinterpret_cast<const uint4 *>(a.x + row * a.x_row + e0);
-      uint32_t top = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
-      top = max(top & 0xFFFFu, top >> 16);
-      const unsigned mask = 0xFFFFu << (threadIdx.x & 16);
-#pragma unroll
-      for (int off = 8; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(mask, top, off));
-      // a block with infinities or NaN is scaled down, so that nothing finite joins them
-      const int e = (int)(top >> 7), shift = e == 255 ? -120 : min(126, 141 - max(e, 1));
-      const float f = __int_as_float((127 + shift) << 23);
-      v = make_uint4(scaled_pair(v.x, f), scaled_pair(v.y, f), scaled_pair(v.z, f), scaled_pair(v.w, f));
-      *reinterpret_cast<uint4 *>(xs + (((block * 4 + (sub & 3)) * a.m + row) * 4 + (sub >> 2)) * 16) = v;
-      if (sub == 0) x_scale[block * 8 * kTiles + row] = __int_as_float((127 - shift) << 23) * scale;
-    }
-    __syncthreads();
-
-    for (int block = c0 + k_warp; block < c1; block += 2) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kWoStages - 2) : "memory");
-      const uint32_t from = ring + take * kWoStage;
-      uint4 w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = wo_lds16(from + i * 512);
-      const uint4 sf = wo_lds16(from + 4 * 512);
-      take = take + 1 == kWoStages ? 0 : take + 1;
-      load();
-      const uint32_t sw[4] = {sf.x, sf.y, sf.z, sf.w};
-      uint32_t s[4][2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t two = e4m3x2_to_f16(sw[i] >> ((t & 1) * 16));
-        s[i][0] = __byte_perm(two, two, 0x1010);
-        s[i][1] = __byte_perm(two, two, 0x3232);
+      for (int r = 0; r < 4; ++r) {
+        raw[half][r] = make_uint4(0, 0, 0, 0);
+        if (4 * half + r < m && in_k) raw[half][r] = *reinterpret_cast<const uint4 *>(from);
+        from += a.x_row;
       }
-      float d[2][kTiles][4];
+    }
+  };
+  auto convert_x = [&]() {
+    const float scale = scale_of * a.scale;
+    __syncwarp();  // the space is free
+    // rows are converted four at a time, since each is a chain of exchanges, or one or two
+    auto rows = [&](auto count, int half) {
+      constexpr int kRows = decltype(count)::value;
+      uint32_t top[kRows];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int r = 0; r < kRows; ++r) {
+        const uint4 v = raw[half][r];
+        top[r] = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+        top[r] = max(top[r] & 0xFFFFu, top[r] >> 16);
+      }
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n)
+      for (int off = 8; off > 0; off >>= 1)  // over the 16 lanes of 128 elements
 #pragma unroll
-          for (int j = 0; j < 4; ++j) d[i][n][j] = 0.0f;
+        for (int r = 0; r < kRows; ++r) top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], off));
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const uint4 v = raw[half][r];
+        const int row = 4 * half + r;
+        // a block with infinities or NaN is scaled down, so that nothing finite joins them
+        const int e = (int)(top[r] >> 7), shift = e == 255 ? -120 : min(126, 141 - max(e, 1));
+        const float f = __int_as_float((127 + shift) << 23);
+        *reinterpret_cast<uint4 *>(x_space + row * 512 + (lane ^ (((lane >> 3) & 1) | ((r & 1) << 1))) * 16) =
+            make_uint4(scaled_pair(v.x, f), scaled_pair(v.y, f), scaled_pair(v.z, f), scaled_pair(v.w, f));
+        if ((lane & 15) == 0) factors[(lane >> 4) * 8 + row] = __int_as_float((127 - shift) << 23) * scale;
+      }
+    };
+    if (m == 1) {
+      rows(std::integral_constant<int, 1>(), 0);
+    } else if (m == 2) {
+      rows(std::integral_constant<int, 2>(), 0);
+    } else {
+      rows(std::integral_constant<int, 4>(), 0);
+      if (m > 4) rows(std::integral_constant<int, 4>(), 1);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        uint4 x[kTiles];
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) {
-          x[n] = make_uint4(0, 0, 0, 0);
-          if (8 * n + g < a.m) x[n] = wo_lds16(xs_addr + ((((block - c0) * 4 + q) * a.m + 8 * n + g) * 4 + t) * 16);
-        }
-        uint32_t h[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e2m1_to_f16(q == 0 ? w[i].x : q == 1 ? w[i].y : q == 2 ? w[i].z : w[i].w, h[i]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) h[i][j] = mul_f16x2(h[i][j], s[i][q >> 1]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n) {
-            mma_f16(d[i][n], h[2 * i][0], h[2 * i + 1][0], h[2 * i][1], h[2 * i + 1][1], x[n].x, x[n].y);
-            mma_f16(d[i][n], h[2 * i][2], h[2 * i + 1][2], h[2 * i][3], h[2 * i + 1][3], x[n].z, x[n].w);
-          }
+        const int c = b * 16 + t * 4 + q;
+        x[b][q] = make_uint4(0, 0, 0, 0);
+        if (g < m) x[b][q] = *reinterpret_cast<const uint4 *>(x_space + g * 512 + (c ^ ((t >> 1) | ((g & 1) << 1))) * 16);
       }
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n) {
-        // columns behind the activation's last row: their products are 0, and their scales are not there
-        const float f0 = 8 * n + 2 * t < a.m ? x_scale[(block - c0) * 8 * kTiles + 8 * n + 2 * t] : 0.0f;
-        const float f1 = 8 * n + 2 * t + 1 < a.m ? x_scale[(block - c0) * 8 * kTiles + 8 * n + 2 * t + 1] : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          acc[i][n][0] += d[i][n][0] * f0;
-          acc[i][n][1] += d[i][n][1] * f1;
-          acc[i][n][2] += d[i][n][2] * f0;
-          acc[i][n][3] += d[i][n][3] * f1;
-        }
-      }
-    }
-  }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+  };
 
-  // float parts [k_warp][column][row of the tile] over the activation's space, then the sum over the cluster's CTAs and their k_warps
-  __syncthreads();
-  float *part = reinterpret_cast<float *>(xs);
+  // the activation ahead of the weight: behind the first tiles of all SMs it took 5600 cycles to arrive
+  if (a.passes == 1) load_x(k_first);
+#pragma unroll 1
+  for (int i = 0; i < kWoStages; ++i) load();
+  if (a.passes == 1) {
+    convert_x();
+    __syncthreads();  // the warps' sums take the activation's space
+  }
+
+  // lane (g, t) takes row (g >> 1) + 4 (g & 1) of eight, so that what eight lanes read at once lies in different banks
+  const int my_row = (g >> 1) | ((g & 1) << 2);
+  // (the second 128 elements' codes lie at the same offset ^ 64)
+  const uint32_t my_codes = codes + my_row * 128 + ((t ^ my_row) << 4), my_codes2 = my_codes ^ 64;
+  const uint32_t my_scales = scales + my_row * 16 + (t >> 1) * 128 + (t & 1) * 2;
+  const int per_tile = 16 * m;
+  const bool col0 = 2 * t < m, col1 = 2 * t + 1 < m;
+  int take = 0, flip = 0;
+  unsigned phases = 0;
+  for (int chunk = j0; chunk < j1; chunk += a.chunk, flip ^= 1) {
+    const int end = min(chunk + a.chunk, j1);
+    float *part = parts + flip * (a.parts_bytes / 8);
+    for (int pass = 0; pass < a.passes; ++pass) {
+      if (a.passes > 1) {
+        load_x(k_first + pass * k_pass);
+        convert_x();
+      }
+      if (!works) continue;
+      for (int pair = (chunk >> 1) + row_group; 2 * pair < end; pair += a.row_groups) {
+        if (!ptx::mbar_wait(bars + take, (phases >> take) & 1, gave_up)) {
+          *gave_up = 1;
+          if (a.error_flag != nullptr) atomicExch(a.error_flag, kWeightOnlyTimeout);
+        }
+        __syncwarp();
+        phases ^= 1u << take;
+#pragma unroll 1
+        for (int half = 2 * pair < chunk ? 1 : 0; half < (2 * pair + 1 < end ? 2 : 1); ++half) {
+          const uint32_t at = take * kWoCodes + half * 2048, from_sf = my_scales + take * kWoScales + half * 8;
+          float acc[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t from = (b == 0 ? my_codes : my_codes2) + at;
+            const uint4 w0 = wo_lds16(from), w1 = wo_lds16(from + 1024);
+            // the scale factors of this lane's two groups of 16 elements, of both rows
+            const __half2 s0 = e4m3x2_to_f16(wo_lds2(from_sf + b * 256)), s1 = e4m3x2_to_f16(wo_lds2(from_sf + b * 256 + 4));
+            float d[4];
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n)
+            for (int q = 0; q < 4; ++q) {
+              uint32_t h0[4], h1[4];
+              e2m1_to_f16(q == 0 ? w0.x : q == 1 ? w0.y : q == 2 ? w0.z : w0.w, h0);
+              e2m1_to_f16(q == 0 ? w1.x : q == 1 ? w1.y : q == 2 ? w1.z : w1.w, h1);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        part[(k_warp * 8 * kTiles + 8 * n + 2 * t + (j & 1)) * kWoPitch + 32 * (2 * i + (j >> 1)) + 8 * row_warp + g] = acc[i][n][j];
-  if (a.splits > 1)
-    ptx::cluster_sync();
-  else
-    __syncthreads();
-  const int rank = a.splits > 1 ? (int)ptx::cluster_ctarank() : 0;
-  for (int i = rank * kWoThreads + threadIdx.x; i < 128 * a.m; i += a.splits * kWoThreads) {
-    const int col = i >> 7, r = i & 127, row = blockIdx.y * 128 + r;
-    float sum = 0.0f;
-    for (int c = 0; c < a.splits; ++c) {
+              for (int c = 0; c < 4; ++c) {
+                h0[c] = mul_f16x2(h0[c], q < 2 ? __low2half2(s0) : __high2half2(s0));
+                h1[c] = mul_f16x2(h1[c], q < 2 ? __low2half2(s1) : __high2half2(s1));
+              }
+              if (q == 0)
+                mma_f16_from0(d, h0[0], h1[0], h0[1], h1[1], x[b][q].x, x[b][q].y);
+              else
+                mma_f16(d, h0[0], h1[0], h0[1], h1[1], x[b][q].x, x[b][q].y);
+              mma_f16(d, h0[2], h1[2], h0[3], h1[3], x[b][q].z, x[b][q].w);
+            }
+            const float2 f = *reinterpret_cast<const float2 *>(factors + b * 8 + 2 * t);
 #pragma unroll
-      for (int kw = 0; kw < 2; ++kw) {
-        float *from = part + (kw * 8 * kTiles + col) * kWoPitch + r;
-        float v;
-        if (a.splits > 1)
-          asm volatile(
-              "{\n\t.reg .b32 remote;\n\tmapa.shared::cluster.u32 remote, %1, %2;\n\tld.shared::cluster.f32 %0, [remote];\n\t}"
-              : "=f"(v)
-              : "r"(ptx::smem_u32(from)), "r"(c)
-              : "memory");
-        else
-          v = *from;
-        sum += v;
+            for (int c = 0; c < 4; ++c) acc[c] = b == 0 ? d[c] * (c & 1 ? f.y : f.x) : fmaf(d[c], c & 1 ? f.y : f.x, acc[c]);
+          }
+          // [tile][slice][column][row of the tile]
+          float *to = part + ((2 * pair + half - chunk) * a.slices + slice_in) * per_tile + 32 * t + my_row;
+          if (pass > 0) {
+            if (col0) acc[0] += to[0], acc[2] += to[8];
+            if (col1) acc[1] += to[16], acc[3] += to[24];
+          }
+          if (col0) to[0] = acc[0], to[8] = acc[2];
+          if (col1) to[16] = acc[1], to[24] = acc[3];
+        }
+        take ^= 1;
+        __syncwarp();  // the stage is free
+        load();
       }
     }
-    if (row < a.n) {
-      float y = sum;
-      if (a.bias != nullptr) y += __bfloat162float(a.bias[row]);
-      a.y[(long long)col * a.n + row] = __float2bfloat16_rn(y);
+    __syncthreads();
+    const int count = (end - chunk) * per_tile;
+    float *sum_of = sums + flip * (kWoSums / 4);
+    const unsigned magic = a.per_tile_magic[blockIdx.z];
+    auto finish = [&](int i, float y) {
+      const int tile = (int)__umulhi((unsigned)i, magic), rest = i - tile * per_tile, col = row_first + (rest >> 4), r = rest & 15;
+      const int row = tile_row(chunk + tile) + (r >> 3) * 32 + (r & 7);
+      if (row < a.n) {
+        if (a.bias != nullptr) y += __bfloat162float(a.bias[row]);
+        a.y[(long long)col * a.n + row] = __float2bfloat16_rn(y);
+      }
+    };
+    for (int i = threadIdx.x; i < count; i += kWoThreads) {
+      const int tile = (int)__umulhi((unsigned)i, magic), rest = i - tile * per_tile;
+      const float *from = part + tile * a.slices * per_tile + rest;
+      float v[kWoWarps], y = 0.0f;  // all loads, then the sum
+#pragma unroll
+      for (int s = 0; s < kWoWarps; ++s) v[s] = s < a.slices ? from[s * per_tile] : 0.0f;
+#pragma unroll
+      for (int s = 0; s < kWoWarps; ++s) y += v[s];
+      if (a.cluster == 1)
+        finish(i, y);
+      else
+        sum_of[i] = y;
+    }
+    if (a.cluster > 1) {
+      __syncwarp();
+      ptx::cluster_sync();
+      for (int i = blockIdx.x * kWoThreads + threadIdx.x; i < count; i += a.cluster * kWoThreads) {
+        float v[kWoClusterMost], y = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kWoClusterMost; ++r) v[r] = r < a.cluster ? ld_cluster_f32(ptx::smem_u32(sum_of + i), r) : 0.0f;
+#pragma unroll
+        for (int r = 0; r < kWoClusterMost; ++r) y += v[r];
+        finish(i, y);
+      }
     }
   }
   __syncwarp();
-  if (a.splits > 1) ptx::cluster_sync();  // a CTA's memory is read until here
+  if (a.cluster > 1) ptx::cluster_sync();  // a CTA's memory is read until here
 }
 
 int wo_sm_count() {
@@ -277,22 +402,47 @@ int wo_sm_count() {
   return sms[dev];
 }
 
+// Clusters of `size` CTAs that run at once, one CTA per SM: fewer than SMs / size, since a cluster lies within a GPC.
+template <typename Kernel>
+cudaError_t wo_clusters(Kernel kernel, int size, int *clusters) {
+  static int known[64][kWoClusterMost + 1] = {};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (size == 1 || dev < 0 || dev >= 64) {
+    *clusters = wo_sm_count() / size;
+    return cudaSuccess;
+  }
+  int &of = known[dev][size];
+  if (of == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)size);
+    cfg.blockDim = dim3(kWoThreads);
+    cfg.dynamicSmemBytes = kWoSmem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    err = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (err != cudaSuccess) return err;
+    of = n > 0 ? n : 1;
+  }
+  *clusters = of;
+  return cudaSuccess;
+}
+
 }  // namespace
 
 cudaError_t run_weight_only(const void *x, long long x_row, int m, int n, int k, const void *qw, const void *sf, const float *scale_dev,
-                            float scale, const void *bias, void *y, cudaStream_t stream) {
+                            float scale, const void *bias, void *y, int *error_flag, cudaStream_t stream) {
   if (m < 1 || m > kWeightOnlyMaxRows || n < 1 || k < 64 || k % 64 != 0) return cudaErrorInvalidValue;
-  const int tiles = (n + 127) / 128, blocks = (k + 127) / 128;
-  if (tiles > 65535) return cudaErrorInvalidValue;
-  int splits = 2 * wo_sm_count() / tiles;
-  if (splits > 8) splits = 8;
-  if (splits > blocks / 2) splits = blocks / 2;
-  if (splits < 1) splits = 1;
   WeightOnlyArgs a;
   a.x = static_cast<const __nv_bfloat16 *>(x);
   a.x_row = x_row;
-  a.qw = static_cast<const unsigned char *>(qw);
-  a.sf = static_cast<const unsigned char *>(sf);
+  a.error_flag = error_flag;
   a.scale_dev = scale_dev;
   a.scale = scale;
   a.bias = static_cast<const __nv_bfloat16 *>(bias);
@@ -300,25 +450,62 @@ cudaError_t run_weight_only(const void *x, long long x_row, int m, int n, int k,
   a.m = m;
   a.n = n;
   a.k = k;
-  a.splits = splits;
-  const auto kernel = m <= 8 ? weight_only_kernel<1> : weight_only_kernel<2>;
+  const int slices = (k - 1) / kWoSlice + 1;
+  a.cluster = (slices + kWoWarps - 1) / kWoWarps;
+  if (a.cluster > kWoClusterMost) a.cluster = kWoClusterMost;
+  a.passes = (slices + a.cluster * kWoWarps - 1) / (a.cluster * kWoWarps);
+  while (a.passes > 1 && (slices + a.cluster * a.passes - 1) / (a.cluster * a.passes) * (m > 8 ? 8 : m) * 64 * 2 > kWoParts - kWoWarps * kWoXWarp) ++a.passes;
+  a.slices = (slices + a.cluster * a.passes - 1) / (a.cluster * a.passes);
+  a.row_groups = kWoWarps / a.slices;
+  const int left = n % 128;  // a last block of few rows has empty tiles at its end
+  a.tiles = n / 128 * 8 + (left == 0 ? 0 : left > 64 ? 8 : left >= 32 ? 7 : 2 * ((left + 7) / 8) - 1);
+  const auto kernel = weight_only_kernel;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWoSmem);
   if (err != cudaSuccess) return err;
+  int clusters = 0;
+  err = wo_clusters(kernel, a.cluster, &clusters);
+  if (err != cudaSuccess) return err;
+  // more than eight rows: half of the clusters for each eight, side by side, so that the second to read a row of the weight finds it in L2
+  const int eights = m > 8 ? 2 : 1, rows = m > 8 ? 8 : m;
+  clusters = clusters / eights > 0 ? clusters / eights : 1;
+  a.per_cluster = (a.tiles + clusters - 1) / clusters;
+  a.parts_at = a.passes == 1 ? 0 : kWoWarps * kWoXWarp;
+  a.parts_bytes = (kWoParts - a.parts_at) & ~7;
+  // all tiles at once, or half of the space at a time; at most as many as the sums of a cluster's CTAs have room for
+  const int tile_bytes = a.slices * rows * 64, room = a.parts_bytes / 2 / tile_bytes;
+  a.chunk = a.per_cluster * tile_bytes <= a.parts_bytes ? a.per_cluster : room;
+  if (a.cluster > 1 && a.chunk > kWoSums / (rows * 64)) a.chunk = kWoSums / (rows * 64) < room ? kWoSums / (rows * 64) : room;
+  if (a.chunk < 1) return cudaErrorInvalidValue;
+  for (int i = 0; i < eights; ++i) {
+    const int per_tile = 16 * (i == 0 ? rows : m - 8);
+    a.per_tile_magic[i] = (unsigned)(((1ULL << 32) + per_tile - 1) / per_tile);
+  }
+  if (a.chunk < a.row_groups && a.row_groups > 1) a.row_groups = a.chunk;
+  const int used = (a.tiles + a.per_cluster - 1) / a.per_cluster;
+  // codes: 8 rows x 128 bytes at a time; scale factors: blocks of 128 rows, tiles of 64 elements, 8 rows x 16 bytes of 4 tiles at a time
+  CUtensorMap map_w, map_sf;
+  const cuuint64_t w_dims[2] = {(cuuint64_t)k / 2, (cuuint64_t)n}, w_strides[1] = {(cuuint64_t)k / 2};
+  const cuuint32_t w_box[2] = {128, 8};
+  const cuuint64_t sf_dims[3] = {512, (cuuint64_t)k / 64, ((cuuint64_t)n + 127) / 128}, sf_strides[2] = {512, (cuuint64_t)k / 64 * 512};
+  const cuuint32_t sf_box[3] = {128, 4, 1};
+  if (!make_tensor_map(&map_w, 2, qw, w_dims, w_strides, w_box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tensor_map(&map_sf, 3, sf, sf_dims, sf_strides, sf_box, CU_TENSOR_MAP_SWIZZLE_NONE))
+    return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)splits;
+  attr[1].val.clusterDim.x = (unsigned)a.cluster;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)splits, (unsigned)tiles);
+  cfg.gridDim = dim3((unsigned)a.cluster, (unsigned)used, (unsigned)eights);
   cfg.blockDim = dim3(kWoThreads);
   cfg.dynamicSmemBytes = kWoSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = splits > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  cfg.numAttrs = a.cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, map_w, map_sf, a);
 }
 
 }  // namespace sharq

@@ -30,7 +30,7 @@ _NO_FLAG = torch.zeros(1, dtype=torch.int32, device="cpu")
 _PREPARE_TIMEOUTS_SEEN = 0
 _BAD_EXPERT = 0x401  # kPlanBadExpert of csrc/decoder_ops.cu
 _BAD_CACHE_INDEX = 0x402  # kBadCacheIndex of csrc/decode_ops.cuh
-_ATTENTION_TIMEOUT = 0x403  # kAttentionTimeout of csrc/decode_ops.cuh
+_ATTENTION_TIMEOUT, _WEIGHT_ONLY_TIMEOUT = 0x403, 0x404  # kAttentionTimeout, kWeightOnlyTimeout of csrc/decode_ops.cuh
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -79,8 +79,9 @@ def check_device_errors(device=None) -> None:
             if code == _BAD_CACHE_INDEX:
                 raise RuntimeError("sharq_b200 paged cache: a position, length, sequence or page was outside the cache or its tables "
                                    f"on cuda:{idx}")
-            if code == _ATTENTION_TIMEOUT:
-                raise RuntimeError(f"sharq_b200 paged_attention: a wait for a copy ran out on cuda:{idx}; outputs are undefined")
+            if code in (_ATTENTION_TIMEOUT, _WEIGHT_ONLY_TIMEOUT):
+                name = "paged_attention" if code == _ATTENTION_TIMEOUT else "weight_only_linear"
+                raise RuntimeError(f"sharq_b200 {name}: a wait for a copy ran out on cuda:{idx}; outputs are undefined")
             raise RuntimeError(f"sharq_b200 GEMM kernel reported a timed-out wait (code {code}) on cuda:{idx}")
 
 
@@ -553,7 +554,8 @@ def weight_only_linear(x: torch.Tensor, qw: torch.Tensor, sfw_dense: torch.Tenso
     1-element CUDA float32 tensor.  float32 sums, one rounding.  One launch, and no quantisation of the activation: for decode
     steps of few tokens, which read the weight once either way."""
     scale_t = weight_scale if isinstance(weight_scale, torch.Tensor) else None
-    return _lib.native().weight_only_linear(x, qw, sfw_dense, scale_t, 1.0 if scale_t is not None else float(weight_scale), bias, out)
+    return _lib.native().weight_only_linear(x, qw, sfw_dense, scale_t, 1.0 if scale_t is not None else float(weight_scale), bias, out,
+                                              _error_flag(x.device))
 
 
 # --------------------------------------------------------------------------- grouped (mixture-of-experts) launches

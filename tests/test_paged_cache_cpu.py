@@ -93,7 +93,7 @@ def test_weight_only_arguments_that_are_refused():
     one, odd = ctypes.c_void_p(256), ctypes.c_void_p(264)
 
     def refuse(message, x=one, x_row=256, m=2, n=128, k=256, qw=one):
-        assert L.sharq_weight_only_linear(x, x_row, m, n, k, qw, one, None, 1.0, None, one, None) != 0
+        assert L.sharq_weight_only_linear(x, x_row, m, n, k, qw, one, None, 1.0, None, one, None, None) != 0
         assert message in L.sharq_last_error()
 
     refuse(b"null buffer", x=None)

@@ -39,7 +39,8 @@ def check(got, x, w, scale, bias=None):
 
 
 SHAPES = [(1, 4096, 4096), (16, 128, 64), (3, 1, 64), (8, 130, 192), (9, 257, 14336), (5, 1000, 18944), (16, 4608, 3584), (1, 128, 128),
-          (7, 37888, 256), (2, 300, 320), (13, 129, 4032), (1, 64, 32768), (4, 40000, 448)]
+          (7, 37888, 256), (2, 300, 320), (13, 129, 4032), (1, 64, 32768), (4, 40000, 448),
+          (16, 136, 65536), (3, 200, 36864), (2, 5000, 512)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
