@@ -409,8 +409,10 @@ int sharq_rope_append_paged(const void *qkv_bf16, int64_t row_stride, int rows, 
  * q_row / q_head elements between sequences / heads (multiples of 8), out bf16 [sequences, heads, head_dim].  A sequence of length 0 gives
  * zeros.  A length that is negative or more than the page table holds, or a page outside the cache, makes the rows of that sequence NaN and
  * stores 0x402 in *error_flag (may be NULL; 0x403: a wait ran out).  head_dim 64 or 128; heads a multiple of kv_heads.  workspace:
- * sharq_paged_attention_workspace_bytes(heads, kv_heads, head_dim) bytes of scratch, 16-byte aligned, not shared by calls that overlap. */
-size_t sharq_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
+ * sharq_paged_attention_workspace_bytes(heads, cache) bytes of scratch (0: none, by the shape of the cache and its table alone), 16-byte aligned,
+ * not shared by calls that overlap.  Where the table holds few tokens per sequence the call is one launch without scratch, else two: a
+ * table cut to the pages of the longest sequence (max_pages) is the faster one. */
+size_t sharq_paged_attention_workspace_bytes(int heads, const sharq_paged_cache *cache);
 int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int heads, const sharq_paged_cache *cache,
                           const int *lengths, float scale, void *out_bf16, void *workspace, size_t workspace_bytes, int *error_flag,
                           void *stream);

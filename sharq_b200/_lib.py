@@ -99,7 +99,7 @@ SIGNATURES = {
     "sharq_fused_rmsnorm_sparse_residual_quantize_x_noalloc": (
         c_int, [_P, _P, c_float, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P]),
     "sharq_rope_append_paged": (c_int, [_P, c_int64, c_int, c_int, _P, _P, c_int, _P, _P, _P, _P, _P, _P, _P]),
-    "sharq_paged_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "sharq_paged_attention_workspace_bytes": (c_size_t, [c_int, _P]),
     "sharq_paged_attention": (c_int, [_P, c_int64, c_int64, c_int, _P, _P, c_float, _P, _P, c_size_t, _P, _P]),
     "sharq_weight_only_linear": (c_int, [_P, c_int64, c_int, c_int, c_int, _P, _P, _P, c_float, _P, _P, _P, _P]),
     "sharq_noalloc_max_rows": (c_int, []),

@@ -787,9 +787,11 @@ int sharq_rope_append_paged(const void *qkv_bf16, int64_t row_stride, int rows, 
                     "rope_append_paged");
 }
 
-size_t sharq_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
-  if (heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
-  return sharq::paged_attention_workspace_bytes(heads, kv_heads, head_dim);
+size_t sharq_paged_attention_workspace_bytes(int heads, const sharq_paged_cache *cache) {
+  sharq::PagedCache c;
+  bool fp8 = false;
+  if (paged_cache(cache, &c, &fp8) || heads <= 0 || heads % c.kv_heads != 0) return 0;
+  return sharq::paged_attention_workspace_bytes(heads, c, fp8);
 }
 
 int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int heads, const sharq_paged_cache *cache,
@@ -798,7 +800,7 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
   sharq::PagedCache c;
   bool fp8 = false;
   if (paged_cache(cache, &c, &fp8)) return 1;
-  SHARQ_REQUIRE(q_bf16 && lengths && out_bf16 && workspace, "null buffer");
+  SHARQ_REQUIRE(q_bf16 && lengths && out_bf16, "null buffer");
   SHARQ_REQUIRE(c.head_dim == 64 || c.head_dim == 128, "head_dim must be 64 or 128, got %d", c.head_dim);
   SHARQ_REQUIRE(heads > 0 && heads % c.kv_heads == 0 && heads <= 65536, "heads must be a positive multiple of kv_heads, at most 65536");
   SHARQ_REQUIRE((int64_t)c.seqs * heads <= 0x7fffffff &&
@@ -806,8 +808,8 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
                 "too many sequences, or a page table for too many tokens");
   SHARQ_REQUIRE(q_row >= 0 && q_head >= 0 && q_row % 8 == 0 && q_head % 8 == 0, "the strides of q must be multiples of 8");
   SHARQ_REQUIRE(aligned16(q_bf16) && aligned16(out_bf16) && aligned16(workspace), "buffers must be 16-byte aligned");
-  const size_t need = sharq::paged_attention_workspace_bytes(heads, c.kv_heads, c.head_dim);
-  SHARQ_REQUIRE(workspace_bytes >= need, "workspace too small: need %zu bytes", need);
+  const size_t need = sharq::paged_attention_workspace_bytes(heads, c, fp8);
+  SHARQ_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "workspace too small: need %zu bytes", need);
   return check_cuda(sharq::run_paged_attention(q_bf16, q_row, q_head, heads, c, fp8, lengths, scale, out_bf16, workspace, error_flag,
                                                as_stream(stream)),
                     "paged_attention");

@@ -32,7 +32,7 @@ cudaError_t run_rope_append_paged(const void *qkv, long long row_stride, int row
                                   void *q_out, void *k_out, int *error_flag, cudaStream_t stream);
 
 // One query row per sequence of the cache's page table (cache.head_dim 64 or 128, heads a multiple of cache.kv_heads).
-size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
+size_t paged_attention_workspace_bytes(int heads, const PagedCache &cache, bool fp8);
 cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head, int heads, const PagedCache &cache, bool fp8,
                                 const int *lengths, float scale, void *out, void *workspace, int *error_flag, cudaStream_t stream);
 
@@ -40,5 +40,16 @@ cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head
 constexpr int kWeightOnlyMaxRows = 16;
 cudaError_t run_weight_only(const void *x, long long x_row, int m, int n, int k, const void *qw, const void *sf, const float *scale_dev,
                             float scale, const void *bias, void *y, int *error_flag, cudaStream_t stream);
+
+// Leave for `bytes` of shared memory, asked for once per kernel and device (ready: a static array per kernel).
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, bool (&ready)[64]) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess || (dev >= 0 && dev < 64 && ready[dev])) return err;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess && dev >= 0 && dev < 64) ready[dev] = true;
+  return err;
+}
 
 }  // namespace sharq

@@ -24,8 +24,8 @@
 //
 // e4m3 caches go through f16: their values are exact in it, queries are scaled to it by a power of two per head (a value below 2^-39 of its
 // head's largest is lost), and probabilities carry a factor of 2^10, so that those down to 2^-24 of the maximum keep f16's full precision.  For bf16
-// caches the probabilities are rounded to bf16 for the product with the values (half a unit in the 8th bit, as the output itself); their sum is
-// taken before that rounding, in float.
+// caches the probabilities enter as the sum of two bf16 numbers, 16 bits (rounded to one they made half of the result's error, and the reading of the
+// cache hides the second product).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         for (int j = 0; j < 2; ++j) base[n][j] = (m[n][j] == -INFINITY ? 0.0f : m[n][j]) - (kFp8 ? kF16Lift : 0.0f);
 #pragma unroll
       for (int b = 0; b < kTokens / 16; ++b) {
-        uint32_t pb[kN][2];
+        uint32_t pb[kN][2], pb_lo[kN][2];
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
           float p[4];
@@ -564,8 +564,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
             p[j] = exp2_approx(s[b][n][j] - base[n][j & 1]);
             l[n][j & 1] += p[j];
           }
-          pb[n][0] = movmatrix(kFp8 ? pack_f16(p[0], p[1]) : pack_bf16(p[0], p[1]));
-          pb[n][1] = movmatrix(kFp8 ? pack_f16(p[2], p[3]) : pack_bf16(p[2], p[3]));
+          if (kFp8) {
+            pb[n][0] = movmatrix(pack_f16(p[0], p[1]));
+            pb[n][1] = movmatrix(pack_f16(p[2], p[3]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t hi = pack_bf16(p[2 * j], p[2 * j + 1]);
+              pb[n][j] = movmatrix(hi);
+              pb_lo[n][j] = movmatrix(pack_bf16(p[2 * j] - __uint_as_float(hi << 16), p[2 * j + 1] - __uint_as_float(hi & 0xFFFF0000u)));
+            }
+          }
         }
         if (!kFp8) {
 #pragma unroll
@@ -573,7 +582,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
             uint32_t w[4];
             ldmatrix4_trans(w, (values + b * 2048 + v_lane + (i / 4) * T::kHalf) ^ ((i % 4) * 32));
 #pragma unroll
-            for (int n = 0; n < kN; ++n) mma16816<kFp8>(o[i][n], w, pb[n][0], pb[n][1]);
+            for (int n = 0; n < kN; ++n) {
+              mma16816<kFp8>(o[i][n], w, pb[n][0], pb[n][1]);
+              mma16816<kFp8>(o[i][n], w, pb_lo[n][0], pb_lo[n][1]);
+            }
           }
         } else {
           // lane (g, t) takes D / 8 neighbouring elements of four tokens: rows g and g + 8 of tile i are its elements 2 i and 2 i + 1
@@ -1015,10 +1027,11 @@ cudaError_t launch(AttnArgs a, const PagedCache &c, int ctas, cudaStream_t strea
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const int items = c.kv_heads * a.chunks;
-  const int splits = direct_splits(a.seqs, items, (paged_capacity(c) + T::kTokens - 1) / T::kTokens, ctas);
+  const int splits = direct_splits(a.seqs, items, (paged_capacity(c) - 1) / T::kTokens + 1, ctas);
   if (splits > 0) {
     const auto kernel = paged_attention_kernel<D, kFp8, kCols, true>;
-    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    static bool ready[64] = {};
+    const cudaError_t err = allow_smem(kernel, kSmem, ready);
     if (err != cudaSuccess) return err;
     a.stretch_shift = __builtin_ctz((unsigned)(splits * kAttnWarps));
     attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -1029,7 +1042,8 @@ cudaError_t launch(AttnArgs a, const PagedCache &c, int ctas, cudaStream_t strea
     return cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, a, c);
   }
   const auto kernel = paged_attention_kernel<D, kFp8, kCols, false>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static bool ready[64] = {};
+  cudaError_t err = allow_smem(kernel, kSmem, ready);
   if (err != cudaSuccess) return err;
   cfg.gridDim = dim3((unsigned)ctas);
   err = cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, a, c);
@@ -1044,9 +1058,11 @@ int attn_ctas() { return 2 * attn_sm_count(); }
 
 }  // namespace
 
-size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
-  const size_t cols = heads / kv_heads <= 8 ? 8 : 16, places = 2 * (size_t)attn_ctas();
-  return places * cols * (head_dim + 2) * sizeof(float);
+size_t paged_attention_workspace_bytes(int heads, const PagedCache &cache, bool fp8) {
+  const int group = heads / cache.kv_heads, items = cache.kv_heads * ((group + 15) / 16), cols = group <= 8 ? 8 : 16;
+  const int tokens = cache.head_dim * (fp8 ? 1 : 2) > 128 ? 16 : 32;  // as Tile has it
+  if (direct_splits(cache.seqs, items, (paged_capacity(cache) - 1) / tokens + 1, attn_ctas()) > 0) return 0;
+  return 2 * (size_t)attn_ctas() * cols * (cache.head_dim + 2) * sizeof(float);
 }
 
 cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head, int heads, const PagedCache &cache, bool fp8,

@@ -45,13 +45,22 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return lo | hi << 16;
 }
 
-// eight neighbouring elements of a head into the cache
+// Eight neighbouring elements of a head into the cache.  The quotient by the scale is the float division's, by its residual from a product with
+// the correctly rounded reciprocal (Markstein); 1024 and more saturate in e4m3 whatever the last bits, and a zero keeps its sign.  (16 divisions: 103 instead of 85 us for 16384 rows.)
 template <bool kFp8>
-__device__ __forceinline__ void store8(char *at, const float (&f)[8], float scale) {
+__device__ __forceinline__ void store8(char *at, const float (&f)[8], float scale, float reciprocal) {
   if (kFp8) {
     float q[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(f[j], scale);
+    for (int j = 0; j < 8; ++j) {
+      q[j] = f[j] * reciprocal;
+      const float residual = __fmaf_rn(-q[j], scale, f[j]);
+      if (fabsf(q[j]) < 1024.0f && q[j] != 0.0f) q[j] = __fmaf_rn(residual, reciprocal, q[j]);
+    }
+    if (!(scale > 0x1p-100f && scale < 0x1p100f)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(f[j], scale);
+    }
     *reinterpret_cast<uint2 *>(at) = make_uint2(e4m3x4(q[0], q[1], q[2], q[3]), e4m3x4(q[4], q[5], q[6], q[7]));
   } else {
     *reinterpret_cast<uint4 *>(at) = pack8(f);
@@ -64,85 +73,82 @@ struct AppendArgs {
   const int *positions, *sequences;
   __nv_bfloat16 *q_out, *k_out;
   int *error_flag;
-  int rows, heads, table_rows, rows_per_cta;
+  int rows, heads, table_rows, page_shift;  // page_shift: log2 of the page size, -1 if it is no power of two
 };
 
-// A thread takes 8 elements of the first half of a head and their 8 partners of the second half; a row's threads are those of one CTA
-// (several rows share one while a row has few).
+// A thread takes 8 elements of the first half of a head and their 8 partners of the second half: threadIdx = (vector of the half head, head, row of the
+// CTA), so that nothing is divided to find them.  What it rotates is loaded first, and the row's place is found meanwhile: a thread that
+// looked the place up before it loaded anything took 98 us for 16384 rows of 36 heads of 128.
 template <bool kFp8>
-__global__ void __launch_bounds__(512) rope_append_kernel(AppendArgs a, PagedCache c) {
-  ptx::grid_launch_dependents();
+__global__ void __launch_bounds__(512) rope_append_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ PagedCache c) {
+  const int half = c.head_dim >> 1, v = threadIdx.x, row = blockIdx.x * blockDim.z + threadIdx.z, all_heads = a.heads + 2 * c.kv_heads;
   ptx::grid_dependency_wait();
-  const int half = c.head_dim >> 1;
-  const unsigned vecs = (unsigned)half >> 3;
-  const unsigned per_row = (unsigned)(a.heads + 2 * c.kv_heads) * vecs;
-  unsigned i = threadIdx.x, row = blockIdx.x;
-  if (a.rows_per_cta > 1) {
-    const unsigned in_cta = i / per_row;
-    i -= in_cta * per_row;
-    row = row * a.rows_per_cta + in_cta;
-    if (in_cta >= (unsigned)a.rows_per_cta) return;
-  }
-  if (row >= (unsigned)a.rows) return;
-  const int position = a.positions[row];
-  const int seq = a.sequences != nullptr ? a.sequences[row] : (int)row;
+  ptx::grid_launch_dependents();
+  if (row >= a.rows) return;
+  const int position = a.positions[row], seq = a.sequences != nullptr ? a.sequences[row] : row;
+  const __nv_bfloat16 *x = a.qkv + row * a.row_stride + v * 8;
+  int head = blockIdx.y * blockDim.y + threadIdx.y;
+  if (head >= all_heads) return;
+  uint4 w1 = *reinterpret_cast<const uint4 *>(x + head * c.head_dim), w2 = *reinterpret_cast<const uint4 *>(x + head * c.head_dim + half);
   const bool padding = position < 0;
-  bool good = !padding && position < a.table_rows && position < paged_capacity(c) && seq >= 0 && seq < c.seqs;
-  int page = 0;
-  if (good) {
-    page = c.page_table[seq * c.table_stride + position / c.page_size];
-    good = page >= 0 && page < c.pages;
-  }
-  if (!good && !padding && i == 0 && a.error_flag != nullptr) atomicExch(a.error_flag, kBadCacheIndex);
-  const long long slot = page * c.page_stride + (position % c.page_size) * c.token_stride;
-  const size_t table = (size_t)position * c.head_dim;
-  for (; i < per_row; i += blockDim.x) {
-    const int head = (int)(i / vecs), v = (int)(i % vecs);
-    const int kv = head - a.heads;  // key head, or kv_heads + value head
-    float x1[8], x2[8];
-    if (good) {
-      const __nv_bfloat16 *x = a.qkv + row * a.row_stride + (size_t)head * c.head_dim + v * 8;
-      unpack8(*reinterpret_cast<const uint4 *>(x), x1);
-      unpack8(*reinterpret_cast<const uint4 *>(x + half), x2);
-      if (kv < c.kv_heads) {
-        float c1[8], c2[8], s1[8], s2[8];
-        unpack8(*reinterpret_cast<const uint4 *>(a.cos_t + table + v * 8), c1);
-        unpack8(*reinterpret_cast<const uint4 *>(a.cos_t + table + v * 8 + half), c2);
-        unpack8(*reinterpret_cast<const uint4 *>(a.sin_t + table + v * 8), s1);
-        unpack8(*reinterpret_cast<const uint4 *>(a.sin_t + table + v * 8 + half), s2);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float o1 = __fadd_rn(__fmul_rn(x1[j], c1[j]), -__fmul_rn(x2[j], s1[j]));
-          x2[j] = __fadd_rn(__fmul_rn(x2[j], c2[j]), __fmul_rn(x1[j], s2[j]));
-          x1[j] = o1;
-        }
-      }
-    } else {
-      // a padding row gives zeros, a row without a place NaN; neither touches the cache
-      const float fill = padding ? 0.0f : __int_as_float(0x7fffffff);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x1[j] = x2[j] = fill;
-    }
+  const bool in_tables = !padding && position < a.table_rows && position < paged_capacity(c) && seq >= 0 && seq < c.seqs;
+  const int kv = head - a.heads;  // key head, or kv_heads + value head
+  uint4 wc1, wc2, ws1, ws2;
+  int page = 0, in_page = 0;
+  if (in_tables) {
     if (kv < c.kv_heads) {
-      __nv_bfloat16 *out = nullptr;
-      if (kv < 0)
-        out = a.q_out + ((size_t)row * a.heads + head) * c.head_dim + v * 8;
-      else if (a.k_out != nullptr)
-        out = a.k_out + ((size_t)row * c.kv_heads + kv) * c.head_dim + v * 8;
-      if (out != nullptr) {
-        *reinterpret_cast<uint4 *>(out) = pack8(x1);
-        *reinterpret_cast<uint4 *>(out + half) = pack8(x2);
-      }
+      const __nv_bfloat16 *cos_at = a.cos_t + (size_t)position * c.head_dim + v * 8, *sin_at = a.sin_t + (size_t)position * c.head_dim + v * 8;
+      wc1 = *reinterpret_cast<const uint4 *>(cos_at);
+      wc2 = *reinterpret_cast<const uint4 *>(cos_at + half);
+      ws1 = *reinterpret_cast<const uint4 *>(sin_at);
+      ws2 = *reinterpret_cast<const uint4 *>(sin_at + half);
     }
-    if (kv >= 0 && good) {
-      const bool value = kv >= c.kv_heads;
-      const int h = value ? kv - c.kv_heads : kv;
-      const int size = kFp8 ? 1 : 2;
-      char *at = (value ? c.v : c.k) + slot + h * c.head_stride + v * 8 * size;
-      const float scale = kFp8 ? (value ? c.v_scale : c.k_scale)[h] : 1.0f;
-      store8<kFp8>(at, x1, scale);
-      store8<kFp8>(at + half * size, x2, scale);
+    const int entry = a.page_shift >= 0 ? position >> a.page_shift : position / c.page_size;
+    in_page = position - entry * c.page_size;
+    page = c.page_table[seq * c.table_stride + entry];
+  }
+  const bool good = in_tables && page >= 0 && page < c.pages;
+  if (!good && !padding && head == 0 && v == 0 && a.error_flag != nullptr) atomicExch(a.error_flag, kBadCacheIndex);
+  float x1[8], x2[8];
+  unpack8(w1, x1);
+  unpack8(w2, x2);
+  if (!good) {
+    // a padding row gives zeros, a row without a place NaN; neither touches the cache
+    const float fill = padding ? 0.0f : __int_as_float(0x7fffffff);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x1[j] = x2[j] = fill;
+  } else if (kv < c.kv_heads) {
+    float c1[8], c2[8], s1[8], s2[8];
+    unpack8(wc1, c1);
+    unpack8(wc2, c2);
+    unpack8(ws1, s1);
+    unpack8(ws2, s2);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {  // the products are exact
+      const float o1 = __fmaf_rn(x1[j], c1[j], -__fmul_rn(x2[j], s1[j]));
+      x2[j] = __fmaf_rn(x2[j], c2[j], __fmul_rn(x1[j], s2[j]));
+      x1[j] = o1;
     }
+  }
+  if (kv < c.kv_heads) {
+    __nv_bfloat16 *out = nullptr;
+    if (kv < 0)
+      out = a.q_out + ((size_t)row * a.heads + head) * c.head_dim + v * 8;
+    else if (a.k_out != nullptr)
+      out = a.k_out + ((size_t)row * c.kv_heads + kv) * c.head_dim + v * 8;
+    if (out != nullptr) {
+      *reinterpret_cast<uint4 *>(out) = pack8(x1);
+      *reinterpret_cast<uint4 *>(out + half) = pack8(x2);
+    }
+  }
+  if (kv >= 0 && good) {
+    const bool value = kv >= c.kv_heads;
+    const int kv_head = value ? kv - c.kv_heads : kv, size = kFp8 ? 1 : 2;
+    char *at = (value ? c.v : c.k) + page * c.page_stride + in_page * c.token_stride + kv_head * c.head_stride + v * 8 * size;
+    const float scale = kFp8 ? (value ? c.v_scale : c.k_scale)[kv_head] : 1.0f;
+    const float reciprocal = kFp8 ? __frcp_rn(scale) : 1.0f;
+    store8<kFp8>(at, x1, scale, reciprocal);
+    store8<kFp8>(at + half * size, x2, scale, reciprocal);
   }
 }
 
@@ -152,7 +158,6 @@ cudaError_t run_rope_append_paged(const void *qkv, long long row_stride, int row
                                   int table_rows, const int *positions, const int *sequences, const PagedCache &cache, bool fp8,
                                   void *q_out, void *k_out, int *error_flag, cudaStream_t stream) {
   if (rows <= 0) return cudaSuccess;
-  const long long per_row = (long long)(heads + 2 * cache.kv_heads) * (cache.head_dim / 16);
   AppendArgs a;
   a.qkv = static_cast<const __nv_bfloat16 *>(qkv);
   a.cos_t = static_cast<const __nv_bfloat16 *>(cos_t);
@@ -166,14 +171,19 @@ cudaError_t run_rope_append_paged(const void *qkv, long long row_stride, int row
   a.rows = rows;
   a.heads = heads;
   a.table_rows = table_rows;
-  a.rows_per_cta = per_row < 64 ? (int)(128 / per_row) : 1;
-  const int threads = per_row > 512 ? 512 : (int)((a.rows_per_cta * per_row + 31) / 32 * 32);
+  a.page_shift = (cache.page_size & (cache.page_size - 1)) == 0 ? __builtin_ctz((unsigned)cache.page_size) : -1;
+  // CTAs of up to 512 threads, all heads of a row in equal shares; short rows share one of 128
+  const int vecs = cache.head_dim / 16, all_heads = heads + 2 * cache.kv_heads;
+  const int shares = (all_heads * vecs + 511) / 512, share = (all_heads + shares - 1) / shares;
+  int together = 128 / (share * vecs);
+  if (together < 1 || shares > 1) together = 1;
+  if (together > 64) together = 64;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)((rows + a.rows_per_cta - 1) / a.rows_per_cta));
-  cfg.blockDim = dim3((unsigned)threads);
+  cfg.gridDim = dim3((unsigned)((rows + together - 1) / together), (unsigned)shares);
+  cfg.blockDim = dim3((unsigned)vecs, (unsigned)share, (unsigned)together);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;

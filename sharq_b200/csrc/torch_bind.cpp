@@ -455,7 +455,7 @@ void check_indices(const Tensor &t, int64_t n, const at::Device &dev, const char
     fail(std::string(name) + " must be a contiguous CUDA int32 vector with " + std::to_string(n) + " entries on the device of the input");
 }
 
-// -> (q [rows, heads, head_dim], k [rows, kv_heads, head_dim] or an empty tensor)
+// -> q [rows, heads, head_dim] and, with return_k, k [rows, kv_heads, head_dim]
 std::vector<Tensor> rope_append_paged(const Tensor &qkv, int64_t heads, int64_t kv_heads, int64_t head_dim, const Tensor &cos,
                                       const Tensor &sin, const Tensor &positions, const Tensor &table, const Tensor &k_cache,
                                       const Tensor &v_cache, const std::optional<Tensor> &sequences,
@@ -483,13 +483,14 @@ std::vector<Tensor> rope_append_paged(const Tensor &qkv, int64_t heads, int64_t 
     need(rows <= c.sequences, "page_table must have a row for every row of qkv when sequences is not given");
   c10::cuda::OptionalCUDAGuard guard(dev);
   Tensor q = empty_like_on(qkv, {rows, heads, head_dim}, at::kBFloat16);
-  Tensor k = empty_like_on(qkv, {return_k ? rows : 0, kv_heads, head_dim}, at::kBFloat16);
+  std::vector<Tensor> out = {q};
+  if (return_k) out.push_back(empty_like_on(qkv, {rows, kv_heads, head_dim}, at::kBFloat16));
   if (rows > 0)
     check(sharq_rope_append_paged(ptr(qkv), rows > 1 ? qkv.stride(0) : qkv.size(1) / 8 * 8, (int)rows, (int)heads, ptr(cos), ptr(sin),
                                   (int)cos.size(0), static_cast<const int *>(ptr(positions)),
-                                  sequences ? static_cast<const int *>(ptr(*sequences)) : nullptr, &c, ptr(q), return_k ? ptr(k) : nullptr,
+                                  sequences ? static_cast<const int *>(ptr(*sequences)) : nullptr, &c, ptr(q), return_k ? ptr(out[1]) : nullptr,
                                   flag_of(flag), stream_of(qkv)));
-  return {q, k};
+  return out;
 }
 
 Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &table, const Tensor &lengths,
@@ -512,10 +513,11 @@ Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_c
   if (seqs == 0) return o;
   sharq_paged_cache used = c;
   used.sequences = (int)seqs;
-  const int64_t ws_bytes = (int64_t)sharq_paged_attention_workspace_bytes((int)heads, c.kv_heads, (int)d);
-  Tensor ws = empty_like_on(q, {ws_bytes}, at::kByte);
+  const int64_t ws_bytes = (int64_t)sharq_paged_attention_workspace_bytes((int)heads, &used);
+  Tensor ws;
+  if (ws_bytes > 0) ws = empty_like_on(q, {ws_bytes}, at::kByte);
   check(sharq_paged_attention(ptr(q), seqs > 1 ? q.stride(0) : 0, heads > 1 ? q.stride(1) : 0, (int)heads, &used,
-                              static_cast<const int *>(ptr(lengths)), (float)(scale ? *scale : 1.0 / std::sqrt((double)d)), ptr(o), ptr(ws),
+                              static_cast<const int *>(ptr(lengths)), (float)(scale ? *scale : 1.0 / std::sqrt((double)d)), ptr(o), ws_bytes > 0 ? ptr(ws) : nullptr,
                               (size_t)ws_bytes, flag_of(flag), stream_of(q)));
   return o;
 }

@@ -460,7 +460,8 @@ cudaError_t run_weight_only(const void *x, long long x_row, int m, int n, int k,
   const int left = n % 128;  // a last block of few rows has empty tiles at its end
   a.tiles = n / 128 * 8 + (left == 0 ? 0 : left > 64 ? 8 : left >= 32 ? 7 : 2 * ((left + 7) / 8) - 1);
   const auto kernel = weight_only_kernel;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWoSmem);
+  static bool ready[64] = {};
+  cudaError_t err = allow_smem(kernel, kWoSmem, ready);
   if (err != cudaSuccess) return err;
   int clusters = 0;
   err = wo_clusters(kernel, a.cluster, &clusters);

@@ -213,9 +213,9 @@ def rope_append_paged(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: in
     p % page_size of page page_table[sequence, p // page_size] (int32).  float32 arithmetic, one rounding per result.  A negative
     position is padding (zeros, nothing appended); a place outside the tables or the cache gives NaN, appends nothing and is reported by
     check_device_errors.  No two rows may have the same place."""
-    q, k = _lib.native().rope_append_paged(qkv, heads, kv_heads, head_dim, cos, sin, positions, page_table, k_cache, v_cache,
-                                           sequences, k_scale, v_scale, return_k, _error_flag(qkv.device))
-    return (q, k) if return_k else q
+    out = _lib.native().rope_append_paged(qkv, heads, kv_heads, head_dim, cos, sin, positions, page_table, k_cache, v_cache,
+                                            sequences, k_scale, v_scale, return_k, _error_flag(qkv.device))
+    return out if return_k else out[0]
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,

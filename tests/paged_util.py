@@ -64,10 +64,10 @@ def attention_bound(out, size, reach, dim, longest, fp8):
     """How far the kernel may be from attention64, element by element.
     A score is a float sum of dim exact products: off by at most (dim + 4) * 2^-23 of the sum of their sizes (`reach`), the multiplication by
     the scale and the exponential's argument among the 4; a probability is off by that, relative, twice (its own and its sum's).  It is
-    rounded to bf16 (2^-8) or f16 (2^-11) for the product, and the product's float sum has at most longest + 16 roundings of 2^-23 and the
+    rounded to two bf16 numbers (2^-16) or to f16 (2^-11) for the product, and the product's float sum has at most longest + 16 roundings of 2^-23 and the
     joins.  All that in units of sum p |v|; the result is rounded to bf16 once (2^-8)."""
     score = (dim + 4) * 2.0 ** -23 * reach
-    rounding = 2.0 ** -11 if fp8 else 2.0 ** -8
+    rounding = 2.0 ** -11 if fp8 else 2.0 ** -16
     return (rounding + 2 * score * (1 + score) + 2 * (longest + 64) * 2.0 ** -23) * size + 2.0 ** -8 * (1 + 2.0 ** -7) * out.abs() + 1e-30
 
 

@@ -46,8 +46,11 @@ def test_other_arguments_that_are_refused():
 
     L = _lib.lib()
     one, odd = ctypes.c_void_p(256), ctypes.c_void_p(258)
-    need = L.sharq_paged_attention_workspace_bytes(4, 2, 128)
-    assert need > 0 and L.sharq_paged_attention_workspace_bytes(0, 2, 128) == 0
+    # a table of few tokens needs no scratch, one of many does, arguments that are refused have none
+    long = dict(max_pages=10000, page_table_stride=10000)
+    need = L.sharq_paged_attention_workspace_bytes(4, cache(**long))
+    assert need > 0 and L.sharq_paged_attention_workspace_bytes(4, cache()) == 0
+    assert L.sharq_paged_attention_workspace_bytes(0, cache(**long)) == 0 and L.sharq_paged_attention_workspace_bytes(3, cache(**long)) == 0
 
     def attend(message, q=one, q_row=512, q_head=128, heads=4, c=None, ws=need):
         assert L.sharq_paged_attention(q, q_row, q_head, heads, c or cache(), one, 0.1, one, one, ws, None, None) != 0
@@ -59,7 +62,7 @@ def test_other_arguments_that_are_refused():
     attend(b"too many sequences", c=cache(sequences=2 ** 30))
     attend(b"multiples of 8", q_row=516)
     attend(b"16-byte aligned", q=odd)
-    attend(b"workspace too small", ws=need - 1)
+    attend(b"workspace too small", ws=need - 1, c=cache(**long))
 
     def append(message, qkv=one, stride=1024, rows=2, heads=4, table=64, c=None):
         assert L.sharq_rope_append_paged(qkv, stride, rows, heads, one, one, table, one, None, c or cache(), one, None, None, None) != 0

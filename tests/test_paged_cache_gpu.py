@@ -293,3 +293,29 @@ def test_refusals():
     # nothing to do
     assert ops.paged_attention(q[:0], k, v, table, n[:0]).shape == (0, 4, 128)
     assert ops.rope_append_paged(qkv[:0], 4, 2, 128, cos, sin, n[:0], table, k, v).shape == (0, 4, 128)
+
+
+def test_append_divides_as_a_float_division():
+    """Every finite bf16 value, infinities and NaN, by scales of many sizes, in a cache of e4m3 values: the bits of a float division, clamped
+    and converted (a NaN's sign aside)."""
+    from sharq_b200 import ops
+
+    dim = 128
+    values = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16).view(512, dim)
+    g = torch.Generator().manual_seed(4)
+    scales = torch.cat((torch.rand(40, generator=g) * 0.1 + 1e-4, 2.0 ** torch.arange(-20, 20, 8).float(), torch.tensor([1.9999999, 3e-33, 1e-39, 7e35])))
+    kv = scales.numel()
+    qkv = torch.zeros(512, (1 + 2 * kv) * dim, dtype=torch.bfloat16)
+    qkv[:, (1 + kv) * dim:] = values.repeat(1, kv)
+    table, pages = P.make_table([512], 16, 0, 1)
+    k, v = (torch.zeros(pages, kv, 16, dim, dtype=torch.float8_e4m3fn, device="cuda") for _ in range(2))
+    cos, sin = P.rope_tables(512, dim)
+    at = torch.arange(512, dtype=torch.int32).cuda()
+    ops.rope_append_paged(qkv.cuda(), 1, kv, dim, cos, sin, at, table, k, v, sequences=torch.zeros_like(at), k_scale=scales.cuda(),
+                          v_scale=scales.cuda())
+    ops.check_device_errors()
+    got = v[table[0].long()].transpose(1, 2).reshape(512, kv, dim)
+    want = (values.cuda().float()[:, None] / scales.cuda()[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+    nan = want.float().isnan()
+    assert torch.equal(got.float().isnan(), nan)
+    assert torch.equal(got.view(torch.uint8)[~nan], want.view(torch.uint8)[~nan])
