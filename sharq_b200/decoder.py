@@ -1,4 +1,4 @@
-"""Minimal decoder stacks (Llama / Qwen2 shaped) built on the SharQ linears, for prefill.
+"""Minimal decoder stacks (Llama / Qwen2 shaped) built on the SharQ linears, for prefill and decode steps.
 
 The reference wraps HuggingFace decoder layers (model/qLlamaLayer.py:50-257,
 model/qQwenLayer.py) written against transformers 4.44; those wrappers read attributes
@@ -10,11 +10,14 @@ decoder with the same call pattern on the quantized path:
 * the input and post-attention RMSNorms are fused into the prepare of the following
   linears; the decoder layer never runs them separately - model/qLlamaLayer.py:219-221
 * o_proj and down_proj take the plain (non-RMSNorm) prepare
-* attention itself is stock `scaled_dot_product_attention` with grouped KV heads; it is not
+* attention of a prompt is stock `scaled_dot_product_attention` with grouped KV heads; it is not
   part of the accelerated path.  The rotary embedding runs in place on the merged qkv output
   (one kernel, ops.rope_inplace_) and SwiGLU is fused with the prepare of down_proj
   (prepare_input_swiglu); both give the bits of the ATen compositions they replace, which
-  `fused_glue=False` still runs.
+  `fused_glue=False` still runs
+* with a paged cache (SharqDecoder.new_cache) the rotary embedding also appends keys and values to it
+  (ops.rope_append_paged, one rounding per element), and decode() runs one token per sequence through the
+  layers, with attention over the cache (ops.paged_attention)
 
 Tensor parallelism (`world` > 1): attention heads and the FFN width are sharded; qkv and
 gate_up are column-parallel, o_proj and down_proj row-parallel with an all-reduce.
@@ -28,6 +31,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
+from .kv_cache import LayerCache, PagedKVCache
 from .qlinear import QLinearLayer, methods_kept
 from .tp import RowParallelSharqLinear, head_layout, padded_size, shard_bounds
 
@@ -186,18 +190,24 @@ class SharqDecoderLayer(torch.nn.Module):
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, delta: torch.Tensor = None,
-                return_delta: bool = False):
+                return_delta: bool = False, kv: LayerCache = None, weight_only: bool = False):
         """x: [B, S, hidden] bf16 -> same shape.  delta: an addend of x that the caller has not
         applied yet (the previous layer's down_proj output); with return_delta the layer returns
         (x_mid, d) whose sum is its output, so that the next layer can fold the add into the
-        statistics pass of its first prepare."""
+        statistics pass of its first prepare.  kv: this layer's part of a paged cache, to which the keys and values go;
+        with kv.lengths (S = 1) the attention runs over it.  weight_only: the linears take the activations unquantised
+        (at most 16 rows; expert FFNs as ever)."""
+        if weight_only:
+            if self.mode != "SHARQ":
+                raise ValueError("weight_only is a form of the SHARQ mode")
+            return self._forward_weight_only(x, cos, sin, delta, return_delta, kv)
         if self.mode != "SHARQ":
             if delta is not None:
                 x = x + delta
             if self.world > 1:
-                y = self._forward_comparison_tp(x, cos, sin)
+                y = self._forward_comparison_tp(x, cos, sin, kv)
             else:
-                y = self.forward_reference(x, cos, sin) if self.mode == "BF16" else self._forward_nvfp4(x, cos, sin)
+                y = self.forward_reference(x, cos, sin, kv) if self.mode == "BF16" else self._forward_nvfp4(x, cos, sin, kv)
             return (y, None) if return_delta else y
         cfg = self.cfg
         b, s, h = x.shape
@@ -209,9 +219,7 @@ class SharqDecoderLayer(torch.nn.Module):
                 x2 = x2 + delta.reshape(b * s, h)
             prep = self.qkv.prepare_input_rmsnorm(x2, self.input_norm, cfg.eps)
         qkv = self.qkv.apply_prepared(prep)
-        q, k, v = _split_heads(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, self.fused_glue)
-        attn = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
-        attn2 = attn.transpose(1, 2).reshape(b * s, self.local_heads * cfg.head_dim)
+        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, self.fused_glue, kv)
         o = self.o_proj(attn2)
         if cfg.experts > 0:
             if self.fused_glue and h <= 8192:
@@ -247,8 +255,29 @@ class SharqDecoderLayer(torch.nn.Module):
         return (x2 + d).view(b, s, h)
 
     @torch.no_grad()
+    def _forward_weight_only(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, delta: torch.Tensor, return_delta: bool,
+                             kv: LayerCache):
+        """The layer on the 4-bit weights with unquantised activations: RMSNorm, attention and SwiGLU between four products that
+        read the weight once and quantise nothing (QLinearLayer.forward_weight_only)."""
+        cfg = self.cfg
+        b, s, h = x.shape
+        x2 = x.reshape(b * s, h)
+        hn, x2 = _add_norm(x2, None if delta is None else delta.reshape(b * s, h), self.input_norm, cfg.eps)
+        qkv = self.qkv.forward_weight_only(hn)
+        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, self.fused_glue, kv)
+        o = self.o_proj.reduce(self.o_proj.local.forward_weight_only(attn2))
+        hn, x2 = _add_norm(x2, o, self.post_norm, cfg.eps)
+        if cfg.experts > 0:
+            d = self._moe(hn)
+        else:
+            d = self.down.reduce(self.down.local.forward_weight_only(_swiglu(self.gate_up.forward_weight_only(hn), self.fused_glue)))
+        if return_delta:
+            return x2.view(b, s, h), d.view(b, s, h)
+        return (x2 + d).view(b, s, h)
+
+    @torch.no_grad()
     def forward_sequence_parallel(self, sp, prepared, x_local: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, b: int,
-                                  s: int, next_gamma: torch.Tensor):
+                                  s: int, next_gamma: torch.Tensor, kv: LayerCache = None):
         """One layer with the residual stream sharded by rows over the ranks (tp.SequenceParallelContext).
         prepared: the RMSNorm-prepared input of qkv for ALL b*s rows (from the previous transition);
         x_local: this rank's rows of the residual stream.  The two transitions (after o_proj with this
@@ -257,9 +286,7 @@ class SharqDecoderLayer(torch.nn.Module):
         residual, prepares the local rows (RMSNorm fused) and all-gathers the packed activation.  -> (prepared input of the next layer's qkv, x_local)."""
         cfg = self.cfg
         qkv = self.qkv.apply_prepared(prepared)
-        q, k, v = _split_heads(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, True)
-        attn = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
-        attn2 = attn.transpose(1, 2).reshape(b * s, self.local_heads * cfg.head_dim)
+        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, True, kv)
         self.o_proj.local.apply_prepared(self.o_proj.local.prepare_input(attn2), scatter=sp.scatter)
         prepared, x_local = sp.transition(x_local, self.post_norm, cfg.eps)
         self.down.local.apply_prepared(_prepare_down(self.gate_up, prepared, self.down.local), scatter=sp.scatter)
@@ -350,7 +377,7 @@ class SharqDecoderLayer(torch.nn.Module):
         return ops.moe_combine(y, dest, selected.contiguous(), routing.contiguous(), residual=residual)
 
     @torch.no_grad()
-    def _forward_comparison_tp(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+    def _forward_comparison_tp(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, kv: LayerCache = None) -> torch.Tensor:
         """The dense-NVFP4 or bf16 layer on this rank's weight shards: column-parallel qkv and gate_up,
         row-parallel o_proj and down_proj whose partial outputs are written into symmetric memory and
         summed by the same all-reduce kernel the SharQ layers use (torch.distributed where that is
@@ -379,9 +406,7 @@ class SharqDecoderLayer(torch.nn.Module):
         else:
             nv = self.nv
             qkv = nv["qkv"].apply_prepared(nv["qkv"].prepare_input_rmsnorm(x2, self.input_norm, cfg.eps))
-        q, k, v = _split_heads(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, self.fused_glue)
-        attn = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
-        attn2 = attn.transpose(1, 2).reshape(m, self.local_heads * cfg.head_dim)
+        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, self.fused_glue, kv)
         if self.mode == "BF16":
             o = row_parallel(lambda out: torch.mm(attn2, r["o"].T, out=out) if out is not None else attn2 @ r["o"].T, h)
         else:
@@ -399,21 +424,18 @@ class SharqDecoderLayer(torch.nn.Module):
         return (x2 + d).view(b, s, h)
 
     @torch.no_grad()
-    def _forward_nvfp4(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+    def _forward_nvfp4(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, kv: LayerCache = None) -> torch.Tensor:
         cfg, nv = self.cfg, self.nv
         b, s, h = x.shape
         x2 = x.reshape(b * s, h)
         qkv = nv["qkv"].apply_prepared(nv["qkv"].prepare_input_rmsnorm(x2, self.input_norm, cfg.eps))
-        nq = cfg.heads * cfg.head_dim
-        q, k, v = _split_heads(qkv, b, s, cfg.heads, cfg.kv_heads, cfg.head_dim, cos, sin, self.fused_glue)
-        attn = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
-        x2 = x2 + nv["o"](attn.transpose(1, 2).reshape(b * s, nq))
+        x2 = x2 + nv["o"](_attention(qkv, b, s, cfg.heads, cfg.kv_heads, cfg.head_dim, cos, sin, self.fused_glue, kv))
         gu = nv["gate_up"].apply_prepared(nv["gate_up"].prepare_input_rmsnorm(x2, self.post_norm, cfg.eps))
         x2 = x2 + nv["down"](_swiglu(gu, self.fused_glue))
         return x2.view(b, s, h)
 
     @torch.no_grad()
-    def forward_reference(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+    def forward_reference(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, kv: LayerCache = None) -> torch.Tensor:
         """The same layer with the unquantised bf16 weights (single rank, keep_reference=True)."""
         cfg, r = self.cfg, self.ref
         b, s, h = x.shape
@@ -424,11 +446,8 @@ class SharqDecoderLayer(torch.nn.Module):
 
         x2 = x.reshape(b * s, h)
         qkv = F.linear(norm(x2, self.input_norm), r["qkv"], r["qkv_bias"])
-        nq = cfg.heads * cfg.head_dim
         glue = "gate_up" in r  # BF16 comparison mode; the accuracy reference of a SharQ layer stays pure ATen
-        q, k, v = _split_heads(qkv, b, s, cfg.heads, cfg.kv_heads, cfg.head_dim, cos, sin, glue)
-        attn = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
-        x2 = x2 + F.linear(attn.transpose(1, 2).reshape(b * s, nq), r["o"])
+        x2 = x2 + F.linear(_attention(qkv, b, s, cfg.heads, cfg.kv_heads, cfg.head_dim, cos, sin, glue, kv), r["o"])
         y = norm(x2, self.post_norm)
         if cfg.experts > 0:
             routing, selected = _route(y, self.router, cfg.top_k)
@@ -513,6 +532,32 @@ def _split_heads(qkv: torch.Tensor, b: int, s: int, heads: int, kv_heads: int, d
     return q, k, v
 
 
+def _attention(qkv: torch.Tensor, b: int, s: int, heads: int, kv_heads: int, d: int, cos: torch.Tensor, sin: torch.Tensor, fused: bool,
+               kv: LayerCache = None) -> torch.Tensor:
+    """Attention of a merged qkv activation [b*s, (heads + 2*kv_heads)*d] -> [b*s, heads*d]: causal over the s tokens, which with kv are
+    also appended to the cache, or, with kv.lengths, of one token per sequence over the cache."""
+    if kv is None:
+        q, k, v = _split_heads(qkv, b, s, heads, kv_heads, d, cos, sin, fused)
+    else:
+        got = ops.rope_append_paged(qkv, heads, kv_heads, d, kv.cos, kv.sin, kv.positions, kv.table, kv.k, kv.v, sequences=kv.sequences,
+                                    k_scale=kv.k_scale, v_scale=kv.v_scale, return_k=kv.lengths is None)
+        if kv.lengths is not None:
+            return ops.paged_attention(got, kv.k, kv.v, kv.table, kv.lengths, k_scale=kv.k_scale, v_scale=kv.v_scale).view(b * s, heads * d)
+        q, k = (x.view(b, s, -1, d).transpose(1, 2) for x in got)
+        v = qkv[:, (heads + kv_heads) * d:].view(b, s, kv_heads, d).transpose(1, 2)
+    attn = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
+    return attn.transpose(1, 2).reshape(b * s, heads * d)
+
+
+def _add_norm(x: torch.Tensor, addend: torch.Tensor, weight: torch.Tensor, eps: float):
+    """(rmsnorm(x + addend) in bf16, x + addend), the addend optional."""
+    if x.shape[1] <= 8192 and x.shape[1] % 8 == 0:
+        got = ops.add_rmsnorm(x.contiguous(), weight, eps, residual=None if addend is None else addend.contiguous())
+        return (got, x) if addend is None else got
+    x = x if addend is None else x + addend
+    return _rmsnorm(x, weight, eps), x
+
+
 def _prepare_down(gate_up, prepared, down):
     """down.prepare_input_swiglu(gate_up.apply_prepared(prepared)), for a QLinearLayer in one GEMM launch where it can be."""
     if isinstance(gate_up, QLinearLayer):
@@ -536,7 +581,7 @@ def _local_column(w_local: torch.Tensor, w_full: torch.Tensor, bias):
 
 
 class SharqDecoder(torch.nn.Module):
-    """Embedding -> N decoder layers -> final norm -> (bf16) lm_head on the last token."""
+    """Embedding -> N decoder layers -> final norm -> (bf16) lm_head on the last token; with a cache one decode step after the other."""
 
     def __init__(self, cfg: DecoderConfig, device, world: int = 1, rank: int = 0, seed: int = 0,
                  keep_reference: bool = False, mode: str = "SHARQ", fused_glue: bool = True, reduce_hook=None):
@@ -568,10 +613,18 @@ class SharqDecoder(torch.nn.Module):
         return tp.sequence_parallel_context(m, self.cfg.hidden, None, self.embed.device)
 
     @torch.no_grad()
-    def prefill(self, token_ids: torch.Tensor, reference: bool = False) -> torch.Tensor:
+    def prefill(self, token_ids: torch.Tensor, reference: bool = False, cache: PagedKVCache = None) -> torch.Tensor:
         """token_ids [B, S] -> logits of the last position [B, vocab] (float32).
-        reference=True runs the unquantised bf16 layers (needs keep_reference=True)."""
+        reference=True runs the unquantised bf16 layers (needs keep_reference=True).  cache: an empty cache of B sequences, which
+        then holds the prompts (decode)."""
         b, s = token_ids.shape
+        kvs = [None] * len(self.layers)
+        if cache is not None:
+            if b != cache.sequences or any(cache.lengths):
+                raise ValueError("prefill takes an empty cache with a sequence for every prompt")
+            cache.reserve([s] * b)
+            positions, sequences = cache.prompt_step(s)
+            kvs = [cache.layer(i, positions, sequences, None) for i in range(len(self.layers))]
         cos, sin = rope_tables(s, self.cfg.head_dim, self.cfg.rope_theta, self.embed.device)
         sp = None if reference else self._sequence_parallel_context(b * s)
         if sp is not None:
@@ -582,7 +635,7 @@ class SharqDecoder(torch.nn.Module):
             prepared, x_local = sp.transition(x_local, self.layers[0].input_norm, self.cfg.eps, use_partial=False)
             for i, layer in enumerate(self.layers):
                 nxt = self.layers[i + 1].input_norm if i + 1 < len(self.layers) else self.final_norm
-                prepared, x_local = layer.forward_sequence_parallel(sp, prepared, x_local, cos, sin, b, s, nxt)
+                prepared, x_local = layer.forward_sequence_parallel(sp, prepared, x_local, cos, sin, b, s, nxt, kvs[i])
             # the last position of every sequence lives on one rank: sum the zero-padded rows over ranks
             last = torch.zeros((b, self.cfg.hidden), dtype=torch.float32, device=x_local.device)
             for bi in range(b):  # python indices only: this runs under stream capture
@@ -593,13 +646,56 @@ class SharqDecoder(torch.nn.Module):
         else:
             x = self.embed[token_ids]
             delta = None
-            for layer in self.layers:
+            for layer, kv in zip(self.layers, kvs):
                 if reference:
-                    x = layer.forward_reference(x, cos, sin)
+                    x = layer.forward_reference(x, cos, sin, kv)
                 else:
-                    x, delta = layer(x, cos, sin, delta=delta, return_delta=True)
+                    x, delta = layer(x, cos, sin, delta=delta, return_delta=True, kv=kv)
             if delta is not None:
                 x = x + delta
             last = x[:, -1, :].float()
+        if cache is not None:
+            cache.advance([s] * b)
+        return self._logits(last)
+
+    def new_cache(self, sequences: int, max_tokens: int, page_size: int = 64, pages: int = None, dtype: torch.dtype = torch.bfloat16,
+                  k_scale: torch.Tensor = None, v_scale: torch.Tensor = None) -> PagedKVCache:
+        """A paged cache for this model's (this rank's) key/value heads, see PagedKVCache."""
+        cos, sin = rope_tables(max_tokens, self.cfg.head_dim, self.cfg.rope_theta, self.embed.device)
+        return PagedKVCache(len(self.layers), self.layers[0].local_kv, self.cfg.head_dim, sequences, max_tokens, cos, sin, page_size, pages,
+                            dtype, k_scale, v_scale)
+
+    @torch.no_grad()
+    def decode(self, token_ids: torch.Tensor, cache: PagedKVCache, reference: bool = False, weight_only: bool = False) -> torch.Tensor:
+        """One more token of every sequence of the cache: token_ids [B] -> logits of the next one [B, vocab] (float32).
+        weight_only: the linears take the activations unquantised (at most 16 sequences).  reference: as in prefill."""
+        b = int(token_ids.shape[0])
+        if token_ids.dim() != 1 or b != cache.sequences:
+            raise ValueError("decode takes one token for every sequence of the cache")
+        if weight_only and b > 16:
+            raise ValueError(f"weight_only takes at most 16 sequences, got {b}")
+        cache.reserve([1] * b)
+        logits = self.decode_step(token_ids, cache, cache.device_lengths, cache.device_lengths + 1, reference, weight_only)
+        cache.advance([1] * b)
+        return logits
+
+    @torch.no_grad()
+    def decode_step(self, token_ids: torch.Tensor, cache: PagedKVCache, positions: torch.Tensor, lengths: torch.Tensor,
+                    reference: bool = False, weight_only: bool = False) -> torch.Tensor:
+        """The device part of decode, for capture in a CUDA graph: positions and lengths (int32 [B], device) of the new tokens and of the
+        sequences with them, whose pages have been reserved; the cache's own lengths stay."""
+        x, delta = self.embed[token_ids][:, None], None
+        for i, layer in enumerate(self.layers):
+            kv = cache.layer(i, positions, None, lengths)
+            if reference:
+                x = layer.forward_reference(x, kv.cos, kv.sin, kv)
+            else:
+                x, delta = layer(x, kv.cos, kv.sin, delta=delta, return_delta=True, kv=kv, weight_only=weight_only)
+        if delta is not None:
+            x = x + delta
+        return self._logits(x[:, -1, :].float())
+
+    def _logits(self, last: torch.Tensor) -> torch.Tensor:
+        """Final norm and lm_head of hidden states [B, hidden] (float32)."""
         last = last * torch.rsqrt(last.pow(2).mean(-1, keepdim=True) + self.cfg.eps) * self.final_norm.float()
         return (last.to(torch.bfloat16) @ self.lm_head.T).float()

@@ -111,16 +111,28 @@ SHAPES = [  # sequences' lengths, heads, kv_heads, dim, page size
     ([40, 41], 36, 2, 128, 1),                 # 18: two pieces, pages of one token
     ([300] * 40, 9, 3, 128, 32),               # many equal sequences
     ([3000, 1] + [0] * 5 + [64] * 70, 10, 2, 64, 256),
+    ([20000, 5], 8, 8, 128, 64),               # parts of one (sequence, head) over many CTAs
+    ([37 * i % 190 for i in range(331)], 8, 2, 128, 16),  # more sequences than a warp looks at at once
 ]
 
 
+def wide(table, page):
+    """The table with room for 200000 tokens per sequence: the form of attention goes by the room, not by the lengths."""
+    out = torch.full((table.shape[0], 200000 // page), -1, dtype=torch.int32, device="cuda")
+    out[:, :table.shape[1]] = table
+    return out
+
+
+@pytest.mark.parametrize("room", ["short", "wide"])
 @pytest.mark.parametrize("order", ["hnd", "nhd"])
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("lengths,heads,kv,dim,page", SHAPES)
-def test_attention(lengths, heads, kv, dim, page, fp8, order):
+def test_attention(lengths, heads, kv, dim, page, fp8, order, room):
     from sharq_b200 import ops
 
     table, pages = P.make_table(lengths, page, 2, seed=len(lengths))
+    if room == "wide":
+        table = wide(table, page)
     k, v, ks, vs = P.make_cache(pages, kv, page, dim, fp8, 7, order)
     g = torch.Generator().manual_seed(11)
     # rows of a merged activation: the heads of a row are contiguous, the rows are not
@@ -139,9 +151,10 @@ def test_attention(lengths, heads, kv, dim, page, fp8, order):
     assert torch.equal(again, got)
 
 
+@pytest.mark.parametrize("room", ["short", "wide"])
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_attention_ignores_what_lies_behind_a_sequence(dim, fp8):
+def test_attention_ignores_what_lies_behind_a_sequence(dim, fp8, room):
     """NaN and infinities in slots behind the length and in pages of nobody, bad entries behind the last page."""
     from sharq_b200 import ops
 
@@ -153,6 +166,8 @@ def test_attention_ignores_what_lies_behind_a_sequence(dim, fp8):
         for j in range(n):
             used[int(table[i, j // page]), j % page] = True
     used = used.cuda()
+    if room == "wide":
+        table = wide(table, page)
     q = torch.randn(4, 6, dim, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
     n = torch.tensor(lengths, dtype=torch.int32).cuda()
     clean = ops.paged_attention(q, k, v, table, n, k_scale=ks, v_scale=vs)
@@ -162,19 +177,22 @@ def test_attention_ignores_what_lies_behind_a_sequence(dim, fp8):
     ops.check_device_errors()
 
 
-def test_attention_reports_bad_lengths_and_pages():
+@pytest.mark.parametrize("room", ["short", "wide"])
+def test_attention_reports_bad_lengths_and_pages(room):
     from sharq_b200 import ops
 
     page, dim = 16, 128
     for fp8 in (False, True):
         table, pages = P.make_table([64, 64, 64, 64, 64], page, 1, 1)
+        if room == "wide":
+            table = wide(table, page)
         k, v, ks, vs = P.make_cache(pages, 2, page, dim, fp8, 7)
         q = torch.randn(5, 8, dim, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
         good = ops.paged_attention(q, k, v, table, torch.full((5,), 64, dtype=torch.int32).cuda(), k_scale=ks, v_scale=vs)
         ops.check_device_errors()
         table[3, 2] = -1
         table[4, 3] = pages
-        n = torch.tensor([64, -1, 65, 64, 64], dtype=torch.int32).cuda()
+        n = torch.tensor([64, -1, table.shape[1] * page + 1, 64, 64], dtype=torch.int32).cuda()
         got = ops.paged_attention(q, k, v, table, n, k_scale=ks, v_scale=vs)
         with pytest.raises(RuntimeError, match="paged cache"):
             ops.check_device_errors()
@@ -319,3 +337,67 @@ def test_append_divides_as_a_float_division():
     nan = want.float().isnan()
     assert torch.equal(got.float().isnan(), nan)
     assert torch.equal(got.view(torch.uint8)[~nan], want.view(torch.uint8)[~nan])
+
+
+def _attention_inputs(seed, lengths, heads=8, kv=2, dim=128, page=16, fp8=False, room="wide"):
+    table, pages = P.make_table(lengths, page, 1, seed)
+    k, v, ks, vs = P.make_cache(pages, kv, page, dim, fp8, seed)
+    q = torch.randn(len(lengths), heads, dim, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).cuda()
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    return (q, k, v, wide(table, page) if room == "wide" else table, n), dict(k_scale=ks, v_scale=vs)
+
+
+@pytest.mark.parametrize("room", ["short", "wide"])
+def test_attention_on_two_streams_and_in_two_graphs(room):
+    """Calls that overlap have scratch of their own; a replay reads the lengths that are there then."""
+    from sharq_b200 import ops
+
+    calls = [_attention_inputs(1, [3000, 17, 400], room=room), _attention_inputs(2, [2500, 1, 0, 90], fp8=True, room=room)]
+    want = [ops.paged_attention(*a, **kw) for a, kw in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    outs = [[torch.empty_like(w) for _ in range(30)] for w in want]
+    for i in range(30):
+        for s, (a, kw), o in zip(streams, calls, outs):
+            with torch.cuda.stream(s):
+                ops.paged_attention(*a, **kw, out=o[i])
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(w, x) for x in o)
+    graphs = []
+    for a, kw in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops.paged_attention(*a, **kw)
+        graphs.append((g, out))
+    for _ in range(5):
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for w, (_, out) in zip(want, graphs):
+        assert torch.equal(w, out)
+    (q, k, v, table, n), kw = calls[0]
+    n.copy_(torch.tensor([5, 0, 399], dtype=torch.int32))
+    graphs[0][0].replay()
+    assert torch.equal(graphs[0][1], ops.paged_attention(q, k, v, table, n, **kw))
+    ops.check_device_errors()
+
+
+def test_attention_of_shared_pages_drafts_and_broadcast_queries():
+    """A sequence in several rows with lengths of its own, pages that sequences share, queries of one head for all, into its own queries."""
+    from sharq_b200 import ops
+
+    (q, k, v, table, n), kw = _attention_inputs(3, [300, 40], room="short")
+    rows = torch.tensor([0, 0, 0, 1]).cuda()
+    lengths = [298, 299, 300, 40]
+    table4 = table[rows].contiguous()
+    table4[3, 0] = table4[0, 0]  # a shared prefix
+    one = q[:1, :1].expand(4, 8, 128)
+    got = ops.paged_attention(one, k, v, table4, torch.tensor(lengths, dtype=torch.int32).cuda())
+    out, size, reach = P.attention64(one, P.values64(k, None), P.values64(v, None), table4, lengths)
+    assert bool(((got.double() - out).abs() <= P.attention_bound(out, size, reach, 128, 300, False)).all())
+    want = ops.paged_attention(q, k, v, table, n)
+    assert ops.paged_attention(q, k, v, table, n, out=q) is not None
+    assert torch.equal(q, want)
+    ops.check_device_errors()
