@@ -46,7 +46,8 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 }
 
 // Eight neighbouring elements of a head into the cache.  The quotient by the scale is the float division's, by its residual from a product with
-// the correctly rounded reciprocal (Markstein); 1024 and more saturate in e4m3 whatever the last bits, and a zero keeps its sign.  (16 divisions: 103 instead of 85 us for 16384 rows.)
+// the correctly rounded reciprocal (Markstein); 1024 and more saturate in e4m3 whatever the last bits, and a zero
+// keeps its sign.  (16 divisions: 102.5 instead of 91.2 us for 16384 rows of 36 heads of 128, one head per thread.)
 template <bool kFp8>
 __device__ __forceinline__ void store8(char *at, const float (&f)[8], float scale, float reciprocal) {
   if (kFp8) {
@@ -76,10 +77,16 @@ struct AppendArgs {
   int rows, heads, table_rows, page_shift;  // page_shift: log2 of the page size, -1 if it is no power of two
 };
 
-// A thread takes 8 elements of the first half of a head and their 8 partners of the second half: threadIdx = (vector of the half head, head, row of the
-// CTA), so that nothing is divided to find them.  What it rotates is loaded first, and the row's place is found meanwhile: a thread that
-// looked the place up before it loaded anything took 98 us for 16384 rows of 36 heads of 128.
-template <bool kFp8>
+// Heads per thread: one for few rows, where only the way to the result counts, and three from kManyRows rows on, whose loads are in flight
+// together.  One / three, 48 heads of 128, us: 1 row 1.67 / 2.07, 64 rows 1.79 / 2.23, 256 rows 2.61 / 2.71, 512 rows 5.08 / 4.63, 2048 rows
+// 13.9 / 12.8, 16384 rows in e4m3 91.2 / 82.
+constexpr int kManyRows = 512, kHeadsOfMany = 3;
+
+// A thread takes 8 elements of the first half of a head and their 8 partners of the second half: threadIdx = (vector of the half head, head,
+// row of the CTA), so that nothing is divided to find them; its further heads are blockDim.y apart and share the row's place and the tables.
+// What it rotates is loaded first, and the row's place is found meanwhile: a thread that looked the place up before it loaded anything took
+// 98 us for 16384 rows of 36 heads of 128, 61.7 now (79 % of the rate of a copy).
+template <bool kFp8, int kHeads>
 __global__ void __launch_bounds__(512) rope_append_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ PagedCache c) {
   const int half = c.head_dim >> 1, v = threadIdx.x, row = blockIdx.x * blockDim.z + threadIdx.z, all_heads = a.heads + 2 * c.kv_heads;
   ptx::grid_dependency_wait();
@@ -87,16 +94,21 @@ __global__ void __launch_bounds__(512) rope_append_kernel(const __grid_constant_
   if (row >= a.rows) return;
   const int position = a.positions[row], seq = a.sequences != nullptr ? a.sequences[row] : row;
   const __nv_bfloat16 *x = a.qkv + row * a.row_stride + v * 8;
-  int head = blockIdx.y * blockDim.y + threadIdx.y;
-  if (head >= all_heads) return;
-  uint4 w1 = *reinterpret_cast<const uint4 *>(x + head * c.head_dim), w2 = *reinterpret_cast<const uint4 *>(x + head * c.head_dim + half);
+  const int head0 = blockIdx.y * blockDim.y * kHeads + threadIdx.y;
+  uint4 w1[kHeads], w2[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int head = head0 + i * blockDim.y;
+    if (head >= all_heads) break;
+    w1[i] = *reinterpret_cast<const uint4 *>(x + head * c.head_dim);
+    w2[i] = *reinterpret_cast<const uint4 *>(x + head * c.head_dim + half);
+  }
   const bool padding = position < 0;
   const bool in_tables = !padding && position < a.table_rows && position < paged_capacity(c) && seq >= 0 && seq < c.seqs;
-  const int kv = head - a.heads;  // key head, or kv_heads + value head
   uint4 wc1, wc2, ws1, ws2;
   int page = 0, in_page = 0;
   if (in_tables) {
-    if (kv < c.kv_heads) {
+    if (head0 < a.heads + c.kv_heads) {
       const __nv_bfloat16 *cos_at = a.cos_t + (size_t)position * c.head_dim + v * 8, *sin_at = a.sin_t + (size_t)position * c.head_dim + v * 8;
       wc1 = *reinterpret_cast<const uint4 *>(cos_at);
       wc2 = *reinterpret_cast<const uint4 *>(cos_at + half);
@@ -108,47 +120,52 @@ __global__ void __launch_bounds__(512) rope_append_kernel(const __grid_constant_
     page = c.page_table[seq * c.table_stride + entry];
   }
   const bool good = in_tables && page >= 0 && page < c.pages;
-  if (!good && !padding && head == 0 && v == 0 && a.error_flag != nullptr) atomicExch(a.error_flag, kBadCacheIndex);
-  float x1[8], x2[8];
-  unpack8(w1, x1);
-  unpack8(w2, x2);
-  if (!good) {
-    // a padding row gives zeros, a row without a place NaN; neither touches the cache
-    const float fill = padding ? 0.0f : __int_as_float(0x7fffffff);
+  if (!good && !padding && head0 == 0 && v == 0 && a.error_flag != nullptr) atomicExch(a.error_flag, kBadCacheIndex);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x1[j] = x2[j] = fill;
-  } else if (kv < c.kv_heads) {
-    float c1[8], c2[8], s1[8], s2[8];
-    unpack8(wc1, c1);
-    unpack8(wc2, c2);
-    unpack8(ws1, s1);
-    unpack8(ws2, s2);
+  for (int i = 0; i < kHeads; ++i) {
+    const int head = head0 + i * blockDim.y, kv = head - a.heads;  // key head, or kv_heads + value head
+    if (head >= all_heads) break;
+    float x1[8], x2[8];
+    unpack8(w1[i], x1);
+    unpack8(w2[i], x2);
+    if (!good) {
+      // a padding row gives zeros, a row without a place NaN; neither touches the cache
+      const float fill = padding ? 0.0f : __int_as_float(0x7fffffff);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {  // the products are exact
-      const float o1 = __fmaf_rn(x1[j], c1[j], -__fmul_rn(x2[j], s1[j]));
-      x2[j] = __fmaf_rn(x2[j], c2[j], __fmul_rn(x1[j], s2[j]));
-      x1[j] = o1;
+      for (int j = 0; j < 8; ++j) x1[j] = x2[j] = fill;
+    } else if (kv < c.kv_heads) {
+      float c1[8], c2[8], s1[8], s2[8];
+      unpack8(wc1, c1);
+      unpack8(wc2, c2);
+      unpack8(ws1, s1);
+      unpack8(ws2, s2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {  // the products are exact
+        const float o1 = __fmaf_rn(x1[j], c1[j], -__fmul_rn(x2[j], s1[j]));
+        x2[j] = __fmaf_rn(x2[j], c2[j], __fmul_rn(x1[j], s2[j]));
+        x1[j] = o1;
+      }
     }
-  }
-  if (kv < c.kv_heads) {
-    __nv_bfloat16 *out = nullptr;
-    if (kv < 0)
-      out = a.q_out + ((size_t)row * a.heads + head) * c.head_dim + v * 8;
-    else if (a.k_out != nullptr)
-      out = a.k_out + ((size_t)row * c.kv_heads + kv) * c.head_dim + v * 8;
-    if (out != nullptr) {
-      *reinterpret_cast<uint4 *>(out) = pack8(x1);
-      *reinterpret_cast<uint4 *>(out + half) = pack8(x2);
+    if (kv < c.kv_heads) {
+      __nv_bfloat16 *out = nullptr;
+      if (kv < 0)
+        out = a.q_out + ((size_t)row * a.heads + head) * c.head_dim + v * 8;
+      else if (a.k_out != nullptr)
+        out = a.k_out + ((size_t)row * c.kv_heads + kv) * c.head_dim + v * 8;
+      if (out != nullptr) {
+        *reinterpret_cast<uint4 *>(out) = pack8(x1);
+        *reinterpret_cast<uint4 *>(out + half) = pack8(x2);
+      }
     }
-  }
-  if (kv >= 0 && good) {
-    const bool value = kv >= c.kv_heads;
-    const int kv_head = value ? kv - c.kv_heads : kv, size = kFp8 ? 1 : 2;
-    char *at = (value ? c.v : c.k) + page * c.page_stride + in_page * c.token_stride + kv_head * c.head_stride + v * 8 * size;
-    const float scale = kFp8 ? (value ? c.v_scale : c.k_scale)[kv_head] : 1.0f;
-    const float reciprocal = kFp8 ? __frcp_rn(scale) : 1.0f;
-    store8<kFp8>(at, x1, scale, reciprocal);
-    store8<kFp8>(at + half * size, x2, scale, reciprocal);
+    if (kv >= 0 && good) {
+      const bool value = kv >= c.kv_heads;
+      const int kv_head = value ? kv - c.kv_heads : kv, size = kFp8 ? 1 : 2;
+      char *at = (value ? c.v : c.k) + page * c.page_stride + in_page * c.token_stride + kv_head * c.head_stride + v * 8 * size;
+      const float scale = kFp8 ? (value ? c.v_scale : c.k_scale)[kv_head] : 1.0f;
+      const float reciprocal = kFp8 ? __frcp_rn(scale) : 1.0f;
+      store8<kFp8>(at, x1, scale, reciprocal);
+      store8<kFp8>(at + half * size, x2, scale, reciprocal);
+    }
   }
 }
 
@@ -172,9 +189,10 @@ cudaError_t run_rope_append_paged(const void *qkv, long long row_stride, int row
   a.heads = heads;
   a.table_rows = table_rows;
   a.page_shift = (cache.page_size & (cache.page_size - 1)) == 0 ? __builtin_ctz((unsigned)cache.page_size) : -1;
-  // CTAs of up to 512 threads, all heads of a row in equal shares; short rows share one of 128
-  const int vecs = cache.head_dim / 16, all_heads = heads + 2 * cache.kv_heads;
-  const int shares = (all_heads * vecs + 511) / 512, share = (all_heads + shares - 1) / shares;
+  // CTAs of up to 512 threads, the heads of a row in equal shares; short rows share one of 128
+  const int vecs = cache.head_dim / 16, all_heads = heads + 2 * cache.kv_heads, per = rows >= kManyRows ? kHeadsOfMany : 1;
+  const int most = 512 / vecs * per, shares = (all_heads + most - 1) / most;
+  const int share = ((all_heads + shares - 1) / shares + per - 1) / per;
   int together = 128 / (share * vecs);
   if (together < 1 || shares > 1) together = 1;
   if (together > 64) together = 64;
@@ -187,7 +205,9 @@ cudaError_t run_rope_append_paged(const void *qkv, long long row_stride, int row
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fp8 ? rope_append_kernel<true> : rope_append_kernel<false>, a, cache);
+  const auto kernel = per == 1 ? (fp8 ? rope_append_kernel<true, 1> : rope_append_kernel<false, 1>)
+                               : (fp8 ? rope_append_kernel<true, kHeadsOfMany> : rope_append_kernel<false, kHeadsOfMany>);
+  return cudaLaunchKernelEx(&cfg, kernel, a, cache);
 }
 
 }  // namespace sharq

@@ -2,19 +2,28 @@
 //
 //   y[m, n] = bf16(scale * sum_k x[m, k] * e2m1[n, k] * ue4m3[n, k / 16] + bias[n])
 //
-// on the payload and the dense scale factors that a quantised linear holds.  Reading the weight (9/16 byte per element) is what it costs.
-// At that rate an SM gets some 42 elements per clock, so the instructions per element count: a pair of codes is one conversion to f16 (exact), its
-// scale one packed product (exact: 2 x 4 significant bits, between 2^-10 and 2688), and mma.sync.m16n8k16 with 16 rows of weight as
-// the large operand does the rest.  The k positions of an instruction may stand for any elements as long as both operands agree, so
-// lane (g, t) takes 32 neighbouring elements of a row, 16 bytes, straight from where it copied them.
+// on the payload and the dense scale factors that a quantised linear holds.  Reading the weight (9/16 byte per element) is what it has to
+// do: at the rate of a copy an SM gets some 42 elements per clock, so the instructions per element count.  A pair of codes is one
+// conversion to f16 (exact), its scale one packed product (exact: 2 x 4 significant bits, between 2^-10 and 2688), and mma.sync.m16n8k16 with 16
+// rows of weight as the large operand does the rest, from registers: the fifth generation's instructions would want the scaled weight
+// in shared memory first, and have no use for so few columns.  The k positions of an instruction may stand for any elements as long
+// as both operands agree, so lane (g, t) takes 32 neighbouring elements of a row, 16 bytes, straight from where they were copied.
 //
-// A warp keeps 256 elements of K of the activation in registers, as f16 operands, and streams that slice of the weight's rows past them, 16 rows at a
-// time, through a ring of its own (tensor-map copies; cp.async needs a pass of the load unit for every row of every copy, half of its time).  f16 is reached by scaling 128 elements of a row by
-// the power of two that takes their largest to [2^14, 2^15): exact but for elements below 2^-39 of it.  Sums are float.  A CTA's 16 warps cover
-// 4096 elements of K (or fewer, and several rows at a time), the CTAs of a cluster the rest; the clusters take equal shares of the rows.  The
-// warps' float sums of some rows meet in shared memory, those of CTAs in distributed shared memory, each added up in a fixed order: the same bits from
-// call to call, no scratch and no second launch.  (With tiles of 128 rows per CTA and the activation in shared memory, 323 instead of SOME
-// instructions per 16 rows x 256 and uneven shares: 28672 x 4096 with one row 19.8 us, with 16 rows 38.)
+// A warp keeps 256 elements of K of up to eight rows of the activation in registers, as f16 operands, and streams that slice of the weight's
+// rows past them, 16 rows at a time, through a ring of its own (tensor-map copies of two such tiles, two stages; with cp.async every 16
+// bytes of every lane passed the load unit, half of the time).  f16 is reached by scaling 128 elements of a row by the power of two that takes their
+// largest to [2^14, 2^15): exact but for elements below 2^-39 of it.  Sums are float; the weight's scale is in the factors of the
+// blocks of 128, so that no sum overflows that the result would not.  A CTA's 16 warps cover 4096 elements of K (or fewer, and several rows at a
+// time), the CTAs of a cluster the rest; the clusters take equal shares of the rows.  The warps' sums of some rows meet in shared memory,
+// those of CTAs in distributed shared memory, each added up in a fixed order: the same bits from call to call, no scratch and no second launch.
+// More than eight rows are two halves of the grid, the second of which reads the weight from L2.
+//
+// 28672 x 4096: one row 14.9 us (4.4 TB/s, 67 % of the rate of a copy), 16 rows 34; 4096 x 4096, one row: 4.8 us.  (Tiles of 128 rows per CTA with
+// the activation in shared memory, 323 instead of 265 instructions per 16 rows x 256 and uneven shares: 19.8, 38 and 6.6.)  The loop's
+// instructions take 6.8 us of the 14.9 to issue, beside the copies' 10; the activation's way to the registers comes before, the join after.
+// Both eights of 16 rows in one warp, the weight converted once, took 40 us instead of 34 and, for 13 rows of 4608 x 3584,
+// 13.6 instead of 8.1: every SM then reads all of the activation, its operands leave too few registers, and the sums have
+// room for two tiles at a time.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -61,6 +61,39 @@ def test_append(rows, heads, kv, dim, page, fp8, order):
     assert torch.equal(only, q)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+# rows whose threads take several heads, in numbers of heads that leave some without; heads that fill a CTA to the last thread
+@pytest.mark.parametrize("rows,heads,kv,dim,page", [(700, 5, 1, 64, 8), (515, 70, 5, 128, 32), (512, 2, 1, 16, 1), (600, 13, 2, 80, 5),
+                                                    (2, 510, 1, 80, 4), (513, 510, 1, 80, 4)])
+def test_append_of_many_rows_or_heads(rows, heads, kv, dim, page, fp8):
+    test_append(rows, heads, kv, dim, page, fp8, "hnd")
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_append_of_many_rows_equals_appends_of_few(fp8):
+    from sharq_b200 import ops
+
+    rows, heads, kv, dim, page = 1200, 7, 2, 64, 16
+    g = torch.Generator().manual_seed(3)
+    table, pages = P.make_table([600, 600], page, 2, 5)
+    table[1, 20] = pages + 3  # no such page
+    cos, sin = P.rope_tables(600, dim)
+    qkv = torch.randn(rows, (heads + 2 * kv) * dim, generator=g).to(torch.bfloat16).cuda()
+    sequences = torch.arange(rows, dtype=torch.int32).cuda() % 2
+    positions = torch.arange(rows, dtype=torch.int32).cuda() // 2
+    positions[::13] = -1
+    positions[70] = 600  # outside the tables
+    a, b = (P.make_cache(pages, kv, page, dim, fp8, 3) for _ in range(2))
+    qa, ka = _append(ops, qkv, heads, kv, dim, cos, sin, positions, table, a, sequences=sequences, return_k=True)
+    parts = [_append(ops, qkv[i:i + 200], heads, kv, dim, cos, sin, positions[i:i + 200], table, b, sequences=sequences[i:i + 200], return_k=True)
+             for i in range(0, rows, 200)]
+    with pytest.raises(RuntimeError, match="cache"):
+        ops.check_device_errors()
+    for got, want in ((qa, torch.cat([p[0] for p in parts])), (ka, torch.cat([p[1] for p in parts])), (a[0], b[0]), (a[1], b[1])):
+        assert torch.equal(got.contiguous().view(torch.uint8), want.contiguous().view(torch.uint8))
+    assert bool(ka[70].isnan().all()) and not bool(ka[13].any())
+
+
 def test_append_of_rows_without_sequences_equals_listed_ones():
     from sharq_b200 import ops
 
