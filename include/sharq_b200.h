@@ -382,7 +382,7 @@ int sharq_tp_reduce_rmsnorm_prepare_allgather(const void *partial_blocks, const 
  *
  * k and v are device arrays [pages][kv_heads][page_size][head_dim] of bf16 or, when k_scale and v_scale are given (float [kv_heads] on the
  * device), of e4m3 values that stand for value * scale[head].  The strides (in elements, the same for both, multiples of 16 bytes) may
- * order the first three dimensions in any way; head_dim elements are contiguous.  Token j of sequence s lies in slot j % page_size of
+ * order the first three dimensions in any way, without overlap; head_dim elements are contiguous.  Token j of sequence s lies in slot j % page_size of
  * page page_table[s * page_table_stride + j / page_size]; entries behind a sequence's last page are not read. */
 typedef struct sharq_paged_cache {
   void *k, *v;
@@ -407,7 +407,7 @@ int sharq_rope_append_paged(const void *qkv_bf16, int64_t row_stride, int rows, 
 /* Attention of one new token per sequence over the cache: out[s, h] = sum_j softmax_j(scale * q[s, h] . k[j]) v[j] over the first
  * lengths[s] tokens of sequence s (the new one among them), query head h reading key/value head h / (heads / kv_heads).  q bf16 with
  * q_row / q_head elements between sequences / heads (multiples of 8), out bf16 [sequences, heads, head_dim].  A sequence of length 0 gives
- * zeros.  A length that is negative or more than the page table holds, or a page outside the cache, makes the rows of that sequence NaN and
+ * zeros.  A length that is negative or more than the page table holds (or 2^31 - 65536), or a page outside the cache, makes the rows of that sequence NaN and
  * stores 0x402 in *error_flag (may be NULL; 0x403: a wait ran out).  head_dim 64 or 128; heads a multiple of kv_heads.  workspace:
  * sharq_paged_attention_workspace_bytes(heads, cache) bytes of scratch (0: none, by the shape of the cache and its table alone), 16-byte aligned,
  * not shared by calls that overlap.  Where the table holds few tokens per sequence the call is one launch without scratch, else two: a
@@ -420,7 +420,7 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
 /* Product of m (1 to 16) unquantised bf16 rows (x_row elements between them, a multiple of 8) with a 4-bit weight:
  * y[m, n] = bf16(scale * scale_dev[0] * sum_k x[m, k] * W[n, k] + bias[n]), W = payload qw [n, k/2] times the dense scale factors sfw_dense, as
  * sharq_quantize_w32_shared and sharq_quantize_nvfp4 make them.  scale_dev (float on the device) and bias (bf16 [n]) may be NULL.  Float
- * sums, one rounding.  k % 64 == 0; x, qw and sfw_dense 16-byte aligned.  A wait that ran out stores 0x404 in *error_flag (may be NULL). */
+ * sums, one rounding.  k % 64 == 0, k <= 2^24; x, qw and sfw_dense 16-byte aligned.  A wait that ran out stores 0x404 in *error_flag (may be NULL). */
 int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, int k, const void *qw, const void *sfw_dense,
                              const float *scale_dev, float scale, const void *bias_bf16, void *y_bf16, int *error_flag, void *stream);
 

@@ -73,6 +73,12 @@ int paged_cache(const sharq_paged_cache *c, sharq::PagedCache *out, bool *fp8) {
   return 0;
 }
 
+// Strides that step over a head's elements at least (a dimension of one element needs none).
+bool strides_reach(const sharq_paged_cache &c) {
+  return (c.pages == 1 || c.page_stride >= c.head_dim) && (c.kv_heads == 1 || c.head_stride >= c.head_dim) &&
+         (c.page_size == 1 || c.token_stride >= c.head_dim);
+}
+
 }  // namespace
 
 extern "C" {
@@ -777,6 +783,7 @@ int sharq_rope_append_paged(const void *qkv_bf16, int64_t row_stride, int rows, 
   SHARQ_REQUIRE(qkv_bf16 && cos_bf16 && sin_bf16 && positions && q_out_bf16, "null buffer");
   SHARQ_REQUIRE(rows >= 0 && heads > 0 && table_rows > 0, "rows must be >= 0, heads and table_rows positive");
   SHARQ_REQUIRE(c.head_dim % 16 == 0 && c.head_dim <= 256, "head_dim must be a multiple of 16, at most 256, got %d", c.head_dim);
+  SHARQ_REQUIRE(strides_reach(*cache), "elements of the cache must not overlap");
   SHARQ_REQUIRE((int64_t)heads + 2 * (int64_t)c.kv_heads <= 65536, "at most 65536 heads in a row");
   SHARQ_REQUIRE(row_stride >= ((int64_t)heads + 2 * (int64_t)c.kv_heads) * c.head_dim && row_stride % 8 == 0,
                 "row_stride must cover all heads and be a multiple of 8");
@@ -802,6 +809,7 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
   if (paged_cache(cache, &c, &fp8)) return 1;
   SHARQ_REQUIRE(q_bf16 && lengths && out_bf16, "null buffer");
   SHARQ_REQUIRE(c.head_dim == 64 || c.head_dim == 128, "head_dim must be 64 or 128, got %d", c.head_dim);
+  SHARQ_REQUIRE(strides_reach(*cache), "elements of the cache must not overlap");
   SHARQ_REQUIRE(heads > 0 && heads % c.kv_heads == 0 && heads <= 65536, "heads must be a positive multiple of kv_heads, at most 65536");
   SHARQ_REQUIRE((int64_t)c.seqs * heads <= 0x7fffffff &&
                     (int64_t)c.seqs * (sharq::paged_capacity(c) / 16 + 4) <= 0x70000000 / (c.kv_heads * (int64_t)((heads / c.kv_heads + 15) / 16)),
@@ -821,6 +829,7 @@ int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, in
   SHARQ_REQUIRE(m >= 1 && m <= sharq::kWeightOnlyMaxRows, "weight_only_linear takes 1 to %d rows, got %d", sharq::kWeightOnlyMaxRows, m);
   SHARQ_REQUIRE(n > 0 && n <= 65535 * 128, "N must be in [1, %d], got %d", 65535 * 128, n);
   SHARQ_REQUIRE(k > 0 && k % 64 == 0, "weight_only_linear requires K to be a multiple of 64, got %d", k);
+  SHARQ_REQUIRE(k <= 1 << 24, "weight_only_linear takes K up to %d, got %d", 1 << 24, k);
   SHARQ_REQUIRE(m == 1 || (x_row >= k && x_row % 8 == 0), "the rows of x must not overlap and be a multiple of 8 elements apart");
   SHARQ_REQUIRE(aligned16(x_bf16) && aligned16(qw) && aligned16(sfw_dense), "x, qw and sfw_dense must be 16-byte aligned");
   return check_cuda(sharq::run_weight_only(x_bf16, x_row, m, n, k, qw, sfw_dense, scale_dev, scale, bias_bf16, y_bf16, error_flag,

@@ -21,10 +21,10 @@ struct PagedCache {
   int seqs, max_pages, pages, page_size, kv_heads, head_dim;
 };
 
-// Tokens that a row of the page table can hold, within an int.
+// Tokens that a row of the page table can hold, within an int, and so far from its end that the tokens of a few tiles beyond are too.
 __host__ __device__ inline int paged_capacity(const PagedCache &c) {
   const long long n = (long long)c.max_pages * c.page_size;
-  return n > 0x7fffffffLL ? 0x7fffffff : (int)n;
+  return n > 0x7fff0000LL ? 0x7fff0000 : (int)n;
 }
 
 cudaError_t run_rope_append_paged(const void *qkv, long long row_stride, int rows, int heads, const void *cos_t, const void *sin_t,

@@ -25,7 +25,8 @@
 // e4m3 caches go through f16: their values are exact in it, queries are scaled to it by a power of two per head (a value below 2^-39 of its
 // head's largest is lost), and probabilities carry a factor of 2^10, so that those down to 2^-24 of the maximum keep f16's full precision.  For bf16
 // caches the probabilities enter as the sum of two bf16 numbers, 16 bits (rounded to one they made half of the result's error, and the reading of the
-// cache hides the second product).
+// cache hides the second product); both are positive, for an infinite value has an infinite product with either.  They carry a factor of 2^-32, so that
+// no sum of finite values overflows; 2^-94 of the maximum and less is 0.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -42,7 +43,7 @@ namespace {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-constexpr float kF16Lift = 10.0f;
+constexpr float kF16Lift = 10.0f, kBf16Lift = -32.0f;  // log2 of a factor of the probabilities
 constexpr int kItemCost = 2;
 constexpr int kStretchLeast = 4;
 constexpr int kAttnClusterMost = 8;
@@ -552,7 +553,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 #pragma unroll
       for (int n = 0; n < kN; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) base[n][j] = (m[n][j] == -INFINITY ? 0.0f : m[n][j]) - (kFp8 ? kF16Lift : 0.0f);
+        for (int j = 0; j < 2; ++j) base[n][j] = (m[n][j] == -INFINITY ? 0.0f : m[n][j]) - (kFp8 ? kF16Lift : kBf16Lift);
 #pragma unroll
       for (int b = 0; b < kTokens / 16; ++b) {
         uint32_t pb[kN][2], pb_lo[kN][2];
@@ -570,9 +571,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           } else {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const uint32_t hi = pack_bf16(p[2 * j], p[2 * j + 1]);
-              pb[n][j] = movmatrix(hi);
-              pb_lo[n][j] = movmatrix(pack_bf16(p[2 * j] - __uint_as_float(hi << 16), p[2 * j + 1] - __uint_as_float(hi & 0xFFFF0000u)));
+              // the upper half of the bits, and what they leave, with the last bit set: never 0 beside an upper half that is not
+              const uint32_t x = __float_as_uint(p[2 * j]) | 1, y = __float_as_uint(p[2 * j + 1]) | 1;
+              pb[n][j] = movmatrix(__byte_perm(x, y, 0x7632));
+              pb_lo[n][j] = movmatrix(pack_bf16(__uint_as_float(x) - __uint_as_float(x & 0xFFFF0000u),
+                                                __uint_as_float(y) - __uint_as_float(y & 0xFFFF0000u)));
             }
           }
         }

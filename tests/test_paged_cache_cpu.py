@@ -111,3 +111,24 @@ def test_weight_only_arguments_that_are_refused():
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.weight_only_linear(torch.zeros(1, 64, dtype=torch.bfloat16), torch.zeros(4, 32, dtype=torch.uint8),
                                torch.zeros(512, dtype=torch.uint8), 1.0)
+
+
+@pytest.mark.parametrize("change", [dict(page_stride=0), dict(head_stride=0), dict(token_stride=0), dict(token_stride=64)])
+def test_caches_whose_elements_overlap_are_refused(change):
+    from sharq_b200 import _lib
+
+    L = _lib.lib()
+    one = ctypes.c_void_p(256)
+    assert L.sharq_paged_attention(one, 512, 128, 4, cache(**change), one, 0.1, one, one, 1 << 30, None, None) != 0
+    assert b"must not overlap" in L.sharq_last_error()
+    assert L.sharq_rope_append_paged(one, 1024, 2, 4, one, one, 64, one, None, cache(**change), one, None, None, None) != 0
+    assert b"must not overlap" in L.sharq_last_error()
+
+
+def test_a_weight_whose_rows_are_too_long_is_refused():
+    from sharq_b200 import _lib
+
+    L = _lib.lib()
+    one = ctypes.c_void_p(256)
+    assert L.sharq_weight_only_linear(one, 2 ** 31 - 64, 1, 1, 2 ** 31 - 64, one, one, None, 1.0, None, one, None, None) != 0
+    assert b"K up to" in L.sharq_last_error()

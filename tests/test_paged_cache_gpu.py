@@ -434,3 +434,48 @@ def test_attention_of_shared_pages_drafts_and_broadcast_queries():
     assert ops.paged_attention(q, k, v, table, n, out=q) is not None
     assert torch.equal(q, want)
     ops.check_device_errors()
+
+
+@pytest.mark.parametrize("room", ["short", "wide"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_with_infinite_and_with_the_largest_values(dim, room):
+    """An infinite value of a token that counts is infinite in the result, whatever its probability; the mean of finite ones is finite."""
+    from sharq_b200 import ops
+
+    lengths, page, kv = [1, 40, 700, 5000], 16, 2
+    table, pages = P.make_table(lengths, page, 1, 1)
+    k, v, _, _ = P.make_cache(pages, kv, page, dim, False, 7)
+    largest = torch.finfo(torch.bfloat16).max
+    v[..., 5] = float("inf")
+    v[..., 6] = -float("inf")
+    v[..., 7] = largest
+    v[..., 8] = -largest
+    for i, n in enumerate(lengths):  # one token of every sequence
+        v[table[i, (n // 2) // page].long(), :, n // 2 % page, 9] = float("inf")
+    if room == "wide":
+        table = wide(table, page)
+    q = torch.randn(4, 6, dim, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    got = ops.paged_attention(q, k, v, table, n)
+    ops.check_device_errors()
+    assert bool((got[..., [5, 9]] == float("inf")).all()) and bool((got[..., 6] == -float("inf")).all())
+    # the mean is the largest value but for roundings of some 2^-23 of it, which bf16 does not see
+    assert bool((got[..., 7] == largest).all()) and bool((got[..., 8] == -largest).all())
+    rest = [d for d in range(dim) if d not in (5, 6, 7, 8, 9)]
+    out, size, reach = P.attention64(q, P.values64(k, None), P.values64(v, None), table, lengths)
+    bound = P.attention_bound(out, size, reach, dim, max(lengths), False)
+    assert bool(((got.double() - out).abs() <= bound)[..., rest].all())
+
+
+def test_a_length_near_the_end_of_an_int_is_reported():
+    from sharq_b200 import ops
+
+    page = 65536
+    k, v = (torch.zeros(1, 1, page, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    table = torch.zeros(2, 32768, dtype=torch.int32, device="cuda")
+    q = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    n = torch.tensor([2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    got = ops.paged_attention(q, k, v, table, n)
+    with pytest.raises(RuntimeError, match="paged cache"):
+        ops.check_device_errors()
+    assert bool(got.isnan().all())
