@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 
 // Eight neighbouring elements of a head into the cache.  The quotient by the scale is the float division's, by its residual from a product with
 // the correctly rounded reciprocal (Markstein); 1024 and more saturate in e4m3 whatever the last bits, and a zero
-// keeps its sign.  (16 divisions: 102.5 instead of 91.2 us for 16384 rows of 36 heads of 128, one head per thread.)
+// keeps its sign.  (16 divisions: 78 instead of 73 us for 16384 rows of 48 heads of 128.)
 template <bool kFp8>
 __device__ __forceinline__ void store8(char *at, const float (&f)[8], float scale, float reciprocal) {
   if (kFp8) {
@@ -78,16 +78,17 @@ struct AppendArgs {
 };
 
 // Heads per thread: one for few rows, where only the way to the result counts, and three from kManyRows rows on, whose loads are in flight
-// together.  One / three, 48 heads of 128, us: 1 row 1.67 / 2.07, 64 rows 1.79 / 2.23, 256 rows 2.61 / 2.71, 512 rows 5.08 / 4.63, 2048 rows
-// 13.9 / 12.8, 16384 rows in e4m3 91.2 / 82.
+// together.  One / three, 48 heads of 128, us: 1 row 1.7 / 2.3, 64 rows 1.8 / 2.3, 256 rows 2.4 / 2.9, 512 rows 5.0 / 4.4, 2048 rows
+// 16.1 / 12.0, 16384 rows in e4m3 114 / 73.  (Two: 77.)
 constexpr int kManyRows = 512, kHeadsOfMany = 3;
 
 // A thread takes 8 elements of the first half of a head and their 8 partners of the second half: threadIdx = (vector of the half head, head,
 // row of the CTA), so that nothing is divided to find them; its further heads are blockDim.y apart and share the row's place and the tables.
 // What it rotates is loaded first, and the row's place is found meanwhile: a thread that looked the place up before it loaded anything took
-// 98 us for 16384 rows of 36 heads of 128, 61.7 now (79 % of the rate of a copy).
+// 98 us for 16384 rows of 36 heads of 128, 53.5 now (91 % of the rate of a copy).  With the 84 registers that the compiler takes without the
+// second bound (64) it is 61.7, for want of warps: what it has to spill costs less.
 template <bool kFp8, int kHeads>
-__global__ void __launch_bounds__(512) rope_append_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ PagedCache c) {
+__global__ void __launch_bounds__(512, 2) rope_append_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ PagedCache c) {
   const int half = c.head_dim >> 1, v = threadIdx.x, row = blockIdx.x * blockDim.z + threadIdx.z, all_heads = a.heads + 2 * c.kv_heads;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();

@@ -683,7 +683,8 @@ class SharqDecoder(torch.nn.Module):
     def decode_step(self, token_ids: torch.Tensor, cache: PagedKVCache, positions: torch.Tensor, lengths: torch.Tensor,
                     reference: bool = False, weight_only: bool = False) -> torch.Tensor:
         """The device part of decode, for capture in a CUDA graph: positions and lengths (int32 [B], device) of the new tokens and of the
-        sequences with them, whose pages have been reserved; the cache's own lengths stay."""
+        sequences with them, whose pages have been reserved; the cache's own lengths stay.  A graph reads the page table as wide as it was
+        at the capture: reserve the tokens of all replays before it."""
         x, delta = self.embed[token_ids][:, None], None
         for i, layer in enumerate(self.layers):
             kv = cache.layer(i, positions, None, lengths)

@@ -230,7 +230,7 @@ class QLinearLayer(nn.Module):
     def forward_weight_only(self, x: torch.Tensor) -> torch.Tensor:
         """The layer on an unquantised activation [..., in_features] of at most 16 rows: the 4-bit weight is the only quantised
         operand, one launch (ops.weight_only_linear).  For decode steps of few tokens, which read the weight once either way."""
-        x2 = x.reshape(-1, x.shape[-1]).to(torch.bfloat16)
+        x2 = x.reshape(-1, x.shape[-1]).to(torch.bfloat16).contiguous()
         sf = self.scale_w_dense if self.quant_type == "SHARQ" else self.scale_w
         bias = self.bias
         folded = bias if (bias is not None and bias.dtype == torch.bfloat16 and bias.dim() == 1 and bias.is_contiguous()

@@ -162,3 +162,16 @@ def test_refusals():
     refuse("must not overlap", x[:1].expand(2, 256), qw, sf, 1.0)
     refuse("16-byte aligned", torch.zeros(2, 260, dtype=torch.bfloat16).cuda().view(-1)[4:516].view(2, 256), qw, sf, 1.0)
     assert ops.weight_only_linear(x[:0], qw, sf, 1.0).shape == (0, 128)
+
+
+def test_layer_takes_activations_of_any_stride():
+    from sharq_b200.qlinear import QLinearLayer
+
+    g = torch.Generator().manual_seed(2)
+    w = torch.nn.Linear(192, 40, bias=True)
+    w.weight.data = (0.05 * torch.randn(40, 192, generator=g))
+    layer = QLinearLayer(w.to(torch.bfloat16).cuda(), quant_type="SHARQ")
+    x = torch.randn(192, 6, generator=g).to(torch.bfloat16).cuda().t()
+    whole = torch.randn(5, 200, generator=g).to(torch.bfloat16).cuda()
+    for strided in (x, whole[:, 3:195], whole[:1, 3:195].expand(4, 192)):
+        assert torch.equal(layer.forward_weight_only(strided), layer.forward_weight_only(strided.clone(memory_format=torch.contiguous_format)))
