@@ -10,7 +10,7 @@
 // as both operands agree, so lane (g, t) takes 32 neighbouring elements of a row, 16 bytes, straight from where they were copied.
 //
 // A warp keeps 256 elements of K of up to eight rows of the activation in registers, as f16 operands, and streams that slice of the weight's
-// rows past them, 16 rows at a time, through a ring of its own (tensor-map copies of two such tiles, two stages; with cp.async every 16
+// rows past them, 16 rows at a time, through a ring of its own (one tensor-map copy for each, two of them a stage; with cp.async every 16
 // bytes of every lane passed the load unit, half of the time).  f16 is reached by scaling 128 elements of a row by the power of two that takes their
 // largest to [2^14, 2^15): exact but for elements below 2^-39 of it.  Sums are float; the weight's scale is in the factors of the
 // blocks of 128, so that no sum overflows that the result would not.  A CTA's 16 warps cover 4096 elements of K (or fewer, and several rows at a
@@ -18,12 +18,12 @@
 // those of CTAs in distributed shared memory, each added up in a fixed order: the same bits from call to call, no scratch and no second launch.
 // More than eight rows are two halves of the grid, the second of which reads the weight from L2.
 //
-// 28672 x 4096: one row 14.9 us (4.4 TB/s, 67 % of the rate of a copy), 16 rows 34; 4096 x 4096, one row: 4.8 us.  (Tiles of 128 rows per CTA with
-// the activation in shared memory, 323 instead of 265 instructions per 16 rows x 256 and uneven shares: 19.8, 38 and 6.6.)  The loop's
-// instructions take 6.8 us of the 14.9 to issue, beside the copies' 10; the activation's way to the registers comes before, the join after.
-// Both eights of 16 rows in one warp, the weight converted once, took 40 us instead of 34 and, for 13 rows of 4608 x 3584,
-// 13.6 instead of 8.1: every SM then reads all of the activation, its operands leave too few registers, and the sums have
-// room for two tiles at a time.
+// 28672 x 4096: one row 14.5 us (4.6 TB/s, 70 % of the rate of a copy), 8 rows 17.6, 16 rows 28.9; 4096 x 4096, one row: 4.9 us.  (Tiles of 128
+// rows per CTA with the activation in shared memory, 323 instead of 265 instructions per 16 rows x 256 and uneven shares: 19.8, 38 with 16
+// rows and 6.6.)  The loop's instructions take 7 us to issue, beside the copies' 10; the activation's way to the registers comes before, the
+// join after.  Both eights of 16 rows in one warp, the weight converted once for 128 elements of K of each, took 34 us instead of 29 and, for
+// 13 rows of 4608 x 3584, 8.8 instead of 8.0: twice as many parts to join, and clusters of two CTAs where one does.  Joining a chunk of rows while
+// the next is multiplied gained nothing.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -41,18 +41,19 @@ namespace {
 
 constexpr int kWoWarps = 16;
 constexpr int kWoThreads = 32 * kWoWarps;
-constexpr int kWoSlice = 256;               // elements of K of a warp
 constexpr int kWoStages = 2;
-constexpr int kWoCodes = 32 * 128, kWoScales = 4 * 128;  // 32 rows x 256 codes; 8 rows x 16 bytes of scale factors for each of 4 x 64 elements
-constexpr int kWoRing = kWoStages * (kWoCodes + kWoScales);
-constexpr int kWoParts = 70144;             // bytes for the warps' float sums: of all of a CTA's tiles, or of two chunks of them
-constexpr int kWoSums = 6144;               // for a CTA's float sums of a chunk, twice
-constexpr int kWoXWarp = 8 * 512;            // of a warp's slice of 8 rows on its way to the registers
+constexpr int kWoSums = 6144;     // bytes for a CTA's float sums of a chunk, twice
+constexpr int kWoXWarp = 4096;    // of a warp's slice of the activation on its way to the registers
 constexpr int kWoClusterMost = 8;
-constexpr int kWoFactors = kWoWarps * kWoRing + kWoParts + 2 * kWoSums;
-constexpr int kWoBars = kWoFactors + kWoWarps * 64;  // the barriers behind it all, and the flag of a wait that ran out
-constexpr int kWoSmem = kWoBars + kWoWarps * kWoStages * 8 + 8;
-static_assert(kWoSmem <= 232448 && kWoWarps * kWoXWarp <= kWoParts, "what a CTA can have");
+constexpr int kWoSmem = 232448;
+constexpr int kWoSlice = 256;                                 // elements of K of a warp
+constexpr int kWoBox = 8 * kWoSlice / 2;                      // bytes of the codes of 8 rows
+constexpr int kWoCodes = 4 * kWoBox, kWoScales = 4 * 128;     // of 32 rows; 8 rows x 16 bytes of scale factors for each of 4 x 64 elements
+constexpr int kWoRing = kWoStages * (kWoCodes + kWoScales);
+constexpr int kWoBars = kWoSmem - kWoWarps * kWoStages * 8 - 16;  // the barriers behind it all, and the flag of a wait that ran out
+constexpr int kWoFactors = kWoBars - kWoWarps * 64;
+constexpr int kWoParts = kWoFactors - 2 * kWoSums - kWoWarps * kWoRing;  // for the warps' float sums: of all of a CTA's tiles, or of two chunks of them
+static_assert(kWoWarps * kWoXWarp <= kWoParts && kWoParts % 16 == 0 && kWoBars % 16 == 0, "what a CTA can have");
 
 __device__ __forceinline__ uint4 wo_lds16(uint32_t smem) {
   uint4 v;
@@ -101,15 +102,6 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float f) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// a float of CTA `rank`'s shared memory (addr: this CTA's address of the same variable); not volatile, so that loads go out together
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, int rank) {
-  uint32_t remote;
-  float v;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
-  return v;
-}
-
 __device__ __forceinline__ void copy_2d(uint32_t dst, const CUtensorMap *m, int c0, int c1, uint64_t *bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(m),
                "r"(ptx::smem_u32(bar)), "r"(c0), "r"(c1)
@@ -118,6 +110,12 @@ __device__ __forceinline__ void copy_2d(uint32_t dst, const CUtensorMap *m, int 
 __device__ __forceinline__ void copy_3d(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, uint64_t *bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(m),
                "r"(ptx::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+
+__device__ __forceinline__ void copy_4d(uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2, int c3, uint64_t *bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(m),
+               "r"(ptx::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
 }
 
@@ -136,18 +134,23 @@ struct WeightOnlyArgs {
   int cluster;      // CTAs
   int tiles;        // of 16 rows, of the whole weight
   int per_cluster;  // tiles
-  int chunk;        // tiles whose sums are joined at a time
+  int chunk;        // pairs of tiles whose sums are joined at a time
+  int whole;        // blocks of 128 rows
   int parts_at, parts_bytes;  // of the space of kWoParts bytes, for the warps' sums; they are all of it unless the activation is read more than once
-  unsigned per_tile_magic[2]; // ceil(2^32 / (16 rows)) of the first and second eight rows
+  unsigned per_tile_magic[2];  // ceil(2^32 / floats of a tile's sums) for the first and the second eight rows
+  bool by_four;             // four neighbouring results are one store, and so many of the bias one load
 };
 
 // Tile j: rows 32 i + 8 c + g of a block of 128, i = 2 h and 2 h + 1, with c = j / 2 % 4 and h = j % 2: the scale factors of a pair of tiles, for
 // 64 elements of K, are 16 neighbouring bytes per g.  Pairs are copied together; a share of the rows may begin or end within one.
 __device__ __forceinline__ int tile_row(int j) { return (j >> 3) * 128 + (j & 1) * 64 + ((j >> 1) & 3) * 8; }
 
-// blockIdx.x: CTA of the cluster, blockIdx.y: cluster, blockIdx.z: eight rows of the activation.
+// blockIdx.x: CTA of the cluster, blockIdx.y: cluster, blockIdx.z: eight rows of the activation.  kPasses: a cluster goes along K several times
+// (more than 32768 elements), which in the same kernel cost all others a tenth of their time, for the registers.
+template <bool kPasses>
 __global__ void __launch_bounds__(kWoThreads, 1)
-    weight_only_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_sf, const __grid_constant__ WeightOnlyArgs a) {
+    weight_only_kernel(const __grid_constant__ CUtensorMap map_tiles, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_sf,
+                       const __grid_constant__ WeightOnlyArgs a) {
   extern __shared__ __align__(1024) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row_first = blockIdx.z * 8, m = min(8, a.m - row_first);
@@ -159,7 +162,7 @@ __global__ void __launch_bounds__(kWoThreads, 1)
   if (lane == 0) {
     for (int i = 0; i < kWoStages; ++i) ptx::mbar_init(bars + i, 1);
     ptx::fence_barrier_init();
-    ptx::tma_prefetch_desc(&map_w);
+    ptx::tma_prefetch_desc(&map_tiles);
     ptx::tma_prefetch_desc(&map_sf);
   }
   unsigned char *space = smem + kWoWarps * kWoRing;
@@ -170,12 +173,12 @@ __global__ void __launch_bounds__(kWoThreads, 1)
   const int j0 = blockIdx.y * a.per_cluster, j1 = min(j0 + a.per_cluster, a.tiles);
   const int k_first = (blockIdx.x * a.slices + slice_in) * kWoSlice, k_pass = a.cluster * a.slices * kWoSlice;
 
-  // The pairs of this warp in order: those of its row group, pass by pass within a chunk of tiles whose sums are joined together.
-  int l_chunk = j0, l_pass = 0, l_pair = (j0 >> 1) + row_group, l_end = min(j0 + a.chunk, j1), put = 0, k0 = k_first;
-  if (!works || 2 * l_pair >= l_end) l_chunk = j1;  // fewer pairs than row groups
+  // The pairs of this warp in order: those of its row group, pass by pass within a chunk of pairs whose sums are joined together.
+  const int p0 = j0 >> 1, p1 = (j1 + 1) >> 1;
+  int l_chunk = p0, l_pass = 0, l_pair = works ? p0 + row_group : p1, put = 0, k0 = k_first;
   __syncthreads();
   const bool chosen = ptx::elect_one();
-  if (l_chunk < j1 && chosen) {
+  if (l_pair < p1 && chosen) {
     // the first rows into L2, where they may be as old as they like: ahead of the wait for the kernels before
 #pragma unroll 1
     for (int i = 0; i < 4; ++i) ptx::tma_prefetch_l2_2d(&map_w, k0 / 2, tile_row(2 * l_pair) + 32 * i);
@@ -184,26 +187,29 @@ __global__ void __launch_bounds__(kWoThreads, 1)
   ptx::grid_launch_dependents();
 
   auto load = [&]() {
-    if (l_chunk < j1) {
+    if (l_pair < p1) {
       if (chosen) {
         // rows and elements that are not there come as zeros
-        const int from = 2 * l_pair < l_chunk ? 2 : 0, to = 2 * l_pair + 1 < l_end ? 4 : 2, row = tile_row(2 * l_pair);
-        ptx::mbar_arrive_expect_tx(bars + put, (to - from) * 1024 + kWoScales);
-        for (int i = from; i < to; ++i) copy_2d(codes + put * kWoCodes + i * 1024, &map_w, k0 / 2, row + 32 * i, bars + put);
-        copy_3d(scales + put * kWoScales, &map_sf, (l_pair & 3) * 128, k0 / 64, l_pair >> 2, bars + put);
+        const int from = 2 * l_pair < j0 ? 1 : 0, to = 2 * l_pair + 1 < j1 ? 2 : 1, block = l_pair >> 2;
+        ptx::mbar_arrive_expect_tx(bars + put, (to - from) * 2 * kWoBox + kWoScales);
+        for (int h = from; h < to; ++h) {
+          const uint32_t dst = codes + put * kWoCodes + h * 2 * kWoBox;
+          if (block < a.whole) {
+            copy_4d(dst, &map_tiles, k0 / 2, (l_pair & 3) * 8, 2 * h, block, bars + put);
+          } else {
+            copy_2d(dst, &map_w, k0 / 2, tile_row(2 * l_pair + h), bars + put);
+            copy_2d(dst + kWoBox, &map_w, k0 / 2, tile_row(2 * l_pair + h) + 32, bars + put);
+          }
+        }
+        copy_3d(scales + put * kWoScales, &map_sf, (l_pair & 3) * 128, k0 / 64, block, bars + put);
       }
       l_pair += a.row_groups;
-      if (2 * l_pair >= l_end) {
+      if (kPasses && l_pair >= min(l_chunk + a.chunk, p1)) {  // one row group
         if (++l_pass == a.passes) {
           l_pass = 0;
           l_chunk += a.chunk;
-          l_end = min(l_chunk + a.chunk, j1);
-          while (l_chunk < j1 && 2 * ((l_chunk >> 1) + row_group) >= l_end) {  // no pair of this row group in the chunk
-            l_chunk += a.chunk;
-            l_end = min(l_chunk + a.chunk, j1);
-          }
         }
-        l_pair = (l_chunk >> 1) + row_group;
+        l_pair = l_chunk;
         k0 = k_first + l_pass * k_pass;
       }
     }
@@ -214,23 +220,20 @@ __global__ void __launch_bounds__(kWoThreads, 1)
   // the weight's scale goes into the factors of the activation's blocks, so that a sum is in the result's range on its way
   const float scale_of = a.scale_dev != nullptr ? *a.scale_dev : 1.0f;
   uint4 x[2][4];
-  // The slice's 512 bytes of a row, 16 per lane; as f16 through shared memory to the lanes that multiply them.  Piece c of row r lies at
-  // c ^ (c / 8 % 2 + 2 (r % 2)): the four pieces of eight lanes that read at once are in different banks.
+  // A lane loads 16 bytes of every row of the warp's slice, and they go as f16 through shared memory to the lanes that multiply them.  Piece c of
+  // row r lies at c ^ (c / 8 % 2 + 2 (r % 2)): the four pieces of eight lanes that read at once are in different banks.
   unsigned char *x_space = space + warp * kWoXWarp;
   float *factors = reinterpret_cast<float *>(smem + kWoFactors) + warp * 16;  // [block of 128 elements][column]: what its sum is multiplied by
-  uint4 raw[2][4];  // of eight rows at a time
+  uint4 raw[8];
   auto load_x = [&](int from_k) {
     const bool in_k = works && from_k + lane * 8 < a.k;
     const __nv_bfloat16 *from = a.x + row_first * a.x_row + from_k + lane * 8;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (4 * half >= m) break;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        raw[half][r] = make_uint4(0, 0, 0, 0);
-        if (4 * half + r < m && in_k) raw[half][r] = *reinterpret_cast<const uint4 *>(from);
-        from += a.x_row;
-      }
+    for (int i = 0; i < 8; ++i) {
+      if (i % 4 == 0 && i >= m) break;
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (i < m && in_k) raw[i] = *reinterpret_cast<const uint4 *>(from);
+      from += a.x_row;
     }
   };
   auto convert_x = [&]() {
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(kWoThreads, 1)
       uint32_t top[kRows];
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        const uint4 v = raw[half][r];
+        const uint4 v = raw[4 * half + r];
         top[r] = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
         top[r] = max(top[r] & 0xFFFFu, top[r] >> 16);
       }
@@ -252,12 +255,12 @@ __global__ void __launch_bounds__(kWoThreads, 1)
         for (int r = 0; r < kRows; ++r) top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], off));
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        const uint4 v = raw[half][r];
+        const uint4 v = raw[4 * half + r];
         const int row = 4 * half + r;
         // a block with infinities or NaN is scaled down, so that nothing finite joins them
         const int e = (int)(top[r] >> 7), shift = e == 255 ? -120 : min(126, 141 - max(e, 1));
         const float f = __int_as_float((127 + shift) << 23);
-        *reinterpret_cast<uint4 *>(x_space + row * 512 + (lane ^ (((lane >> 3) & 1) | ((r & 1) << 1))) * 16) =
+        *reinterpret_cast<uint4 *>(x_space + row * kWoSlice * 2 + (lane ^ (((lane >> 3) & 1) | ((row & 1) << 1))) * 16) =
             make_uint4(scaled_pair(v.x, f), scaled_pair(v.y, f), scaled_pair(v.z, f), scaled_pair(v.w, f));
         if ((lane & 15) == 0) factors[(lane >> 4) * 8 + row] = __int_as_float((127 - shift) << 23) * scale;
       }
@@ -277,39 +280,40 @@ __global__ void __launch_bounds__(kWoThreads, 1)
       for (int q = 0; q < 4; ++q) {
         const int c = b * 16 + t * 4 + q;
         x[b][q] = make_uint4(0, 0, 0, 0);
-        if (g < m) x[b][q] = *reinterpret_cast<const uint4 *>(x_space + g * 512 + (c ^ ((t >> 1) | ((g & 1) << 1))) * 16);
+        if (g < m) x[b][q] = *reinterpret_cast<const uint4 *>(x_space + g * kWoSlice * 2 + (c ^ ((t >> 1) | ((g & 1) << 1))) * 16);
       }
     __syncwarp();
   };
 
   // the activation ahead of the weight: behind the first tiles of all SMs it took 5600 cycles to arrive
-  if (a.passes == 1) load_x(k_first);
+  if (!kPasses) load_x(k_first);
 #pragma unroll 1
   for (int i = 0; i < kWoStages; ++i) load();
-  if (a.passes == 1) {
+  if (!kPasses) {
     convert_x();
     __syncthreads();  // the warps' sums take the activation's space
   }
 
   // lane (g, t) takes row (g >> 1) + 4 (g & 1) of eight, so that what eight lanes read at once lies in different banks
+  // (and the second 128 elements' codes lie at the same offset ^ 64)
   const int my_row = (g >> 1) | ((g & 1) << 2);
-  // (the second 128 elements' codes lie at the same offset ^ 64)
-  const uint32_t my_codes = codes + my_row * 128 + ((t ^ my_row) << 4), my_codes2 = my_codes ^ 64;
+  const uint32_t my_codes = codes + my_row * 128 + ((t ^ my_row) << 4);
   const uint32_t my_scales = scales + my_row * 16 + (t >> 1) * 128 + (t & 1) * 2;
-  const int per_tile = 16 * m;
-  const bool col0 = 2 * t < m, col1 = 2 * t + 1 < m;
+  // A tile's sums: [column odd][row of the tile / 8][column / 2][row % 8], so that what a warp stores at once lies in different banks.
+  const int pairs = (m + 1) >> 1, per_tile = 32 * pairs;
+  const unsigned magic = a.per_tile_magic[blockIdx.z];
   int take = 0, flip = 0;
   unsigned phases = 0;
-  for (int chunk = j0; chunk < j1; chunk += a.chunk, flip ^= 1) {
-    const int end = min(chunk + a.chunk, j1);
+  for (int chunk = p0; chunk < p1; chunk += a.chunk, flip ^= 1) {
+    const int end = min(chunk + a.chunk, p1);
     float *part = parts + flip * (a.parts_bytes / 8);
-    for (int pass = 0; pass < a.passes; ++pass) {
-      if (a.passes > 1) {
+    for (int pass = 0; pass < (kPasses ? a.passes : 1); ++pass) {
+      if (kPasses) {
         load_x(k_first + pass * k_pass);
         convert_x();
       }
       if (!works) continue;
-      for (int pair = (chunk >> 1) + row_group; 2 * pair < end; pair += a.row_groups) {
+      for (int pair = chunk + row_group; pair < end; pair += a.row_groups) {
         if (!ptx::mbar_wait(bars + take, (phases >> take) & 1, gave_up)) {
           *gave_up = 1;
           if (a.error_flag != nullptr) atomicExch(a.error_flag, kWeightOnlyTimeout);
@@ -317,13 +321,13 @@ __global__ void __launch_bounds__(kWoThreads, 1)
         __syncwarp();
         phases ^= 1u << take;
 #pragma unroll 1
-        for (int half = 2 * pair < chunk ? 1 : 0; half < (2 * pair + 1 < end ? 2 : 1); ++half) {
-          const uint32_t at = take * kWoCodes + half * 2048, from_sf = my_scales + take * kWoScales + half * 8;
+        for (int half = 2 * pair < j0 ? 1 : 0; half < (2 * pair + 1 < j1 ? 2 : 1); ++half) {
+          const uint32_t at = take * kWoCodes + half * 2 * kWoBox, from_sf = my_scales + take * kWoScales + half * 8;
           float acc[4];
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            const uint32_t from = (b == 0 ? my_codes : my_codes2) + at;
-            const uint4 w0 = wo_lds16(from), w1 = wo_lds16(from + 1024);
+            const uint32_t from = (my_codes ^ (b * 64)) + at;
+            const uint4 w0 = wo_lds16(from), w1 = wo_lds16(from + kWoBox);
             // the scale factors of this lane's two groups of 16 elements, of both rows
             const __half2 s0 = e4m3x2_to_f16(wo_lds2(from_sf + b * 256)), s1 = e4m3x2_to_f16(wo_lds2(from_sf + b * 256 + 4));
             float d[4];
@@ -347,14 +351,12 @@ __global__ void __launch_bounds__(kWoThreads, 1)
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[c] = b == 0 ? d[c] * (c & 1 ? f.y : f.x) : fmaf(d[c], c & 1 ? f.y : f.x, acc[c]);
           }
-          // [tile][slice][column][row of the tile]
-          float *to = part + ((2 * pair + half - chunk) * a.slices + slice_in) * per_tile + 32 * t + my_row;
-          if (pass > 0) {
-            if (col0) acc[0] += to[0], acc[2] += to[8];
-            if (col1) acc[1] += to[16], acc[3] += to[24];
+          if (t < pairs) {
+            float *to = part + ((2 * (pair - chunk) + half) * a.slices + slice_in) * per_tile + t * 8 + my_row;
+            const int step = pairs * 8;
+            if (kPasses && pass > 0) acc[0] += to[0], acc[2] += to[step], acc[1] += to[2 * step], acc[3] += to[3 * step];
+            to[0] = acc[0], to[step] = acc[2], to[2 * step] = acc[1], to[3 * step] = acc[3];
           }
-          if (col0) to[0] = acc[0], to[8] = acc[2];
-          if (col1) to[16] = acc[1], to[24] = acc[3];
         }
         take ^= 1;
         __syncwarp();  // the stage is free
@@ -362,25 +364,43 @@ __global__ void __launch_bounds__(kWoThreads, 1)
       }
     }
     __syncthreads();
-    const int count = (end - chunk) * per_tile;
-    float *sum_of = sums + flip * (kWoSums / 4);
-    const unsigned magic = a.per_tile_magic[blockIdx.z];
-    auto finish = [&](int i, float y) {
-      const int tile = (int)__umulhi((unsigned)i, magic), rest = i - tile * per_tile, col = row_first + (rest >> 4), r = rest & 15;
-      const int row = tile_row(chunk + tile) + (r >> 3) * 32 + (r & 7);
-      if (row < a.n) {
-        if (a.bias != nullptr) y += __bfloat162float(a.bias[row]);
-        a.y[(long long)col * a.n + row] = __float2bfloat16_rn(y);
+    // from the first to the last of the chunk's tiles
+    const int first = (max(2 * chunk, j0) - 2 * chunk) * per_tile / 4, count = (min(2 * end, j1) - 2 * chunk) * per_tile / 4;
+    float4 *sum_of = reinterpret_cast<float4 *>(sums + flip * (kWoSums / 4));
+    // four rows of a column at a time
+    auto add = [](float4 &y, const float4 &v) { y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w; };
+    auto finish = [&](int i, float4 y) {
+      const int tile = (int)__umulhi((unsigned)i * 4, magic), rest = i * 4 - tile * per_tile;
+      const int pair = rest >> 3, v = (pair >= pairs) + (pair >= 2 * pairs) + (pair >= 3 * pairs);
+      const int col = 2 * (pair - v * pairs) + (v >> 1), row = tile_row(2 * chunk + tile) + (v & 1) * 32 + (rest & 7);
+      if (row >= a.n || col >= m) return;
+      __nv_bfloat16 *to = a.y + (long long)(row_first + col) * a.n + row;
+      if (a.by_four) {
+        if (a.bias != nullptr) {
+          const uint2 w = *reinterpret_cast<const uint2 *>(a.bias + row);
+          add(y, make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u)));
+        }
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(y.x, y.y), hi = __floats2bfloat162_rn(y.z, y.w);
+        *reinterpret_cast<uint2 *>(to) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+      } else {
+        const float of_row[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (row + j < a.n) to[j] = __float2bfloat16_rn(of_row[j] + (a.bias != nullptr ? __bfloat162float(a.bias[row + j]) : 0.0f));
       }
     };
-    for (int i = threadIdx.x; i < count; i += kWoThreads) {
-      const int tile = (int)__umulhi((unsigned)i, magic), rest = i - tile * per_tile;
-      const float *from = part + tile * a.slices * per_tile + rest;
-      float v[kWoWarps], y = 0.0f;  // all loads, then the sum
+    for (int i = first + threadIdx.x; i < count; i += kWoThreads) {
+      const int tile = (int)__umulhi((unsigned)i * 4, magic);
+      const float4 *from = reinterpret_cast<const float4 *>(part + tile * (a.slices - 1) * per_tile) + i;  // tile * slices * per_tile + rest
+      float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int s = 0; s < kWoWarps; ++s) v[s] = s < a.slices ? from[s * per_tile] : 0.0f;
+      for (int s0 = 0; s0 < kWoWarps; s0 += 8) {
+        float4 v[8];  // all loads, then the sum
 #pragma unroll
-      for (int s = 0; s < kWoWarps; ++s) y += v[s];
+        for (int s = 0; s < 8; ++s) v[s] = s0 + s < a.slices ? from[(s0 + s) * (per_tile >> 2)] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) add(y, v[s]);
+      }
       if (a.cluster == 1)
         finish(i, y);
       else
@@ -389,12 +409,13 @@ __global__ void __launch_bounds__(kWoThreads, 1)
     if (a.cluster > 1) {
       __syncwarp();
       ptx::cluster_sync();
-      for (int i = blockIdx.x * kWoThreads + threadIdx.x; i < count; i += a.cluster * kWoThreads) {
-        float v[kWoClusterMost], y = 0.0f;
+      for (int i = first + blockIdx.x * kWoThreads + threadIdx.x; i < count; i += a.cluster * kWoThreads) {
+        float4 v[kWoClusterMost], y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int r = 0; r < kWoClusterMost; ++r) v[r] = r < a.cluster ? ld_cluster_f32(ptx::smem_u32(sum_of + i), r) : 0.0f;
+        for (int r = 0; r < kWoClusterMost; ++r)
+          v[r] = r < a.cluster ? ptx::ld_cluster_f32x4(ptx::smem_u32(sum_of + i), r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int r = 0; r < kWoClusterMost; ++r) y += v[r];
+        for (int r = 0; r < kWoClusterMost; ++r) add(y, v[r]);
         finish(i, y);
       }
     }
@@ -463,42 +484,55 @@ cudaError_t run_weight_only(const void *x, long long x_row, int m, int n, int k,
   a.cluster = (slices + kWoWarps - 1) / kWoWarps;
   if (a.cluster > kWoClusterMost) a.cluster = kWoClusterMost;
   a.passes = (slices + a.cluster * kWoWarps - 1) / (a.cluster * kWoWarps);
-  while (a.passes > 1 && (slices + a.cluster * a.passes - 1) / (a.cluster * a.passes) * (m > 8 ? 8 : m) * 64 * 2 > kWoParts - kWoWarps * kWoXWarp) ++a.passes;
+  const int rows = m > 8 ? 8 : m, per_tile = 32 * ((rows + 1) / 2);  // floats
+  while (a.passes > 1 && (slices + a.cluster * a.passes - 1) / (a.cluster * a.passes) * per_tile * 4 * 4 > ((kWoParts - kWoWarps * kWoXWarp) & ~31)) ++a.passes;
   a.slices = (slices + a.cluster * a.passes - 1) / (a.cluster * a.passes);
-  a.row_groups = kWoWarps / a.slices;
+  a.row_groups = a.passes == 1 ? kWoWarps / a.slices : 1;
   const int left = n % 128;  // a last block of few rows has empty tiles at its end
   a.tiles = n / 128 * 8 + (left == 0 ? 0 : left > 64 ? 8 : left >= 32 ? 7 : 2 * ((left + 7) / 8) - 1);
-  const auto kernel = weight_only_kernel;
-  static bool ready[64] = {};
-  cudaError_t err = allow_smem(kernel, kWoSmem, ready);
+  const auto kernel = a.passes > 1 ? weight_only_kernel<true> : weight_only_kernel<false>;
+  static bool ready[2][64] = {};
+  cudaError_t err = allow_smem(kernel, kWoSmem, ready[a.passes > 1]);
   if (err != cudaSuccess) return err;
   int clusters = 0;
   err = wo_clusters(kernel, a.cluster, &clusters);
   if (err != cudaSuccess) return err;
   // more than eight rows: half of the clusters for each eight, side by side, so that the second to read a row of the weight finds it in L2
-  const int eights = m > 8 ? 2 : 1, rows = m > 8 ? 8 : m;
+  const int eights = m > 8 ? 2 : 1;
   clusters = clusters / eights > 0 ? clusters / eights : 1;
   a.per_cluster = (a.tiles + clusters - 1) / clusters;
   a.parts_at = a.passes == 1 ? 0 : kWoWarps * kWoXWarp;
-  a.parts_bytes = (kWoParts - a.parts_at) & ~7;
-  // all tiles at once, or half of the space at a time; at most as many as the sums of a cluster's CTAs have room for
-  const int tile_bytes = a.slices * rows * 64, room = a.parts_bytes / 2 / tile_bytes;
-  a.chunk = a.per_cluster * tile_bytes <= a.parts_bytes ? a.per_cluster : room;
-  if (a.cluster > 1 && a.chunk > kWoSums / (rows * 64)) a.chunk = kWoSums / (rows * 64) < room ? kWoSums / (rows * 64) : room;
-  if (a.chunk < 1) return cudaErrorInvalidValue;
-  for (int i = 0; i < eights; ++i) {
-    const int per_tile = 16 * (i == 0 ? rows : m - 8);
-    a.per_tile_magic[i] = (unsigned)(((1ULL << 32) + per_tile - 1) / per_tile);
+  a.parts_bytes = (kWoParts - a.parts_at) & ~31;  // two halves of float4s
+  // all tiles at once, or half of the space at a time; at most as many as the sums of a cluster's CTAs have room for; in pairs
+  const int tile_bytes = a.slices * per_tile * 4, all = (a.per_cluster + 1) / 2, of_sums = kWoSums / (per_tile * 8);
+  a.chunk = all;
+  if (2 * all * tile_bytes > a.parts_bytes || (a.cluster > 1 && all > of_sums)) {
+    a.chunk = a.parts_bytes / 2 / (2 * tile_bytes);
+    if (a.cluster > 1 && a.chunk > of_sums) a.chunk = of_sums;
+    if (a.chunk > a.row_groups) a.chunk -= a.chunk % a.row_groups;  // the pairs of a row group follow one another at equal distances
   }
-  if (a.chunk < a.row_groups && a.row_groups > 1) a.row_groups = a.chunk;
+  if (a.chunk < 1) return cudaErrorInvalidValue;
+  if (a.row_groups > a.chunk) a.row_groups = a.chunk;
+  for (int i = 0; i < eights; ++i) {
+    const int floats = i == 0 ? per_tile : 32 * ((m - 8 + 1) / 2);
+    a.per_tile_magic[i] = (unsigned)(((1ULL << 32) + floats - 1) / floats);
+  }
   const int used = (a.tiles + a.per_cluster - 1) / a.per_cluster;
-  // codes: 8 rows x 128 bytes at a time; scale factors: blocks of 128 rows, tiles of 64 elements, 8 rows x 16 bytes of 4 tiles at a time
-  CUtensorMap map_w, map_sf;
+  a.whole = n / 128;
+  a.by_four = n % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 7) == 0 && (reinterpret_cast<uintptr_t>(a.bias) & 7) == 0;
+  CUtensorMap map_tiles, map_w, map_sf;
+  // codes: 8 rows x 128 bytes at a time
   const cuuint64_t w_dims[2] = {(cuuint64_t)k / 2, (cuuint64_t)n}, w_strides[1] = {(cuuint64_t)k / 2};
-  const cuuint32_t w_box[2] = {128, 8};
+  const cuuint32_t w_box[2] = {kWoSlice / 2, 8};
+  // and, in whole blocks of 128 rows, a tile's 16 rows in one copy
+  const cuuint64_t t_dims[4] = {(cuuint64_t)k / 2, 32, 4, (cuuint64_t)(a.whole > 0 ? a.whole : 1)};
+  const cuuint64_t t_strides[3] = {(cuuint64_t)k / 2, (cuuint64_t)k / 2 * 32, (cuuint64_t)k / 2 * 128};
+  const cuuint32_t t_box[4] = {kWoSlice / 2, 8, 2, 1};
+  // scale factors: blocks of 128 rows, tiles of 64 elements, 8 rows x 16 bytes of 4 tiles at a time
   const cuuint64_t sf_dims[3] = {512, (cuuint64_t)k / 64, ((cuuint64_t)n + 127) / 128}, sf_strides[2] = {512, (cuuint64_t)k / 64 * 512};
-  const cuuint32_t sf_box[3] = {128, 4, 1};
-  if (!make_tensor_map(&map_w, 2, qw, w_dims, w_strides, w_box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+  const cuuint32_t sf_box[3] = {128, kWoSlice / 64, 1};
+  const CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B;
+  if (!make_tensor_map(&map_tiles, 4, qw, t_dims, t_strides, t_box, swizzle) || !make_tensor_map(&map_w, 2, qw, w_dims, w_strides, w_box, swizzle) ||
       !make_tensor_map(&map_sf, 3, sf, sf_dims, sf_strides, sf_box, CU_TENSOR_MAP_SWIZZLE_NONE))
     return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
@@ -515,7 +549,7 @@ cudaError_t run_weight_only(const void *x, long long x_row, int m, int n, int k,
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = a.cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, map_w, map_sf, a);
+  return cudaLaunchKernelEx(&cfg, kernel, map_tiles, map_w, map_sf, a);
 }
 
 }  // namespace sharq

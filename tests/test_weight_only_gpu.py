@@ -175,3 +175,22 @@ def test_layer_takes_activations_of_any_stride():
     whole = torch.randn(5, 200, generator=g).to(torch.bfloat16).cuda()
     for strided in (x, whole[:, 3:195], whole[:1, 3:195].expand(4, 192)):
         assert torch.equal(layer.forward_weight_only(strided), layer.forward_weight_only(strided.clone(memory_format=torch.contiguous_format)))
+
+
+# shares of the rows whose sums are joined in several turns, in one CTA and in clusters, beginning and ending within a pair of tiles
+@pytest.mark.parametrize("m,n,k", [(8, 20000, 4096), (7, 28701, 4096), (16, 20000, 4096), (15, 9002, 14336), (9, 12345, 2048), (4, 16000, 8192),
+                                   (2, 30000, 14336), (16, 20000, 512), (11, 3001, 20480)])
+def test_products_joined_in_turns(m, n, k):
+    from sharq_b200 import ops
+
+    g = torch.Generator().manual_seed(m + n + k)
+    qw, sf = random_weight(n, k, m + n + k)
+    x = torch.randn(m, k, generator=g).to(torch.bfloat16).cuda()
+    bias = torch.randn(n, generator=g).to(torch.bfloat16).cuda() if m % 2 else None
+    got = ops.weight_only_linear(x, qw, sf, 0.25, bias=bias)
+    ops.check_device_errors()
+    for i in range(0, n, 4096):  # in pieces of whole blocks of 128 rows
+        rows = min(4096, n - i)
+        w = weight64(qw[i:i + rows], sf[i * k // 16:])
+        check(got[:, i:i + rows], x, w, 0.25, None if bias is None else bias[i:i + rows])
+    assert torch.equal(ops.weight_only_linear(x, qw, sf, 0.25, bias=bias), got)
