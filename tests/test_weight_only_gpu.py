@@ -194,3 +194,20 @@ def test_products_joined_in_turns(m, n, k):
         w = weight64(qw[i:i + rows], sf[i * k // 16:])
         check(got[:, i:i + rows], x, w, 0.25, None if bias is None else bias[i:i + rows])
     assert torch.equal(ops.weight_only_linear(x, qw, sf, 0.25, bias=bias), got)
+
+
+@pytest.mark.parametrize("m,n", [(1, 4096), (1, 4098), (12, 512)])
+def test_results_and_biases_at_any_element(m, n):
+    from sharq_b200 import ops
+
+    qw, sf = random_weight(n, 512, 3)
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(m, 512, generator=g).to(torch.bfloat16).cuda()
+    bias = torch.randn(n + 1, generator=g).to(torch.bfloat16).cuda()
+    want = ops.weight_only_linear(x, qw, sf, 0.5, bias=bias[1:].clone())
+    for shift in (0, 1, 2):
+        room = torch.full((m * n + 8,), 7.0, dtype=torch.bfloat16, device="cuda")
+        out = room[shift:shift + m * n].view(m, n)
+        assert ops.weight_only_linear(x, qw, sf, 0.5, bias=bias[1:], out=out) is not None
+        assert torch.equal(out, want)
+        assert bool((room[:shift] == 7).all()) and bool((room[shift + m * n:] == 7).all())
