@@ -13,6 +13,8 @@ Extra ops that the reference does not have (all optional for a drop-in):
   sharq_linear_forward           the op name the reference's vLLM plugin probes for
   sharq_linear_gemm              fused sparse+residual GEMM on a prepared activation
   scaled_sparse_residual_quantize_x   prepare with the host-side amax/divide folded in
+  rope_append_paged, paged_attention, weight_only_linear   the operators of a decode step: rotary embedding with the append to
+                                 a paged key/value cache, attention over it, few unquantised rows times a 4-bit weight
 """
 from __future__ import annotations
 
