@@ -47,8 +47,8 @@ constexpr float kF16Lift = 10.0f, kBf16Lift = -32.0f;  // log2 of a factor of th
 constexpr int kItemCost = 2;
 constexpr int kStretchLeast = 4;
 constexpr int kAttnClusterMost = 8;
-constexpr int kDirectTiles = 3;  // tiles of a warp that a cluster is sized for, and for which it is taken at most
-constexpr int kDirectMost = 16;
+constexpr int kDirectTiles = 3;  // tiles of a warp that a cluster is sized for, and for which it is taken at most, where its like fill two fifths
+constexpr int kDirectMost = 16, kDirectFew = 10;  // of the SMs, and where they do not
 
 __device__ __forceinline__ uint4 ld_shared16(uint32_t smem) {
   uint4 v;
@@ -998,13 +998,17 @@ bool encode(CUtensorMap *map, char *base, const PagedCache &c, int size, int box
 
 unsigned magic_of(int d) { return (unsigned)(((1ULL << 32) + d - 1) / d); }  // for divide(), which does not use it for 1
 
-// CTAs of the direct form's clusters, 0 for the list of tiles.
+// CTAs of the direct form's clusters, 0 for the list of tiles; from sizes of tensors alone, so that a captured call keeps its form.  One launch with
+// a join in the cluster saves some 4 us of the list's two, but a cluster reads only what its few CTAs can, and more clusters than run at
+// once begin one behind the other.  Direct / list, us, 8 heads of 128 in bf16: 1 x 97 tokens 4.1 / 9.0, 1 x 4096 10.9 / 11.7, 1 x 5000 12.4 / 12.1 (10
+// tiles per warp, 64 CTAs), 1 x 6000 13.8 / 12.5, 2 x 7000 16.5 / 17.0 (128 CTAs), 8 x 4000 24.1 / 28.0, 64 x 64 9.6 / 11.4, 74 x 400 25.0 / 27.8,
+// 90 x 60 13.1 / 12.5 (720 clusters of one CTA), in e4m3 14.0 / 9.6, 128 x 64 16.8 / 11.0, 128 x 256 31.6 / 30.4.
 int direct_splits(int seqs, int items, int most_tiles, int ctas) {
   const long long pairs = (long long)seqs * items;
+  if (pairs > 2 * ctas || items > 65535 || seqs > 65535) return 0;
   int splits = 1;
   while (splits < kAttnClusterMost && splits * kAttnWarps * kDirectTiles < most_tiles && pairs * splits * 2 <= ctas) splits *= 2;
-  if (items > 65535 || seqs > 65535) return 0;
-  return (pairs * splits <= ctas || splits == 1) && most_tiles <= splits * kAttnWarps * kDirectMost ? splits : 0;
+  return most_tiles <= splits * kAttnWarps * (pairs * splits * 5 >= 2 * ctas ? kDirectMost : kDirectFew) ? splits : 0;
 }
 
 template <int D, bool kFp8, int kCols>
