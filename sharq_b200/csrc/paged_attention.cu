@@ -47,8 +47,7 @@ constexpr float kF16Lift = 10.0f, kBf16Lift = -32.0f;  // log2 of a factor of th
 constexpr int kItemCost = 2;
 constexpr int kStretchLeast = 4;
 constexpr int kAttnClusterMost = 8;
-constexpr int kDirectTiles = 3;  // tiles of a warp that a cluster is sized for, and for which it is taken at most, where its like fill two fifths
-constexpr int kDirectMost = 16, kDirectFew = 10;  // of the SMs, and where they do not
+constexpr int kDirectMost = 16, kDirectFew = 10;  // tiles of a warp for which a cluster is taken at most, where its like fill two fifths of the SMs or not
 
 __device__ __forceinline__ uint4 ld_shared16(uint32_t smem) {
   uint4 v;
@@ -1003,11 +1002,19 @@ unsigned magic_of(int d) { return (unsigned)(((1ULL << 32) + d - 1) / d); }  // 
 // once begin one behind the other.  Direct / list, us, 8 heads of 128 in bf16: 1 x 97 tokens 4.1 / 9.0, 1 x 4096 10.9 / 11.7, 1 x 5000 12.4 / 12.1 (10
 // tiles per warp, 64 CTAs), 1 x 6000 13.8 / 12.5, 2 x 7000 16.5 / 17.0 (128 CTAs), 8 x 4000 24.1 / 28.0, 64 x 64 9.6 / 11.4, 74 x 400 25.0 / 27.8,
 // 90 x 60 13.1 / 12.5 (720 clusters of one CTA), in e4m3 14.0 / 9.6, 128 x 64 16.8 / 11.0, 128 x 256 31.6 / 30.4.
+// A cluster has CTAs until its warps have a tile each, as long as SMs are free (1 x 400 tokens 4.9 us, with three tiles each 5.4; in e4m3
+// 1 x 700 5.5 and 7.4); two tiles each in a single CTA are as fast, for there the CTAs have nothing to join (1 x 97: 4.1, in two CTAs 4.6); where CTAs
+// share an SM four each (4 x 400 6.6, with one 6.9; 16 x 200 7.1 and 7.6).  (Eight warps to a CTA or sixteen CTAs to a cluster: 1 x 4096 10.2 or 9.9
+// instead of 10.9, but 1 x 1024 6.5 instead of 5.8, and sixteen clusters of that size do not run at once; four stages instead of two: the same.)
 int direct_splits(int seqs, int items, int most_tiles, int ctas) {
   const long long pairs = (long long)seqs * items;
   if (pairs > 2 * ctas || items > 65535 || seqs > 65535) return 0;
   int splits = 1;
-  while (splits < kAttnClusterMost && splits * kAttnWarps * kDirectTiles < most_tiles && pairs * splits * 2 <= ctas) splits *= 2;
+  while (splits < kAttnClusterMost && pairs * splits * 2 <= ctas) {
+    const int enough = pairs * splits * 4 > ctas ? 4 : splits == 1 ? 2 : 1;  // tiles per warp
+    if (most_tiles <= splits * kAttnWarps * enough) break;
+    splits *= 2;
+  }
   return most_tiles <= splits * kAttnWarps * (pairs * splits * 5 >= 2 * ctas ? kDirectMost : kDirectFew) ? splits : 0;
 }
 
