@@ -18,7 +18,7 @@
 // those of CTAs in distributed shared memory, each added up in a fixed order: the same bits from call to call, no scratch and no second launch.
 // More than eight rows are two halves of the grid, the second of which reads the weight from L2.
 //
-// 28672 x 4096: one row 14.5 us (4.6 TB/s, 70 % of the rate of a copy), 8 rows 17.6, 16 rows 28.9; 4096 x 4096, one row: 4.9 us.  (Tiles of 128
+// 28672 x 4096: one row 14.5 us (4.6 TB/s, 70 % of the rate of a copy), 8 rows 17.2, 16 rows 28.8; 4096 x 4096, one row: 4.9 us.  (Tiles of 128
 // rows per CTA with the activation in shared memory, 323 instead of 265 instructions per 16 rows x 256 and uneven shares: 19.8, 38 with 16
 // rows and 6.6.)  The loop's instructions take 7 us to issue, beside the copies' 10; the activation's way to the registers comes before, the
 // join after.  Both eights of 16 rows in one warp, the weight converted once for 128 elements of K of each, took 34 us instead of 29 and, for
@@ -178,8 +178,10 @@ __global__ void __launch_bounds__(kWoThreads, 1)
   int l_chunk = p0, l_pass = 0, l_pair = works ? p0 + row_group : p1, put = 0, k0 = k_first;
   __syncthreads();
   const bool chosen = ptx::elect_one();
-  if (l_pair < p1 && chosen) {
-    // the first rows into L2, where they may be as old as they like: ahead of the wait for the kernels before
+  if (m <= 3 && l_pair < p1 && chosen) {
+    // The first rows into L2, where they may be as old as they like: ahead of the wait for the kernels before.  More rows of the activation arrive
+    // later for it: 28672 x 4096 with / without, 2 rows 14.6 / 15.2 us, 3 rows 15.1 / 15.3, 4 rows 15.7 / 15.5, 6 rows 17.5 / 17.0; 4096 x 4096
+    // 5.0 / 4.9, 5.4 / 4.9, 5.4 / 5.3, 6.3 / 5.8.  (Of both stages: 15.6 instead of 14.5 with one row.)
 #pragma unroll 1
     for (int i = 0; i < 4; ++i) ptx::tma_prefetch_l2_2d(&map_w, k0 / 2, tile_row(2 * l_pair) + 32 * i);
   }
