@@ -479,3 +479,24 @@ def test_a_length_near_the_end_of_an_int_is_reported():
     with pytest.raises(RuntimeError, match="paged cache"):
         ops.check_device_errors()
     assert bool(got.isnan().all())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim,group", [(64, 3), (128, 12), (128, 1), (64, 16)])
+def test_attention_of_few_sequences_at_every_size_of_cluster(dim, group, fp8):
+    """Tables of one to some hundred tiles, with sequences that leave warps and CTAs of their cluster without a token."""
+    from sharq_b200 import ops
+
+    page, kv = 16, 2
+    for longest in (1, 16, 17, 33, 128, 129, 255, 257, 400, 513, 1000, 1025, 2049, 3000):
+        for lengths in ([longest], [longest, 0, 1, longest // 2 + 1, longest // 3]):
+            table, pages = P.make_table(lengths, page, 1, seed=longest)
+            k, v, ks, vs = P.make_cache(pages, kv, page, dim, fp8, longest)
+            g = torch.Generator().manual_seed(longest)
+            q = torch.randn(len(lengths), kv * group, dim, generator=g).to(torch.bfloat16).cuda()
+            n = torch.tensor(lengths, dtype=torch.int32).cuda()
+            got = ops.paged_attention(q, k, v, table, n, k_scale=ks, v_scale=vs)
+            out, size, reach = P.attention64(q, P.values64(k, ks), P.values64(v, vs), table, lengths)
+            bound = P.attention_bound(out, size, reach, dim, longest, fp8)
+            assert bool(((got.double() - out).abs() <= bound).all()), (longest, lengths)
+    ops.check_device_errors()
