@@ -155,20 +155,26 @@ struct __align__(16) Part {
   int seq, item;  // item: head and chunk, -1: nothing
   int begins, tiles_left;
 };
-// Shared memory of a CTA: the rings (the swizzle wants 1024 bytes), then the part at the beginning of every warp's stretch (the one at the end goes
-// to the warp's ring, which is free by then), two parts' maxima and sums per warp, their descriptions, barriers and the flag of a wait that ran out.
-template <int D, bool kFp8, int kCols>
+// Forms of the kernel: the list of tiles, and the direct one with two or three CTAs per SM.
+constexpr int kList = 0, kDirectTwo = 1, kDirectThree = 2;
+
+// Shared memory of a CTA: the rings (the swizzle wants 1024 bytes), then the part at the beginning of every warp's stretch (the one at the end, and
+// the only one of the direct form, goes to the warp's ring, which is free by then), two parts' maxima and sums per warp, their descriptions,
+// barriers and the flag of a wait that ran out.  CTAs: per SM.
+template <int D, bool kFp8, int kCols, int kForm>
 struct Layout {
+  static constexpr bool kDirect = kForm != kList;
+  static constexpr int kCtas = kForm == kDirectThree ? 3 : 2;
   static constexpr int kStages = 2;
   static constexpr int kRing = kStages * Tile<D, kFp8>::kStage;
   static constexpr int kPart = D * kCols * 4;
   static constexpr int kParts = kAttnWarps * kRing;
-  static constexpr int kMl = kParts + kAttnWarps * kPart;
+  static constexpr int kMl = kParts + (kDirect ? 0 : kAttnWarps * kPart);
   static constexpr int kInfo = kMl + 2 * kAttnWarps * kCols * 8;
   static constexpr int kBars = kInfo + 2 * kAttnWarps * (int)sizeof(Part);
   static constexpr int kFlag = kBars + kAttnWarps * kStages * 8;
   static constexpr int kTotal = kFlag + 8;
-  static_assert(kPart <= kRing && kTotal <= 115712, "a part fits a ring, two CTAs an SM");
+  static_assert(kPart <= kRing && kCtas * (kTotal + 1024) <= 233472, "a part fits a ring, the CTAs an SM");
 };
 
 // A length as the kernel uses it: one that the page table cannot hold counts as an empty sequence whose rows come out as NaN.
@@ -269,12 +275,13 @@ __device__ __forceinline__ int locate(Place &at, int u, const AttnArgs &a, const
 
 // kCols: columns for query heads (8 or 16).  kDirect: a cluster per (sequence, head chunk), blockIdx = (rank, head chunk, sequence), whose warps take equal
 // stretches of its tiles and whose CTAs join their parts through distributed shared memory; nothing is left for a second launch.
-template <int D, bool kFp8, int kCols, bool kDirect>
-__global__ void __launch_bounds__(kAttnThreads, 2)
+template <int D, bool kFp8, int kCols, int kForm>
+__global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::kCtas))
     paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const __grid_constant__ AttnArgs a, const __grid_constant__ PagedCache c) {
   using T = Tile<D, kFp8>;
-  using L = Layout<D, kFp8, kCols>;
+  using L = Layout<D, kFp8, kCols, kForm>;
+  constexpr bool kDirect = L::kDirect;
   constexpr int kTokens = T::kTokens, kN = kCols / 8, kStages = L::kStages;
   constexpr float kLazy = kFp8 ? 4.0f : 8.0f;  // f16: 2^(10 + 4) at most
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -668,7 +675,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     } else {
       // [element][column], with the maxima and sums beside it
       const int slot = 2 * warp + (begins ? 1 : 0);
-      float *part = reinterpret_cast<float *>(begins ? smem + warp * L::kRing : smem + L::kParts + warp * L::kPart);
+      float *part = reinterpret_cast<float *>(kDirect || begins ? smem + warp * L::kRing : smem + L::kParts + warp * L::kPart);
       float *part_ml = reinterpret_cast<float *>(smem + L::kMl) + slot * kCols * 2;
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
@@ -701,7 +708,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     const float4 *of_ml = reinterpret_cast<const float4 *>(smem + L::kMl + (i * kCols + col0) * 8);
     const float4 p = of_ml[0], q = of_ml[1];
     const float of[4] = {p.x, p.z, q.x, q.z}, s[4] = {p.y, p.w, q.y, q.w};
-    const float4 *x = reinterpret_cast<const float4 *>((i & 1) != 0 ? smem + (i >> 1) * L::kRing : smem + L::kParts + (i >> 1) * L::kPart);
+    const float4 *x = reinterpret_cast<const float4 *>(kDirect || (i & 1) != 0 ? smem + (i >> 1) * L::kRing : smem + L::kParts + (i >> 1) * L::kPart);
     float f[4], f_old[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -1022,7 +1029,7 @@ int direct_splits(int seqs, int items, int most_tiles, int ctas) {
 template <int D, bool kFp8, int kCols>
 cudaError_t launch(AttnArgs a, const PagedCache &c, int ctas, cudaStream_t stream) {
   using T = Tile<D, kFp8>;
-  constexpr int kSmem = Layout<D, kFp8, kCols>::kTotal;
+  constexpr int kSmem = Layout<D, kFp8, kCols, kList>::kTotal;
   int box = c.page_size & -c.page_size;
   if (box > T::kTokens) box = T::kTokens;
   a.box_shift = __builtin_ctz((unsigned)box);
@@ -1044,9 +1051,15 @@ cudaError_t launch(AttnArgs a, const PagedCache &c, int ctas, cudaStream_t strea
   const int items = c.kv_heads * a.chunks;
   const int splits = direct_splits(a.seqs, items, (paged_capacity(c) - 1) / T::kTokens + 1, ctas);
   if (splits > 0) {
-    const auto kernel = paged_attention_kernel<D, kFp8, kCols, true>;
-    static bool ready[64] = {};
-    const cudaError_t err = allow_smem(kernel, kSmem, ready);
+    // Three CTAs per SM where two would leave some for a second turn, and three do not (48 x 128 tokens of 8 heads 8.0 instead of 10.7 us; with
+    // fewer, or more than three can take, it is slower: 8 x 4000 26.3 instead of 24.2, 64 x 256 18.1 instead of 16.9).
+    const long long all = (long long)a.seqs * items * splits;
+    const bool three = kCols == 8 && all > ctas && 2 * all <= 3 * ctas;
+    const auto kernel = three ? paged_attention_kernel<D, kFp8, kCols, kCols == 8 ? kDirectThree : kDirectTwo> : paged_attention_kernel<D, kFp8, kCols, kDirectTwo>;
+    // (with the smaller form's need three of two's would fit)
+    cfg.dynamicSmemBytes = three ? Layout<D, kFp8, kCols, kDirectThree>::kTotal : kSmem;
+    static bool ready[2][64] = {};
+    const cudaError_t err = allow_smem(kernel, (int)cfg.dynamicSmemBytes, ready[three]);
     if (err != cudaSuccess) return err;
     a.stretch_shift = __builtin_ctz((unsigned)(splits * kAttnWarps));
     attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -1056,7 +1069,7 @@ cudaError_t launch(AttnArgs a, const PagedCache &c, int ctas, cudaStream_t strea
     cfg.gridDim = dim3((unsigned)splits, (unsigned)items, (unsigned)a.seqs);
     return cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, a, c);
   }
-  const auto kernel = paged_attention_kernel<D, kFp8, kCols, false>;
+  const auto kernel = paged_attention_kernel<D, kFp8, kCols, kList>;
   static bool ready[64] = {};
   cudaError_t err = allow_smem(kernel, kSmem, ready);
   if (err != cudaSuccess) return err;
