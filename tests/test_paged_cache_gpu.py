@@ -500,3 +500,24 @@ def test_attention_of_few_sequences_at_every_size_of_cluster(dim, group, fp8):
             bound = P.attention_bound(out, size, reach, dim, longest, fp8)
             assert bool(((got.double() - out).abs() <= bound).all()), (longest, lengths)
     ops.check_device_errors()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+# clusters of one CTA in numbers that fill two, three and more CTAs per SM, and more than the direct form takes
+@pytest.mark.parametrize("seqs,heads,kv,dim,longest", [(37, 32, 8, 128, 300), (38, 32, 8, 128, 300), (55, 8, 8, 64, 200), (111, 12, 4, 128, 500),
+                                                       (56, 32, 8, 64, 100), (74, 32, 8, 128, 90), (75, 32, 8, 128, 90), (45, 72, 8, 128, 150)])
+def test_attention_of_many_short_sequences(seqs, heads, kv, dim, longest, fp8):
+    from sharq_b200 import ops
+
+    lengths = [(i * 37) % (longest + 1) for i in range(seqs - 1)] + [longest]
+    page = 16
+    table, pages = P.make_table(lengths, page, 1, seed=seqs)
+    k, v, ks, vs = P.make_cache(pages, kv, page, dim, fp8, 5)
+    q = torch.randn(seqs, heads, dim, generator=torch.Generator().manual_seed(seqs)).to(torch.bfloat16).cuda()
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    got = ops.paged_attention(q, k, v, table, n, k_scale=ks, v_scale=vs)
+    ops.check_device_errors()
+    out, size, reach = P.attention64(q, P.values64(k, ks), P.values64(v, vs), table, lengths)
+    bound = P.attention_bound(out, size, reach, dim, longest, fp8)
+    assert bool(((got.double() - out).abs() <= bound).all()), float(((got.double() - out).abs() / bound).max())
+    assert torch.equal(ops.paged_attention(q, k, v, table, n, k_scale=ks, v_scale=vs), got)
