@@ -152,7 +152,7 @@ static_assert(Tile<128, false>::kStage == 8192 && Tile<64, true>::kStage == 8192
 
 // What a warp leaves of an item that does not lie within its stretch.
 struct __align__(16) Part {
-  int seq, item;  // item: head and chunk, -1: nothing
+  int seq, item;  // item: which (head, chunk) of the sequence, below 2^17; -1: nothing
   int begins, tiles_left;
 };
 // Forms of the kernel: the list of tiles, and the direct one with two or three CTAs per SM.
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
           *reinterpret_cast<float2 *>(part + d1 * kCols + 8 * n + 2 * t) = make_float2(o[i][n][2], o[i][n][3]);
         }
       }
-      if (lane == 0) info[slot] = {at.seq, at.head << 16 | at.chunk, begins, n_tiles - at.end};
+      if (lane == 0) info[slot] = {at.seq, at.head * a.chunks + at.chunk, begins, n_tiles - at.end};
     }
   }
 
@@ -807,8 +807,9 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
     const bool same = now.item == run.item && now.seq == run.seq;
     if (run.item >= 0 && !same) {
       if (run.begins && run.tiles_left == 0) {
+        const int head = a.chunks == 1 ? run.item : run.item / a.chunks, chunk = run.item - head * a.chunks;
 #pragma unroll
-        for (int v = 0; v < kVecs; ++v) write(run.seq, run.item >> 16, run.item & 0xFFFF, v * kAttnThreads + threadIdx.x, acc[v]);
+        for (int v = 0; v < kVecs; ++v) write(run.seq, head, chunk, v * kAttnThreads + threadIdx.x, acc[v]);
       } else {
         // the part of an item that began in an earlier CTA goes to this CTA's first place, of one that goes on in a later one to the second
         const int place = 2 * blockIdx.x + (run.begins ? 1 : 0);

@@ -521,3 +521,22 @@ def test_attention_of_many_short_sequences(seqs, heads, kv, dim, longest, fp8):
     bound = P.attention_bound(out, size, reach, dim, longest, fp8)
     assert bool(((got.double() - out).abs() <= bound).all()), float(((got.double() - out).abs() / bound).max())
     assert torch.equal(ops.paged_attention(q, k, v, table, n, k_scale=ks, v_scale=vs), got)
+
+
+@pytest.mark.parametrize("kv,group,lengths", [(40000, 1, [65]), (33000, 1, [33, 1, 97]), (3000, 20, [70])])
+def test_attention_of_very_many_heads(kv, group, lengths):
+    """Items whose tiles fall to several warps at every index of a head, and of a piece of a group, that the interface takes."""
+    from sharq_b200 import ops
+
+    page, dim = 16, 64
+    table, pages = P.make_table(lengths, page, 1, seed=3)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    k, v = (torch.randn(pages, kv, page, dim, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    q = torch.randn(len(lengths), kv * group, dim, generator=g, device="cuda", dtype=torch.bfloat16)
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    got = torch.full_like(q, 7.0)
+    ops.paged_attention(q, k, v, table, n, out=got)
+    ops.check_device_errors()
+    out, size, reach = P.attention64(q, P.values64(k, None), P.values64(v, None), table, lengths)
+    bound = P.attention_bound(out, size, reach, dim, max(lengths), False)
+    assert bool(((got.double() - out).abs() <= bound).all()), float(((got.double() - out).abs() / bound).max())
