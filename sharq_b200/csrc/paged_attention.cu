@@ -753,6 +753,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
       mine_ml[threadIdx.x * 2] = make_float4(top[0], sum[0], top[1], sum[1]);
       mine_ml[threadIdx.x * 2 + 1] = make_float4(top[2], sum[2], top[3], sum[3]);
     }
+    __syncwarp();  // a few lanes have stored
     ptx::cluster_sync();
     // the CTAs take turns at 128 of the part's float4s, and sum in rank order
     for (int vec = blockIdx.x * kAttnThreads + threadIdx.x; vec < kVecs * kAttnThreads; vec += gridDim.x * kAttnThreads) {
