@@ -74,7 +74,7 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t smem)
 }
 __device__ __forceinline__ uint32_t movmatrix(uint32_t w) {  // transpose of an 8 x 8 matrix of 16-bit elements, two per lane
   uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));  // volatile: stays ahead of a branch that uses it
   return r;
 }
 
@@ -660,6 +660,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
           }
           if (!kFp8) {
             // [element][column] to [column][element]
+            __syncwarp();  // the stores before are of some lanes only
             const uint32_t w0 = movmatrix(pack_bf16(y[0], y[1])), w1 = movmatrix(pack_bf16(y[2], y[3]));
             if (8 * n + g < cols) {
               *reinterpret_cast<uint32_t *>(out + (8 * n + g) * D + 16 * i + 2 * t) = w0;

@@ -359,9 +359,9 @@ __global__ void __launch_bounds__(kWoThreads, 1)
             if (kPasses && pass > 0) acc[0] += to[0], acc[2] += to[step], acc[1] += to[2 * step], acc[3] += to[3 * step];
             to[0] = acc[0], to[step] = acc[2], to[2 * step] = acc[1], to[3 * step] = acc[3];
           }
+          __syncwarp();  // the next products are the whole warp's; and the stage is free
         }
         take ^= 1;
-        __syncwarp();  // the stage is free
         load();
       }
     }
