@@ -155,6 +155,8 @@ struct __align__(16) Part {
   int seq, item;  // item: which (head, chunk) of the sequence, below 2^17; -1: nothing
   int begins, tiles_left;
 };
+// A warp's wait ran out: it copies and waits for nothing more, and what is left of its stretch comes out as NaN.
+constexpr unsigned kLost = 1u << 31;
 // Forms of the kernel: the list of tiles, and the direct one with two or three CTAs per SM.
 constexpr int kList = 0, kDirectTwo = 1, kDirectThree = 2;
 
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
     }
   };
   int put = 0;              // stage that is filled next
-  unsigned bad_stages = 0;  // stages with a piece of no page
+  unsigned bad_stages = 0;  // stages with a piece of no page, and kLost
   auto load = [&]() {
     if (next.left > 0) {
       const uint32_t stage = ring + put * T::kStage;
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
         if (token < next.tokens) held_page = c.page_table[next.seq * c.table_stride + (a.page_shift >= 0 ? token >> a.page_shift : token / c.page_size)];
       }
       bool any_bad = false;
-      const bool chosen = ptx::elect_one();
+      const bool chosen = ptx::elect_one() && (bad_stages & kLost) == 0;
       if (chosen) ptx::mbar_arrive_expect_tx(bars + put, (pieces << a.box_shift) * 256 * T::kHalves);
       for (int i = 0; i < pieces; ++i) {
         int page = __shfl_sync(0xffffffffu, held_page, piece0 + i - held_first);
@@ -463,10 +465,14 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
       load();
       const uint32_t keys = ring + take * T::kStage, values = keys + T::kBytes;
       bool poison = (bad_stages >> take) & 1;
-      if (!ptx::mbar_wait(bars + take, (phases >> take) & 1, gave_up)) {
-        *gave_up = 1;
+      if (!__all_sync(0xffffffffu, (bad_stages & kLost) == 0 && ptx::mbar_wait(bars + take, (phases >> take) & 1, gave_up))) {
+        if ((bad_stages & kLost) == 0) {
+          for (int i = 0; i < kStages; ++i) ptx::mbar_drain(bars + i, (phases >> i) & 1);
+          *gave_up = 1;
+          if (a.error_flag != nullptr) atomicExch(a.error_flag, kAttentionTimeout);
+          bad_stages |= kLost;
+        }
         poison = true;
-        if (a.error_flag != nullptr) atomicExch(a.error_flag, kAttentionTimeout);
       }
       __syncwarp();
       phases ^= 1u << take;

@@ -84,6 +84,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volati
   }
 }
 
+// Behind a wait that gave up: until the copies that are counted on the barrier have landed, or as long again, whatever the abort flag says.
+// What a copy may still write must not become another CTA's memory.  (With nothing on its way it takes the whole limit.)
+__device__ __forceinline__ void mbar_drain(uint64_t *bar, uint32_t parity) {
+  const long long start = clock64();
+  while (!mbar_try_wait(bar, parity) && clock64() - start <= kWaitLimitCycles) {
+  }
+}
+
 // For barriers that another CTA of the cluster arrives on; orders no memory.
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity) {
   uint32_t ok;

@@ -49,6 +49,7 @@ constexpr int kWoSmem = 232448;
 constexpr int kWoSlice = 256;                                 // elements of K of a warp
 constexpr int kWoBox = 8 * kWoSlice / 2;                      // bytes of the codes of 8 rows
 constexpr int kWoCodes = 4 * kWoBox, kWoScales = 4 * 128;     // of 32 rows; 8 rows x 16 bytes of scale factors for each of 4 x 64 elements
+constexpr unsigned kWoLost = 1u << 31;  // a lane's wait ran out: it waits for nothing more, and the one that copies copies nothing more (a vote took 3 %)
 constexpr int kWoRing = kWoStages * (kWoCodes + kWoScales);
 constexpr int kWoBars = kWoSmem - kWoWarps * kWoStages * 8 - 16;  // the barriers behind it all, and the flag of a wait that ran out
 constexpr int kWoFactors = kWoBars - kWoWarps * 64;
@@ -188,9 +189,10 @@ __global__ void __launch_bounds__(kWoThreads, 1)
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
+  unsigned phases = 0;  // parity of every stage's barrier, and kWoLost
   auto load = [&]() {
     if (l_pair < p1) {
-      if (chosen) {
+      if (chosen && (phases & kWoLost) == 0) {
         // rows and elements that are not there come as zeros
         const int from = 2 * l_pair < j0 ? 1 : 0, to = 2 * l_pair + 1 < j1 ? 2 : 1, block = l_pair >> 2;
         ptx::mbar_arrive_expect_tx(bars + put, (to - from) * 2 * kWoBox + kWoScales);
@@ -305,7 +307,6 @@ __global__ void __launch_bounds__(kWoThreads, 1)
   const int pairs = (m + 1) >> 1, per_tile = 32 * pairs;
   const unsigned magic = a.per_tile_magic[blockIdx.z];
   int take = 0, flip = 0;
-  unsigned phases = 0;
   for (int chunk = p0; chunk < p1; chunk += a.chunk, flip ^= 1) {
     const int end = min(chunk + a.chunk, p1);
     float *part = parts + flip * (a.parts_bytes / 8);
@@ -316,9 +317,11 @@ __global__ void __launch_bounds__(kWoThreads, 1)
       }
       if (!works) continue;
       for (int pair = chunk + row_group; pair < end; pair += a.row_groups) {
-        if (!ptx::mbar_wait(bars + take, (phases >> take) & 1, gave_up)) {
+        if ((phases & kWoLost) == 0 && !ptx::mbar_wait(bars + take, (phases >> take) & 1, gave_up)) {
+          for (int i = 0; i < kWoStages; ++i) ptx::mbar_drain(bars + i, (phases >> i) & 1);
           *gave_up = 1;
           if (a.error_flag != nullptr) atomicExch(a.error_flag, kWeightOnlyTimeout);
+          phases |= kWoLost;
         }
         __syncwarp();
         phases ^= 1u << take;

@@ -1,0 +1,38 @@
+"""A kernel of the decode step whose wait for a copy runs out leaves nothing behind that still writes.
+
+A copy that lands late would write into the shared memory of whichever CTA is there by then, and a barrier that is armed again while its
+copy is on its way counts wrongly.  Making a copy late needs a GPU that stalls, so the sources are held to the rule instead: a lane whose
+wait has failed waits (with a limit of its own) for all that is on its way, and the lane that copies requests nothing more.
+"""
+import re
+
+import pytest
+
+from sharq_b200._build import CSRC
+from tests.test_dependent_launch_cpu import _block, _code
+
+
+# the attention's lanes agree on it by a vote, as what follows is for whole warps; in the products the lane that copies is the same for good
+@pytest.mark.parametrize("name,lost,stages,wait", [
+    ("paged_attention.cu", r"\(bad_stages & kLost\)", "kStages", r"if \(!__all_sync\(0xffffffffu, {lost} == 0 && ptx::mbar_wait\("),
+    ("weight_only.cu", r"\(phases & kWoLost\)", "kWoStages", r"if \({lost} == 0 && !ptx::mbar_wait\(")])
+def test_a_wait_that_ran_out(name, lost, stages, wait):
+    code = _code(CSRC / name)
+    assert code.count("mbar_wait(") == 1
+    at = code.rindex("if (", 0, code.index("mbar_wait("))
+    assert re.match(wait.format(lost=lost), code[at:])
+    if name == "weight_only.cu":
+        assert re.findall(r"\S+ \S+ \w+ = ptx::elect_one\(\)", code) == ["const bool chosen = ptx::elect_one()"]
+    given_up = _block(code, at)
+    drain = re.search(rf"for \(int i = 0; i < {stages}; \+\+i\) ptx::mbar_drain\(bars \+ i, \(phases >> i\) & 1\);", given_up)
+    assert drain and drain.start() < given_up.index("*gave_up = 1")
+    assert re.search(r"(bad_stages \|= kLost|phases \|= kWoLost);", given_up)
+    # the one lane that arms a barrier and issues copies does so only while the warp has lost nothing
+    assert code.count("mbar_arrive_expect_tx(") == 1
+    ahead = code[:code.index("mbar_arrive_expect_tx(")]
+    assert re.search(rf"chosen (=|&&)[^;{{]*{lost} == 0[^;{{]*(;|\{{)\s*(if \(chosen\) |[^}}]*)ptx::$", ahead)
+
+
+def test_the_second_wait_is_bounded_too():
+    code = _code(CSRC / "sm100_ptx.cuh")
+    assert "clock64() - start <= kWaitLimitCycles" in _block(code, code.index("void mbar_drain("))
