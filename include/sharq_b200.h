@@ -420,7 +420,8 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
 /* Product of m (1 to 16) unquantised bf16 rows (x_row elements between them, a multiple of 8) with a 4-bit weight:
  * y[m, n] = bf16(scale * scale_dev[0] * sum_k x[m, k] * W[n, k] + bias[n]), W = payload qw [n, k/2] times the dense scale factors sfw_dense, as
  * sharq_quantize_w32_shared and sharq_quantize_nvfp4 make them.  scale_dev (float on the device) and bias (bf16 [n]) may be NULL.  Float
- * sums, one rounding.  k % 64 == 0, k <= 2^24; x, qw and sfw_dense 16-byte aligned.  A wait that ran out stores 0x404 in *error_flag (may be NULL). */
+ * sums, one rounding.  k % 64 == 0, k <= 2^24; x, qw and sfw_dense 16-byte aligned.  A wait that ran out makes the results that it held up NaN and stores
+ * 0x404 in *error_flag (may be NULL). */
 int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, int k, const void *qw, const void *sfw_dense,
                              const float *scale_dev, float scale, const void *bias_bf16, void *y_bf16, int *error_flag, void *stream);
 

@@ -372,6 +372,7 @@ __global__ void __launch_bounds__(kWoThreads, 1)
     // from the first to the last of the chunk's tiles
     const int first = (max(2 * chunk, j0) - 2 * chunk) * per_tile / 4, count = (min(2 * end, j1) - 2 * chunk) * per_tile / 4;
     float4 *sum_of = reinterpret_cast<float4 *>(sums + flip * (kWoSums / 4));
+    const bool lost = *gave_up != 0;  // a warp of this CTA had no weight to multiply
     // four rows of a column at a time
     auto add = [](float4 &y, const float4 &v) { y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w; };
     auto finish = [&](int i, float4 y) {
@@ -406,6 +407,7 @@ __global__ void __launch_bounds__(kWoThreads, 1)
 #pragma unroll
         for (int s = 0; s < 8; ++s) add(y, v[s]);
       }
+      if (lost) y.x = y.y = y.z = y.w = __int_as_float(0x7fffffff);
       if (a.cluster == 1)
         finish(i, y);
       else

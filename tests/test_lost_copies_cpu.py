@@ -36,3 +36,13 @@ def test_a_wait_that_ran_out(name, lost, stages, wait):
 def test_the_second_wait_is_bounded_too():
     code = _code(CSRC / "sm100_ptx.cuh")
     assert "clock64() - start <= kWaitLimitCycles" in _block(code, code.index("void mbar_drain("))
+
+
+def test_products_without_their_weight_are_nan():
+    """Every sum that a CTA takes of its warps' parts behind a wait that ran out, whether it goes out or to the other CTAs of a cluster."""
+    code = _code(CSRC / "weight_only.cu")
+    at = code.index("const bool lost = *gave_up != 0;")
+    assert "__syncthreads();" in code[code.rindex("}", 0, at):at]  # behind the warps' last wait
+    sums = _block(code, code.index("for (int i = first + threadIdx.x; i < count;", at))
+    poison = sums.index("if (lost) y.x = y.y = y.z = y.w = __int_as_float(0x7fffffff);")
+    assert sums.rindex("add(y, v[s])") < poison < sums.index("finish(i, y)") and poison < sums.index("sum_of[i] = y")
