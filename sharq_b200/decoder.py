@@ -660,7 +660,9 @@ class SharqDecoder(torch.nn.Module):
 
     def new_cache(self, sequences: int, max_tokens: int, page_size: int = 64, pages: int = None, dtype: torch.dtype = torch.bfloat16,
                   k_scale: torch.Tensor = None, v_scale: torch.Tensor = None) -> PagedKVCache:
-        """A paged cache for this model's (this rank's) key/value heads, see PagedKVCache."""
+        """A paged cache for this model's (this rank's) key/value heads, see PagedKVCache.  Heads of 64 or 128, which ops.paged_attention takes."""
+        if self.cfg.head_dim not in (64, 128):
+            raise ValueError(f"decode steps take heads of 64 or 128, not {self.cfg.head_dim}")
         cos, sin = rope_tables(max_tokens, self.cfg.head_dim, self.cfg.rope_theta, self.embed.device)
         return PagedKVCache(len(self.layers), self.layers[0].local_kv, self.cfg.head_dim, sequences, max_tokens, cos, sin, page_size, pages,
                             dtype, k_scale, v_scale)
