@@ -66,9 +66,11 @@ class DecoderConfig:
                                        rope_theta=1e6, qkv_bias=True), **kw})
 
 
-def rope_tables(seq: int, head_dim: int, theta: float, device) -> tuple[torch.Tensor, torch.Tensor]:
-    inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, device=device, dtype=torch.float32) / head_dim))
-    ang = torch.outer(torch.arange(seq, device=device, dtype=torch.float32), inv)
+def rope_tables(seq: int, head_dim: int, theta: float, device, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16 cosines and sines [seq, head_dim] of the rotary embedding.  dtype: of the angles.  In float32 they are off by up to 2^-24 of the
+    position and as much again, more than the rounding to bf16 of a cosine from some 32000 positions on."""
+    inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, device=device, dtype=dtype) / head_dim))
+    ang = torch.outer(torch.arange(seq, device=device, dtype=dtype), inv)
     emb = torch.cat((ang, ang), dim=-1)
     return emb.cos().to(torch.bfloat16), emb.sin().to(torch.bfloat16)
 
@@ -663,7 +665,7 @@ class SharqDecoder(torch.nn.Module):
         """A paged cache for this model's (this rank's) key/value heads, see PagedKVCache.  Heads of 64 or 128, which ops.paged_attention takes."""
         if self.cfg.head_dim not in (64, 128):
             raise ValueError(f"decode steps take heads of 64 or 128, not {self.cfg.head_dim}")
-        cos, sin = rope_tables(max_tokens, self.cfg.head_dim, self.cfg.rope_theta, self.embed.device)
+        cos, sin = rope_tables(max_tokens, self.cfg.head_dim, self.cfg.rope_theta, self.embed.device, torch.float64)  # as long as a cache may be
         return PagedKVCache(len(self.layers), self.layers[0].local_kv, self.cfg.head_dim, sequences, max_tokens, cos, sin, page_size, pages,
                             dtype, k_scale, v_scale)
 
