@@ -26,6 +26,7 @@ Weights are random (N(0, 0.02)): there are no checkpoints in this environment.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Sequence
 
 import torch
 import torch.nn.functional as F
@@ -615,18 +616,24 @@ class SharqDecoder(torch.nn.Module):
         return tp.sequence_parallel_context(m, self.cfg.hidden, None, self.embed.device)
 
     @torch.no_grad()
-    def prefill(self, token_ids: torch.Tensor, reference: bool = False, cache: PagedKVCache = None) -> torch.Tensor:
+    def prefill(self, token_ids: torch.Tensor, reference: bool = False, cache: PagedKVCache = None,
+                sequences: Sequence[int] = None) -> torch.Tensor:
         """token_ids [B, S] -> logits of the last position [B, vocab] (float32).
-        reference=True runs the unquantised bf16 layers (needs keep_reference=True).  cache: an empty cache of B sequences, which
-        then holds the prompts (decode)."""
+        reference=True runs the unquantised bf16 layers (needs keep_reference=True).  cache: holds the prompts afterwards (decode), as its
+        sequences, which are B and empty, or as those listed in sequences, which are B and empty, whatever the others hold."""
         b, s = token_ids.shape
         kvs = [None] * len(self.layers)
+        if cache is None and sequences is not None:
+            raise ValueError("sequences are those of a cache")
         if cache is not None:
-            if b != cache.sequences or any(cache.lengths):
-                raise ValueError("prefill takes an empty cache with a sequence for every prompt")
-            cache.reserve([s] * b)
-            positions, sequences = cache.prompt_step(s)
-            kvs = [cache.layer(i, positions, sequences, None) for i in range(len(self.layers))]
+            which = cache.chosen(sequences)
+            if b != len(which) or any(cache.lengths[i] for i in which):
+                raise ValueError("prefill takes an empty cache with a sequence for every prompt" if sequences is None else
+                                 "prefill takes one empty sequence of the cache for every prompt")
+            counts = cache.counts(which, s)
+            cache.reserve(counts)
+            positions, rows = cache.prompt_step(s, sequences)
+            kvs = [cache.layer(i, positions, rows, None) for i in range(len(self.layers))]
         cos, sin = rope_tables(s, self.cfg.head_dim, self.cfg.rope_theta, self.embed.device)
         sp = None if reference else self._sequence_parallel_context(b * s)
         if sp is not None:
@@ -657,7 +664,7 @@ class SharqDecoder(torch.nn.Module):
                 x = x + delta
             last = x[:, -1, :].float()
         if cache is not None:
-            cache.advance([s] * b)
+            cache.advance(counts)
         return self._logits(last)
 
     def new_cache(self, sequences: int, max_tokens: int, page_size: int = 64, pages: int = None, dtype: torch.dtype = torch.bfloat16,
@@ -670,28 +677,35 @@ class SharqDecoder(torch.nn.Module):
                             dtype, k_scale, v_scale)
 
     @torch.no_grad()
-    def decode(self, token_ids: torch.Tensor, cache: PagedKVCache, reference: bool = False, weight_only: bool = False) -> torch.Tensor:
-        """One more token of every sequence of the cache: token_ids [B] -> logits of the next one [B, vocab] (float32).
-        weight_only: the linears take the activations unquantised (at most 16 sequences).  reference: as in prefill."""
+    def decode(self, token_ids: torch.Tensor, cache: PagedKVCache, reference: bool = False, weight_only: bool = False,
+               sequences: Sequence[int] = None) -> torch.Tensor:
+        """One more token of every sequence of the cache (an empty one begins with it), or of those listed in sequences, in that order:
+        token_ids [B] -> logits of the next one [B, vocab] (float32).  weight_only: the linears take the activations unquantised (at most 16 sequences).  reference: as in prefill."""
+        which = cache.chosen(sequences)
         b = int(token_ids.shape[0])
-        if token_ids.dim() != 1 or b != cache.sequences:
-            raise ValueError("decode takes one token for every sequence of the cache")
+        if token_ids.dim() != 1 or b != len(which):
+            raise ValueError("decode takes one token for every sequence of the cache" + ("" if sequences is None else " that is listed"))
         if weight_only and b > 16:
             raise ValueError(f"weight_only takes at most 16 sequences, got {b}")
-        cache.reserve([1] * b)
-        logits = self.decode_step(token_ids, cache, cache.device_lengths, cache.device_lengths + 1, reference, weight_only)
-        cache.advance([1] * b)
+        counts = cache.counts(which, 1)
+        cache.reserve(counts)
+        rows = None if sequences is None else torch.tensor(which, device=cache.table.device)
+        positions = cache.device_lengths if rows is None else cache.device_lengths[rows]
+        logits = self.decode_step(token_ids, cache, positions, positions + 1, reference, weight_only, rows)
+        cache.advance(counts)
         return logits
 
     @torch.no_grad()
     def decode_step(self, token_ids: torch.Tensor, cache: PagedKVCache, positions: torch.Tensor, lengths: torch.Tensor,
-                    reference: bool = False, weight_only: bool = False) -> torch.Tensor:
+                    reference: bool = False, weight_only: bool = False, rows: torch.Tensor = None) -> torch.Tensor:
         """The device part of decode, for capture in a CUDA graph: positions and lengths (int32 [B], device) of the new tokens and of the
-        sequences with them, whose pages have been reserved; the cache's own lengths stay.  A graph reads the page table as wide as it was
+        sequences with them, whose pages have been reserved; the cache's own lengths stay.  rows (int64 [B], device, different): the sequences
+        of the cache that the tokens belong to, default all of them in order.  A graph reads the page table as wide as it was
         at the capture: reserve the tokens of all replays before it."""
         x, delta = self.embed[token_ids][:, None], None
+        table = cache.held_table(rows)
         for i, layer in enumerate(self.layers):
-            kv = cache.layer(i, positions, None, lengths)
+            kv = cache.layer(i, positions, None, lengths, table)
             if reference:
                 x = layer.forward_reference(x, kv.cos, kv.sin, kv)
             else:

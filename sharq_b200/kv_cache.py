@@ -89,21 +89,42 @@ class PagedKVCache:
             self.device_lengths += torch.tensor(list(counts), dtype=torch.int32, device=self.table.device)
 
     def free(self, sequence: int) -> None:
-        """Gives the pages of a sequence back; it is empty then."""
+        """Gives the pages of a sequence back; it is empty then, and another prompt may take its place (SharqDecoder.prefill with sequences)."""
         self._free += reversed(self._held[sequence])
         self._held[sequence] = []
         self.lengths[sequence] = 0
         self.device_lengths[sequence] = 0
 
-    def prompt_step(self, tokens: int):
-        """(positions, sequences) int32 of `tokens` new tokens of every sequence, sequence after sequence."""
-        device = self.table.device
-        positions = (self.device_lengths[:, None] + torch.arange(tokens, dtype=torch.int32, device=device)).reshape(-1)
-        return positions, torch.arange(self.sequences, dtype=torch.int32, device=device).repeat_interleave(tokens)
+    def chosen(self, sequences: Optional[Sequence[int]]) -> list[int]:
+        """The sequences that a step is for: all of them, or those listed, each once."""
+        which = list(range(self.sequences)) if sequences is None else [int(i) for i in sequences]
+        if not which or len(set(which)) != len(which) or not all(0 <= i < self.sequences for i in which):
+            raise ValueError(f"sequences must be different numbers below {self.sequences}, got {which}")
+        return which
 
-    def layer(self, index: int, positions: torch.Tensor, sequences: Optional[torch.Tensor], lengths: Optional[torch.Tensor]) -> LayerCache:
-        """Layer `index` for a step; the page table is cut to what the longest sequence holds."""
-        held = max(1, max(len(h) for h in self._held))
+    def counts(self, which: Sequence[int], tokens: int) -> list[int]:
+        """For reserve and advance: `tokens` of every sequence in `which`, none of the others."""
+        listed = set(which)
+        return [tokens if i in listed else 0 for i in range(self.sequences)]
+
+    def prompt_step(self, tokens: int, sequences: Optional[Sequence[int]] = None):
+        """(positions, sequences) int32 of `tokens` new tokens of every sequence, or of those listed, sequence after sequence."""
+        device = self.table.device
+        first, which = self.device_lengths, torch.arange(self.sequences, dtype=torch.int32, device=device)
+        if sequences is not None:
+            which = torch.tensor(self.chosen(sequences), dtype=torch.int32, device=device)
+            first = first[which.long()]
+        positions = (first[:, None] + torch.arange(tokens, dtype=torch.int32, device=device)).reshape(-1)
+        return positions, which.repeat_interleave(tokens)
+
+    def held_table(self, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The page table cut to what the longest sequence holds, of all sequences or of those in rows (int64, device)."""
+        table = self.table[:, :max(1, max(len(h) for h in self._held))]
+        return table if rows is None else table[rows]
+
+    def layer(self, index: int, positions: torch.Tensor, sequences: Optional[torch.Tensor], lengths: Optional[torch.Tensor],
+              table: Optional[torch.Tensor] = None) -> LayerCache:
+        """Layer `index` for a step.  table: the rows of the page table that belong to the step's rows, default held_table()."""
         return LayerCache(self.k[index], self.v[index], None if self.k_scale is None else self.k_scale[index],
-                          None if self.v_scale is None else self.v_scale[index], self.table[:, :held], positions, sequences, lengths,
-                          self.cos, self.sin)
+                          None if self.v_scale is None else self.v_scale[index], self.held_table() if table is None else table, positions,
+                          sequences, lengths, self.cos, self.sin)
