@@ -23,11 +23,13 @@
 // The maximum is raised only when a score exceeds it by more than kLazy (then probabilities stay below 2^kLazy, and the sum and the output
 // are relative to the same value): raising it costs shuffles and a pass over the output.
 //
-// e4m3 caches go through f16: their values are exact in it, queries are scaled to it by a power of two per head (a value below 2^-39 of its
-// head's largest is lost), and probabilities carry a factor of 2^10, so that those down to 2^-24 of the maximum keep f16's full precision.  For bf16
-// caches the probabilities enter as the sum of two bf16 numbers, 16 bits (rounded to one they made half of the result's error, and the reading of the
-// cache hides the second product); both are positive, for an infinite value has an infinite product with either.  They carry a factor of 2^-32, so that
-// no sum of finite values overflows; 2^-94 of the maximum and less is 0.
+// e4m3 caches go through f16: their values are exact in it, queries are scaled to it by a power of two per head (exact down to 2^-31 of the head's
+// largest, off by at most 2^-39 of that below), and probabilities carry a factor of 2^10, so that those down to 2^-24 of the maximum keep f16's full
+// precision.  The probabilities enter as the sum of two numbers: for bf16 caches two bf16 numbers, 16 bits (rounded to one they made half of the result's
+// error, and the reading of the cache hides the second product; both are positive, for an infinite value has an infinite product with either), for e4m3 caches
+// two f16 numbers, 21 bits (with one, values that nearly cancel came out several steps off; it costs nothing for 128 sequences of 33 to 8192 tokens, 1 % for
+// 8 x 2048 tokens of 8 heads, 7 % for 20 x 2000).  For bf16 caches they carry a factor of 2^-32, so that no sum of finite values overflows; 2^-94 of the
+// maximum and less is 0.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -579,8 +581,13 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
             l[n][j & 1] += p[j];
           }
           if (kFp8) {
-            pb[n][0] = movmatrix(pack_f16(p[0], p[1]));
-            pb[n][1] = movmatrix(pack_f16(p[2], p[3]));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              // the upper 11 bits, and what they leave
+              const float x = __uint_as_float(__float_as_uint(p[2 * j]) & 0xFFFFE000u), y = __uint_as_float(__float_as_uint(p[2 * j + 1]) & 0xFFFFE000u);
+              pb[n][j] = movmatrix(pack_f16(x, y));
+              pb_lo[n][j] = movmatrix(pack_f16(p[2 * j] - x, p[2 * j + 1] - y));
+            }
           } else {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -630,6 +637,8 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
             for (int n = 0; n < kN; ++n) {
               mma16816<kFp8>(o[2 * i][n], even, pb[n][0], pb[n][1]);
               mma16816<kFp8>(o[2 * i + 1][n], odd, pb[n][0], pb[n][1]);
+              mma16816<kFp8>(o[2 * i][n], even, pb_lo[n][0], pb_lo[n][1]);
+              mma16816<kFp8>(o[2 * i + 1][n], odd, pb_lo[n][0], pb_lo[n][1]);
             }
           }
         }

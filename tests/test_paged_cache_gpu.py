@@ -540,3 +540,28 @@ def test_attention_of_very_many_heads(kv, group, lengths):
     out, size, reach = P.attention64(q, P.values64(k, None), P.values64(v, None), table, lengths)
     bound = P.attention_bound(out, size, reach, dim, max(lengths), False)
     assert bool(((got.double() - out).abs() <= bound).all()), float(((got.double() - out).abs() / bound).max())
+
+
+@pytest.mark.parametrize("room", ["short", "wide"])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim,group", [(64, 3), (128, 4), (128, 12)])
+def test_attention_of_values_that_nearly_cancel(dim, group, fp8, room):
+    """Values of +-448 under probabilities that differ by a few thousandths: 11 bits of a probability are too few for the difference, with
+    a cache of either type.  (16 bits, as attention_bound has them for bf16.)"""
+    from sharq_b200 import ops
+
+    lengths, page, kv = [2, 34, 4, 1], 16, 2
+    table, pages = P.make_table(lengths, page, 1, seed=4)
+    g = torch.Generator().manual_seed(group)
+    k = torch.randn(pages, kv, page, dim, generator=g).to(torch.float8_e4m3fn)
+    sign = 1 - 2 * (torch.arange(page) % 2)
+    v = (448.0 * sign[None, None, :, None]).expand(pages, kv, page, dim).to(torch.float8_e4m3fn).contiguous()
+    k, v = (x.cuda() if fp8 else x.float().to(torch.bfloat16).cuda() for x in (k, v))
+    ks, vs = (torch.tensor([1.0, 0.25], device="cuda"), torch.tensor([0.5, 1.0], device="cuda")) if fp8 else (None, None)
+    q = (2.0 ** -7 * torch.randn(len(lengths), kv * group, dim, generator=g)).to(torch.bfloat16).cuda()
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    got = ops.paged_attention(q, k, v, wide(table, page) if room == "wide" else table, n, k_scale=ks, v_scale=vs)
+    ops.check_device_errors()
+    out, size, reach = P.attention64(q, P.values64(k, ks), P.values64(v, vs), table, lengths)
+    bound = P.attention_bound(out, size, reach, dim, max(lengths), False)
+    assert bool(((got.double() - out).abs() <= bound).all()), float(((got.double() - out).abs() / bound).max())
