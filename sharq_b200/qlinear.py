@@ -236,7 +236,7 @@ class QLinearLayer(nn.Module):
         folded = bias if (bias is not None and bias.dtype == torch.bfloat16 and bias.dim() == 1 and bias.is_contiguous()
                           and bias.numel() == self.out_features) else None
         y = ops.weight_only_linear(x2, self.weight_q, sf, self.weight_scale_host, bias=folded)
-        return (y if folded is bias else y + bias).reshape(*x.shape[:-1], -1)
+        return (y if folded is bias else y + bias).reshape(*x.shape[:-1], self.out_features)
 
 
 QLINEAR_METHODS = {name: vars(QLinearLayer)[name] for name in ("prepare_input", "prepare_input_swiglu", "apply_prepared")}

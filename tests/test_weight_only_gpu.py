@@ -211,3 +211,15 @@ def test_results_and_biases_at_any_element(m, n):
         assert ops.weight_only_linear(x, qw, sf, 0.5, bias=bias[1:], out=out) is not None
         assert torch.equal(out, want)
         assert bool((room[:shift] == 7).all()) and bool((room[shift + m * n:] == 7).all())
+
+
+@pytest.mark.parametrize("shape", [(0, 256), (2, 0, 256), (256,), (1, 1, 3, 256)])
+def test_layer_forward_of_every_shape(shape):
+    """No rows, a single one without a dimension of its own, and several dimensions."""
+    from sharq_b200.qlinear import QLinearLayer
+
+    layer = QLinearLayer(torch.nn.Linear(256, 320, bias=True), quant_type="SHARQ", device="cuda")
+    x = torch.randn(shape, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).cuda()
+    got = layer.forward_weight_only(x)
+    assert got.shape == (*shape[:-1], 320)
+    assert torch.equal(got.reshape(-1, 320), layer.forward_weight_only(x.reshape(-1, 256)))
