@@ -118,9 +118,13 @@ class PagedKVCache:
         return positions, which.repeat_interleave(tokens)
 
     def held_table(self, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """The page table cut to what the longest sequence holds, of all sequences or of those in rows (int64, device)."""
+        """The page table cut to what the longest sequence holds, of all sequences or of those in rows (int64, device).  A row of no
+        sequence has no pages, which the kernels report."""
         table = self.table[:, :max(1, max(len(h) for h in self._held))]
-        return table if rows is None else table[rows]
+        if rows is None:
+            return table
+        there = (rows >= 0) & (rows < self.sequences)
+        return torch.where(there[:, None], table[rows.clamp(0, self.sequences - 1)], -1)
 
     def layer(self, index: int, positions: torch.Tensor, sequences: Optional[torch.Tensor], lengths: Optional[torch.Tensor],
               table: Optional[torch.Tensor] = None) -> LayerCache:

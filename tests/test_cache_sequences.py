@@ -26,6 +26,8 @@ def test_a_step_of_some_sequences():
     layer = cache.layer(0, positions, None, None, cache.held_table(rows))
     assert torch.equal(layer.table, cache.table[[2, 1], :2])
     assert torch.equal(cache.layer(0, positions, None, None).table, cache.table[:, :2])
+    strange = cache.held_table(torch.tensor([1, 3, -1, 2 ** 40]))  # of no sequence: no pages
+    assert torch.equal(strange[0], cache.table[1, :2]) and bool((strange[1:] == -1).all()) and strange.dtype == torch.int32
 
 
 @pytest.mark.parametrize("sequences", [[], [3], [-1], [0, 0], [0, 1, 2, 0]])
@@ -158,3 +160,25 @@ def test_refusals_of_some_sequences():
     with pytest.raises(ValueError, match="empty cache"):
         model.prefill(ids, cache=cache)
     assert cache.lengths == [0, 5, 0]
+
+
+@pytest.mark.gpu
+def test_a_step_of_no_sequence_is_reported():
+    from sharq_b200 import ops
+    from sharq_b200.decoder import SharqDecoder
+
+    cfg = small()
+    model = SharqDecoder(cfg, torch.device("cuda"), seed=3)
+    ids = torch.randint(0, cfg.vocab, (2, 9), generator=torch.Generator().manual_seed(1)).cuda()
+    cache = model.new_cache(2, 32, page_size=16)
+    model.prefill(ids[:, :8], cache=cache)
+    cache.reserve([1, 1])
+    before = cache.k.view(torch.int16).clone()
+    positions = torch.tensor([8, 8], dtype=torch.int32).cuda()
+    logits = model.decode_step(ids[:, 8], cache, positions, positions + 1, weight_only=True, rows=torch.tensor([1, 2]).cuda())
+    with pytest.raises(RuntimeError, match="paged cache"):
+        ops.check_device_errors()
+    assert bool(torch.isfinite(logits[0]).all()) and bool(logits[1].isnan().all())
+    page = cache._held[1][0]  # only the other sequence's token went into the cache
+    before[:, page, :, 8] = cache.k.view(torch.int16)[:, page, :, 8]
+    assert torch.equal(cache.k.view(torch.int16), before)
