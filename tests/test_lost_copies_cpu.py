@@ -12,17 +12,13 @@ from sharq_b200._build import CSRC
 from tests.test_dependent_launch_cpu import _block, _code
 
 
-# the attention's lanes agree on it by a vote, as what follows is for whole warps; in the products the lane that copies is the same for good
-@pytest.mark.parametrize("name,lost,stages,wait", [
-    ("paged_attention.cu", r"\(bad_stages & kLost\)", "kStages", r"if \(!__all_sync\(0xffffffffu, {lost} == 0 && ptx::mbar_wait\("),
-    ("weight_only.cu", r"\(phases & kWoLost\)", "kWoStages", r"if \({lost} == 0 && !ptx::mbar_wait\(")])
-def test_a_wait_that_ran_out(name, lost, stages, wait):
+@pytest.mark.parametrize("name,lost,stages", [("paged_attention.cu", r"\(bad_stages & kLost\)", "kStages"),
+                                              ("weight_only.cu", r"\(phases & kWoLost\)", "kWoStages")])
+def test_a_wait_that_ran_out(name, lost, stages):
     code = _code(CSRC / name)
     assert code.count("mbar_wait(") == 1
     at = code.rindex("if (", 0, code.index("mbar_wait("))
-    assert re.match(wait.format(lost=lost), code[at:])
-    if name == "weight_only.cu":
-        assert re.findall(r"\S+ \S+ \w+ = ptx::elect_one\(\)", code) == ["const bool chosen = ptx::elect_one()"]
+    assert re.match(rf"if \({lost} == 0 && !ptx::mbar_wait\(", code[at:])
     given_up = _block(code, at)
     drain = re.search(rf"for \(int i = 0; i < {stages}; \+\+i\) ptx::mbar_drain\(bars \+ i, \(phases >> i\) & 1\);", given_up)
     assert drain and drain.start() < given_up.index("*gave_up = 1")
@@ -46,3 +42,13 @@ def test_products_without_their_weight_are_nan():
     sums = _block(code, code.index("for (int i = first + threadIdx.x; i < count;", at))
     poison = sums.index("if (lost) y.x = y.y = y.z = y.w = __int_as_float(0x7fffffff);")
     assert sums.rindex("add(y, v[s])") < poison < sums.index("finish(i, y)") and poison < sums.index("sum_of[i] = y")
+
+
+def test_attention_behind_a_lost_tile_is_nan():
+    """Every item that the lane takes part in from then on, finished or left as a part, by the sum of its probabilities."""
+    code = _code(CSRC / "paged_attention.cu")
+    at = code.index("const float lost = (bad_stages & kLost) != 0 ? __int_as_float(0x7fffffff) : 0.0f;")
+    tiles, added = code.index("for (int tile = at.tile; tile < at.end; ++tile)"), code.index("l[n][j] += lost;", at)
+    assert tiles + len(_block(code, tiles)) <= at
+    assert code.index("l[n][j] += __shfl_xor_sync(", at) > added
+    assert added < code.index("__fdividef(kFp8 ? c.v_scale[kv] : 1.0f, l[n][j])") and added < code.index("make_float4(m[n][0], l[n][0], m[n][1], l[n][1])")
