@@ -85,7 +85,7 @@ constexpr int kManyRows = 512, kHeadsOfMany = 3;
 // A thread takes 8 elements of the first half of a head and their 8 partners of the second half: threadIdx = (vector of the half head, head,
 // row of the CTA), so that nothing is divided to find them; its further heads are blockDim.y apart and share the row's place and the tables.
 // What it rotates is loaded first, and the row's place is found meanwhile: a thread that looked the place up before it loaded anything took
-// 98 us for 16384 rows of 36 heads of 128, 53.5 now (91 % of the rate of a copy).  With the 84 registers that the compiler takes without the
+// 98 us for 16384 rows of 36 heads of 128, 53.5 to 55 now (91 to 89 % of the rate of a copy).  With the 84 registers that the compiler takes without the
 // second bound (64) it is 61.7, for want of warps: what it has to spill costs less.
 template <bool kFp8, int kHeads>
 __global__ void __launch_bounds__(512, 2) rope_append_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ PagedCache c) {

@@ -12,16 +12,16 @@
 // A warp keeps 256 elements of K of up to eight rows of the activation in registers, as f16 operands, and streams that slice of the weight's
 // rows past them, 16 rows at a time, through a ring of its own (one tensor-map copy for each, two of them a stage; with cp.async every 16
 // bytes of every lane passed the load unit, half of the time).  f16 is reached by scaling 128 elements of a row by the power of two that takes their
-// largest to [2^14, 2^15): exact but for elements below 2^-39 of it.  Sums are float; the weight's scale is in the factors of the
+// largest to [2^14, 2^15): exact down to 2^-31 of it, and off by at most 2^-39 of it below that, where f16's numbers end.  Sums are float; the weight's scale is in the factors of the
 // blocks of 128, so that no sum overflows that the result would not.  A CTA's 16 warps cover 4096 elements of K (or fewer, and several rows at a
 // time), the CTAs of a cluster the rest; the clusters take equal shares of the rows.  The warps' sums of some rows meet in shared memory,
 // those of CTAs in distributed shared memory, each added up in a fixed order: the same bits from call to call, no scratch and no second launch.
 // More than eight rows are two halves of the grid, the second of which reads the weight from L2.
 //
-// 28672 x 4096: one row 14.5 us (4.6 TB/s, 70 % of the rate of a copy), 8 rows 17.2, 16 rows 28.8; 4096 x 4096, one row: 4.9 us.  (Tiles of 128
+// 28672 x 4096: one row 14.1 us (4.7 TB/s, 72 % of the rate of a copy), 8 rows 17.1, 16 rows 27.9; 4096 x 4096, one row: 4.8 us.  (Tiles of 128
 // rows per CTA with the activation in shared memory, 323 instead of 265 instructions per 16 rows x 256 and uneven shares: 19.8, 38 with 16
-// rows and 6.6.)  The loop's instructions take 7 us to issue, beside the copies' 10; the activation's way to the registers comes before, the
-// join after.  Both eights of 16 rows in one warp, the weight converted once for 128 elements of K of each, took 34 us instead of 29 and, for
+// rows and 6.6.)  The loop's instructions take 7 us to issue, below the copies' 10: what bounds it are the copies and the 4 us around
+// the loop, in which they stand still, the activation's way to the registers before it and the join after.  Both eights of 16 rows in one warp, the weight converted once for 128 elements of K of each, took 34 us instead of 29 and, for
 // 13 rows of 4608 x 3584, 8.8 instead of 8.0: twice as many parts to join, and clusters of two CTAs where one does.  Joining a chunk of rows while
 // the next is multiplied gained nothing.
 #include <cuda.h>
