@@ -425,6 +425,48 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
 int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, int k, const void *qw, const void *sfw_dense,
                              const float *scale_dev, float scale, const void *bias_bf16, void *y_bf16, int *error_flag, void *stream);
 
+/* Pages and places of a step's tokens, from lengths on the device.  Sequence i holds lengths[i] tokens in the first
+ * ceil(lengths[i] / page_size) pages of its row of page_table [sequences, max_pages] (page_table_stride entries between rows); the free pages are
+ * free_pages[0 .. free_count[0]), a stack of room for free_pages_size.  In this order:
+ *   - sequences with released[i] != 0 (NULL: none) put their pages back on the stack, in ascending order, each its last page first, and are empty;
+ *   - counts[i] new tokens of every sequence get their pages from the top of the stack, in ascending order of the sequences, and lengths[i] grows
+ *     by them.  A sequence gets all of what it asks for or nothing: where the pages do not suffice for it and those ahead of it, it gets
+ *     nothing, and neither does any later one that needs a page.
+ * page_table, lengths, free_pages and free_count are changed in place; entries that no sequence holds, or behind the free ones, stay as they are.
+ * offsets [sequences + 1] are the counts' sums: the rows of sequence i are offsets[i] .. offsets[i + 1].  positions[r] and row_sequences[r]
+ * of the `rows` rows are a row's place for sharq_rope_append_paged: position -1 in the rows of a sequence that got nothing, and -1 with
+ * sequence 0 behind the last.
+ * A length, count, sum of counts above `rows` or number of free pages that cannot be makes the sequences that it concerns get nothing and stores 0x405 in
+ * *error_flag (may be NULL).  No workspace; calls on one cache must not overlap. */
+int sharq_plan_paged_step(int *page_table, int64_t page_table_stride, int sequences, int max_pages, int page_size, int *lengths,
+                          const int *counts, const unsigned char *released, int *free_pages, int free_pages_size, int *free_count,
+                          int rows, int *offsets, int *positions, int *row_sequences, int *error_flag, void *stream);
+
+/* Penalties for repeated tokens, biases and masks on logits [rows, vocab] (float, or bf16 with bf16 != 0), into out of the same type, which may be
+ * the logits themselves but must not overlap them otherwise.  tokens [rows, width] (int32, or int64 with wide_tokens != 0) is the history of
+ * every row, of which the first lengths[r] count and the first prompt_lengths[r] (NULL: none) of those are the prompt; a negative one is padding.
+ *   x = x > 0 ? x / repetition[r] : x * repetition[r]      for tokens of the history
+ *   x = x - frequency[r] * n - presence[r]                 for tokens that follow the prompt, n times
+ *   x = x + bias_values[j]                                 for every j in bias_offsets[r] .. bias_offsets[r + 1] with that bias_ids[j]
+ *   x = -inf                                               where bit (token % 32) of mask[r * mask_stride + token / 32] is not set
+ * in double, rounded once; a logit that nothing concerns stays as it is.  Each of tokens with lengths, the penalties, the biases and the mask
+ * may be NULL.  Strides in elements (words for the mask, which has ceil(vocab / 32) in a row).  What lies outside its range (a length, an offset, a token of vocab or more,
+ * the token of a bias) is passed over and stores 0x406 in *error_flag (may be NULL).  rows <= 65535. */
+typedef struct sharq_logit_rules {
+  const void *tokens;
+  int64_t tokens_stride;
+  int width, wide_tokens;
+  const int *lengths, *prompt_lengths;
+  const float *repetition, *presence, *frequency;
+  const int *bias_offsets, *bias_ids;
+  const float *bias_values;
+  int biases;
+  const unsigned *mask;
+  int64_t mask_stride;
+} sharq_logit_rules;
+int sharq_adjust_logits(const void *logits, int64_t logits_stride, void *out, int64_t out_stride, int rows, int vocab, int bf16,
+                        const sharq_logit_rules *rules, int *error_flag, void *stream);
+
 /* Test/tuning hook: how many SM clock cycles a cross-GPU wait of the all-reduce and transition
  * kernels may take before the kernel gives up, stores its error code and returns (0 restores the
  * defaults of two to ten seconds).  Applies to launches made after the call. */

@@ -823,6 +823,56 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
                     "paged_attention");
 }
 
+int sharq_plan_paged_step(int *page_table, int64_t page_table_stride, int sequences, int max_pages, int page_size, int *lengths,
+                          const int *counts, const unsigned char *released, int *free_pages, int free_pages_size, int *free_count,
+                          int rows, int *offsets, int *positions, int *row_sequences, int *error_flag, void *stream) {
+  SHARQ_REQUIRE(page_table && lengths && counts && free_count && offsets, "null buffer");
+  SHARQ_REQUIRE(sequences > 0 && max_pages > 0 && page_size > 0, "sequences, max_pages and page_size must be positive");
+  SHARQ_REQUIRE(page_table_stride >= max_pages || sequences == 1, "page_table_stride must cover max_pages");
+  SHARQ_REQUIRE(free_pages_size >= 0 && (free_pages_size == 0 || free_pages), "free_pages must have room for free_pages_size pages");
+  SHARQ_REQUIRE(rows >= 0 && (rows == 0 || (positions && row_sequences)), "rows must be >= 0, with a place for each");
+  const sharq::StepPlan p = {page_table, page_table_stride, sequences, max_pages, page_size, lengths, counts, released, free_pages,
+                             free_pages_size, free_count, rows, offsets, positions, row_sequences, error_flag};
+  return check_cuda(sharq::run_step_plan(p, as_stream(stream)), "plan_paged_step");
+}
+
+int sharq_adjust_logits(const void *logits, int64_t logits_stride, void *out, int64_t out_stride, int rows, int vocab, int bf16,
+                        const sharq_logit_rules *rules, int *error_flag, void *stream) {
+  SHARQ_REQUIRE(logits && out && rules, "null buffer");
+  SHARQ_REQUIRE(rows >= 1 && rows <= 65535 && vocab >= 1 && vocab <= 0x7ff00000, "rows must be in [1, 65535], vocab in [1, 2^31 - 2^20]");
+  SHARQ_REQUIRE(rows == 1 || (logits_stride >= vocab && out_stride >= vocab), "rows must not overlap");
+  SHARQ_REQUIRE(rules->lengths ? rules->tokens || rules->width == 0 : !rules->tokens, "tokens and lengths go together");
+  SHARQ_REQUIRE(rules->lengths || !(rules->prompt_lengths || rules->repetition || rules->presence || rules->frequency),
+                "prompt_lengths and the penalties need tokens");
+  SHARQ_REQUIRE(!rules->lengths || (rules->width >= 0 && (rows == 1 || rules->tokens_stride >= 0)), "the width of tokens must be >= 0");
+  SHARQ_REQUIRE(rules->biases >= 0 && (rules->bias_offsets || rules->biases == 0) && (rules->biases == 0 || (rules->bias_ids && rules->bias_values)),
+                "biases go with bias_offsets, bias_ids and bias_values");
+  SHARQ_REQUIRE(!rules->mask || rows == 1 || rules->mask_stride >= 0, "the stride of the mask must be >= 0");
+  sharq::LogitRules a = {};
+  a.logits = logits;
+  a.out = out;
+  a.logits_stride = logits_stride;
+  a.out_stride = out_stride;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.tokens = rules->tokens;
+  a.tokens_stride = rules->tokens_stride;
+  a.width = rules->width;
+  a.lengths = rules->lengths;
+  a.prompt_lengths = rules->prompt_lengths;
+  a.repetition = rules->repetition;
+  a.presence = rules->presence;
+  a.frequency = rules->frequency;
+  a.bias_offsets = rules->bias_offsets;
+  a.bias_ids = rules->bias_ids;
+  a.bias_values = rules->bias_values;
+  a.biases = rules->biases;
+  a.mask = rules->mask;
+  a.mask_stride = rules->mask_stride;
+  a.error_flag = error_flag;
+  return check_cuda(sharq::run_logit_rules(a, bf16 != 0, rules->wide_tokens != 0, as_stream(stream)), "adjust_logits");
+}
+
 int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, int k, const void *qw, const void *sfw_dense,
                              const float *scale_dev, float scale, const void *bias_bf16, void *y_bf16, int *error_flag, void *stream) {
   SHARQ_REQUIRE(x_bf16 && qw && sfw_dense && y_bf16, "null buffer");

@@ -1,5 +1,6 @@
 // Host launchers of the decode-step kernels: the paged key/value cache (paged_cache.cu), attention of one new token per
-// sequence over it (paged_attention.cu), and products of few rows with a 4-bit weight (weight_only.cu).
+// sequence over it (paged_attention.cu), products of few rows with a 4-bit weight (weight_only.cu), pages and places of a step's tokens
+// (step_plan.cu), and penalties, biases and masks on logits (logit_rules.cu).
 #pragma once
 #include <cuda_runtime.h>
 
@@ -11,6 +12,8 @@ constexpr int kBadCacheIndex = 0x402;  // error code: a position, length, sequen
 
 constexpr int kAttentionTimeout = 0x403;  // error code: a wait for a copy ran out
 constexpr int kWeightOnlyTimeout = 0x404;
+constexpr int kBadStepPlan = 0x405;     // error code: a length, count or number of free pages that the cache cannot have
+constexpr int kBadLogitRules = 0x406;   // error code: a token, length or offset outside its range
 
 // A position of a sequence in the cache; also what the kernels check before every access.
 struct PagedCache {
@@ -40,6 +43,44 @@ cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head
 constexpr int kWeightOnlyMaxRows = 16;
 cudaError_t run_weight_only(const void *x, long long x_row, int m, int n, int k, const void *qw, const void *sf, const float *scale_dev,
                             float scale, const void *bias, void *y, int *error_flag, cudaStream_t stream);
+
+// Pages and places of a step's tokens (step_plan.cu); the fields as sharq_plan_paged_step has them.
+struct StepPlan {
+  int *table;
+  long long table_stride;
+  int sequences, max_pages, page_size;
+  int *lengths;
+  const int *counts;
+  const unsigned char *released;
+  int *stack;
+  int stack_size;
+  int *free_count;
+  int rows;
+  int *offsets, *positions, *row_sequences;
+  int *error_flag;
+};
+cudaError_t run_step_plan(const StepPlan &plan, cudaStream_t stream);
+
+// Penalties, biases and masks on logits (logit_rules.cu); the fields as sharq_logit_rules has them.
+struct LogitRules {
+  const void *logits;
+  void *out;
+  long long logits_stride, out_stride;
+  int rows, vocab;
+  const void *tokens;
+  long long tokens_stride;
+  int width;
+  const int *lengths, *prompt_lengths;
+  const float *repetition, *presence, *frequency;
+  const int *bias_offsets, *bias_ids;
+  const float *bias_values;
+  int biases;
+  const unsigned *mask;
+  long long mask_stride;
+  int *error_flag;
+  int slice;  // tokens of a CTA, the launcher's choice
+};
+cudaError_t run_logit_rules(const LogitRules &rules, bool bf16, bool wide_ids, cudaStream_t stream);
 
 // Leave for `bytes` of shared memory, asked for once per kernel and device (ready: a static array per kernel).
 template <typename Kernel>

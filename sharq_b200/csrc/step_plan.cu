@@ -1,0 +1,202 @@
+// Pages and places of a step's tokens from the sequences' lengths, in one launch.  16 sequences of one token: 9 us; 1000 sequences, 60 prompts: 19 us.
+//
+//   need_i = ceil((length_i + count_i) / P) - ceil(length_i / P),   row r belongs to the i with offsets_i <= r < offsets_i + count_i
+//
+// The pages that sequence i takes from the stack of free ones, and its rows, lie at prefix sums of need and count over the sequences ahead of it.
+// There is next to nothing to read or write: what counts is the chain of dependent steps.  So one cluster does it all, and every CTA of it scans all
+// sequences for itself (a thread each, a block's worth at a time) instead of waiting for another's sums; pages and rows are dealt out over the cluster, and found
+// by a binary search in the block's sums in shared memory.  Within the cluster, barriers separate what is read from what is overwritten: pages that
+// ended sequences give back are on the stack before any is taken, and lengths change when everyone has read them.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "decode_ops.cuh"
+#include "sm100_ptx.cuh"
+
+namespace sharq {
+
+namespace {
+
+constexpr int kPlanThreadsMost = 1024;
+constexpr int kPlanCluster = 8;
+
+struct Sums {
+  long long a, b;
+};
+
+// Inclusive sums over the block's threads; total: of all of them.  scratch: one per warp.
+__device__ __forceinline__ Sums block_scan(Sums x, Sums *scratch, Sums *total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long a = __shfl_up_sync(0xffffffffu, x.a, off), b = __shfl_up_sync(0xffffffffu, x.b, off);
+    if (lane >= off) x.a += a, x.b += b;
+  }
+  __syncthreads();  // scratch may still be read from the scan before
+  if (lane == 31) scratch[warp] = x;
+  __syncthreads();
+  // every warp sums the warps ahead of it by itself
+  Sums of = lane < warps ? scratch[lane] : Sums{0, 0};
+  Sums ahead = lane < warp ? of : Sums{0, 0};
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    of.a += __shfl_xor_sync(0xffffffffu, of.a, off);
+    of.b += __shfl_xor_sync(0xffffffffu, of.b, off);
+    ahead.a += __shfl_xor_sync(0xffffffffu, ahead.a, off);
+    ahead.b += __shfl_xor_sync(0xffffffffu, ahead.b, off);
+  }
+  *total = of;
+  return {x.a + ahead.a, x.b + ahead.b};
+}
+
+// the first of `n` ascending sums that is more than x, which the last one is
+__device__ __forceinline__ int first_above(const long long *sums, int n, long long x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (sums[mid] > x)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreadsMost) step_plan_kernel(const __grid_constant__ StepPlan p) {
+  __shared__ Sums scratch[32];
+  __shared__ long long need_ends[kPlanThreadsMost], row_ends[kPlanThreadsMost];
+  __shared__ int held_of[kPlanThreadsMost], given_of[kPlanThreadsMost];  // given_of: length ahead of the new tokens, -1: nothing is given
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const int rank = blockIdx.x, at0 = rank * threads + tid, step = gridDim.x * threads;
+  const long long capacity = (long long)p.max_pages * p.page_size;
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const int free_given = *p.free_count;
+  bool bad = free_given < 0 || free_given > p.stack_size;
+  const bool no_stack = bad;
+  long long free_now = no_stack ? 0 : free_given;
+
+  if (p.released != nullptr) {  // ended sequences put their pages back, the last page first
+    long long before = 0;
+    for (int i0 = 0; i0 < p.sequences; i0 += threads) {
+      const int i = i0 + tid;
+      long long back = 0;
+      if (i < p.sequences && p.released[i] != 0) {
+        const int length = p.lengths[i];
+        if (length < 0 || length > capacity)
+          bad = true;
+        else
+          back = ((long long)length + p.page_size - 1) / p.page_size;
+      }
+      Sums total;
+      const Sums ends = block_scan({back, 0}, scratch, &total);
+      need_ends[tid] = ends.a;
+      held_of[tid] = (int)back;
+      __syncthreads();
+      for (long long q = at0; q < total.a; q += step) {
+        const int s = first_above(need_ends, threads, q);
+        const long long page = q - (need_ends[s] - held_of[s]), to = free_now + before + need_ends[s] - 1 - page;
+        if (!no_stack && to < p.stack_size)
+          p.stack[to] = p.table[(long long)(i0 + s) * p.table_stride + page];
+        else
+          bad = true;
+      }
+      before += total.a;
+      __syncthreads();  // the sums have been read
+    }
+    free_now = no_stack ? 0 : min(free_now + before, (long long)p.stack_size);
+    __syncwarp();
+    ptx::cluster_sync();
+  }
+
+  long long need_before = 0, rows_before = 0, taken = 0;
+  for (int i0 = 0; i0 < p.sequences; i0 += threads) {
+    const int i = i0 + tid;
+    int length = 0, count = 0, held = 0;
+    long long need = 0;
+    bool fits = false, keeps = true;  // keeps: its length stays as it is
+    if (i < p.sequences) {
+      length = p.lengths[i];
+      count = p.counts[i];
+      if (p.released != nullptr && p.released[i] != 0) length = 0, keeps = false;
+      fits = length >= 0 && count >= 0 && (long long)length + count <= capacity;
+      if (!fits) bad = true;
+      count = max(count, 0);
+      if (fits) {
+        held = (int)(((long long)length + p.page_size - 1) / p.page_size);
+        need = ((long long)length + count + p.page_size - 1) / p.page_size - held;
+      }
+    }
+    Sums total;
+    Sums ends = block_scan({need, count}, scratch, &total);
+    const long long row_end = rows_before + ends.b;
+    const bool given = fits && !no_stack && (need == 0 || need_before + ends.a <= free_now) && row_end <= p.rows;
+    if (fits && row_end > p.rows) bad = true;
+    need_ends[tid] = ends.a;
+    row_ends[tid] = ends.b;
+    held_of[tid] = held;
+    given_of[tid] = given ? length : -1;
+    // every CTA has read these sequences' lengths, and the number of free pages
+    __syncthreads();
+    ptx::cluster_sync();
+    if (rank == 0 && i < p.sequences) {
+      p.offsets[i + 1] = (int)min(row_end, (long long)p.rows);
+      if (given)
+        p.lengths[i] = length + count;
+      else if (!keeps)
+        p.lengths[i] = 0;
+    }
+    for (long long q = at0; q < total.a; q += step) {
+      const int s = first_above(need_ends, threads, q);
+      if (given_of[s] < 0) continue;
+      const long long start = s > 0 ? need_ends[s - 1] : 0;
+      p.table[(long long)(i0 + s) * p.table_stride + held_of[s] + (q - start)] = p.stack[free_now - 1 - need_before - q];
+    }
+    const long long rows_here = min(total.b, p.rows - min(rows_before, (long long)p.rows));
+    for (long long q = at0; q < rows_here; q += step) {
+      const int s = first_above(row_ends, threads, q);
+      const long long start = s > 0 ? row_ends[s - 1] : 0;
+      p.positions[rows_before + q] = given_of[s] < 0 ? -1 : given_of[s] + (int)(q - start);
+      p.row_sequences[rows_before + q] = i0 + s;
+    }
+    // what was given: the pages of all that fit, which are those of the sequences at the front
+    Sums given_total;
+    block_scan({given ? need : 0, 0}, scratch, &given_total);
+    taken += given_total.a;
+    need_before += total.a;
+    rows_before += total.b;
+  }
+  for (long long r = min(rows_before, (long long)p.rows) + at0; r < p.rows; r += step) {
+    p.positions[r] = -1;
+    p.row_sequences[r] = 0;
+  }
+  if (rank == 0 && tid == 0) {
+    p.offsets[0] = 0;
+    if (!no_stack) *p.free_count = (int)(free_now - taken);
+  }
+  if (bad && p.error_flag != nullptr) atomicCAS(p.error_flag, 0, kBadStepPlan);
+}
+
+}  // namespace
+
+cudaError_t run_step_plan(const StepPlan &p, cudaStream_t stream) {
+  // a thread per sequence as far as a block goes; a cluster where there is more to write than its first CTA does in a few turns
+  const int threads = p.sequences <= 128 ? 128 : p.sequences <= 256 ? 256 : 1024;
+  const bool wide = (long long)p.rows + p.sequences > 4 * threads;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kPlanCluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(wide ? kPlanCluster : 1);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = wide ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, step_plan_kernel, p);
+}
+
+}  // namespace sharq

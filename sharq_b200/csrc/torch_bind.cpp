@@ -17,6 +17,7 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/sharq_b200.h"
@@ -548,6 +549,114 @@ Tensor weight_only_linear(const Tensor &x, const Tensor &qw, const Tensor &sf, c
   return y;
 }
 
+// -> offsets [sequences + 1], positions [rows], sequences [rows], views of one allocation
+std::vector<Tensor> plan_paged_step(const Tensor &table, const Tensor &lengths, const Tensor &counts, const Tensor &free_pages,
+                                    const Tensor &free_count, int64_t page_size, int64_t rows, const std::optional<Tensor> &released,
+                                    const Tensor &flag) {
+  need(table.is_cuda() && table.scalar_type() == at::kInt && table.dim() == 2 && table.numel() > 0 && (table.size(1) <= 1 || table.stride(1) == 1),
+       "page_table must be a CUDA int32 matrix [sequences, pages] with unit column stride");
+  const at::Device dev = table.device();
+  const int64_t n = table.size(0);
+  need(n < INT32_MAX && table.size(1) <= INT32_MAX, "page_table is too large");
+  need(n == 1 || table.stride(0) >= table.size(1), "rows of page_table must not overlap");
+  check_indices(lengths, n, dev, "lengths");
+  check_indices(counts, n, dev, "counts");
+  need(free_pages.dim() == 1 && free_pages.size(0) <= INT32_MAX, "free_pages must be a contiguous CUDA int32 vector on the device of the input");
+  check_indices(free_pages, free_pages.size(0), dev, "free_pages");
+  check_indices(free_count, 1, dev, "free_count");
+  need(page_size > 0 && page_size <= INT32_MAX, "page_size must be positive");
+  need(rows >= 0 && rows <= INT32_MAX, "rows must be in [0, 2^31)");
+  if (released)
+    need((is_plain(*released, at::kBool) || is_plain(*released, at::kByte)) && released->device() == dev && released->dim() == 1 && released->size(0) == n,
+         "released must be a contiguous CUDA bool vector with one entry per sequence");
+  c10::cuda::OptionalCUDAGuard guard(dev);
+  Tensor out = empty_like_on(table, {n + 1 + 2 * rows}, at::kInt);
+  int *at = static_cast<int *>(ptr(out));
+  check(sharq_plan_paged_step(static_cast<int *>(ptr(table)), n > 1 ? table.stride(0) : table.size(1), (int)n, (int)table.size(1), (int)page_size,
+                              static_cast<int *>(ptr(lengths)), static_cast<const int *>(ptr(counts)),
+                              released ? static_cast<const unsigned char *>(ptr(*released)) : nullptr, static_cast<int *>(ptr(free_pages)),
+                              (int)free_pages.size(0), static_cast<int *>(ptr(free_count)), (int)rows, at, at + n + 1, at + n + 1 + rows,
+                              flag_of(flag), stream_of(table)));
+  return {out.narrow(0, 0, n + 1), out.narrow(0, n + 1, rows), out.narrow(0, n + 1 + rows, rows)};
+}
+
+using OptionalTensor = std::optional<Tensor>;
+
+Tensor adjust_logits(const Tensor &logits, const OptionalTensor &tokens, const OptionalTensor &lengths, const OptionalTensor &prompt_lengths,
+                     const OptionalTensor &repetition, const OptionalTensor &presence, const OptionalTensor &frequency,
+                     const std::optional<std::vector<Tensor>> &bias, const OptionalTensor &mask, const OptionalTensor &out, const Tensor &flag) {
+  need(logits.is_cuda() && (logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16) && logits.dim() == 2 &&
+           (logits.size(1) <= 1 || logits.stride(1) == 1),
+       "logits must be a CUDA float32 or bfloat16 matrix [rows, vocab] with unit column stride");
+  const at::Device dev = logits.device();
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  need(vocab > 0 && vocab <= 0x7ff00000 && rows <= 65535, "logits must have at most 65535 rows of 1 to 2^31 - 2^20 tokens");
+  need(rows <= 1 || logits.stride(0) >= vocab, "rows of logits must not overlap");
+  sharq_logit_rules r = {};
+  need(tokens.has_value() == lengths.has_value(), "tokens and lengths go together");
+  if (tokens) {
+    need(tokens->is_cuda() && tokens->device() == dev && (tokens->scalar_type() == at::kInt || tokens->scalar_type() == at::kLong) &&
+             tokens->dim() == 2 && tokens->size(0) == rows && tokens->size(1) <= INT32_MAX && (tokens->size(1) <= 1 || tokens->stride(1) == 1),
+         "tokens must be a CUDA int32 or int64 matrix with a row per row of logits and unit column stride, on their device");
+    check_indices(*lengths, rows, dev, "lengths");
+    r.tokens = ptr(*tokens);
+    r.tokens_stride = rows > 1 ? tokens->stride(0) : 0;
+    r.width = (int)tokens->size(1);
+    r.wide_tokens = tokens->scalar_type() == at::kLong;
+    r.lengths = static_cast<const int *>(ptr(*lengths));
+  }
+  if (prompt_lengths) {
+    check_indices(*prompt_lengths, rows, dev, "prompt_lengths");
+    r.prompt_lengths = static_cast<const int *>(ptr(*prompt_lengths));
+  }
+  const std::pair<const OptionalTensor *, const float **> penalties[3] = {{&repetition, &r.repetition}, {&presence, &r.presence}, {&frequency, &r.frequency}};
+  for (const auto &p : penalties)
+    if (p.first->has_value()) {
+      const Tensor &t = **p.first;
+      need(is_plain(t, at::kFloat) && t.device() == dev && t.dim() == 1 && t.size(0) == rows,
+           "repetition, presence and frequency must be contiguous CUDA float32 vectors with one entry per row of logits");
+      *p.second = static_cast<const float *>(ptr(t));
+    }
+  need(tokens || !(prompt_lengths || repetition || presence || frequency), "prompt_lengths and the penalties need tokens");
+  if (bias) {
+    need(bias->size() == 3, "bias must be (offsets, ids, values)");
+    const Tensor &ids = (*bias)[1], &values = (*bias)[2];
+    check_indices((*bias)[0], rows + 1, dev, "offsets of the biases");
+    need(ids.dim() == 1 && ids.size(0) <= INT32_MAX, "ids of the biases must be a vector");
+    check_indices(ids, ids.size(0), dev, "ids of the biases");
+    need(is_plain(values, at::kFloat) && values.device() == dev && values.sizes() == ids.sizes(),
+         "values of the biases must be a contiguous CUDA float32 vector with one entry per id");
+    r.bias_offsets = static_cast<const int *>(ptr((*bias)[0]));
+    r.bias_ids = static_cast<const int *>(ptr(ids));
+    r.bias_values = static_cast<const float *>(ptr(values));
+    r.biases = (int)ids.size(0);
+  }
+  if (mask) {
+    need(mask->is_cuda() && mask->device() == dev && mask->scalar_type() == at::kInt && mask->dim() == 2 && mask->size(0) == rows &&
+             mask->size(1) == (vocab + 31) / 32 && (mask->size(1) <= 1 || mask->stride(1) == 1),
+         "mask must be a CUDA int32 matrix [rows, ceil(vocab / 32)] with unit column stride, on the device of logits");
+    r.mask = static_cast<const unsigned *>(ptr(*mask));
+    r.mask_stride = rows > 1 ? mask->stride(0) : 0;
+  }
+  if (out)
+    need(out->is_cuda() && out->device() == dev && out->scalar_type() == logits.scalar_type() && out->sizes() == logits.sizes() &&
+             (vocab <= 1 || out->stride(1) == 1) && (rows <= 1 || out->stride(0) >= vocab),
+         "out must be a CUDA matrix like logits");
+  if (out && ptr(*out) != ptr(logits)) {
+    const char *a = static_cast<const char *>(ptr(logits)), *b = static_cast<const char *>(ptr(*out));
+    const int64_t size = logits.element_size(), last = rows > 0 ? rows - 1 : 0;
+    need(a + (last * logits.stride(0) + vocab) * size <= b || b + (last * out->stride(0) + vocab) * size <= a, "out must be logits or not overlap them");
+  } else if (out) {
+    need(rows <= 1 || out->stride(0) == logits.stride(0), "out must be logits or not overlap them");
+  }
+  c10::cuda::OptionalCUDAGuard guard(dev);
+  Tensor o = out ? *out : empty_like_on(logits, {rows, vocab}, logits.scalar_type());
+  if (rows == 0) return o;
+  check(sharq_adjust_logits(ptr(logits), rows > 1 ? logits.stride(0) : vocab, ptr(o), rows > 1 ? o.stride(0) : vocab, (int)rows, (int)vocab,
+                            logits.scalar_type() == at::kBFloat16, &r, flag_of(flag), stream_of(logits)));
+  return o;
+}
+
 // The GIL is released while a call allocates and launches (a launch waits when the queue of the GPU is full).
 template <typename... Args>
 auto as_tuple(std::vector<Tensor> (*fn)(Args...)) {
@@ -583,6 +692,8 @@ PYBIND11_MODULE(sharq_native, m) {
   m.def("rope_append_paged", as_tuple(&rope_append_paged));
   m.def("paged_attention", &paged_attention, nogil());
   m.def("weight_only_linear", &weight_only_linear, nogil());
+  m.def("plan_paged_step", as_tuple(&plan_paged_step));
+  m.def("adjust_logits", &adjust_logits, nogil());
   m.def("rope_inplace", &rope_inplace, nogil());
   m.def("linear_gemm", &linear_gemm, nogil());
   m.def("linear_forward", &linear_forward, nogil());

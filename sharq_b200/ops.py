@@ -33,6 +33,7 @@ _PREPARE_TIMEOUTS_SEEN = 0
 _BAD_EXPERT = 0x401  # kPlanBadExpert of csrc/decoder_ops.cu
 _BAD_CACHE_INDEX = 0x402  # kBadCacheIndex of csrc/decode_ops.cuh
 _ATTENTION_TIMEOUT, _WEIGHT_ONLY_TIMEOUT = 0x403, 0x404  # kAttentionTimeout, kWeightOnlyTimeout of csrc/decode_ops.cuh
+_BAD_STEP_PLAN, _BAD_LOGIT_RULES = 0x405, 0x406  # kBadStepPlan, kBadLogitRules of csrc/decode_ops.cuh
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -81,6 +82,11 @@ def check_device_errors(device=None) -> None:
             if code == _BAD_CACHE_INDEX:
                 raise RuntimeError("sharq_b200 paged cache: a position, length, sequence or page was outside the cache or its tables "
                                    f"on cuda:{idx}")
+            if code == _BAD_STEP_PLAN:
+                raise RuntimeError("sharq_b200 plan_paged_step: a length, count or number of free pages was one that the cache cannot have "
+                                   f"on cuda:{idx}")
+            if code == _BAD_LOGIT_RULES:
+                raise RuntimeError(f"sharq_b200 adjust_logits: a token, length or offset was outside its range on cuda:{idx}")
             if code in (_ATTENTION_TIMEOUT, _WEIGHT_ONLY_TIMEOUT):
                 name = "paged_attention" if code == _ATTENTION_TIMEOUT else "weight_only_linear"
                 raise RuntimeError(f"sharq_b200 {name}: a wait for a copy ran out on cuda:{idx}; outputs are undefined")
@@ -230,6 +236,34 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     outside the cache makes that sequence's rows NaN and is reported by check_device_errors.  A sequence may stand in several
     rows with lengths of their own (drafted tokens).  The same bits from call to call."""
     return _lib.native().paged_attention(q, k_cache, v_cache, page_table, lengths, scale, k_scale, v_scale, out, _error_flag(q.device))
+
+
+def plan_paged_step(page_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                    page_size: int, rows: int, released: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Pages and places of a step's tokens, handed out on the device in one launch: sequence i, which holds lengths[i] tokens in the pages of its row
+    of page_table [sequences, pages], gets counts[i] more -> (offsets [sequences + 1], positions [rows], sequences [rows]), the places that
+    rope_append_paged takes, sequence after sequence.  All int32.  page_table, lengths, free_pages (a stack, of which the first
+    free_count[0] are free) and free_count [1] change in place.  Sequences with released (bool) give their pages back first and are empty.  Where the
+    pages do not suffice for a sequence and those ahead of it, it gets nothing: its length stays and its rows have position -1, as rows behind the
+    last have.  A length, count, sum of counts above `rows` or free_count that cannot be is reported by check_device_errors, and its sequences get nothing."""
+    return _lib.native().plan_paged_step(page_table, lengths, counts, free_pages, free_count, page_size, rows, released,
+                                         _error_flag(page_table.device))
+
+
+def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                  prompt_lengths: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
+                  presence: Optional[torch.Tensor] = None, frequency: Optional[torch.Tensor] = None,
+                  bias: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None, mask: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Penalties for repeated tokens, biases and a mask on logits [rows, vocab] (float32 or bfloat16) -> a new tensor, or out, which may be
+    logits.  tokens [rows, width] (int32 or int64; negative: padding) is every row's history, of which the first lengths[r] (int32) count and the first
+    prompt_lengths[r] of those are the prompt.  A logit x becomes, with float32 [rows] penalties, each optional:
+    x / repetition where it is positive, else x * repetition, for tokens of the history; less frequency * n + presence for a token that
+    follows the prompt n times; plus its biases, (offsets int32 [rows + 1], ids int32, values float32): entries offsets[r] to offsets[r + 1] belong
+    to row r, the same token's add up; and -inf where bit token % 32 of mask[r, token // 32] (int32) is not set.  float64 arithmetic, one rounding; other logits
+    stay as they are.  Lengths, offsets and tokens out of range are passed over and reported by check_device_errors."""
+    return _lib.native().adjust_logits(logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, None if bias is None else list(bias),
+                                       mask, out, _error_flag(logits.device))
 
 
 def scatter_add_scaled_(out: torch.Tensor, y: torch.Tensor, rows: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
