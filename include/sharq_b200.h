@@ -425,6 +425,21 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
 int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, int k, const void *qw, const void *sfw_dense,
                              const float *scale_dev, float scale, const void *bias_bf16, void *y_bf16, int *error_flag, void *stream);
 
+/* Attention of ragged prompts, causal, with a sliding window and first keys that stay visible.  q [rows, heads, head_dim], k and v
+ * [k_rows, kv_heads, head_dim], bf16, with *_row / *_head elements between rows / heads (positive multiples of 8), out bf16 [rows, heads, head_dim].
+ * Sequence s has the queries offsets[s] .. offsets[s + 1] and the keys k_offsets[s] .. k_offsets[s + 1] (NULL: the queries' rows), whose last ones belong to
+ * its queries: the i-th of n queries has position p = keys - n + i, and sees the key at position j where
+ *   j <= p and (p - j < window or j < sinks)          (window 0: every j <= p)
+ * out = sum_j softmax_j(scale * q . k[j]) v[j] over those; a query that sees none gives zeros.  Query head h reads key/value head
+ * h / (heads / kv_heads).  With fill != 0 rows of out ahead of the first sequence and behind the last become zeros, else they stay as they are.
+ * Sums and softmax statistics are float; probabilities enter the product with the values as bf16.  Offsets (int32, on the device) that go back or leave
+ * [0, rows] make their sequence empty, those of keys make its rows NaN, and store 0x407 in *error_flag (may be NULL; 0x408: a wait ran out, results
+ * are undefined).  head_dim 64 or 128, heads a multiple of kv_heads, rows and k_rows at most 2^30; no workspace. */
+int sharq_prompt_attention(const void *q_bf16, int64_t q_row, int64_t q_head, const void *k_bf16, int64_t k_row, int64_t k_head,
+                           const void *v_bf16, int64_t v_row, int64_t v_head, int rows, int k_rows, int heads, int kv_heads, int head_dim,
+                           const int *offsets, const int *k_offsets, int sequences, int window, int sinks, float scale, void *out_bf16,
+                           int fill, int *error_flag, void *stream);
+
 /* Pages and places of a step's tokens, from lengths on the device.  Sequence i holds lengths[i] tokens in the first
  * ceil(lengths[i] / page_size) pages of its row of page_table [sequences, max_pages] (page_table_stride entries between rows); the free pages are
  * free_pages[0 .. free_count[0]), a stack of room for free_pages_size.  In this order:

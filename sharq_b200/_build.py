@@ -24,6 +24,7 @@ BIND_SOURCE = CSRC / "torch_bind.cpp"
 HEADER = PKG.parent / "include" / "sharq_b200.h"
 SOURCES = ["prepare.cu", "prepare_static.cu", "sp_transition.cu", "quant.cu", "gemm.cu", "allreduce.cu", "decoder_ops.cu",
            "paged_cache.cu", "paged_attention.cu", "weight_only.cu", "step_plan.cu", "logit_rules.cu",
+           "prompt_attention.cu",
            "c_api.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

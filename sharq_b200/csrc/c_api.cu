@@ -823,6 +823,48 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
                     "paged_attention");
 }
 
+int sharq_prompt_attention(const void *q_bf16, int64_t q_row, int64_t q_head, const void *k_bf16, int64_t k_row, int64_t k_head,
+                           const void *v_bf16, int64_t v_row, int64_t v_head, int rows, int k_rows, int heads, int kv_heads, int head_dim,
+                           const int *offsets, const int *k_offsets, int sequences, int window, int sinks, float scale, void *out_bf16,
+                           int fill, int *error_flag, void *stream) {
+  SHARQ_REQUIRE(q_bf16 && k_bf16 && v_bf16 && offsets && out_bf16, "null buffer");
+  SHARQ_REQUIRE(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128, got %d", head_dim);
+  SHARQ_REQUIRE(rows >= 1 && rows <= 1 << 30 && k_rows >= 1 && k_rows <= 1 << 30, "rows and k_rows must be in [1, 2^30]");
+  SHARQ_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads <= 65536, "heads must be a positive multiple of kv_heads, at most 65536");
+  SHARQ_REQUIRE(sequences > 0 && sequences <= 1 << 28, "sequences must be in [1, 2^28]");
+  SHARQ_REQUIRE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
+  SHARQ_REQUIRE(k_offsets || k_rows == rows, "without k_offsets there is a key for every query");
+  const int64_t strides[6] = {q_row, q_head, k_row, k_head, v_row, v_head};
+  for (const int64_t s : strides)
+    SHARQ_REQUIRE(s > 0 && s % 8 == 0 && s < (int64_t)1 << 38, "the strides of q, k and v must be positive multiples of 8");
+  SHARQ_REQUIRE(aligned16(q_bf16) && aligned16(k_bf16) && aligned16(v_bf16) && aligned16(out_bf16), "buffers must be 16-byte aligned");
+  sharq::PromptAttention p = {};
+  p.q = q_bf16;
+  p.k = k_bf16;
+  p.v = v_bf16;
+  p.q_row = q_row;
+  p.q_head = q_head;
+  p.k_row = k_row;
+  p.k_head = k_head;
+  p.v_row = v_row;
+  p.v_head = v_head;
+  p.rows = rows;
+  p.k_rows = k_rows;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.head_dim = head_dim;
+  p.offsets = offsets;
+  p.k_offsets = k_offsets;
+  p.seqs = sequences;
+  p.window = window == 0 || window > 1 << 30 ? 1 << 30 : window;
+  p.sinks = window == 0 ? 0 : sinks;
+  p.scale = scale;
+  p.out = out_bf16;
+  p.fill = fill != 0;
+  p.error_flag = error_flag;
+  return check_cuda(sharq::run_prompt_attention(p, as_stream(stream)), "prompt_attention");
+}
+
 int sharq_plan_paged_step(int *page_table, int64_t page_table_stride, int sequences, int max_pages, int page_size, int *lengths,
                           const int *counts, const unsigned char *released, int *free_pages, int free_pages_size, int *free_count,
                           int rows, int *offsets, int *positions, int *row_sequences, int *error_flag, void *stream) {

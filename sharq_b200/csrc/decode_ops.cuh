@@ -1,6 +1,6 @@
 // Host launchers of the decode-step kernels: the paged key/value cache (paged_cache.cu), attention of one new token per
 // sequence over it (paged_attention.cu), products of few rows with a 4-bit weight (weight_only.cu), pages and places of a step's tokens
-// (step_plan.cu), and penalties, biases and masks on logits (logit_rules.cu).
+// (step_plan.cu), penalties, biases and masks on logits (logit_rules.cu), and attention of ragged prompts (prompt_attention.cu).
 #pragma once
 #include <cuda_runtime.h>
 
@@ -14,6 +14,8 @@ constexpr int kAttentionTimeout = 0x403;  // error code: a wait for a copy ran o
 constexpr int kWeightOnlyTimeout = 0x404;
 constexpr int kBadStepPlan = 0x405;     // error code: a length, count or number of free pages that the cache cannot have
 constexpr int kBadLogitRules = 0x406;   // error code: a token, length or offset outside its range
+constexpr int kBadOffsets = 0x407;      // error code: offsets of prompts that go back, or beyond the rows
+constexpr int kPromptTimeout = 0x408;   // error code: a wait inside the attention of prompts ran out
 
 // A position of a sequence in the cache; also what the kernels check before every access.
 struct PagedCache {
@@ -81,6 +83,20 @@ struct LogitRules {
   int slice;  // tokens of a CTA, the launcher's choice
 };
 cudaError_t run_logit_rules(const LogitRules &rules, bool bf16, bool wide_ids, cudaStream_t stream);
+
+// Attention of ragged prompts (prompt_attention.cu); the fields as sharq_prompt_attention has them, strides in elements.
+struct PromptAttention {
+  const void *q, *k, *v;
+  long long q_row, q_head, k_row, k_head, v_row, v_head;
+  int rows, k_rows, heads, kv_heads, head_dim;
+  const int *offsets, *k_offsets;
+  int seqs, window, sinks;
+  float scale;
+  void *out;
+  bool fill;
+  int *error_flag;
+};
+cudaError_t run_prompt_attention(const PromptAttention &p, cudaStream_t stream);
 
 // Leave for `bytes` of shared memory, asked for once per kernel and device (ready: a static array per kernel).
 template <typename Kernel>

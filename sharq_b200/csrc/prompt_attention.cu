@@ -1,0 +1,779 @@
+// Attention of ragged prompts: causal, with a sliding window and a few first keys that stay visible.  32768 tokens of 32 / 8 heads of
+// 128 under a window of 4096: 2.38 ms, 867 TFLOP/s; 200 tokens: 14.6 us.
+//
+//   out[i, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q[i, h] . k_j - max),   j <= p and (p - j < window or j < sinks),   p the position of query i
+//
+// Two products of 128 x 128 x head_dim per block of queries and tile of keys, on the tensor cores (tcgen05, bf16): S = Q K^T into tensor memory, the
+// exponentials back into it as bf16 in the place of S, O += P V from there.  The exponentials take the
+// special function unit as long as the products take the tensor cores (128 x 128: 1024 cycles of 16, and twice 512).
+//
+// A CTA works on two blocks of 128 query rows, so that one's exponentials run under the other's products, and goes from item to item by itself.  The
+// query heads of a key/value head are rows of the same block, token after token (4 heads: 32 tokens of each): what a narrow window lets a
+// block see is then as few tiles as can be.  The keys that a block may see are one list: the first ones, filled up to a multiple of 8, then those of the window
+// from its first one on, which a tile in the middle joins by copies of 8 keys.
+//
+// Warps 0-3 and 4-7 hold a row per thread: maximum, exponentials and sum need no other thread.  The maximum is raised only where a score exceeds it by
+// more than 2^kLazy, for the raise is a pass over O.  Probabilities carry a factor of 2^-32, so that no sum of finite values overflows, and
+// enter the product as bf16, as in the library attention of prompts without a window: off by 2^-9 each, which leaves a result about as near as its own
+// rounding to bf16.  (As two bf16 numbers, as the decode step has them, the second product would be a third more work for the tensor cores.)
+//
+// A masked key has probability 0, which a value that is not finite (another sequence's, or memory that nothing has written) would turn to NaN.  Two
+// warps look for such values in every tile where something is masked; a tile that has one is multiplied row by row, visible keys only, in plain float.
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include <cstdint>
+
+#include "decode_ops.cuh"
+#include "sm100_ptx.cuh"
+#include "tensor_map.cuh"
+
+namespace sharq {
+
+namespace {
+
+constexpr int kTile = 128;  // keys of a tile, rows of a block
+constexpr int kBlocks = 2;
+constexpr int kSoftmaxWarps = 4 * kBlocks, kLoadWarp = kSoftmaxWarps, kMmaWarp = kLoadWarp + 1, kCheckWarp = kMmaWarp + 1, kCheckWarps = 2;
+constexpr int kThreads = 32 * (kCheckWarp + kCheckWarps);
+constexpr int kItemSlots = 2;
+constexpr int kSoftmaxRegisters = 200, kOtherRegisters = 96;
+static_assert(128 * kBlocks * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreads * 168, "the shares of the registers that the block was launched with");
+constexpr float kLazy = 8.0f, kLift = -32.0f;  // in powers of two
+
+template <int D>
+struct Sizes {
+  static constexpr int kHalves = D / 64;           // rows lie 128 bytes apart: a row of 256 bytes in two halves
+  static constexpr int kHalf = kTile * 128;
+  static constexpr int kBytes = kHalf * kHalves;   // of a tile, or of a block of queries
+  static constexpr int kStages = D == 128 ? 5 : 9;
+  static constexpr int kControl = kBlocks * kBytes + kStages * kBytes;
+  static constexpr int kTotal = kControl + 1024;
+  static constexpr int kOutCol = kBlocks * kTile;  // tensor memory: scores of the blocks, then their outputs
+};
+static_assert(Sizes<128>::kTotal <= 232448 && Sizes<64>::kTotal <= 232448, "shared memory of a CTA");
+
+struct Args {
+  const int *offsets, *k_offsets;
+  __nv_bfloat16 *out;
+  int rows, k_rows, seqs;
+  int heads, kv_heads, group, chunks, chunk_heads, tokens;  // chunk_heads: query heads of a block; tokens: of a block
+  int window, sinks;  // window: 2^30 for none
+  float scale_log2;   // scale * log2(e)
+  bool fill;          // rows of no sequence become zeros
+  int *error_flag;
+};
+
+// What a CTA works on: `count` tokens from row `row0` on, the first at position `first`, of heads kv and chunk.  Their keys are a list of `s_pad` first ones
+// and those from position `base` on, of which there are `total` in all, in `tiles` tiles.
+struct Item {
+  int state;  // 0: no more items, 1: an item, 2: one whose keys are not known (its rows come out as NaN)
+  int row0, count, first, kv, chunk;
+  int k_row0, base, s_pad, total, tiles;
+};
+
+__device__ __forceinline__ void set_keys(Item &it, int keys, int window, int sinks) {
+  const int last = it.first + it.count - 1, end = min(last + 1, keys);  // last < keys
+  if (end <= 0) {
+    it.base = it.s_pad = it.total = it.tiles = 0;
+    return;
+  }
+  const int low = max(0, it.first - window + 1), s = min(sinks, end), pad = (s + 7) & ~7;
+  it.base = low;
+  it.s_pad = 0;
+  if (s > 0) {
+    if (low > pad)
+      it.s_pad = pad;
+    else
+      it.base = 0;
+  }
+  it.total = it.s_pad + end - it.base;
+  it.tiles = (it.total + kTile - 1) / kTile;
+}
+
+// Whether some query of the item does not see some key of the tile.
+__device__ __forceinline__ bool is_masked(const Item &it, int tile, int window, int sinks) {
+  const int v0 = tile * kTile, v1 = v0 + kTile - 1;
+  if (v0 < it.s_pad) return v1 >= sinks;
+  const int k0 = it.base + v0 - it.s_pad, k1 = k0 + kTile - 1, last = it.first + it.count - 1;
+  return k1 > it.first || !(k0 > last - window || k1 < sinks);
+}
+
+// Which keys of the list a query sees: [low, high) and those below `sinks`.
+struct Seen {
+  int low, high, sinks;
+};
+__device__ __forceinline__ Seen seen_by(const Item &it, int position, int window, int sinks) {
+  return {it.s_pad + max(position - window + 1 - it.base, 0), it.s_pad + position + 1 - it.base, max(0, min(sinks, position + 1))};
+}
+__device__ __forceinline__ unsigned bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
+__device__ __forceinline__ unsigned seen_word(const Seen &s, int v0) {  // of the keys v0 .. v0 + 31
+  return (bits_below(s.high - v0) & ~bits_below(s.low - v0)) | bits_below(s.sinks - v0);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {  // 2 units in the last place; 0 below 2^-126
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t *>(&v);
+}
+
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld_x4(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr)
+               : "memory");
+}
+
+// bf16 operands, float sums; A and B in shared memory, both with K contiguous (B: with N contiguous, kind::f16's transposed form), or A in tensor memory
+template <int N, bool kTransposeB>
+__device__ __forceinline__ constexpr uint32_t make_idesc_bf16() {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((kTransposeB ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 128 bytes of a head x ... of a [128 bytes][rows or heads][...] array; see encode()
+__device__ __forceinline__ void copy_4d(uint32_t dst, const CUtensorMap *m, int c1, int c2, int c3, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(m), "r"(ptx::smem_u32(bar)), "r"(0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// O of a thread's row += P V of a tile whose values are not all finite, visible keys only.  s: the row's, from the tile's first key on; first_tile: O holds nothing yet.
+template <int D>
+__device__ __noinline__ void multiply_visible(uint32_t tmem_p, uint32_t tmem_o, uint32_t values, Seen s, bool first_tile) {
+  for (int c = 0; c < D; c += 32) {
+    uint32_t o[32];
+    if (first_tile) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = 0;
+    } else {
+      ptx::tmem_ld_32x32b_x32(tmem_o + c, o);
+      ptx::tmem_ld_wait();
+    }
+    for (int k0 = 0; k0 < kTile; k0 += 8) {
+      uint32_t p[4];
+      tmem_ld_x4(tmem_p + k0 / 2, p);
+      ptx::tmem_ld_wait();
+      const unsigned word = seen_word(s, k0);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float pk = __uint_as_float(k % 2 == 0 ? p[k / 2] << 16 : p[k / 2] & 0xFFFF0000u);
+        const uint32_t row = values + (c / 64) * Sizes<D>::kHalf + (k0 + k) * 128;
+#pragma unroll
+        for (int piece = 0; piece < 4; ++piece) {
+          const float4 v = ptx::ld_shared_f32x4(row + (((c % 64) / 8 + piece) ^ k) * 16);  // swizzled by the row in eight
+          const float w[4] = {v.x, v.y, v.z, v.w};
+          if ((word >> k & 1) != 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t bits = __float_as_uint(w[i]);
+              uint32_t &lo = o[piece * 8 + 2 * i], &hi = o[piece * 8 + 2 * i + 1];
+              lo = __float_as_uint(fmaf(pk, __uint_as_float(bits << 16), __uint_as_float(lo)));
+              hi = __float_as_uint(fmaf(pk, __uint_as_float(bits & 0xFFFF0000u), __uint_as_float(hi)));
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+    tmem_st_x32(tmem_o + c, o);
+    tmem_st_wait();
+  }
+}
+
+
+// Rows of the sequences seq0 + lane, all lanes: empty behind the last one, and where offsets go back, below an earlier one (`reached`: the highest
+// so far), or leave the rows.
+struct Bounds {
+  int row0, row1;
+  bool bad;
+};
+__device__ __forceinline__ Bounds bounds_of(const Args &a, int seq0, int lane, int *reached) {
+  const int seq = seq0 + lane;
+  Bounds b = {0, 0, false};
+  if (seq < a.seqs) b.row0 = a.offsets[seq], b.row1 = a.offsets[seq + 1];
+  int top = seq < a.seqs && b.row0 <= a.rows ? b.row0 : -1;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, top, off);
+    if (lane >= off) top = max(top, up);
+  }
+  top = max(top, *reached);
+  *reached = __shfl_sync(0xffffffffu, top, 31);
+  b.bad = seq < a.seqs && !(b.row0 >= 0 && b.row0 >= top && b.row0 <= b.row1 && b.row1 <= a.rows);
+  if (b.bad) b.row0 = b.row1 = 0;
+  return b;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k8,
+                            const __grid_constant__ CUtensorMap map_v8, const __grid_constant__ Args a) {
+  using S = Sizes<D>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t queries = ptx::smem_u32(smem), ring = queries + kBlocks * S::kBytes;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kControl);
+  uint64_t *kv_full = bars, *kv_empty = kv_full + kStages, *v_ok = kv_empty + kStages, *q_full = v_ok + kStages, *q_empty = q_full + kBlocks;
+  uint64_t *s_full = q_empty + kBlocks, *p_full = s_full + kBlocks, *o_full = p_full + kBlocks, *item_full = o_full + kBlocks;
+  uint64_t *item_empty = item_full + kItemSlots;
+  uint64_t *drained = item_empty + kItemSlots;  // for products on their way when a wait ran out
+  Item *items = reinterpret_cast<Item *>(drained + 1);
+  volatile int *not_finite = reinterpret_cast<volatile int *>(items + kItemSlots);  // [kStages][kCheckWarps]
+  volatile int *abort_flag = not_finite + kStages * kCheckWarps;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(const_cast<int *>(abort_flag) + 1);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      ptx::mbar_init(kv_full + i, 1);
+      ptx::mbar_init(kv_empty + i, 1);
+      ptx::mbar_init(v_ok + i, kCheckWarps);
+    }
+    for (int i = 0; i < kBlocks; ++i) {
+      ptx::mbar_init(q_full + i, 1);
+      ptx::mbar_init(q_empty + i, 1);
+      ptx::mbar_init(s_full + i, 1);
+      ptx::mbar_init(p_full + i, 4);
+      ptx::mbar_init(o_full + i, 1);
+    }
+    for (int i = 0; i < kItemSlots; ++i) {
+      ptx::mbar_init(item_full + i, 1);
+      ptx::mbar_init(item_empty + i, kSoftmaxWarps + 1 + kCheckWarps);
+    }
+    ptx::mbar_init(drained, 1);
+    ptx::fence_barrier_init();
+    *abort_flag = 0;
+    ptx::tma_prefetch_desc(&map_q);
+    ptx::tma_prefetch_desc(&map_k);
+    ptx::tma_prefetch_desc(&map_v);
+  }
+  if (warp == kMmaWarp) {
+    ptx::tmem_alloc<1>(tmem_slot, 512);
+    ptx::tmem_relinquish<1>();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  ptx::grid_dependency_wait();
+
+  auto give_up = [&]() {
+    *abort_flag = 1;
+    if (a.error_flag != nullptr) atomicExch(a.error_flag, kPromptTimeout);
+  };
+  // the next item's description as the load warp left it; `n`: how many there have been
+  auto next_item = [&](Item &it, int n) {
+    const int slot = n % kItemSlots;
+    if (!ptx::mbar_wait(item_full + slot, (n / kItemSlots) & 1, abort_flag)) {
+      give_up();
+      return false;
+    }
+    it = items[slot];
+    return it.state != 0;
+  };
+  auto next_item_of_warp = [&](Item &it, int n) {  // all lanes, which have the same answer
+    const bool got = next_item(it, n);
+    __syncwarp();
+    if (!__all_sync(0xffffffffu, got)) return false;
+    if (lane == 0) ptx::mbar_arrive(item_empty + n % kItemSlots);
+    return true;
+  };
+
+  if (warp < kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+    const int block = warp / 4, row = (warp % 4) * 32 + lane;
+    const int token = row / a.chunk_heads, head = row % a.chunk_heads;
+    const uint32_t lanes = tmem + ((uint32_t)(warp % 4) << 21);  // 32 lanes of tensor memory per warp
+    const uint32_t tmem_s = lanes + block * kTile, tmem_o = lanes + S::kOutCol + block * D;
+    const bool negative = a.scale_log2 < 0.0f;
+    const float c = fmaxf(fabsf(a.scale_log2), 1.2e-38f);  // not 0: masked scores are -inf, and stay so
+    if (a.fill) {  // rows of no sequence, a share of them per thread
+      const int begin = min(max(a.offsets[0], 0), a.rows), end = min(max(a.offsets[a.seqs], 0), a.rows);
+      const long long width = (long long)a.heads * D / 8, ahead = begin * width, behind = (long long)max(a.rows - max(end, begin), 0) * width;
+      uint4 *out = reinterpret_cast<uint4 *>(a.out);
+      for (long long i = (long long)blockIdx.x * (32 * kSoftmaxWarps) + threadIdx.x; i < ahead + behind; i += (long long)gridDim.x * (32 * kSoftmaxWarps))
+        out[i < ahead ? i : (long long)a.rows * width - behind + (i - ahead)] = make_uint4(0, 0, 0, 0);
+    }
+    unsigned tiles_done = 0, values_done = 0, items_done = 0;  // for the barriers' parities: of this block, of all, of this block
+    Item it;
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      if (!next_item_of_warp(it, n)) break;
+      const unsigned value0 = values_done;
+      values_done += it.tiles;
+      if (it.count <= block * a.tokens) continue;  // nothing for this block
+      const int t = block * a.tokens + token, position = it.first + min(t, it.count - 1);
+      const Seen seen = seen_by(it, position, a.window, a.sinks);
+      float m = -INFINITY, l = 0.0f;  // maximum in powers of two, sum
+      for (int tile = 0; tile < it.tiles; ++tile) {
+        if (!ptx::mbar_wait(s_full + block, tiles_done++ & 1, abort_flag)) {
+          give_up();
+          ok = false;
+        }
+        __syncwarp();
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(tmem_s + 32 * i, s[i]);
+        ptx::tmem_ld_wait();
+        if (negative) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s[i][j] ^= 0x80000000u;
+        }
+        const bool masked = is_masked(it, tile, a.window, a.sinks);
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const unsigned word = seen_word(seen, tile * kTile + 32 * i);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s[i][j] = (word >> j & 1) != 0 ? s[i][j] : 0xff800000u;
+          }
+        }
+        float top[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          top[i] = __uint_as_float(s[i][0]);
+#pragma unroll
+          for (int j = 1; j < 32; ++j) top[i] = fmaxf(top[i], __uint_as_float(s[i][j]));
+        }
+        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+        const bool raise = high > m + kLazy;
+        if (__any_sync(0xffffffffu, raise)) {
+          const float f = raise ? exp2_approx(m - high) : 1.0f;  // from -inf: 0, and nothing to keep
+          if (raise) m = high;
+          l *= f;
+          if (tile > 0) {
+#pragma unroll 1
+            for (int i = 0; i < D; i += 32) {
+              uint32_t o[32];
+              ptx::tmem_ld_32x32b_x32(tmem_o + i, o);
+              ptx::tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st_x32(tmem_o + i, o);
+            }
+          }
+        }
+        // a row with no finite score so far has maximum -inf: its probabilities are 0, not exp(-inf + inf)
+        const float base = (m == -INFINITY ? 0.0f : m) - kLift;
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t p[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float x = exp2_approx(fmaf(__uint_as_float(s[2 * i + j / 16][j % 16 * 2]), c, -base));
+            const float y = exp2_approx(fmaf(__uint_as_float(s[2 * i + j / 16][j % 16 * 2 + 1]), c, -base));
+            sum[0] += x;
+            sum[1] += y;
+            p[j] = pack_bf16(x, y);
+          }
+          tmem_st_x32(tmem_s + 32 * i, p);
+        }
+        l += sum[0] + sum[1];
+        tmem_st_wait();
+        if (masked) {
+          const unsigned value = value0 + tile;
+          if (!ptx::mbar_wait(v_ok + value % kStages, (value / kStages) & 1, abort_flag)) {
+            give_up();
+            ok = false;
+          }
+          __syncwarp();
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          if ((not_finite[value % kStages * kCheckWarps] | not_finite[value % kStages * kCheckWarps + 1]) != 0)
+            multiply_visible<D>(tmem_s, tmem_o, ring + (2 * value + 1) % kStages * S::kBytes,
+                                Seen{seen.low - tile * kTile, seen.high - tile * kTile, seen.sinks - tile * kTile}, tile == 0);
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(p_full + block);
+      }
+      if (!ok) break;
+      const bool there = token < a.tokens && t < it.count && it.chunk * a.chunk_heads + head < a.group;
+      if (it.tiles > 0) {
+        if (!ptx::mbar_wait(o_full + block, items_done++ & 1, abort_flag)) {
+          give_up();
+          ok = false;
+        }
+        __syncwarp();
+        if (!__all_sync(0xffffffffu, ok)) break;
+        ptx::tc_fence_after();
+      }
+      __nv_bfloat16 *out = a.out + ((long long)(it.row0 + t) * a.heads + it.kv * a.group + it.chunk * a.chunk_heads + head) * D;
+      const float f = 1.0f / l;
+#pragma unroll 1
+      for (int i = 0; i < D; i += 32) {
+        uint32_t o[32];
+        if (it.tiles > 0) {
+          ptx::tmem_ld_32x32b_x32(tmem_o + i, o);
+          ptx::tmem_ld_wait();
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[e] = pack_bf16(__uint_as_float(o[j + 2 * e]) * f, __uint_as_float(o[j + 2 * e + 1]) * f);
+            if (position < 0 || it.tiles == 0) w[e] = 0;
+            if (it.state == 2) w[e] = 0x7fff7fffu;
+          }
+          if (there) *reinterpret_cast<uint4 *>(out + i + j) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        __syncwarp();
+      }
+      ptx::tc_fence_before();
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+    if (warp == kLoadWarp) {
+      // blocks of two times `tokens` tokens, of all sequences
+      const int span = kBlocks * a.tokens;
+      int blocks = 0, reached = 0;
+      bool bad = false;
+      for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+        const Bounds b = bounds_of(a, b0, lane, &reached);
+        bad |= b.bad;
+        blocks += (b.row1 - b.row0 + span - 1) / span;
+      }
+      blocks = __reduce_add_sync(0xffffffffu, blocks);
+      const int columns = a.kv_heads * a.chunks;
+      unsigned copies = 0, loads[kBlocks] = {0, 0};
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        const long long at = (long long)blockIdx.x + (long long)n * gridDim.x;
+        Item it;
+        it.state = at < (long long)blocks * columns ? 1 : 0;
+        if (it.state != 0) {
+          const int block = (int)(at / columns), column = (int)(at - (long long)block * columns);
+          it.kv = column / a.chunks;
+          it.chunk = column - it.kv * a.chunks;
+          int before = 0;
+          reached = 0;
+          for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+            const Bounds b = bounds_of(a, b0, lane, &reached);
+            int ends = (b.row1 - b.row0 + span - 1) / span;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+              const int up = __shfl_up_sync(0xffffffffu, ends, off);
+              if (lane >= off) ends += up;
+            }
+            const unsigned over = __ballot_sync(0xffffffffu, before + ends > block);
+            if (over != 0) {
+              const int in = __ffs(over) - 1, seq = b0 + in;
+              const int from = __shfl_sync(0xffffffffu, b.row0, in), to = __shfl_sync(0xffffffffu, b.row1, in);
+              const int index = before + __shfl_sync(0xffffffffu, ends, in) - 1 - block;  // the last block first: it sees most
+              it.row0 = from + index * span;
+              it.count = min(span, to - it.row0);
+              int k0 = from, k1 = to;
+              if (a.k_offsets != nullptr) {
+                k0 = a.k_offsets[seq];
+                k1 = a.k_offsets[seq + 1];
+              }
+              const bool known = k0 >= 0 && k0 <= k1 && k1 <= a.k_rows;
+              it.k_row0 = k0;
+              it.first = (k1 - k0) - (to - from) + index * span;
+              set_keys(it, k1 - k0, a.window, a.sinks);
+              if (!known) {
+                bad = true;
+                it.state = 2;
+                it.tiles = 0;
+              }
+              break;
+            }
+            before += __shfl_sync(0xffffffffu, ends, 31);
+          }
+        }
+        const int slot = n % kItemSlots;
+        if (lane == 0) {
+          if (ptx::mbar_wait(item_empty + slot, ((n / kItemSlots) & 1) ^ 1, abort_flag)) {
+            items[slot] = it;
+            ptx::mbar_arrive(item_full + slot);
+          } else {
+            give_up();
+            ok = false;
+          }
+          if (ok && it.state != 0 && it.tiles > 0) {
+            auto fill = [&](int tile, bool of_keys) {
+              const int stage = copies % kStages;
+              if (!ptx::mbar_wait(kv_empty + stage, ((copies / kStages) & 1) ^ 1, abort_flag)) {
+                give_up();
+                ok = false;
+                return;
+              }
+              const uint32_t to = ring + stage * S::kBytes;
+              const int v0 = tile * kTile;
+              ptx::mbar_arrive_expect_tx(kv_full + stage, S::kBytes);
+              if (v0 + kTile <= it.s_pad || v0 >= it.s_pad) {
+                const int key = v0 < it.s_pad ? v0 : it.base + v0 - it.s_pad;
+                copy_4d(to, of_keys ? &map_k : &map_v, it.k_row0 + key, 0, it.kv, kv_full + stage);
+              } else {  // the first keys end in this tile
+                for (int i = 0; i < kTile; i += 8) {
+                  const int key = v0 + i < it.s_pad ? v0 + i : it.base + v0 + i - it.s_pad;
+                  for (int half = 0; half < S::kHalves; ++half)
+                    copy_4d(to + half * S::kHalf + i * 128, of_keys ? &map_k8 : &map_v8, it.k_row0 + key, half, it.kv, kv_full + stage);
+                }
+              }
+              ++copies;
+            };
+            for (int b = 0; b < kBlocks && ok; ++b) {
+              if (it.count <= b * a.tokens) continue;
+              if (!ptx::mbar_wait(q_empty + b, (loads[b] & 1) ^ 1, abort_flag)) {
+                give_up();
+                ok = false;
+                break;
+              }
+              ++loads[b];
+              ptx::mbar_arrive_expect_tx(q_full + b, a.tokens * a.chunk_heads * D * 2);
+              for (int half = 0; half < S::kHalves; ++half)
+                copy_4d(queries + b * S::kBytes + half * S::kHalf, &map_q, it.kv * a.group + it.chunk * a.chunk_heads, it.row0 + b * a.tokens, half,
+                        q_full + b);
+              if (b == 0) fill(0, true);
+            }
+            for (int tile = 0; tile < it.tiles && ok; ++tile) {
+              if (tile > 0) fill(tile, true);
+              if (ok) fill(tile, false);
+            }
+          }
+        }
+        __syncwarp();
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (it.state == 0) break;
+      }
+      if (__any_sync(0xffffffffu, bad) && lane == 0 && a.error_flag != nullptr) atomicCAS(a.error_flag, 0, kBadOffsets);
+      if (!ok && lane == 0) {  // what is on its way must land before this memory is another CTA's
+        for (unsigned i = copies > kStages ? copies - kStages : 0; i < copies; ++i) ptx::mbar_drain(kv_full + i % kStages, (i / kStages) & 1);
+        for (int b = 0; b < kBlocks; ++b)
+          if (loads[b] > 0) ptx::mbar_drain(q_full + b, (loads[b] - 1) & 1);
+      }
+    } else if (warp == kMmaWarp) {
+      if (ptx::elect_one()) {
+        constexpr uint32_t kScores = make_idesc_bf16<kTile, false>(), kOutputs = make_idesc_bf16<D, true>();
+        unsigned copies = 0, values = 0, loads[kBlocks] = {0, 0}, probs[kBlocks] = {0, 0};
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, unsigned parity) {
+          ok = ok && ptx::mbar_wait(bar, parity & 1, abort_flag);
+          if (!ok) give_up();
+          return ok;
+        };
+        Item it;
+        for (int n = 0; ok; ++n) {
+          if (!next_item(it, n)) break;
+          ptx::mbar_arrive(item_empty + n % kItemSlots);
+          if (it.tiles == 0) continue;
+          const int active = it.count > a.tokens ? 2 : 1;
+          auto scores = [&](int b, unsigned copy, bool last) {  // S of block b and the tile that is copy `copy`
+            const uint32_t keys = ring + copy % kStages * S::kBytes;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t at = (k / 4) * S::kHalf + (k % 4) * 32;
+              mma_ss(tmem + b * kTile, ptx::make_smem_desc(queries + b * S::kBytes + at, 1024, 16, 2), ptx::make_smem_desc(keys + at, 1024, 16, 2), kScores,
+                     k > 0);
+            }
+            ptx::tc_commit<1>(s_full + b);
+            if (last) ptx::tc_commit<1>(q_empty + b);
+          };
+          for (int b = 0; b < active; ++b) {
+            if (!wait(q_full + b, loads[b]++)) break;
+            if (b == 0 && !wait(kv_full + copies % kStages, copies / kStages)) break;
+            ptx::tc_fence_after();
+            scores(b, copies, it.tiles == 1);
+          }
+          if (!ok) break;
+          ptx::tc_commit<1>(kv_empty + copies % kStages);
+          ++copies;
+          for (int tile = 0; tile < it.tiles && ok; ++tile) {
+            const unsigned value = copies, next = copies + 1;
+            const bool more = tile + 1 < it.tiles;
+            if (!wait(kv_full + value % kStages, value / kStages)) break;
+            if (!wait(v_ok + values % kStages, values / kStages)) break;
+            const bool by_rows = (not_finite[values % kStages * kCheckWarps] | not_finite[values % kStages * kCheckWarps + 1]) != 0;
+            ++values;
+            if (more && !wait(kv_full + next % kStages, next / kStages)) break;
+            for (int b = 0; b < active; ++b) {
+              if (!wait(p_full + b, probs[b]++)) break;
+              ptx::tc_fence_after();
+              if (!by_rows) {
+                const uint32_t from = ring + value % kStages * S::kBytes;
+#pragma unroll
+                for (int k = 0; k < kTile / 16; ++k)
+                  mma_ts(tmem + S::kOutCol + b * D, tmem + b * kTile + k * 8, ptx::make_smem_desc(from + k * 2048, 1024, S::kHalf, 2), kOutputs,
+                         tile > 0 || k > 0);
+              }
+              if (b + 1 == active) ptx::tc_commit<1>(kv_empty + value % kStages);
+              if (more)
+                scores(b, next, tile + 2 == it.tiles);
+              else
+                ptx::tc_commit<1>(o_full + b);
+            }
+            if (!ok) break;
+            if (more) ptx::tc_commit<1>(kv_empty + next % kStages);
+            copies += more ? 2 : 1;
+          }
+        }
+        if (!ok) {  // the products that were issued must have ended before their memory is another CTA's
+          ptx::tc_commit<1>(drained);
+          ptx::mbar_drain(drained, 0);
+        }
+      }
+      __syncwarp();
+    } else {
+      const int part = warp - kCheckWarp;
+      unsigned copies = 0, values = 0;
+      Item it;
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        if (!next_item_of_warp(it, n)) break;
+        for (int tile = 0; tile < it.tiles; ++tile, copies += 2, ++values) {
+          const unsigned copy = copies + 1;
+          ok = ptx::mbar_wait(kv_full + copy % kStages, (copy / kStages) & 1, abort_flag);
+          if (!ok) give_up();
+          __syncwarp();
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          bool found = false;
+          if (is_masked(it, tile, a.window, a.sinks)) {
+            const uint32_t from = ring + copy % kStages * S::kBytes + part * (S::kBytes / kCheckWarps) + lane * 16;
+            unsigned top = 0;
+#pragma unroll 8
+            for (int i = 0; i < S::kBytes / kCheckWarps; i += 512) {
+              const float4 v = ptx::ld_shared_f32x4(from + i);
+              top = __vmaxu2(top, __vmaxu2(__float_as_uint(v.x) & 0x7FFF7FFFu, __float_as_uint(v.y) & 0x7FFF7FFFu));
+              top = __vmaxu2(top, __vmaxu2(__float_as_uint(v.z) & 0x7FFF7FFFu, __float_as_uint(v.w) & 0x7FFF7FFFu));
+            }
+            found = max(top & 0xFFFFu, top >> 16) >= 0x7F80u;
+          }
+          const bool any = __any_sync(0xffffffffu, found);
+          if (lane == 0) {
+            not_finite[values % kStages * kCheckWarps + part] = any;
+            ptx::mbar_arrive(v_ok + values % kStages);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<1>(tmem, 512);
+  }
+}
+
+bool encode(CUtensorMap *map, const void *base, int rows, int heads, int halves, long long row_stride, long long head_stride, bool heads_first,
+            int box_rows, int box_heads, int box_halves) {
+  // [128 bytes][heads][rows][halves] for the queries, [128 bytes][rows][halves][heads] for keys and values; strides in elements
+  const cuuint64_t row = (cuuint64_t)row_stride * 2, head = (cuuint64_t)head_stride * 2;
+  if (heads_first) {
+    const cuuint64_t dims[4] = {128, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)halves}, strides[3] = {head, row, 128};
+    const cuuint32_t box[4] = {128, (cuuint32_t)box_heads, (cuuint32_t)box_rows, 1};
+    return make_tensor_map(map, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  const cuuint64_t dims[4] = {128, (cuuint64_t)rows, (cuuint64_t)halves, (cuuint64_t)heads}, strides[3] = {row, 128, head};
+  const cuuint32_t box[4] = {128, (cuuint32_t)box_rows, (cuuint32_t)box_halves, 1};
+  return make_tensor_map(map, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int D>
+cudaError_t launch(const PromptAttention &p, const Args &a, int sms, cudaStream_t stream) {
+  using S = Sizes<D>;
+  CUtensorMap q, k, v, k8, v8;
+  if (!encode(&q, p.q, p.rows, p.heads, S::kHalves, p.q_row, p.q_head, true, a.tokens, a.chunk_heads, 1) ||
+      !encode(&k, p.k, p.k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, kTile, 1, S::kHalves) ||
+      !encode(&v, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, kTile, 1, S::kHalves) ||
+      !encode(&k8, p.k, p.k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, 8, 1, 1) ||
+      !encode(&v8, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, 8, 1, 1))
+    return cudaErrorInvalidValue;
+  static bool ready[64] = {};
+  const cudaError_t err = allow_smem(prompt_attention_kernel<D>, S::kTotal, ready);
+  if (err != cudaSuccess) return err;
+  const long long most = ((long long)p.rows / (kBlocks * a.tokens) + p.seqs) * a.kv_heads * a.chunks;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)(most < sms ? most : sms));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kTotal;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, prompt_attention_kernel<D>, q, k, v, k8, v8, a);
+}
+
+}  // namespace
+
+cudaError_t run_prompt_attention(const PromptAttention &p, cudaStream_t stream) {
+  int dev = 0, sms = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (err != cudaSuccess) return err;
+  Args a = {};
+  a.offsets = p.offsets;
+  a.k_offsets = p.k_offsets;
+  a.out = static_cast<__nv_bfloat16 *>(p.out);
+  a.rows = p.rows;
+  a.k_rows = p.k_rows;
+  a.seqs = p.seqs;
+  a.heads = p.heads;
+  a.kv_heads = p.kv_heads;
+  a.group = p.heads / p.kv_heads;
+  a.chunks = (a.group + kTile - 1) / kTile;
+  a.chunk_heads = (a.group + a.chunks - 1) / a.chunks;
+  a.tokens = kTile / a.chunk_heads;
+  a.window = p.window;
+  a.sinks = p.sinks;
+  a.scale_log2 = p.scale * 1.4426950408889634f;
+  a.fill = p.fill;
+  a.error_flag = p.error_flag;
+  return p.head_dim == 128 ? launch<128>(p, a, sms, stream) : launch<64>(p, a, sms, stream);
+}
+
+}  // namespace sharq

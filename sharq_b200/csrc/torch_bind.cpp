@@ -549,6 +549,59 @@ Tensor weight_only_linear(const Tensor &x, const Tensor &qw, const Tensor &sf, c
   return y;
 }
 
+// A window as the C ABI takes it.
+int window_of(const std::optional<int64_t> &window, int64_t sinks) {
+  need(!window || *window >= 1, "window must be at least 1, or None");
+  need(sinks >= 0, "sinks must not be negative");
+  return !window ? 0 : (int)std::min<int64_t>(*window, INT32_MAX);
+}
+
+Tensor prompt_attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &offsets, const std::optional<int64_t> &window,
+                        int64_t sinks, const std::optional<double> &scale, const std::optional<Tensor> &k_offsets, const std::optional<Tensor> &out,
+                        const Tensor &flag) {
+  need(q.is_cuda(), "q must be a CUDA tensor");
+  const at::Device dev = q.device();
+  const Tensor *held[3] = {&q, &k, &v};
+  for (int i = 0; i < 3; ++i)
+    if (!(held[i]->is_cuda() && held[i]->device() == dev && held[i]->scalar_type() == at::kBFloat16 && held[i]->dim() == 3 &&
+          (held[i]->size(2) <= 1 || held[i]->stride(2) == 1)))
+      fail(std::string(1, "qkv"[i]) + " must be a CUDA bfloat16 tensor [rows, heads, head_dim] whose heads are contiguous, on the device of q");
+  const int64_t rows = q.size(0), heads = q.size(1), d = q.size(2), k_rows = k.size(0), kv_heads = k.size(1);
+  need(k.sizes() == v.sizes(), "k and v must be shaped alike");
+  need(k.size(2) == d && kv_heads > 0 && heads > 0 && heads % kv_heads == 0,
+       "q must have head_dim elements per head and a multiple of the heads of k");
+  if (d != 64 && d != 128) fail("head_dim must be 64 or 128, got " + std::to_string(d));
+  need(rows <= 1 << 30 && k_rows <= 1 << 30 && heads <= 65536, "too many rows or heads");
+  need(offsets.dim() == 1 && offsets.size(0) >= 2 && offsets.size(0) <= 1 << 28, "offsets must have an entry for every sequence and one more");
+  check_indices(offsets, offsets.size(0), dev, "offsets");
+  if (k_offsets)
+    check_indices(*k_offsets, offsets.size(0), dev, "k_offsets");
+  else
+    need(k_rows == rows, "without k_offsets k and v must have a row for every row of q");
+  const int w = window_of(window, sinks);
+  if (out)
+    need(is_plain(*out, at::kBFloat16) && out->device() == dev && out->sizes() == q.sizes(),
+         "out must be a contiguous CUDA bfloat16 tensor shaped like q");
+  int64_t strides[3][2];
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 2; ++j) {  // a dimension of one element has no stride to speak of
+      strides[i][j] = held[i]->size(j) > 1 ? held[i]->stride(j) : d;
+      if (strides[i][j] <= 0 || strides[i][j] % 8 != 0)
+        fail(std::string("strides of ") + "qkv"[i] + " must be positive multiples of 8");
+    }
+  c10::cuda::OptionalCUDAGuard guard(dev);
+  Tensor o = out ? *out : empty_like_on(q, {rows, heads, d}, at::kBFloat16);
+  if (rows == 0) return o;
+  // without any key there is nothing to read: the queries stand for keys that no sequence has
+  const Tensor &keys = k_rows > 0 ? k : q, &values = k_rows > 0 ? v : q;
+  check(sharq_prompt_attention(ptr(q), strides[0][0], strides[0][1], ptr(keys), strides[1][0], strides[1][1], ptr(values), strides[2][0], strides[2][1],
+                               (int)rows, (int)std::max<int64_t>(k_rows, 1), (int)heads, (int)kv_heads, (int)d, static_cast<const int *>(ptr(offsets)),
+                               k_offsets ? static_cast<const int *>(ptr(*k_offsets)) : nullptr, (int)offsets.size(0) - 1, w,
+                               (int)std::min<int64_t>(sinks, INT32_MAX), (float)(scale ? *scale : 1.0 / std::sqrt((double)d)), ptr(o), !out,
+                               flag_of(flag), stream_of(q)));
+  return o;
+}
+
 // -> offsets [sequences + 1], positions [rows], sequences [rows], views of one allocation
 std::vector<Tensor> plan_paged_step(const Tensor &table, const Tensor &lengths, const Tensor &counts, const Tensor &free_pages,
                                     const Tensor &free_count, int64_t page_size, int64_t rows, const std::optional<Tensor> &released,
@@ -692,6 +745,7 @@ PYBIND11_MODULE(sharq_native, m) {
   m.def("rope_append_paged", as_tuple(&rope_append_paged));
   m.def("paged_attention", &paged_attention, nogil());
   m.def("weight_only_linear", &weight_only_linear, nogil());
+  m.def("prompt_attention", &prompt_attention, nogil());
   m.def("plan_paged_step", as_tuple(&plan_paged_step));
   m.def("adjust_logits", &adjust_logits, nogil());
   m.def("rope_inplace", &rope_inplace, nogil());

@@ -34,6 +34,7 @@ _BAD_EXPERT = 0x401  # kPlanBadExpert of csrc/decoder_ops.cu
 _BAD_CACHE_INDEX = 0x402  # kBadCacheIndex of csrc/decode_ops.cuh
 _ATTENTION_TIMEOUT, _WEIGHT_ONLY_TIMEOUT = 0x403, 0x404  # kAttentionTimeout, kWeightOnlyTimeout of csrc/decode_ops.cuh
 _BAD_STEP_PLAN, _BAD_LOGIT_RULES = 0x405, 0x406  # kBadStepPlan, kBadLogitRules of csrc/decode_ops.cuh
+_BAD_OFFSETS, _PROMPT_TIMEOUT = 0x407, 0x408  # kBadOffsets, kPromptTimeout of csrc/decode_ops.cuh
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -87,6 +88,10 @@ def check_device_errors(device=None) -> None:
                                    f"on cuda:{idx}")
             if code == _BAD_LOGIT_RULES:
                 raise RuntimeError(f"sharq_b200 adjust_logits: a token, length or offset was outside its range on cuda:{idx}")
+            if code == _BAD_OFFSETS:
+                raise RuntimeError(f"sharq_b200 prompt_attention: offsets went back or beyond the rows on cuda:{idx}")
+            if code == _PROMPT_TIMEOUT:
+                raise RuntimeError(f"sharq_b200 prompt_attention: a wait ran out on cuda:{idx}; outputs are undefined")
             if code in (_ATTENTION_TIMEOUT, _WEIGHT_ONLY_TIMEOUT):
                 name = "paged_attention" if code == _ATTENTION_TIMEOUT else "weight_only_linear"
                 raise RuntimeError(f"sharq_b200 {name}: a wait for a copy ran out on cuda:{idx}; outputs are undefined")
@@ -236,6 +241,19 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     outside the cache makes that sequence's rows NaN and is reported by check_device_errors.  A sequence may stand in several
     rows with lengths of their own (drafted tokens).  The same bits from call to call."""
     return _lib.native().paged_attention(q, k_cache, v_cache, page_table, lengths, scale, k_scale, v_scale, out, _error_flag(q.device))
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, window: Optional[int] = None, sinks: int = 0,
+                     scale: Optional[float] = None, k_offsets: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of ragged prompts whose rows lie one behind the other: q bf16 [rows, heads, head_dim], k and v bf16
+    [rows, kv_heads, head_dim] (heads contiguous, other strides multiples of 8), head_dim 64 or 128, heads a multiple of kv_heads -> bf16
+    [rows, heads, head_dim].  Sequence s has the rows offsets[s] to offsets[s + 1] (int32, on the device).  With window a query at position p sees
+    the keys at p - window + 1 to p and the first `sinks`, else all up to p.  k_offsets: the rows of k and v that a sequence has, of which the last
+    belong to its queries (a later piece of a prompt); a query ahead of all of its keys gives zeros.  scale: default head_dim ** -0.5.  Float32
+    sums and statistics, probabilities in bf16 for the product with the values, one rounding of the result.  Rows of no sequence are zeros, or with out stay
+    as they are.  Offsets that go back or beyond the rows are reported by check_device_errors: such a sequence has no rows, one with such
+    k_offsets NaN.  The same bits from call to call."""
+    return _lib.native().prompt_attention(q, k, v, offsets, window, sinks, scale, k_offsets, out, _error_flag(q.device))
 
 
 def plan_paged_step(page_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
