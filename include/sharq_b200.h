@@ -417,6 +417,13 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
                           const int *lengths, float scale, void *out_bf16, void *workspace, size_t workspace_bytes, int *error_flag,
                           void *stream);
 
+/* ... of the last `window` tokens of a sequence and its first `sinks`, those that it has (window 0: of all).  Pages with no token that is seen are not
+ * read, and their entries in the table may be anything. */
+size_t sharq_paged_attention_windowed_workspace_bytes(int heads, const sharq_paged_cache *cache, int window, int sinks);
+int sharq_paged_attention_windowed(const void *q_bf16, int64_t q_row, int64_t q_head, int heads, const sharq_paged_cache *cache,
+                                   const int *lengths, float scale, int window, int sinks, void *out_bf16, void *workspace,
+                                   size_t workspace_bytes, int *error_flag, void *stream);
+
 /* Product of m (1 to 16) unquantised bf16 rows (x_row elements between them, a multiple of 8) with a 4-bit weight:
  * y[m, n] = bf16(scale * scale_dev[0] * sum_k x[m, k] * W[n, k] + bias[n]), W = payload qw [n, k/2] times the dense scale factors sfw_dense, as
  * sharq_quantize_w32_shared and sharq_quantize_nvfp4 make them.  scale_dev (float on the device) and bias (bf16 [n]) may be NULL.  Float

@@ -102,6 +102,9 @@ SIGNATURES = {
     "sharq_paged_attention_workspace_bytes": (c_size_t, [c_int, _P]),
     "sharq_paged_attention": (c_int, [_P, c_int64, c_int64, c_int, _P, _P, c_float, _P, _P, c_size_t, _P, _P]),
     "sharq_weight_only_linear": (c_int, [_P, c_int64, c_int, c_int, c_int, _P, _P, _P, c_float, _P, _P, _P, _P]),
+    "sharq_paged_attention_windowed_workspace_bytes": (c_size_t, [c_int, _P, c_int, c_int]),
+    "sharq_paged_attention_windowed": (
+        c_int, [_P, c_int64, c_int64, c_int, _P, _P, c_float, c_int, c_int, _P, _P, c_size_t, _P, _P]),
     "sharq_prompt_attention": (
         c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, _P, _P, c_int, c_int,
                 c_int, c_float, _P, c_int, _P, _P]),

@@ -795,15 +795,26 @@ int sharq_rope_append_paged(const void *qkv_bf16, int64_t row_stride, int rows, 
 }
 
 size_t sharq_paged_attention_workspace_bytes(int heads, const sharq_paged_cache *cache) {
+  return sharq_paged_attention_windowed_workspace_bytes(heads, cache, 0, 0);
+}
+
+size_t sharq_paged_attention_windowed_workspace_bytes(int heads, const sharq_paged_cache *cache, int window, int sinks) {
   sharq::PagedCache c;
   bool fp8 = false;
-  if (paged_cache(cache, &c, &fp8) || heads <= 0 || heads % c.kv_heads != 0) return 0;
-  return sharq::paged_attention_workspace_bytes(heads, c, fp8);
+  if (paged_cache(cache, &c, &fp8) || heads <= 0 || heads % c.kv_heads != 0 || window < 0 || sinks < 0) return 0;
+  return sharq::paged_attention_workspace_bytes(heads, c, fp8, window, sinks);
 }
 
 int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int heads, const sharq_paged_cache *cache,
                           const int *lengths, float scale, void *out_bf16, void *workspace, size_t workspace_bytes, int *error_flag,
                           void *stream) {
+  return sharq_paged_attention_windowed(q_bf16, q_row, q_head, heads, cache, lengths, scale, 0, 0, out_bf16, workspace, workspace_bytes, error_flag,
+                                        stream);
+}
+
+int sharq_paged_attention_windowed(const void *q_bf16, int64_t q_row, int64_t q_head, int heads, const sharq_paged_cache *cache,
+                                   const int *lengths, float scale, int window, int sinks, void *out_bf16, void *workspace,
+                                   size_t workspace_bytes, int *error_flag, void *stream) {
   sharq::PagedCache c;
   bool fp8 = false;
   if (paged_cache(cache, &c, &fp8)) return 1;
@@ -816,10 +827,11 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
                 "too many sequences, or a page table for too many tokens");
   SHARQ_REQUIRE(q_row >= 0 && q_head >= 0 && q_row % 8 == 0 && q_head % 8 == 0, "the strides of q must be multiples of 8");
   SHARQ_REQUIRE(aligned16(q_bf16) && aligned16(out_bf16) && aligned16(workspace), "buffers must be 16-byte aligned");
-  const size_t need = sharq::paged_attention_workspace_bytes(heads, c, fp8);
+  SHARQ_REQUIRE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
+  const size_t need = sharq::paged_attention_workspace_bytes(heads, c, fp8, window, sinks);
   SHARQ_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "workspace too small: need %zu bytes", need);
-  return check_cuda(sharq::run_paged_attention(q_bf16, q_row, q_head, heads, c, fp8, lengths, scale, out_bf16, workspace, error_flag,
-                                               as_stream(stream)),
+  return check_cuda(sharq::run_paged_attention(q_bf16, q_row, q_head, heads, c, fp8, lengths, scale, window, sinks, out_bf16, workspace,
+                                               error_flag, as_stream(stream)),
                     "paged_attention");
 }
 

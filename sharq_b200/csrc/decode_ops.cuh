@@ -37,9 +37,11 @@ cudaError_t run_rope_append_paged(const void *qkv, long long row_stride, int row
                                   void *q_out, void *k_out, int *error_flag, cudaStream_t stream);
 
 // One query row per sequence of the cache's page table (cache.head_dim 64 or 128, heads a multiple of cache.kv_heads).
-size_t paged_attention_workspace_bytes(int heads, const PagedCache &cache, bool fp8);
+// window: tokens that are seen from the last one back, with the first `sinks`; 0: all.
+size_t paged_attention_workspace_bytes(int heads, const PagedCache &cache, bool fp8, int window, int sinks);
 cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head, int heads, const PagedCache &cache, bool fp8,
-                                const int *lengths, float scale, void *out, void *workspace, int *error_flag, cudaStream_t stream);
+                                const int *lengths, float scale, int window, int sinks, void *out, void *workspace, int *error_flag,
+                                cudaStream_t stream);
 
 // y[m, n] = bf16(scale * x . W^T + bias), m rows (1..16) of bf16 against a 4-bit weight with dense scale factors, k % 64 == 0.
 constexpr int kWeightOnlyMaxRows = 16;

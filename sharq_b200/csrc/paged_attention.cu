@@ -136,6 +136,7 @@ struct AttnArgs {
   unsigned stretches_magic, items_magic;  // list: for divide() by the stretches and by the items of a sequence
   int page_shift;                  // log2 of the page size, -1 if it is no power of two
   float scale_log2;                // scale * log2(e)
+  int window, sinks;               // windowed form: tokens that are seen from the last one back, and first ones
   int *error_flag;
 };
 
@@ -192,9 +193,20 @@ __device__ __forceinline__ Length length_of(const AttnArgs &a, const PagedCache 
   const bool bad = n < 0 || n > paged_capacity(c);
   return {bad ? 0 : n, bad};
 }
-template <int kTokens>
-__device__ __forceinline__ int tiles_of(int tokens) {  // an empty sequence has one tile, without tokens
-  return tokens <= kTokens ? 1 : (tokens - 1) / kTokens + 1;
+// Windowed form: a sequence of n tokens is seen but for [sinks, begin), begin = n - window, and the tiles that hold nothing but those, `skip` of them behind the first
+// `front`, are left out of its list of tiles.
+struct Gap {
+  int begin, front, skip;
+};
+template <int kTokens, bool kWindow>
+__device__ __forceinline__ Gap gap_of(const AttnArgs &a, int tokens) {
+  if (!kWindow) return {0, 0, 0};
+  const int begin = max(0, tokens - a.window), front = (int)(((unsigned)min(a.sinks, tokens) + kTokens - 1) / kTokens);
+  return {begin, front, max(0, begin / kTokens - front)};
+}
+template <int kTokens, bool kWindow>
+__device__ __forceinline__ int tiles_of(const AttnArgs &a, int tokens) {  // an empty sequence has one tile, without tokens
+  return (tokens <= kTokens ? 1 : (tokens - 1) / kTokens + 1) - gap_of<kTokens, kWindow>(a, tokens).skip;
 }
 
 // n / d for n < 2^31 with ceil(2^32 / d) at hand (an integer division by a variable takes some hundred cycles): at most one too high
@@ -208,15 +220,15 @@ __device__ __forceinline__ int divide(int n, int d, unsigned magic) {
 struct Place {
   int seq, head, chunk, skip, left, tokens, tile, end;
 };
-template <int kTokens>
+template <int kTokens, bool kWindow>
 __device__ __forceinline__ void enter(Place &p, const AttnArgs &a, const PagedCache &c) {
   p.tokens = length_of(a, c, p.seq).tokens;
   p.tile = max(0, p.skip - kItemCost);
-  p.end = min(tiles_of<kTokens>(p.tokens), p.skip + p.left - kItemCost);
+  p.end = min(tiles_of<kTokens, kWindow>(a, p.tokens), p.skip + p.left - kItemCost);
 }
-template <int kTokens>
+template <int kTokens, bool kWindow>
 __device__ __forceinline__ void leave(Place &p, const AttnArgs &a, const PagedCache &c) {
-  p.left = max(0, p.left - (kItemCost + tiles_of<kTokens>(p.tokens) - p.skip));
+  p.left = max(0, p.left - (kItemCost + tiles_of<kTokens, kWindow>(a, p.tokens) - p.skip));
   if (p.left == 0) return;
   p.skip = 0;
   if (++p.chunk == a.chunks) {
@@ -226,10 +238,10 @@ __device__ __forceinline__ void leave(Place &p, const AttnArgs &a, const PagedCa
   if (p.head == c.kv_heads) {
     p.head = 0;
     ++p.seq;
-    enter<kTokens>(p, a, c);
+    enter<kTokens, kWindow>(p, a, c);
   } else {  // the same sequence's tokens
     p.tile = 0;
-    p.end = min(tiles_of<kTokens>(p.tokens), p.left - kItemCost);
+    p.end = min(tiles_of<kTokens, kWindow>(a, p.tokens), p.left - kItemCost);
   }
 }
 
@@ -237,22 +249,22 @@ __device__ __forceinline__ void leave(Place &p, const AttnArgs &a, const PagedCa
 struct List {
   int total, per;
 };
-template <int kTokens>
+template <int kTokens, bool kWindow>
 __device__ __forceinline__ List list_of(const AttnArgs &a, const PagedCache &c, int items, int stretches, int lane) {
   int per_head = 0;
 #pragma unroll 4
-  for (int b = lane; b < a.seqs; b += 32) per_head += kItemCost + tiles_of<kTokens>(length_of(a, c, b).tokens);
+  for (int b = lane; b < a.seqs; b += 32) per_head += kItemCost + tiles_of<kTokens, kWindow>(a, length_of(a, c, b).tokens);
   const int total = __reduce_add_sync(0xffffffffu, per_head) * items;
   return {total, max(kStretchLeast, divide(total + stretches - 1, stretches, a.stretches_magic))};
 }
 // the item that unit u of the list belongs to, and what of it lies before u -> the item's length
-template <int kTokens>
+template <int kTokens, bool kWindow>
 __device__ __forceinline__ int locate(Place &at, int u, const AttnArgs &a, const PagedCache &c, int items, int lane) {
   int before = 0;
   const int u_head = divide(u, items, a.items_magic);  // in units of a head: a sequence begins at items times what lies before it
   for (int b0 = 0; b0 < a.seqs; b0 += 32) {
     const int b = b0 + lane;
-    const int n_units = b < a.seqs ? kItemCost + tiles_of<kTokens>(length_of(a, c, b).tokens) : 0;
+    const int n_units = b < a.seqs ? kItemCost + tiles_of<kTokens, kWindow>(a, length_of(a, c, b).tokens) : 0;
     int n = n_units;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -280,7 +292,7 @@ __device__ __forceinline__ int locate(Place &at, int u, const AttnArgs &a, const
 
 // kCols: columns for query heads (8 or 16).  kDirect: a cluster per (sequence, head chunk), blockIdx = (rank, head chunk, sequence), whose warps take equal
 // stretches of its tiles and whose CTAs join their parts through distributed shared memory; nothing is left for a second launch.
-template <int D, bool kFp8, int kCols, int kForm>
+template <int D, bool kFp8, int kCols, int kForm, bool kWindow>
 __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::kCtas))
     paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const __grid_constant__ AttnArgs a, const __grid_constant__ PagedCache c) {
@@ -316,17 +328,17 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
     at.head = a.chunks == 1 ? blockIdx.y : blockIdx.y / a.chunks;
     at.chunk = blockIdx.y - at.head * a.chunks;
     at.tokens = length_of(a, c, at.seq).tokens;
-    const int n_tiles = tiles_of<kTokens>(at.tokens), each = (n_tiles + stretches - 1) >> a.stretch_shift;
+    const int n_tiles = tiles_of<kTokens, kWindow>(a, at.tokens), each = (n_tiles + stretches - 1) >> a.stretch_shift;
     at.tile = stretch * each;
     at.end = min(n_tiles, at.tile + each);
     at.left = 1;  // this item and no other
   } else {
-    const List list = list_of<kTokens>(a, c, items, stretches, lane);
+    const List list = list_of<kTokens, kWindow>(a, c, items, stretches, lane);
     const int u0 = stretch * list.per;  // stretches * per: total and a little more
     at.left = max(0, min(list.per, list.total - u0));
     if (at.left > 0) {
-      locate<kTokens>(at, u0, a, c, items, lane);
-      enter<kTokens>(at, a, c);
+      locate<kTokens, kWindow>(at, u0, a, c, items, lane);
+      enter<kTokens, kWindow>(at, a, c);
     }
   }
 
@@ -336,7 +348,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
   auto settle = [&]() {  // moves on to the next item with a tile for this warp
     bool entered = false;
     while (next.tile >= next.end && next.left > 0) {
-      leave<kTokens>(next, a, c);
+      leave<kTokens, kWindow>(next, a, c);
       entered = true;
     }
     if (entered && next.left > 0) {  // its queries on their way to the SM
@@ -352,9 +364,11 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
   auto load = [&]() {
     if (next.left > 0) {
       const uint32_t stage = ring + put * T::kStage;
-      const int live = next.tokens - next.tile * kTokens;  // tokens from this tile on
+      const Gap gap = gap_of<kTokens, kWindow>(a, next.tokens);
+      const int tile = kWindow && next.tile >= gap.front ? next.tile + gap.skip : next.tile;
+      const int live = next.tokens - tile * kTokens;  // tokens from this tile on
       const int pieces = live <= 0 ? 0 : min(boxes, (live + box - 1) >> a.box_shift);
-      const int piece0 = next.tile * boxes;
+      const int piece0 = tile * boxes;
       if (next.seq != held_seq || piece0 < held_first || piece0 + boxes > held_first + 32) {
         held_seq = next.seq;
         held_first = piece0;
@@ -370,7 +384,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
         const int token = (piece0 + i) << a.box_shift;
         const int slot = a.page_shift >= 0 ? token & (c.page_size - 1) : token % c.page_size;
         if ((unsigned)page >= (unsigned)c.pages) {
-          any_bad = true;
+          any_bad |= !(kWindow && token >= a.sinks && token + box <= gap.begin);  // a page that is not seen may be anything
           page = c.pages;  // one behind the last: zeros are filled in
         }
         if (chosen) {
@@ -403,7 +417,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
 
   int take = 0;         // stage that is used next
   unsigned phases = 0;  // parity of every stage's barrier
-  for (; at.left > 0; leave<kTokens>(at, a, c)) {
+  for (; at.left > 0; leave<kTokens, kWindow>(at, a, c)) {
     if (at.tile >= at.end) continue;
     const int kv = at.head, chunk = at.chunk;
     const int cols = min(16, a.group - chunk * 16);  // query heads of the chunk
@@ -464,7 +478,9 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
 #pragma unroll
     for (int n = 0; n < kN; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
 
-    for (int tile = at.tile; tile < at.end; ++tile) {
+    const Gap gap = gap_of<kTokens, kWindow>(a, at.tokens);
+    for (int index = at.tile; index < at.end; ++index) {
+      const int tile = kWindow && index >= gap.front ? index + gap.skip : index;
       load();
       const uint32_t keys = ring + take * T::kStage, values = keys + T::kBytes;
       const bool poison = (bad_stages >> take) & 1;
@@ -516,18 +532,25 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
         for (int n = 0; n < kN; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) s[b][n][j] = (s[b][n][j] + s2[b][n][j]) * sl[n][j & 1];
-      if (live < kTokens || poison) {
+      // rows of the tile that are not seen though they lie ahead of the last token
+      const int hide0 = kWindow ? min(kTokens, max(0, a.sinks - tile * kTokens)) : 0, hide1 = kWindow ? min(kTokens, max(0, gap.begin - tile * kTokens)) : 0;
+      if (live < kTokens || poison || (kWindow && hide0 < hide1)) {
 #pragma unroll
         for (int b = 0; b < kTokens / 16; ++b)
 #pragma unroll
           for (int n = 0; n < kN; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              if (b * 16 + (j >> 1) * 8 + my_token >= live) s[b][n][j] = -INFINITY;
+              const int row = b * 16 + (j >> 1) * 8 + my_token;
+              if (row >= live || (kWindow && row >= hide0 && row < hide1)) s[b][n][j] = -INFINITY;
               if (poison) s[b][n][j] = __int_as_float(0x7fffffff);
             }
         // values behind the sequence: whatever the page or an earlier tile left there must not meet a probability of 0
         for (int i = max(live, 0) * 8 + lane; i < kTokens * 8; i += 32)
+#pragma unroll
+          for (int half = 0; half < T::kHalves; ++half)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(values + half * T::kHalf + i * 16), "r"(0) : "memory");
+        for (int i = hide0 * 8 + lane; i < hide1 * 8; i += 32)
 #pragma unroll
           for (int half = 0; half < T::kHalves; ++half)
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(values + half * T::kHalf + i * 16), "r"(0) : "memory");
@@ -656,7 +679,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], off);
       }
-    const int n_tiles = tiles_of<kTokens>(at.tokens);
+    const int n_tiles = tiles_of<kTokens, kWindow>(a, at.tokens);
     if (begins && at.end == n_tiles) {
       const int raw = a.lengths[at.seq];
       const bool bad = raw < 0 || raw > paged_capacity(c);
@@ -709,7 +732,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
     }
   }
 
-  if (kDirect && tiles_of<kTokens>(at.tokens) == 1) return;  // one warp of the cluster has done it all
+  if (kDirect && tiles_of<kTokens, kWindow>(a, at.tokens) == 1) return;  // one warp of the cluster has done it all
   __syncthreads();
   constexpr int kVecs = D * kCols / 4 / kAttnThreads;  // a thread's float4s of a part; its columns are the same in all of them
   static_assert(kVecs >= 1 && kAttnThreads * 4 % kCols == 0, "every thread has a share of a part");
@@ -861,7 +884,7 @@ constexpr int kJoinSlices = 4;
 constexpr int kJoinBatch = 4;  // parts whose loads are in flight together; more would take registers that the kernel above still holds
 constexpr int kJoinAlone = 8;  // parts that one warp joins
 
-template <int D, int kCols, bool kFp8>
+template <int D, int kCols, bool kFp8, bool kWindow>
 __global__ void __launch_bounds__(32 * kJoinWarps) paged_attention_join_kernel(const __grid_constant__ AttnArgs a,
                                                                                const __grid_constant__ PagedCache c, int ctas) {
   constexpr int kTokens = Tile<D, kFp8>::kTokens, kVecs = D * kCols / (128 * kJoinSlices);  // float4s of a lane
@@ -870,12 +893,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_attention_join_kernel(c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, items = c.kv_heads * a.chunks;
   const int base = blockIdx.x * kJoinWarps;
   {
-    const List list = list_of<kTokens>(a, c, items, kAttnWarps * ctas, lane);
+    const List list = list_of<kTokens, kWindow>(a, c, items, kAttnWarps * ctas, lane);
     const int span = list.per * kAttnWarps, from = (base + warp) * span, to = from + span;
     Place at = {0, 0, 0, 0, 0, 0, 0, 0};
     int parts = 0;
     if (base + warp < ctas && to < list.total) {
-      const int units = locate<kTokens>(at, to, a, c, items, lane), first = to - at.skip + kItemCost;  // unit of the item's first tile
+      const int units = locate<kTokens, kWindow>(at, to, a, c, items, lane), first = to - at.skip + kItemCost;  // unit of the item's first tile
       if (at.skip > 0 && first >= from && first < to) parts = 2 + (units - at.skip - 1) / span;
     }
     if (lane == 0) items_of[warp] = make_int4(at.seq, at.head, at.chunk, parts);
@@ -1046,7 +1069,15 @@ int direct_splits(int seqs, int items, int most_tiles, int ctas) {
   return most_tiles <= splits * kAttnWarps * (pairs * splits * 5 >= 2 * ctas ? kDirectMost : kDirectFew) ? splits : 0;
 }
 
-template <int D, bool kFp8, int kCols>
+// Tiles that the longest sequence of a table may have.
+int tiles_at_most(const PagedCache &c, int tokens, int window, int sinks) {
+  const int all = (paged_capacity(c) - 1) / tokens + 1;
+  if (window == 0) return all;
+  const long long seen = ((long long)sinks + tokens - 1) / tokens + ((long long)window + tokens - 2) / tokens + 1;
+  return seen < all ? (int)seen : all;
+}
+
+template <int D, bool kFp8, int kCols, bool kWindow>
 cudaError_t launch(AttnArgs a, const PagedCache &c, int ctas, cudaStream_t stream) {
   using T = Tile<D, kFp8>;
   constexpr int kSmem = Layout<D, kFp8, kCols, kList>::kTotal;
@@ -1069,13 +1100,14 @@ cudaError_t launch(AttnArgs a, const PagedCache &c, int ctas, cudaStream_t strea
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const int items = c.kv_heads * a.chunks;
-  const int splits = direct_splits(a.seqs, items, (paged_capacity(c) - 1) / T::kTokens + 1, ctas);
+  const int splits = direct_splits(a.seqs, items, tiles_at_most(c, T::kTokens, a.window, a.sinks), ctas);
   if (splits > 0) {
     // Three CTAs per SM where two would leave some for a second turn, and three do not (48 x 128 tokens of 8 heads 8.0 instead of 10.7 us; with
     // fewer, or more than three can take, it is slower: 8 x 4000 26.3 instead of 24.2, 64 x 256 18.1 instead of 16.9).
     const long long all = (long long)a.seqs * items * splits;
     const bool three = kCols == 8 && all > ctas && 2 * all <= 3 * ctas;
-    const auto kernel = three ? paged_attention_kernel<D, kFp8, kCols, kCols == 8 ? kDirectThree : kDirectTwo> : paged_attention_kernel<D, kFp8, kCols, kDirectTwo>;
+    const auto kernel = three ? paged_attention_kernel<D, kFp8, kCols, kCols == 8 ? kDirectThree : kDirectTwo, kWindow>
+                              : paged_attention_kernel<D, kFp8, kCols, kDirectTwo, kWindow>;
     // (with the smaller form's need three of two's would fit)
     cfg.dynamicSmemBytes = three ? Layout<D, kFp8, kCols, kDirectThree>::kTotal : kSmem;
     static bool ready[2][64] = {};
@@ -1089,7 +1121,7 @@ cudaError_t launch(AttnArgs a, const PagedCache &c, int ctas, cudaStream_t strea
     cfg.gridDim = dim3((unsigned)splits, (unsigned)items, (unsigned)a.seqs);
     return cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, a, c);
   }
-  const auto kernel = paged_attention_kernel<D, kFp8, kCols, kList>;
+  const auto kernel = paged_attention_kernel<D, kFp8, kCols, kList, kWindow>;
   static bool ready[64] = {};
   cudaError_t err = allow_smem(kernel, kSmem, ready);
   if (err != cudaSuccess) return err;
@@ -1099,22 +1131,23 @@ cudaError_t launch(AttnArgs a, const PagedCache &c, int ctas, cudaStream_t strea
   cfg.gridDim = dim3((unsigned)((ctas + kJoinWarps - 1) / kJoinWarps), kJoinSlices);
   cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<D, kCols, kFp8>, a, c, ctas);
+  return cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<D, kCols, kFp8, kWindow>, a, c, ctas);
 }
 
 int attn_ctas() { return 2 * attn_sm_count(); }
 
 }  // namespace
 
-size_t paged_attention_workspace_bytes(int heads, const PagedCache &cache, bool fp8) {
+size_t paged_attention_workspace_bytes(int heads, const PagedCache &cache, bool fp8, int window, int sinks) {
   const int group = heads / cache.kv_heads, items = cache.kv_heads * ((group + 15) / 16), cols = group <= 8 ? 8 : 16;
   const int tokens = cache.head_dim * (fp8 ? 1 : 2) > 128 ? 16 : 32;  // as Tile has it
-  if (direct_splits(cache.seqs, items, (paged_capacity(cache) - 1) / tokens + 1, attn_ctas()) > 0) return 0;
+  if (direct_splits(cache.seqs, items, tiles_at_most(cache, tokens, window, sinks), attn_ctas()) > 0) return 0;
   return 2 * (size_t)attn_ctas() * cols * (cache.head_dim + 2) * sizeof(float);
 }
 
 cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head, int heads, const PagedCache &cache, bool fp8,
-                                const int *lengths, float scale, void *out, void *workspace, int *error_flag, cudaStream_t stream) {
+                                const int *lengths, float scale, int window, int sinks, void *out, void *workspace, int *error_flag,
+                                cudaStream_t stream) {
   const int ctas = attn_ctas(), group = heads / cache.kv_heads, cols = group <= 8 ? 8 : 16, d = cache.head_dim;
   AttnArgs a;
   a.q = static_cast<const __nv_bfloat16 *>(q);
@@ -1128,9 +1161,12 @@ cudaError_t run_paged_attention(const void *q, long long q_row, long long q_head
   a.group = group;
   a.chunks = (group + 15) / 16;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.window = window;
+  a.sinks = sinks;
   a.error_flag = error_flag;
-#define SHARQ_ATTN(D, FP8, COLS) \
-  if (d == D && fp8 == FP8 && cols == COLS) return launch<D, FP8, COLS>(a, cache, ctas, stream);
+#define SHARQ_ATTN(D, FP8, COLS)            \
+  if (d == D && fp8 == FP8 && cols == COLS) \
+    return window > 0 ? launch<D, FP8, COLS, true>(a, cache, ctas, stream) : launch<D, FP8, COLS, false>(a, cache, ctas, stream);
   SHARQ_ATTN(128, false, 8)
   SHARQ_ATTN(128, false, 16)
   SHARQ_ATTN(128, true, 8)

@@ -494,9 +494,17 @@ std::vector<Tensor> rope_append_paged(const Tensor &qkv, int64_t heads, int64_t 
   return out;
 }
 
+// A window as the C ABI takes it.
+int window_of(const std::optional<int64_t> &window, int64_t sinks) {
+  need(!window || *window >= 1, "window must be at least 1, or None");
+  need(sinks >= 0, "sinks must not be negative");
+  return !window ? 0 : (int)std::min<int64_t>(*window, INT32_MAX);
+}
+
 Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &table, const Tensor &lengths,
                        const std::optional<double> &scale, const std::optional<Tensor> &k_scale, const std::optional<Tensor> &v_scale,
-                       const std::optional<Tensor> &out, const Tensor &flag) {
+                       const std::optional<Tensor> &out, const Tensor &flag, const std::optional<int64_t> &window, int64_t sinks) {
+  const int w = window_of(window, sinks), first = (int)std::min<int64_t>(sinks, INT32_MAX);
   need(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.stride(2) == 1,
        "q must be a CUDA bfloat16 tensor shaped [sequences, heads, head_dim] whose heads are contiguous");
   const at::Device dev = q.device();
@@ -514,12 +522,12 @@ Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_c
   if (seqs == 0) return o;
   sharq_paged_cache used = c;
   used.sequences = (int)seqs;
-  const int64_t ws_bytes = (int64_t)sharq_paged_attention_workspace_bytes((int)heads, &used);
+  const int64_t ws_bytes = (int64_t)sharq_paged_attention_windowed_workspace_bytes((int)heads, &used, w, first);
   Tensor ws;
   if (ws_bytes > 0) ws = empty_like_on(q, {ws_bytes}, at::kByte);
-  check(sharq_paged_attention(ptr(q), seqs > 1 ? q.stride(0) : 0, heads > 1 ? q.stride(1) : 0, (int)heads, &used,
-                              static_cast<const int *>(ptr(lengths)), (float)(scale ? *scale : 1.0 / std::sqrt((double)d)), ptr(o), ws_bytes > 0 ? ptr(ws) : nullptr,
-                              (size_t)ws_bytes, flag_of(flag), stream_of(q)));
+  check(sharq_paged_attention_windowed(ptr(q), seqs > 1 ? q.stride(0) : 0, heads > 1 ? q.stride(1) : 0, (int)heads, &used,
+                                       static_cast<const int *>(ptr(lengths)), (float)(scale ? *scale : 1.0 / std::sqrt((double)d)), w, first, ptr(o),
+                                       ws_bytes > 0 ? ptr(ws) : nullptr, (size_t)ws_bytes, flag_of(flag), stream_of(q)));
   return o;
 }
 
@@ -547,13 +555,6 @@ Tensor weight_only_linear(const Tensor &x, const Tensor &qw, const Tensor &sf, c
   check(sharq_weight_only_linear(ptr(x), x.stride(0), (int)m, (int)n, (int)k, ptr(qw), ptr(sf), scale_dev, (float)scale,
                                  bias ? ptr(*bias) : nullptr, ptr(y), flag_of(flag), stream_of(x)));
   return y;
-}
-
-// A window as the C ABI takes it.
-int window_of(const std::optional<int64_t> &window, int64_t sinks) {
-  need(!window || *window >= 1, "window must be at least 1, or None");
-  need(sinks >= 0, "sinks must not be negative");
-  return !window ? 0 : (int)std::min<int64_t>(*window, INT32_MAX);
 }
 
 Tensor prompt_attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &offsets, const std::optional<int64_t> &window,

@@ -233,14 +233,16 @@ def rope_append_paged(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: in
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                     scale: Optional[float] = None, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
-                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    out: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     """Attention of one new token per sequence over a paged cache (see rope_append_paged for its layout): q bf16
     [sequences, heads, head_dim] (heads contiguous, other strides multiples of 8), head_dim 64 or 128, heads a multiple of the cache's
     -> bf16 [sequences, heads, head_dim], the softmax of scale * q . k (default head_dim ** -0.5) over the first lengths[s] (int32) tokens
     of every sequence, the new one among them, applied to the values.  Length 0 gives zeros.  A length beyond the page table or a page
     outside the cache makes that sequence's rows NaN and is reported by check_device_errors.  A sequence may stand in several
-    rows with lengths of their own (drafted tokens).  The same bits from call to call."""
-    return _lib.native().paged_attention(q, k_cache, v_cache, page_table, lengths, scale, k_scale, v_scale, out, _error_flag(q.device))
+    rows with lengths of their own (drafted tokens).  The same bits from call to call.  With window only the last `window` tokens of a sequence and its
+    first `sinks` are seen; pages without any of those are not read, and their entries in the table may be anything."""
+    return _lib.native().paged_attention(q, k_cache, v_cache, page_table, lengths, scale, k_scale, v_scale, out, _error_flag(q.device), window,
+                                         sinks)
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, window: Optional[int] = None, sinks: int = 0,
