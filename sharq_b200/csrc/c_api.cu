@@ -877,15 +877,16 @@ int sharq_prompt_attention(const void *q_bf16, int64_t q_row, int64_t q_head, co
   return check_cuda(sharq::run_prompt_attention(p, as_stream(stream)), "prompt_attention");
 }
 
-int sharq_plan_paged_step(int *page_table, int64_t page_table_stride, int sequences, int max_pages, int page_size, int *lengths,
+int sharq_plan_paged_step(int *page_table, int64_t page_table_stride, int sequences, int max_pages, int page_size, int max_tokens, int *lengths,
                           const int *counts, const unsigned char *released, int *free_pages, int free_pages_size, int *free_count,
                           int rows, int *offsets, int *positions, int *row_sequences, int *error_flag, void *stream) {
   SHARQ_REQUIRE(page_table && lengths && counts && free_count && offsets, "null buffer");
   SHARQ_REQUIRE(sequences > 0 && max_pages > 0 && page_size > 0, "sequences, max_pages and page_size must be positive");
+  SHARQ_REQUIRE(max_tokens >= 0, "max_tokens must not be negative");
   SHARQ_REQUIRE(page_table_stride >= max_pages || sequences == 1, "page_table_stride must cover max_pages");
   SHARQ_REQUIRE(free_pages_size >= 0 && (free_pages_size == 0 || free_pages), "free_pages must have room for free_pages_size pages");
   SHARQ_REQUIRE(rows >= 0 && (rows == 0 || (positions && row_sequences)), "rows must be >= 0, with a place for each");
-  const sharq::StepPlan p = {page_table, page_table_stride, sequences, max_pages, page_size, lengths, counts, released, free_pages,
+  const sharq::StepPlan p = {page_table, page_table_stride, sequences, max_pages, page_size, max_tokens, lengths, counts, released, free_pages,
                              free_pages_size, free_count, rows, offsets, positions, row_sequences, error_flag};
   return check_cuda(sharq::run_step_plan(p, as_stream(stream)), "plan_paged_step");
 }

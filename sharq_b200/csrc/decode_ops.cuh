@@ -52,7 +52,7 @@ cudaError_t run_weight_only(const void *x, long long x_row, int m, int n, int k,
 struct StepPlan {
   int *table;
   long long table_stride;
-  int sequences, max_pages, page_size;
+  int sequences, max_pages, page_size, max_tokens;
   int *lengths;
   const int *counts;
   const unsigned char *released;

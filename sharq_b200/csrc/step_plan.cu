@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kPlanThreadsMost) step_plan_kernel(const __gri
   __shared__ int held_of[kPlanThreadsMost], given_of[kPlanThreadsMost];  // given_of: length ahead of the new tokens, -1: nothing is given
   const int tid = threadIdx.x, threads = blockDim.x;
   const int rank = blockIdx.x, at0 = rank * threads + tid, step = gridDim.x * threads;
-  const long long capacity = (long long)p.max_pages * p.page_size;
+  const long long capacity = (long long)p.max_pages * p.page_size, most = p.max_tokens > 0 ? min(capacity, (long long)p.max_tokens) : capacity;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const int free_given = *p.free_count;
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kPlanThreadsMost) step_plan_kernel(const __gri
       length = p.lengths[i];
       count = p.counts[i];
       if (p.released != nullptr && p.released[i] != 0) length = 0, keeps = false;
-      fits = length >= 0 && count >= 0 && (long long)length + count <= capacity;
+      fits = length >= 0 && count >= 0 && (long long)length + count <= most;
       if (!fits) bad = true;
       count = max(count, 0);
       if (fits) {

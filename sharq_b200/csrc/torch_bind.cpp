@@ -606,7 +606,7 @@ Tensor prompt_attention(const Tensor &q, const Tensor &k, const Tensor &v, const
 // -> offsets [sequences + 1], positions [rows], sequences [rows], views of one allocation
 std::vector<Tensor> plan_paged_step(const Tensor &table, const Tensor &lengths, const Tensor &counts, const Tensor &free_pages,
                                     const Tensor &free_count, int64_t page_size, int64_t rows, const std::optional<Tensor> &released,
-                                    const Tensor &flag) {
+                                    const std::optional<int64_t> &max_tokens, const Tensor &flag) {
   need(table.is_cuda() && table.scalar_type() == at::kInt && table.dim() == 2 && table.numel() > 0 && (table.size(1) <= 1 || table.stride(1) == 1),
        "page_table must be a CUDA int32 matrix [sequences, pages] with unit column stride");
   const at::Device dev = table.device();
@@ -620,6 +620,7 @@ std::vector<Tensor> plan_paged_step(const Tensor &table, const Tensor &lengths, 
   check_indices(free_count, 1, dev, "free_count");
   need(page_size > 0 && page_size <= INT32_MAX, "page_size must be positive");
   need(rows >= 0 && rows <= INT32_MAX, "rows must be in [0, 2^31)");
+  need(!max_tokens || *max_tokens > 0, "max_tokens must be positive, or None");
   if (released)
     need((is_plain(*released, at::kBool) || is_plain(*released, at::kByte)) && released->device() == dev && released->dim() == 1 && released->size(0) == n,
          "released must be a contiguous CUDA bool vector with one entry per sequence");
@@ -627,7 +628,7 @@ std::vector<Tensor> plan_paged_step(const Tensor &table, const Tensor &lengths, 
   Tensor out = empty_like_on(table, {n + 1 + 2 * rows}, at::kInt);
   int *at = static_cast<int *>(ptr(out));
   check(sharq_plan_paged_step(static_cast<int *>(ptr(table)), n > 1 ? table.stride(0) : table.size(1), (int)n, (int)table.size(1), (int)page_size,
-                              static_cast<int *>(ptr(lengths)), static_cast<const int *>(ptr(counts)),
+                              max_tokens ? (int)std::min<int64_t>(*max_tokens, INT32_MAX) : 0, static_cast<int *>(ptr(lengths)), static_cast<const int *>(ptr(counts)),
                               released ? static_cast<const unsigned char *>(ptr(*released)) : nullptr, static_cast<int *>(ptr(free_pages)),
                               (int)free_pages.size(0), static_cast<int *>(ptr(free_count)), (int)rows, at, at + n + 1, at + n + 1 + rows,
                               flag_of(flag), stream_of(table)));

@@ -15,6 +15,8 @@ decoder with the same call pattern on the quantized path:
   (one kernel, ops.rope_inplace_) and SwiGLU is fused with the prepare of down_proj
   (prepare_input_swiglu); both give the bits of the ATen compositions they replace, which
   `fused_glue=False` still runs
+* with DecoderConfig.window a token sees the last tokens and the first ones only (ops.prompt_attention for prompts, ops.paged_attention
+  with a window for decode steps)
 * with a paged cache (SharqDecoder.new_cache) the rotary embedding also appends keys and values to it
   (ops.rope_append_paged, one rounding per element), and decode() runs one token per sequence through the
   layers, with attention over the cache (ops.paged_attention)
@@ -33,6 +35,7 @@ import torch.nn.functional as F
 
 from . import ops
 from .kv_cache import LayerCache, PagedKVCache
+from .logit_rules import LogitRules
 from .qlinear import QLinearLayer, methods_kept
 from .tp import RowParallelSharqLinear, head_layout, padded_size, shard_bounds
 
@@ -51,6 +54,8 @@ class DecoderConfig:
     qkv_bias: bool = False
     experts: int = 0  # > 0: sparse mixture-of-experts FFN (Mixtral): `experts` FFNs, `top_k` per token
     top_k: int = 2
+    window: int = 0   # > 0: a token sees the last `window` tokens, itself among them, and the first `sinks`
+    sinks: int = 0
 
     @staticmethod
     def llama3_8b(**kw):
@@ -222,7 +227,7 @@ class SharqDecoderLayer(torch.nn.Module):
                 x2 = x2 + delta.reshape(b * s, h)
             prep = self.qkv.prepare_input_rmsnorm(x2, self.input_norm, cfg.eps)
         qkv = self.qkv.apply_prepared(prep)
-        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, self.fused_glue, kv)
+        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, self.fused_glue, kv, cfg.window, cfg.sinks)
         o = self.o_proj(attn2)
         if cfg.experts > 0:
             if self.fused_glue and h <= 8192:
@@ -267,7 +272,7 @@ class SharqDecoderLayer(torch.nn.Module):
         x2 = x.reshape(b * s, h)
         hn, x2 = _add_norm(x2, None if delta is None else delta.reshape(b * s, h), self.input_norm, cfg.eps)
         qkv = self.qkv.forward_weight_only(hn)
-        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, self.fused_glue, kv)
+        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, self.fused_glue, kv, cfg.window, cfg.sinks)
         o = self.o_proj.reduce(self.o_proj.local.forward_weight_only(attn2))
         hn, x2 = _add_norm(x2, o, self.post_norm, cfg.eps)
         if cfg.experts > 0:
@@ -289,7 +294,7 @@ class SharqDecoderLayer(torch.nn.Module):
         residual, prepares the local rows (RMSNorm fused) and all-gathers the packed activation.  -> (prepared input of the next layer's qkv, x_local)."""
         cfg = self.cfg
         qkv = self.qkv.apply_prepared(prepared)
-        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, True, kv)
+        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, True, kv, cfg.window, cfg.sinks)
         self.o_proj.local.apply_prepared(self.o_proj.local.prepare_input(attn2), scatter=sp.scatter)
         prepared, x_local = sp.transition(x_local, self.post_norm, cfg.eps)
         self.down.local.apply_prepared(_prepare_down(self.gate_up, prepared, self.down.local), scatter=sp.scatter)
@@ -409,7 +414,7 @@ class SharqDecoderLayer(torch.nn.Module):
         else:
             nv = self.nv
             qkv = nv["qkv"].apply_prepared(nv["qkv"].prepare_input_rmsnorm(x2, self.input_norm, cfg.eps))
-        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, self.fused_glue, kv)
+        attn2 = _attention(qkv, b, s, self.local_heads, self.local_kv, cfg.head_dim, cos, sin, self.fused_glue, kv, cfg.window, cfg.sinks)
         if self.mode == "BF16":
             o = row_parallel(lambda out: torch.mm(attn2, r["o"].T, out=out) if out is not None else attn2 @ r["o"].T, h)
         else:
@@ -432,7 +437,7 @@ class SharqDecoderLayer(torch.nn.Module):
         b, s, h = x.shape
         x2 = x.reshape(b * s, h)
         qkv = nv["qkv"].apply_prepared(nv["qkv"].prepare_input_rmsnorm(x2, self.input_norm, cfg.eps))
-        x2 = x2 + nv["o"](_attention(qkv, b, s, cfg.heads, cfg.kv_heads, cfg.head_dim, cos, sin, self.fused_glue, kv))
+        x2 = x2 + nv["o"](_attention(qkv, b, s, cfg.heads, cfg.kv_heads, cfg.head_dim, cos, sin, self.fused_glue, kv, cfg.window, cfg.sinks))
         gu = nv["gate_up"].apply_prepared(nv["gate_up"].prepare_input_rmsnorm(x2, self.post_norm, cfg.eps))
         x2 = x2 + nv["down"](_swiglu(gu, self.fused_glue))
         return x2.view(b, s, h)
@@ -450,7 +455,7 @@ class SharqDecoderLayer(torch.nn.Module):
         x2 = x.reshape(b * s, h)
         qkv = F.linear(norm(x2, self.input_norm), r["qkv"], r["qkv_bias"])
         glue = "gate_up" in r  # BF16 comparison mode; the accuracy reference of a SharQ layer stays pure ATen
-        x2 = x2 + F.linear(_attention(qkv, b, s, cfg.heads, cfg.kv_heads, cfg.head_dim, cos, sin, glue, kv), r["o"])
+        x2 = x2 + F.linear(_attention(qkv, b, s, cfg.heads, cfg.kv_heads, cfg.head_dim, cos, sin, glue, kv, cfg.window, cfg.sinks), r["o"])
         y = norm(x2, self.post_norm)
         if cfg.experts > 0:
             routing, selected = _route(y, self.router, cfg.top_k)
@@ -536,19 +541,30 @@ def _split_heads(qkv: torch.Tensor, b: int, s: int, heads: int, kv_heads: int, d
 
 
 def _attention(qkv: torch.Tensor, b: int, s: int, heads: int, kv_heads: int, d: int, cos: torch.Tensor, sin: torch.Tensor, fused: bool,
-               kv: LayerCache = None) -> torch.Tensor:
+               kv: LayerCache = None, window: int = 0, sinks: int = 0) -> torch.Tensor:
     """Attention of a merged qkv activation [b*s, (heads + 2*kv_heads)*d] -> [b*s, heads*d]: causal over the s tokens, which with kv are
-    also appended to the cache, or, with kv.lengths, of one token per sequence over the cache."""
+    also appended to the cache, or, with kv.lengths, of one token per sequence over the cache.  window > 0: the last `window` tokens and the
+    first `sinks` are seen."""
     if kv is None:
         q, k, v = _split_heads(qkv, b, s, heads, kv_heads, d, cos, sin, fused)
     else:
         got = ops.rope_append_paged(qkv, heads, kv_heads, d, kv.cos, kv.sin, kv.positions, kv.table, kv.k, kv.v, sequences=kv.sequences,
                                     k_scale=kv.k_scale, v_scale=kv.v_scale, return_k=kv.lengths is None)
         if kv.lengths is not None:
-            return ops.paged_attention(got, kv.k, kv.v, kv.table, kv.lengths, k_scale=kv.k_scale, v_scale=kv.v_scale).view(b * s, heads * d)
+            return ops.paged_attention(got, kv.k, kv.v, kv.table, kv.lengths, k_scale=kv.k_scale, v_scale=kv.v_scale, window=window or None,
+                                       sinks=sinks).view(b * s, heads * d)
         q, k = (x.view(b, s, -1, d).transpose(1, 2) for x in got)
         v = qkv[:, (heads + kv_heads) * d:].view(b, s, kv_heads, d).transpose(1, 2)
-    attn = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
+    if window > 0 and fused and qkv.is_cuda:
+        offsets = torch.arange(0, b * s + 1, s, dtype=torch.int32, device=qkv.device)
+        q, k, v = (x.transpose(1, 2).flatten(0, 1) for x in (q, k, v))  # views: rows one behind the other
+        return ops.prompt_attention(q, k, v, offsets, window=window, sinks=sinks).view(b * s, heads * d)
+    seen = None
+    if window > 0:
+        at = torch.arange(s, device=qkv.device)
+        far = at[:, None] - at
+        seen = (far >= 0) & ((far < window) | (at < sinks))
+    attn = F.scaled_dot_product_attention(q, k, v, attn_mask=seen, is_causal=seen is None, enable_gqa=True)
     return attn.transpose(1, 2).reshape(b * s, heads * d)
 
 
@@ -617,23 +633,30 @@ class SharqDecoder(torch.nn.Module):
 
     @torch.no_grad()
     def prefill(self, token_ids: torch.Tensor, reference: bool = False, cache: PagedKVCache = None,
-                sequences: Sequence[int] = None) -> torch.Tensor:
-        """token_ids [B, S] -> logits of the last position [B, vocab] (float32).
+                sequences: Sequence[int] = None, rules: LogitRules = None) -> torch.Tensor:
+        """token_ids [B, S] -> logits of the last position [B, vocab] (float32), with rules as they change them.
         reference=True runs the unquantised bf16 layers (needs keep_reference=True).  cache: holds the prompts afterwards (decode), as its
-        sequences, which are B and empty, or as those listed in sequences, which are B and empty, whatever the others hold."""
+        sequences, which are B and empty, or as those listed in sequences, which are B and empty, whatever the others hold.  In a cache that hands
+        its pages out on the device a prompt takes the place of what its sequence held, and a sequence for which the pages do not suffice stays empty."""
         b, s = token_ids.shape
         kvs = [None] * len(self.layers)
         if cache is None and sequences is not None:
             raise ValueError("sequences are those of a cache")
         if cache is not None:
             which = cache.chosen(sequences)
-            if b != len(which) or any(cache.lengths[i] for i in which):
+            if cache.on_device:
+                if b != len(which) or s > cache.max_tokens:
+                    raise ValueError("prefill takes a sequence of the cache for every prompt, of at most max_tokens")
+                positions, rows = cache.step_places(which, s, restart=True)
+                kvs = [cache.layer(i, positions, rows, None) for i in range(len(self.layers))]
+            elif b != len(which) or any(cache.lengths[i] for i in which):
                 raise ValueError("prefill takes an empty cache with a sequence for every prompt" if sequences is None else
                                  "prefill takes one empty sequence of the cache for every prompt")
-            counts = cache.counts(which, s)
-            cache.reserve(counts)
-            positions, rows = cache.prompt_step(s, sequences)
-            kvs = [cache.layer(i, positions, rows, None) for i in range(len(self.layers))]
+            else:
+                counts = cache.counts(which, s)
+                cache.reserve(counts)
+                positions, rows = cache.prompt_step(s, sequences)
+                kvs = [cache.layer(i, positions, rows, None) for i in range(len(self.layers))]
         cos, sin = rope_tables(s, self.cfg.head_dim, self.cfg.rope_theta, self.embed.device)
         sp = None if reference else self._sequence_parallel_context(b * s)
         if sp is not None:
@@ -663,41 +686,47 @@ class SharqDecoder(torch.nn.Module):
             if delta is not None:
                 x = x + delta
             last = x[:, -1, :].float()
-        if cache is not None:
+        if cache is not None and not cache.on_device:
             cache.advance(counts)
-        return self._logits(last)
+        return self._logits(last, rules)
 
     def new_cache(self, sequences: int, max_tokens: int, page_size: int = 64, pages: int = None, dtype: torch.dtype = torch.bfloat16,
-                  k_scale: torch.Tensor = None, v_scale: torch.Tensor = None) -> PagedKVCache:
+                  k_scale: torch.Tensor = None, v_scale: torch.Tensor = None, on_device: bool = False) -> PagedKVCache:
         """A paged cache for this model's (this rank's) key/value heads, see PagedKVCache.  Heads of 64 or 128, which ops.paged_attention takes."""
         if self.cfg.head_dim not in (64, 128):
             raise ValueError(f"decode steps take heads of 64 or 128, not {self.cfg.head_dim}")
         cos, sin = rope_tables(max_tokens, self.cfg.head_dim, self.cfg.rope_theta, self.embed.device, torch.float64)  # as long as a cache may be
         return PagedKVCache(len(self.layers), self.layers[0].local_kv, self.cfg.head_dim, sequences, max_tokens, cos, sin, page_size, pages,
-                            dtype, k_scale, v_scale)
+                            dtype, k_scale, v_scale, on_device)
 
     @torch.no_grad()
     def decode(self, token_ids: torch.Tensor, cache: PagedKVCache, reference: bool = False, weight_only: bool = False,
-               sequences: Sequence[int] = None) -> torch.Tensor:
+               sequences: Sequence[int] = None, rules: LogitRules = None) -> torch.Tensor:
         """One more token of every sequence of the cache (an empty one begins with it), or of those listed in sequences, in that order:
-        token_ids [B] -> logits of the next one [B, vocab] (float32).  weight_only: the linears take the activations unquantised (at most 16 sequences).  reference: as in prefill."""
+        token_ids [B] -> logits of the next one [B, vocab] (float32).  weight_only: the linears take the activations unquantised (at most 16 sequences).  reference: as in prefill.  rules: change the logits; their rows are
+        those of token_ids.  With a cache that hands its pages out on the device, and all its sequences, the call can be captured in a CUDA graph whose replays go
+        on from token to token; a sequence for which the pages do not suffice keeps its length, and one that has max_tokens, which is reported."""
         which = cache.chosen(sequences)
         b = int(token_ids.shape[0])
         if token_ids.dim() != 1 or b != len(which):
             raise ValueError("decode takes one token for every sequence of the cache" + ("" if sequences is None else " that is listed"))
         if weight_only and b > 16:
             raise ValueError(f"weight_only takes at most 16 sequences, got {b}")
+        if cache.on_device:
+            positions, rows = cache.step_places(which, 1)
+            return self.decode_step(token_ids, cache, positions, positions + 1, reference, weight_only, None if sequences is None else rows.long(),
+                                    rules)
         counts = cache.counts(which, 1)
         cache.reserve(counts)
         rows = None if sequences is None else torch.tensor(which, device=cache.table.device)
         positions = cache.device_lengths if rows is None else cache.device_lengths[rows]
-        logits = self.decode_step(token_ids, cache, positions, positions + 1, reference, weight_only, rows)
+        logits = self.decode_step(token_ids, cache, positions, positions + 1, reference, weight_only, rows, rules)
         cache.advance(counts)
         return logits
 
     @torch.no_grad()
     def decode_step(self, token_ids: torch.Tensor, cache: PagedKVCache, positions: torch.Tensor, lengths: torch.Tensor,
-                    reference: bool = False, weight_only: bool = False, rows: torch.Tensor = None) -> torch.Tensor:
+                    reference: bool = False, weight_only: bool = False, rows: torch.Tensor = None, rules: LogitRules = None) -> torch.Tensor:
         """The device part of decode, for capture in a CUDA graph: positions and lengths (int32 [B], device) of the new tokens and of the
         sequences with them, whose pages have been reserved; the cache's own lengths stay.  rows (int64 [B], device, different): the sequences
         of the cache that the tokens belong to, default all of them in order.  A graph reads the page table as wide as it was
@@ -712,9 +741,10 @@ class SharqDecoder(torch.nn.Module):
                 x, delta = layer(x, kv.cos, kv.sin, delta=delta, return_delta=True, kv=kv, weight_only=weight_only)
         if delta is not None:
             x = x + delta
-        return self._logits(x[:, -1, :].float())
+        return self._logits(x[:, -1, :].float(), rules)
 
-    def _logits(self, last: torch.Tensor) -> torch.Tensor:
-        """Final norm and lm_head of hidden states [B, hidden] (float32)."""
+    def _logits(self, last: torch.Tensor, rules: LogitRules = None) -> torch.Tensor:
+        """Final norm and lm_head of hidden states [B, hidden] (float32), and what the rules make of the logits."""
         last = last * torch.rsqrt(last.pow(2).mean(-1, keepdim=True) + self.cfg.eps) * self.final_norm.float()
-        return (last.to(torch.bfloat16) @ self.lm_head.T).float()
+        logits = (last.to(torch.bfloat16) @ self.lm_head.T).float()
+        return logits if rules is None else rules.apply_(logits)

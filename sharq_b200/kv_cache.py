@@ -2,7 +2,8 @@
 
 The reference leaves the cache to HuggingFace's layers (model/qLlamaLayer.py:143-160).  Pages of `page_size` tokens are handed out as
 sequences grow, so a batch of short and long sequences takes the memory of its tokens; a cache of torch.float8_e4m3fn values takes half of it.
-The page numbers and lengths are kept on the host, where pages are handed out, and on the device, where the kernels read them.
+The page numbers and lengths are kept on the host, where pages are handed out, and on the device, where the kernels read them.  With on_device they
+are handed out there too (ops.plan_paged_step), and the host knows none of them: a captured decode step then grows its sequences by itself.
 """
 from __future__ import annotations
 
@@ -10,6 +11,8 @@ from dataclasses import dataclass
 from typing import Optional, Sequence
 
 import torch
+
+from . import ops
 
 
 @dataclass
@@ -30,9 +33,10 @@ class LayerCache:
 class PagedKVCache:
     def __init__(self, layers: int, kv_heads: int, head_dim: int, sequences: int, max_tokens: int, cos: torch.Tensor, sin: torch.Tensor,
                  page_size: int = 64, pages: Optional[int] = None, dtype: torch.dtype = torch.bfloat16,
-                 k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
+                 k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None, on_device: bool = False):
         """Room for `sequences` sequences of up to max_tokens tokens in `pages` pages (default: enough for all of them).  cos, sin:
-        rotary tables [>= max_tokens, head_dim].  k_scale, v_scale: float32 [layers, kv_heads] of a float8_e4m3fn cache, default 1."""
+        rotary tables [>= max_tokens, head_dim].  k_scale, v_scale: float32 [layers, kv_heads] of a float8_e4m3fn cache, default 1.
+        on_device: pages are handed out by plan(), not by reserve() and advance()."""
         if min(layers, kv_heads, head_dim, sequences, max_tokens, page_size) < 1:
             raise ValueError("sizes of the cache must be positive")
         if cos.shape[0] < max_tokens or cos.shape != sin.shape or cos.shape[1] != head_dim:
@@ -41,7 +45,7 @@ class PagedKVCache:
             raise ValueError(f"a cache holds torch.bfloat16 or torch.float8_e4m3fn, not {dtype}")
         if dtype == torch.bfloat16 and (k_scale is not None or v_scale is not None):
             raise ValueError("k_scale and v_scale belong to a torch.float8_e4m3fn cache")
-        self.max_tokens, self.page_size, self.sequences = max_tokens, page_size, sequences
+        self.max_tokens, self.page_size, self.sequences, self.on_device = max_tokens, page_size, sequences, on_device
         most = -(-max_tokens // page_size)
         pages = sequences * most if pages is None else pages
         device = cos.device
@@ -59,10 +63,41 @@ class PagedKVCache:
         self.device_lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
         self._held: list[list[int]] = [[] for _ in range(sequences)]
         self._free = list(range(pages - 1, -1, -1))
+        if on_device:
+            self.lengths = None
+            self.free_pages = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=device)
+            self.free_count = torch.full((1,), pages, dtype=torch.int32, device=device)
+
+    def plan(self, counts: torch.Tensor, rows: int, released: Optional[torch.Tensor] = None):
+        """counts[i] (int32, on the device) more tokens for every sequence i, which with released (bool) gives back what it holds first ->
+        (offsets, positions, sequences) of the `rows` rows of the step, see ops.plan_paged_step."""
+        if not self.on_device:
+            raise RuntimeError("the pages of this cache are handed out on the host: reserve() and advance()")
+        return ops.plan_paged_step(self.table, self.device_lengths, counts, self.free_pages, self.free_count, self.page_size, rows, released,
+                                   self.max_tokens)
+
+    def step_places(self, which: Sequence[int], tokens: int, restart: bool = False):
+        """plan() of `tokens` new tokens of every sequence in `which` -> (positions, sequences), int32, in the order of `which`.  restart: they begin anew."""
+        device, everyone = self.table.device, list(which) == list(range(self.sequences))
+        if everyone:
+            chosen = torch.ones(self.sequences, dtype=torch.int32, device=device)
+        else:
+            at = torch.tensor(list(which), device=device)
+            chosen = torch.zeros(self.sequences, dtype=torch.int32, device=device).index_fill_(0, at, 1)
+        offsets, positions, sequences = self.plan(chosen * tokens, len(which) * tokens, chosen.bool() if restart else None)
+        if list(which) != sorted(which):
+            row = (offsets[at][:, None] + torch.arange(tokens, device=device)).reshape(-1)
+            positions, sequences = positions[row], sequences[row]
+        return positions, sequences
+
+    def _by_host(self) -> None:
+        if self.on_device:
+            raise RuntimeError("the pages of this cache are handed out on the device: plan()")
 
     def reserve(self, counts: Sequence[int]) -> None:
         """Pages for counts[i] more tokens of sequence i.  Raises RuntimeError, and changes nothing, where a sequence would pass
         max_tokens or the pages do not suffice."""
+        self._by_host()
         if len(counts) != self.sequences or min(counts) < 0:
             raise ValueError("one count of tokens per sequence")
         want = [n + more for n, more in zip(self.lengths, counts)]
@@ -80,6 +115,7 @@ class PagedKVCache:
 
     def advance(self, counts: Sequence[int]) -> None:
         """The tokens that were reserved and appended now belong to their sequences."""
+        self._by_host()
         if len(counts) != self.sequences or any(n + more > len(held) * self.page_size for n, more, held in zip(self.lengths, counts, self._held)):
             raise ValueError("tokens must be reserved before they are counted")
         self.lengths = [n + more for n, more in zip(self.lengths, counts)]
@@ -90,6 +126,10 @@ class PagedKVCache:
 
     def free(self, sequence: int) -> None:
         """Gives the pages of a sequence back; it is empty then, and another prompt may take its place (SharqDecoder.prefill with sequences)."""
+        if self.on_device:
+            ended = torch.zeros(self.sequences, dtype=torch.int32, device=self.table.device).index_fill_(0, torch.tensor([sequence], device=self.table.device), 1)
+            self.plan(torch.zeros_like(ended), 0, ended.bool())
+            return
         self._free += reversed(self._held[sequence])
         self._held[sequence] = []
         self.lengths[sequence] = 0
@@ -109,6 +149,7 @@ class PagedKVCache:
 
     def prompt_step(self, tokens: int, sequences: Optional[Sequence[int]] = None):
         """(positions, sequences) int32 of `tokens` new tokens of every sequence, or of those listed, sequence after sequence."""
+        self._by_host()
         device = self.table.device
         first, which = self.device_lengths, torch.arange(self.sequences, dtype=torch.int32, device=device)
         if sequences is not None:
@@ -118,9 +159,9 @@ class PagedKVCache:
         return positions, which.repeat_interleave(tokens)
 
     def held_table(self, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """The page table cut to what the longest sequence holds, of all sequences or of those in rows (int64, device).  A row of no
+        """The page table cut to what the longest sequence holds, as far as the host knows, of all sequences or of those in rows (int64, device).  A row of no
         sequence has no pages, which the kernels report."""
-        table = self.table[:, :max(1, max(len(h) for h in self._held))]
+        table = self.table if self.on_device else self.table[:, :max(1, max(len(h) for h in self._held))]
         if rows is None:
             return table
         there = (rows >= 0) & (rows < self.sequences)

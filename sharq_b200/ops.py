@@ -259,14 +259,14 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
 
 def plan_paged_step(page_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
-                    page_size: int, rows: int, released: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                    page_size: int, rows: int, released: Optional[torch.Tensor] = None, max_tokens: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Pages and places of a step's tokens, handed out on the device in one launch: sequence i, which holds lengths[i] tokens in the pages of its row
     of page_table [sequences, pages], gets counts[i] more -> (offsets [sequences + 1], positions [rows], sequences [rows]), the places that
     rope_append_paged takes, sequence after sequence.  All int32.  page_table, lengths, free_pages (a stack, of which the first
     free_count[0] are free) and free_count [1] change in place.  Sequences with released (bool) give their pages back first and are empty.  Where the
     pages do not suffice for a sequence and those ahead of it, it gets nothing: its length stays and its rows have position -1, as rows behind the
-    last have.  A length, count, sum of counts above `rows` or free_count that cannot be is reported by check_device_errors, and its sequences get nothing."""
-    return _lib.native().plan_paged_step(page_table, lengths, counts, free_pages, free_count, page_size, rows, released,
+    last have.  No sequence grows beyond max_tokens, or what its row of page_table holds.  A length, count, sum of counts above `rows` or free_count that cannot be is reported by check_device_errors, and its sequences get nothing."""
+    return _lib.native().plan_paged_step(page_table, lengths, counts, free_pages, free_count, page_size, rows, released, max_tokens,
                                          _error_flag(page_table.device))
 
 

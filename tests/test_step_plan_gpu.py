@@ -9,7 +9,7 @@ from sharq_b200 import ops
 pytestmark = pytest.mark.gpu
 
 
-def walk(table, lengths, counts, stack, free, page, rows, released):
+def walk(table, lengths, counts, stack, free, page, rows, released, max_tokens=None):
     """The step on lists, sequence by sequence -> (offsets, positions, sequences, bad); the lists change as the operator's tensors do."""
     most = len(table[0])
     bad = not 0 <= free[0] <= len(stack)
@@ -29,7 +29,7 @@ def walk(table, lengths, counts, stack, free, page, rows, released):
             lengths[i] = 0
     offsets, positions, sequences, short, total = [0], [], [], False, 0
     for i, count in enumerate(counts):
-        fits = lengths[i] >= 0 and count >= 0 and lengths[i] + count <= most * page
+        fits = lengths[i] >= 0 and count >= 0 and lengths[i] + count <= min(most * page, max_tokens or most * page)
         n = max(count, 0)
         total += n
         need = -(-(lengths[i] + count) // page) - -(-lengths[i] // page) if fits else 0
@@ -67,7 +67,7 @@ class Server:
         self.stack = order[at:] + [-9] * (at + room)
         self.free = [spare]
 
-    def step(self, counts, rows, released=None, stride=0):
+    def step(self, counts, rows, released=None, stride=0, max_tokens=None):
         """One step by the operator and by the walk: both have to agree in everything -> (offsets, positions, sequences)."""
         dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
         wide = torch.full((len(self.table), len(self.table[0]) + stride), -3, dtype=torch.int32, device="cuda")
@@ -75,8 +75,9 @@ class Server:
         table.copy_(dev(self.table))
         lengths, stack, free = dev(self.lengths), dev(self.stack), dev(self.free)
         flags = None if released is None else torch.tensor(released, dtype=torch.bool, device="cuda")
-        got = ops.plan_paged_step(table, lengths, dev(counts), stack, free, self.page, rows, released=flags)
-        *want, bad = walk(self.table, self.lengths, list(counts), self.stack, self.free, self.page, rows, released or [False] * len(counts))
+        got = ops.plan_paged_step(table, lengths, dev(counts), stack, free, self.page, rows, released=flags, max_tokens=max_tokens)
+        *want, bad = walk(self.table, self.lengths, list(counts), self.stack, self.free, self.page, rows, released or [False] * len(counts),
+                          max_tokens)
         for g, w in zip(got, want):
             assert g.tolist() == w
         assert table.tolist() == self.table and lengths.tolist() == self.lengths
@@ -140,6 +141,9 @@ def test_what_cannot_be_is_reported(seqs):
         server = Server(good, 16, 9, 3 * seqs, 9)
         server.free = [free]
         server.step([13] * seqs, 13 * seqs, [i % 2 == 0 for i in range(seqs)])
+    server = Server(good, 16, 9, 3 * seqs, 9)
+    server.step([1] * (seqs - 1) + [2], seqs + 1, max_tokens=21)
+    server.step([1] * seqs, seqs, [True] * (seqs // 2) + [False] * (seqs - seqs // 2), max_tokens=1)
     # fewer rows than tokens
     server = Server(good, 16, 9, 3 * seqs, 10)
     server.step([2] * seqs, 2 * seqs - 3)
@@ -186,7 +190,7 @@ def test_refusals():
     for name, value in [("page_table", dev(3, 4).long()), ("page_table", dev(4, 3).T), ("page_table", dev(3)), ("page_table", dev(3, 0)), ("lengths", dev(2)),
                         ("page_table", dev(1, 4).expand(3, 4)), ("lengths", dev(3).long()), ("lengths", dev(6)[::2]), ("counts", dev(3).cpu()),
                         ("free_pages", dev(9).long()), ("free_pages", dev(3, 3)), ("free_count", dev(2)), ("page_size", 0), ("page_size", -4),
-                        ("rows", -1), ("rows", 2 ** 31), ("released", dev(3)), ("released", torch.zeros(2, dtype=torch.bool, device="cuda"))]:
+                        ("rows", -1), ("max_tokens", 0), ("max_tokens", -1), ("rows", 2 ** 31), ("released", dev(3)), ("released", torch.zeros(2, dtype=torch.bool, device="cuda"))]:
         with pytest.raises(RuntimeError):
             ops.plan_paged_step(**{**good, name: value})
     with pytest.raises(RuntimeError, match="CUDA"):
