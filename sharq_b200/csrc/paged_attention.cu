@@ -479,8 +479,8 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
     for (int n = 0; n < kN; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
 
     const Gap gap = gap_of<kTokens, kWindow>(a, at.tokens);
-    for (int index = at.tile; index < at.end; ++index) {
-      const int tile = kWindow && index >= gap.front ? index + gap.skip : index;
+    for (int tile = at.tile; tile < at.end; ++tile) {
+      const int first_token = (kWindow && tile >= gap.front ? tile + gap.skip : tile) * kTokens;
       load();
       const uint32_t keys = ring + take * T::kStage, values = keys + T::kBytes;
       const bool poison = (bad_stages >> take) & 1;
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
       }
       __syncwarp();
       phases ^= 1u << take;
-      const int live = at.tokens - tile * kTokens;  // tokens from this tile on
+      const int live = at.tokens - first_token;  // tokens from this tile on
 
       float s[kTokens / 16][kN][4], s2[kTokens / 16][kN][4];  // [token][column], in two sums: a product waits for the one before it
 #pragma unroll
@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Layout<D, kFp8, kCols, kForm>::
 #pragma unroll
           for (int j = 0; j < 4; ++j) s[b][n][j] = (s[b][n][j] + s2[b][n][j]) * sl[n][j & 1];
       // rows of the tile that are not seen though they lie ahead of the last token
-      const int hide0 = kWindow ? min(kTokens, max(0, a.sinks - tile * kTokens)) : 0, hide1 = kWindow ? min(kTokens, max(0, gap.begin - tile * kTokens)) : 0;
+      const int hide0 = kWindow ? min(kTokens, max(0, a.sinks - first_token)) : 0, hide1 = kWindow ? min(kTokens, max(0, gap.begin - first_token)) : 0;
       if (live < kTokens || poison || (kWindow && hide0 < hide1)) {
 #pragma unroll
         for (int b = 0; b < kTokens / 16; ++b)
