@@ -1,11 +1,14 @@
-// Penalties for repeated tokens, biases and masks on logits, in one launch.  256 rows of 152064 with histories of up to 6000 tokens: 137 us, 2.3 TB/s; one
+// Penalties for repeated tokens, biases and masks on logits, in one launch.  256 rows of 152064 with histories of up to 6000 tokens: 78.6 us, 4.1 TB/s; one
 // row of 128256: 6.0 us.
 //
 //   x' = x > 0 ? x / r : x r   (tokens of the history),   x' - f n - p [n > 0]   (n: how often the answer so far has the token),   + biases,   -inf where masked
 //
 // Bound by reading and writing the logits once.  What touches a logit is known by token, not by place, so a CTA takes a slice of a row, counts the
 // history's tokens that fall into it in a table in shared memory (whole numbers: the order of the atomics does not matter), and passes over its slice once.  A
-// history is read by every CTA of its row, from L2, which is what a wider slice saves.
+// history is read by every CTA of its row, from L2, which is what a wider slice saves; what it concerns becomes a list, so that the few logits that take
+// arithmetic are dealt out evenly, and goes over what the pass has written.  The logits are on their way while the tokens are counted.  (With the arithmetic in the
+// pass, where a warp waits for its few lanes, 182 us; slices of half the width in CTAs of half the size 86; the list's and the biases' logits fetched ahead
+// of the pass 92; the first tokens ahead of the logits 99; the pass alone 47.5, as a copy.)
 //
 // A penalty or a bias may leave little of a logit, so what they touch is computed in double and rounded once; that is a token in hundreds.
 #include <cuda_bf16.h>
@@ -21,7 +24,7 @@ namespace sharq {
 
 namespace {
 
-constexpr unsigned kSeen = 1u << 31, kBiased = 1u << 30, kTwice = 1u << 29, kCount = kTwice - 1;  // of a token's word; the rest counts
+constexpr unsigned kSeen = 1u << 31, kCount = kSeen - 1;  // of a token's word; the rest counts
 
 __device__ __forceinline__ float minus_inf() { return __int_as_float(0xff800000); }
 
@@ -50,11 +53,18 @@ __device__ __forceinline__ double widened(T x) {
     return (double)__bfloat162float(x);
 }
 
+constexpr int kThreads = 512, kSliceMost = 16384;
+
 // T: type of the logits; Id: of the history's tokens; kVec: logits of a 16-byte access, or 1
 template <typename T, typename Id, int kVec>
-__global__ void __launch_bounds__(512) logit_rules_kernel(const __grid_constant__ LogitRules a) {
+__global__ void __launch_bounds__(kThreads, 2) logit_rules_kernel(const __grid_constant__ LogitRules a) {
+  constexpr int kPer = kSliceMost / (kThreads * kVec);  // accesses of a thread
+  // for every token of the slice how often the history has it, and two bits: it has a bias, it has several; then the history's tokens, each once, in any order
   extern __shared__ __align__(16) unsigned words[];
-  const int row = blockIdx.y, tid = threadIdx.x, threads = blockDim.x;
+  __shared__ int listed;
+  unsigned *biased = words + a.slice, *twice = biased + a.slice / 32, *kept = twice + a.slice / 32;  // kept: the mask
+  unsigned short *list = reinterpret_cast<unsigned short *>(kept + a.slice / 32);
+  const int row = blockIdx.y, tid = threadIdx.x;
   const int first = blockIdx.x * a.slice, size = min(a.slice, a.vocab - first);
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
@@ -72,99 +82,114 @@ __global__ void __launch_bounds__(512) logit_rules_kernel(const __grid_constant_
     bias1 = a.bias_offsets[row + 1];
     if (bias0 < 0 || bias1 < bias0 || bias1 > a.biases) bad = true, bias0 = bias1 = 0;
   }
-  const Penalty penalty = {a.repetition == nullptr ? 1.0 : (double)a.repetition[row], a.presence == nullptr ? 0.0 : (double)a.presence[row],
-                           a.frequency == nullptr ? 0.0 : (double)a.frequency[row]};
-  const bool marked = length > 0 || bias1 > bias0;  // the table is in use
-  if (marked) {
-    for (int i = tid * 4; i < a.slice; i += threads * 4) *reinterpret_cast<uint4 *>(words + i) = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    const Id *tokens = static_cast<const Id *>(a.tokens) + row * a.tokens_stride;
-#pragma unroll 4
-    for (int j = tid; j < length; j += threads) {
-      const Id id = tokens[j];
-      const long long at = (long long)id - first;
-      if (at >= 0 && at < size) {
-        if (j < prompt)
-          atomicOr(words + at, kSeen);
-        else
-          atomicAdd(words + at, 1u);
-      } else if ((long long)id >= a.vocab) {
-        bad = true;
-      }
-    }
-    for (int j = bias0 + tid; j < bias1; j += threads) {
-      const long long at = (long long)a.bias_ids[j] - first;
-      if (at >= 0 && at < size) {
-        if (atomicOr(words + at, kBiased) & kBiased) atomicOr(words + at, kTwice);
-      } else if (at + first < 0 || at + first >= a.vocab) {
-        bad = true;
-      }
-    }
-    __syncthreads();
-  }
-
   const T *in = static_cast<const T *>(a.logits) + row * a.logits_stride + first;
   T *out = static_cast<T *>(a.out) + row * a.out_stride + first;
-  const unsigned *mask = a.mask == nullptr ? nullptr : a.mask + row * a.mask_stride + first / 32;
-  const bool in_place = static_cast<const void *>(in) == static_cast<const void *>(out);
+  static_assert(kThreads * 32 >= kSliceMost, "a word of the mask per thread");
+  const unsigned mask = a.mask != nullptr && tid * 32 < size ? a.mask[row * a.mask_stride + first / 32 + tid] : ~0u;
+  const float repetition = a.repetition == nullptr ? 1.0f : a.repetition[row], presence = a.presence == nullptr ? 0.0f : a.presence[row],
+              frequency = a.frequency == nullptr ? 0.0f : a.frequency[row];
   struct __align__(kVec * sizeof(T)) Vec {
     T x[kVec];
   };
-#pragma unroll 4
-  for (int i = tid * kVec; i < size; i += threads * kVec) {
-    const unsigned keep = mask == nullptr ? ~0u : mask[i >> 5] >> (i & 31);
-    Vec v;
-    if (kVec > 1 && i + kVec <= size)
-      v = *reinterpret_cast<const Vec *>(in + i);
+  Vec held[kPer];  // on their way while the history is counted
+#pragma unroll
+  for (int n = 0; n < kPer; ++n) {
+    const int i = (n * kThreads + tid) * kVec;
+    if (i + kVec <= size)
+      held[n] = *reinterpret_cast<const Vec *>(in + i);
     else
 #pragma unroll
       for (int j = 0; j < kVec; ++j)
-        if (i + j < size) v.x[j] = in[i + j];
-    unsigned any = 0, word[kVec];
-    if (marked) {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        word[j] = words[i + j];  // the table ends at a multiple of a vector
-        any |= word[j];
-      }
-      if (any != 0) {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j)
-          if (word[j] != 0) v.x[j] = rounded<T>(penalised(widened<T>(v.x[j]), word[j], penalty));
-      }
-    }
-    constexpr unsigned kAll = (1u << kVec) - 1;
-    if ((keep & kAll) != kAll) {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        if ((keep >> j & 1) == 0) v.x[j] = rounded<T>((double)minus_inf());
-    } else if (in_place && any == 0) {
-      continue;
-    }
-    if (kVec > 1 && i + kVec <= size && (any & kBiased) == 0)
-      *reinterpret_cast<Vec *>(out + i) = v;
-    else
-#pragma unroll
-      for (int j = 0; j < kVec; ++j)  // a biased one comes below, from the logit as it was
-        if (i + j < size && !(marked && (word[j] & kBiased) != 0)) out[i + j] = v.x[j];
+        if (i + j < size) held[n].x[j] = in[i + j];
   }
-  if (bias1 > bias0) {
-    __syncthreads();
-    for (int j = bias0 + tid; j < bias1; j += threads) {
-      const long long at = (long long)a.bias_ids[j] - first;
-      if (at < 0 || at >= size) continue;
-      const unsigned word = atomicAnd(words + at, ~kBiased);
-      if ((word & kBiased) == 0) continue;  // another thread has this token
-      double x = penalised(widened<T>(in[at]), word & ~(kBiased | kTwice), penalty);
-      if ((word & kTwice) == 0) {
-        x += (double)a.bias_values[j];
-      } else {  // a token with several biases: in the order of the list, whoever came first
-        for (int k = bias0; k < bias1; ++k)
-          if ((long long)a.bias_ids[k] - first == at) x += (double)a.bias_values[k];
-      }
-      const bool keeps = mask == nullptr || (mask[at >> 5] >> (at & 31) & 1) != 0;
-      out[at] = keeps ? rounded<T>(x) : rounded<T>((double)minus_inf());
+
+  for (int i = tid * 4; i < a.slice + a.slice / 16; i += kThreads * 4) *reinterpret_cast<uint4 *>(words + i) = make_uint4(0, 0, 0, 0);
+  if (tid == 0) listed = 0;
+  __syncthreads();
+  const Id *tokens = static_cast<const Id *>(a.tokens) + row * a.tokens_stride;
+  auto place = [&](Id id, int *at) {  // in the slice
+    if constexpr (sizeof(Id) == 4) {
+      *at = (int)((unsigned)id - (unsigned)first);
+      return (unsigned)*at < (unsigned)size;
+    } else {
+      *at = (int)(id - first);
+      return id >= first && id - first < size;
     }
+  };
+  constexpr int kBatch = 32 / sizeof(Id);  // a thread's tokens that are on their way together
+  for (int j0 = tid; j0 < length; j0 += kBatch * kThreads) {
+    Id ids[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) ids[u] = j0 + u * kThreads < length ? tokens[j0 + u * kThreads] : (Id)-1;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      int at;
+      if (place(ids[u], &at)) {
+        const unsigned old = j0 + u * kThreads < prompt ? atomicOr(words + at, kSeen) : atomicAdd(words + at, 1u);
+        if (old == 0) list[atomicAdd(&listed, 1)] = (unsigned short)at;
+      } else if (ids[u] >= a.vocab) {
+        bad = true;
+      }
+    }
+  }
+  auto mark = [&](int at) {
+    const unsigned bit = 1u << (at & 31);
+    if ((atomicOr(biased + (at >> 5), bit) & bit) != 0) atomicOr(twice + (at >> 5), bit);
+  };
+  for (int j = bias0 + tid; j < bias1; j += kThreads) {
+    const long long at = (long long)a.bias_ids[j] - first;
+    if (at >= 0 && at < size)
+      mark((int)at);
+    else if (at + first < 0 || at + first >= a.vocab)
+      bad = true;
+  }
+  if (tid * 32 < size) kept[tid] = mask;
+  __syncthreads();
+
+  // the logits as they are, or -inf
+  const bool in_place = static_cast<const void *>(in) == static_cast<const void *>(out);
+#pragma unroll
+  for (int n = 0; n < kPer; ++n) {
+    const int i = (n * kThreads + tid) * kVec;
+    if (i >= size) break;
+    constexpr unsigned kAll = (1u << kVec) - 1;
+    const unsigned keep = kept[i >> 5] >> (i & 31) & kAll;
+    if (in_place && keep == kAll) continue;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+      if ((keep >> j & 1) == 0) held[n].x[j] = rounded<T>((double)minus_inf());
+    if (i + kVec <= size)
+      *reinterpret_cast<Vec *>(out + i) = held[n];
+    else
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        if (i + j < size) out[i + j] = held[n].x[j];
+  }
+  __syncthreads();
+
+  // those that something concerns, from the logits as they were, over what has just been written
+  const Penalty penalty = {repetition, presence, frequency};
+  auto stays = [&](int at) { return (kept[at >> 5] >> (at & 31) & 1) != 0; };
+  const int concerned = listed;
+  for (int j = tid; j < concerned; j += kThreads) {
+    const int at = list[j];
+    if ((biased[at >> 5] >> (at & 31) & 1) == 0 && stays(at)) out[at] = rounded<T>(penalised(widened<T>(in[at]), words[at], penalty));
+  }
+  auto add = [&](int j, int at, T x, float value) {  // bias j
+    if (!stays(at)) return;
+    double bias = (double)value;
+    if ((twice[at >> 5] >> (at & 31) & 1) != 0) {  // one of several: the first of them adds all up, in their order
+      int k = bias0;
+      while (a.bias_ids[k] - first != at) ++k;
+      if (k != j) return;
+      for (++k; k < bias1; ++k)
+        if (a.bias_ids[k] - first == at) bias += (double)a.bias_values[k];
+    }
+    out[at] = rounded<T>(penalised(widened<T>(x), words[at], penalty) + bias);
+  };
+  for (int j = bias0 + tid; j < bias1; j += kThreads) {
+    const long long at = (long long)a.bias_ids[j] - first;
+    if (at >= 0 && at < size) add(j, (int)at, in[at], a.bias_values[j]);
   }
   if (bad && a.error_flag != nullptr) atomicCAS(a.error_flag, 0, kBadLogitRules);
 }
@@ -175,21 +200,24 @@ cudaError_t launch(LogitRules a, cudaStream_t stream) {
   cudaError_t err = cudaGetDevice(&dev);
   if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (err != cudaSuccess) return err;
-  // slices as wide as shared memory lets three CTAs share an SM, but two CTAs for every SM
-  a.slice = 16384;
-  while (a.slice > 1024 && (long long)a.rows * ((a.vocab + a.slice - 1) / a.slice) < 2 * sms) a.slice /= 2;
+  // Equal slices of a row, as many as its tokens need, or as give every SM a CTA, but of 1024 tokens at least
+  const int most = (a.vocab + 1023) / 1024, enough = (a.vocab + kSliceMost - 1) / kSliceMost, wanted = (sms + a.rows - 1) / a.rows;
+  const int slices = wanted > most ? most : wanted > enough ? wanted : enough;
+  a.slice = ((a.vocab + slices - 1) / slices + 127) / 128 * 128;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)((a.vocab + a.slice - 1) / a.slice), (unsigned)a.rows);
-  cfg.blockDim = dim3(a.slice >= 8192 ? 512 : 256);
-  cfg.dynamicSmemBytes = (size_t)a.slice * sizeof(unsigned);
+  cfg.blockDim = dim3(kThreads);
+  const long long concerned = (long long)a.width + a.biases;
+  const int entries = concerned < a.slice ? (int)concerned : a.slice;  // of the list, at most
+  cfg.dynamicSmemBytes = (size_t)(a.slice + a.slice / 32 * 3) * sizeof(unsigned) + (size_t)entries * sizeof(unsigned short);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   static bool ready[64] = {};
-  err = allow_smem(logit_rules_kernel<T, Id, kVec>, 16384 * (int)sizeof(unsigned), ready);
+  err = allow_smem(logit_rules_kernel<T, Id, kVec>, (kSliceMost + kSliceMost / 32 * 3) * (int)sizeof(unsigned) + kSliceMost * (int)sizeof(unsigned short), ready);
   if (err != cudaSuccess) return err;
   return cudaLaunchKernelEx(&cfg, logit_rules_kernel<T, Id, kVec>, a);
 }
