@@ -885,7 +885,8 @@ int sharq_plan_paged_step(int *page_table, int64_t page_table_stride, int sequen
   SHARQ_REQUIRE(max_tokens >= 0, "max_tokens must not be negative");
   SHARQ_REQUIRE(page_table_stride >= max_pages || sequences == 1, "page_table_stride must cover max_pages");
   SHARQ_REQUIRE(free_pages_size >= 0 && (free_pages_size == 0 || free_pages), "free_pages must have room for free_pages_size pages");
-  SHARQ_REQUIRE(rows >= 0 && (rows == 0 || (positions && row_sequences)), "rows must be >= 0, with a place for each");
+  SHARQ_REQUIRE(free_pages_size <= 1 << 30, "free_pages_size must be at most 2^30");
+  SHARQ_REQUIRE(rows >= 0 && rows <= 1 << 30 && (rows == 0 || (positions && row_sequences)), "rows must be in [0, 2^30], with a place for each");
   const sharq::StepPlan p = {page_table, page_table_stride, sequences, max_pages, page_size, max_tokens, lengths, counts, released, free_pages,
                              free_pages_size, free_count, rows, offsets, positions, row_sequences, error_flag};
   return check_cuda(sharq::run_step_plan(p, as_stream(stream)), "plan_paged_step");

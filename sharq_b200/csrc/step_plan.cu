@@ -21,17 +21,20 @@ namespace {
 constexpr int kPlanThreadsMost = 1024;
 constexpr int kPlanCluster = 8;
 
+// Sums of what is not negative, 2^31 - 1 where they would be more: what lies beyond is never given, and such sums may be taken in any grouping.
 struct Sums {
-  long long a, b;
+  int a, b;
 };
+constexpr int kMost = 0x7fffffff;
+__device__ __forceinline__ int plus(int x, int y) { return (int)min((unsigned)x + (unsigned)y, (unsigned)kMost); }
 
 // Inclusive sums over the block's threads; total: of all of them.  scratch: one per warp.
 __device__ __forceinline__ Sums block_scan(Sums x, Sums *scratch, Sums *total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const long long a = __shfl_up_sync(0xffffffffu, x.a, off), b = __shfl_up_sync(0xffffffffu, x.b, off);
-    if (lane >= off) x.a += a, x.b += b;
+    const int a = __shfl_up_sync(0xffffffffu, x.a, off), b = __shfl_up_sync(0xffffffffu, x.b, off);
+    if (lane >= off) x.a = plus(x.a, a), x.b = plus(x.b, b);
   }
   __syncthreads();  // scratch may still be read from the scan before
   if (lane == 31) scratch[warp] = x;
@@ -41,17 +44,17 @@ __device__ __forceinline__ Sums block_scan(Sums x, Sums *scratch, Sums *total) {
   Sums ahead = lane < warp ? of : Sums{0, 0};
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
-    of.a += __shfl_xor_sync(0xffffffffu, of.a, off);
-    of.b += __shfl_xor_sync(0xffffffffu, of.b, off);
-    ahead.a += __shfl_xor_sync(0xffffffffu, ahead.a, off);
-    ahead.b += __shfl_xor_sync(0xffffffffu, ahead.b, off);
+    of.a = plus(of.a, __shfl_xor_sync(0xffffffffu, of.a, off));
+    of.b = plus(of.b, __shfl_xor_sync(0xffffffffu, of.b, off));
+    ahead.a = plus(ahead.a, __shfl_xor_sync(0xffffffffu, ahead.a, off));
+    ahead.b = plus(ahead.b, __shfl_xor_sync(0xffffffffu, ahead.b, off));
   }
   *total = of;
-  return {x.a + ahead.a, x.b + ahead.b};
+  return {plus(x.a, ahead.a), plus(x.b, ahead.b)};
 }
 
 // the first of `n` ascending sums that is more than x, which the last one is
-__device__ __forceinline__ int first_above(const long long *sums, int n, long long x) {
+__device__ __forceinline__ int first_above(const int *sums, int n, int x) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -63,117 +66,149 @@ __device__ __forceinline__ int first_above(const long long *sums, int n, long lo
   return lo;
 }
 
+__device__ __forceinline__ int pages_of(int tokens, int page_size) { return tokens == 0 ? 0 : (tokens - 1) / page_size + 1; }
+
+// Rows [from, to) in groups of four that begin at multiples of four, `step` threads apart: fill(row, &position, &sequence) for each in ascending order.
+template <typename Fill>
+__device__ __forceinline__ void write_rows(const StepPlan &p, int from, int to, int at0, int step, bool aligned, Fill fill) {
+  for (long long r0 = (from & ~3) + 4LL * at0; r0 < to; r0 += 4LL * step) {
+    int position[4], sequence[4], state = -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (r0 + k >= from && r0 + k < to) fill((int)r0 + k, &state, &position[k], &sequence[k]);
+    if (aligned && r0 >= from && r0 + 4 <= to) {
+      *reinterpret_cast<int4 *>(p.positions + r0) = make_int4(position[0], position[1], position[2], position[3]);
+      *reinterpret_cast<int4 *>(p.row_sequences + r0) = make_int4(sequence[0], sequence[1], sequence[2], sequence[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (r0 + k >= from && r0 + k < to) p.positions[r0 + k] = position[k], p.row_sequences[r0 + k] = sequence[k];
+    }
+  }
+}
+
 __global__ void __launch_bounds__(kPlanThreadsMost) step_plan_kernel(const __grid_constant__ StepPlan p) {
   __shared__ Sums scratch[32];
-  __shared__ long long need_ends[kPlanThreadsMost], row_ends[kPlanThreadsMost];
+  __shared__ int need_ends[kPlanThreadsMost], row_ends[kPlanThreadsMost];
   __shared__ int held_of[kPlanThreadsMost], given_of[kPlanThreadsMost];  // given_of: length ahead of the new tokens, -1: nothing is given
+  __shared__ int taken;
   const int tid = threadIdx.x, threads = blockDim.x;
   const int rank = blockIdx.x, at0 = rank * threads + tid, step = gridDim.x * threads;
-  const long long capacity = (long long)p.max_pages * p.page_size, most = p.max_tokens > 0 ? min(capacity, (long long)p.max_tokens) : capacity;
+  const long long room = (long long)p.max_pages * p.page_size;
+  const int capacity = (int)min(room, (long long)kMost), most = p.max_tokens > 0 ? min(capacity, p.max_tokens) : capacity;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(p.positions) | reinterpret_cast<uintptr_t>(p.row_sequences)) & 15) == 0;
+  if (tid == 0) taken = 0;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const int free_given = *p.free_count;
   bool bad = free_given < 0 || free_given > p.stack_size;
   const bool no_stack = bad;
-  long long free_now = no_stack ? 0 : free_given;
+  int free_now = no_stack ? 0 : free_given;
 
   if (p.released != nullptr) {  // ended sequences put their pages back, the last page first
-    long long before = 0;
+    int before = 0;
     for (int i0 = 0; i0 < p.sequences; i0 += threads) {
       const int i = i0 + tid;
-      long long back = 0;
+      int back = 0;
       if (i < p.sequences && p.released[i] != 0) {
         const int length = p.lengths[i];
         if (length < 0 || length > capacity)
           bad = true;
         else
-          back = ((long long)length + p.page_size - 1) / p.page_size;
+          back = pages_of(length, p.page_size);
       }
       Sums total;
       const Sums ends = block_scan({back, 0}, scratch, &total);
       need_ends[tid] = ends.a;
-      held_of[tid] = (int)back;
+      held_of[tid] = back;
       __syncthreads();
-      for (long long q = at0; q < total.a; q += step) {
+      for (int q = at0; q < total.a; q += step) {
         const int s = first_above(need_ends, threads, q);
-        const long long page = q - (need_ends[s] - held_of[s]), to = free_now + before + need_ends[s] - 1 - page;
+        const int page = q - (need_ends[s] - held_of[s]);
+        const long long to = (long long)free_now + before + need_ends[s] - 1 - page;
         if (!no_stack && to < p.stack_size)
           p.stack[to] = p.table[(long long)(i0 + s) * p.table_stride + page];
         else
           bad = true;
       }
-      before += total.a;
+      before = plus(before, total.a);
       __syncthreads();  // the sums have been read
     }
-    free_now = no_stack ? 0 : min(free_now + before, (long long)p.stack_size);
-    __syncwarp();
-    ptx::cluster_sync();
+    free_now = no_stack ? 0 : min(plus(free_now, before), p.stack_size);
+    if (before > 0) {  // the pages are on the stack before any is taken
+      __syncwarp();
+      ptx::cluster_sync();
+    }
   }
 
-  long long need_before = 0, rows_before = 0, taken = 0;
+  int need_before = 0, rows_before = 0;
   for (int i0 = 0; i0 < p.sequences; i0 += threads) {
     const int i = i0 + tid;
-    int length = 0, count = 0, held = 0;
-    long long need = 0;
+    int length = 0, count = 0, held = 0, need = 0;
     bool fits = false, keeps = true;  // keeps: its length stays as it is
     if (i < p.sequences) {
       length = p.lengths[i];
       count = p.counts[i];
       if (p.released != nullptr && p.released[i] != 0) length = 0, keeps = false;
-      fits = length >= 0 && count >= 0 && (long long)length + count <= most;
+      fits = length >= 0 && count >= 0 && length <= most && count <= most - length;
       if (!fits) bad = true;
       count = max(count, 0);
       if (fits) {
-        held = (int)(((long long)length + p.page_size - 1) / p.page_size);
-        need = ((long long)length + count + p.page_size - 1) / p.page_size - held;
+        held = pages_of(length, p.page_size);
+        need = pages_of(length + count, p.page_size) - held;
       }
     }
     Sums total;
-    Sums ends = block_scan({need, count}, scratch, &total);
-    const long long row_end = rows_before + ends.b;
-    const bool given = fits && !no_stack && (need == 0 || need_before + ends.a <= free_now) && row_end <= p.rows;
+    const Sums ends = block_scan({need, count}, scratch, &total);
+    const int row_end = plus(rows_before, ends.b), need_end = plus(need_before, ends.a);
+    const bool given = fits && !no_stack && (need == 0 || need_end <= free_now) && row_end <= p.rows;
     if (fits && row_end > p.rows) bad = true;
     need_ends[tid] = ends.a;
     row_ends[tid] = ends.b;
     held_of[tid] = held;
     given_of[tid] = given ? length : -1;
+    // those that get pages are at the front of those that need some
+    const int end_of_warp = __reduce_max_sync(0xffffffffu, given && need > 0 ? need_end : 0);
+    if ((tid & 31) == 0 && end_of_warp > 0) atomicMax(&taken, end_of_warp);
     // every CTA has read these sequences' lengths, and the number of free pages
     __syncthreads();
     ptx::cluster_sync();
     if (rank == 0 && i < p.sequences) {
-      p.offsets[i + 1] = (int)min(row_end, (long long)p.rows);
+      p.offsets[i + 1] = min(row_end, p.rows);
       if (given)
         p.lengths[i] = length + count;
       else if (!keeps)
         p.lengths[i] = 0;
     }
-    for (long long q = at0; q < total.a; q += step) {
+    const int pages_here = min(total.a, free_now - min(need_before, free_now));
+    for (int q = at0; q < pages_here; q += step) {
       const int s = first_above(need_ends, threads, q);
       if (given_of[s] < 0) continue;
-      const long long start = s > 0 ? need_ends[s - 1] : 0;
+      const int start = s > 0 ? need_ends[s - 1] : 0;
       p.table[(long long)(i0 + s) * p.table_stride + held_of[s] + (q - start)] = p.stack[free_now - 1 - need_before - q];
     }
-    const long long rows_here = min(total.b, p.rows - min(rows_before, (long long)p.rows));
-    for (long long q = at0; q < rows_here; q += step) {
-      const int s = first_above(row_ends, threads, q);
-      const long long start = s > 0 ? row_ends[s - 1] : 0;
-      p.positions[rows_before + q] = given_of[s] < 0 ? -1 : given_of[s] + (int)(q - start);
-      p.row_sequences[rows_before + q] = i0 + s;
-    }
-    // what was given: the pages of all that fit, which are those of the sequences at the front
-    Sums given_total;
-    block_scan({given ? need : 0, 0}, scratch, &given_total);
-    taken += given_total.a;
-    need_before += total.a;
-    rows_before += total.b;
+    const int row0 = min(rows_before, p.rows), row1 = min(plus(rows_before, total.b), p.rows);
+    write_rows(p, row0, row1, at0, step, aligned, [&](int row, int *s, int *position, int *sequence) {
+      const int q = row - row0;
+      if (*s < 0)
+        *s = first_above(row_ends, threads, q);
+      else
+        while (row_ends[*s] <= q) ++*s;
+      const int start = *s > 0 ? row_ends[*s - 1] : 0;
+      *position = given_of[*s] < 0 ? -1 : given_of[*s] + (q - start);
+      *sequence = i0 + *s;
+    });
+    need_before = plus(need_before, total.a);
+    rows_before = plus(rows_before, total.b);
+    if (i0 + threads < p.sequences) __syncthreads();  // the sums have been read
   }
-  for (long long r = min(rows_before, (long long)p.rows) + at0; r < p.rows; r += step) {
-    p.positions[r] = -1;
-    p.row_sequences[r] = 0;
-  }
+  write_rows(p, min(rows_before, p.rows), p.rows, at0, step, aligned, [&](int, int *, int *position, int *sequence) {
+    *position = -1;
+    *sequence = 0;
+  });
   if (rank == 0 && tid == 0) {
     p.offsets[0] = 0;
-    if (!no_stack) *p.free_count = (int)(free_now - taken);
+    if (!no_stack) *p.free_count = free_now - taken;
   }
   if (bad && p.error_flag != nullptr) atomicCAS(p.error_flag, 0, kBadStepPlan);
 }

@@ -615,24 +615,32 @@ std::vector<Tensor> plan_paged_step(const Tensor &table, const Tensor &lengths, 
   need(n == 1 || table.stride(0) >= table.size(1), "rows of page_table must not overlap");
   check_indices(lengths, n, dev, "lengths");
   check_indices(counts, n, dev, "counts");
-  need(free_pages.dim() == 1 && free_pages.size(0) <= INT32_MAX, "free_pages must be a contiguous CUDA int32 vector on the device of the input");
+  need(free_pages.dim() == 1 && free_pages.size(0) <= 1 << 30, "free_pages must be a contiguous CUDA int32 vector of at most 2^30 on the device of the input");
   check_indices(free_pages, free_pages.size(0), dev, "free_pages");
   check_indices(free_count, 1, dev, "free_count");
   need(page_size > 0 && page_size <= INT32_MAX, "page_size must be positive");
-  need(rows >= 0 && rows <= INT32_MAX, "rows must be in [0, 2^31)");
+  need(rows >= 0 && rows <= 1 << 30, "rows must be in [0, 2^30]");
   need(!max_tokens || *max_tokens > 0, "max_tokens must be positive, or None");
   if (released)
     need((is_plain(*released, at::kBool) || is_plain(*released, at::kByte)) && released->device() == dev && released->dim() == 1 && released->size(0) == n,
          "released must be a contiguous CUDA bool vector with one entry per sequence");
   c10::cuda::OptionalCUDAGuard guard(dev);
-  Tensor out = empty_like_on(table, {n + 1 + 2 * rows}, at::kInt);
+  // the parts begin at multiples of 16 bytes, and are made without the dispatcher
+  const int64_t at_rows = (n + 4) & ~int64_t(3), padded = (rows + 3) & ~int64_t(3);
+  const Tensor out = empty_like_on(table, {at_rows + 2 * padded}, at::kInt);
   int *at = static_cast<int *>(ptr(out));
+  auto part = [&](int64_t offset, int64_t size) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(out.storage()), out.key_set(), c10::scalarTypeToTypeMeta(at::kInt));
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({size});
+    return t;
+  };
   check(sharq_plan_paged_step(static_cast<int *>(ptr(table)), n > 1 ? table.stride(0) : table.size(1), (int)n, (int)table.size(1), (int)page_size,
                               max_tokens ? (int)std::min<int64_t>(*max_tokens, INT32_MAX) : 0, static_cast<int *>(ptr(lengths)), static_cast<const int *>(ptr(counts)),
                               released ? static_cast<const unsigned char *>(ptr(*released)) : nullptr, static_cast<int *>(ptr(free_pages)),
-                              (int)free_pages.size(0), static_cast<int *>(ptr(free_count)), (int)rows, at, at + n + 1, at + n + 1 + rows,
+                              (int)free_pages.size(0), static_cast<int *>(ptr(free_count)), (int)rows, at, at + at_rows, at + at_rows + padded,
                               flag_of(flag), stream_of(table)));
-  return {out.narrow(0, 0, n + 1), out.narrow(0, n + 1, rows), out.narrow(0, n + 1 + rows, rows)};
+  return {part(0, n + 1), part(at_rows, rows), part(at_rows + padded, rows)};
 }
 
 using OptionalTensor = std::optional<Tensor>;
