@@ -37,7 +37,7 @@ constexpr int kBlocks = 2;
 constexpr int kSoftmaxWarps = 4 * kBlocks, kLoadWarp = kSoftmaxWarps, kMmaWarp = kLoadWarp + 1, kCheckWarp = kMmaWarp + 1, kCheckWarps = 2;
 constexpr int kThreads = 32 * (kCheckWarp + kCheckWarps);
 constexpr int kItemSlots = 2;
-constexpr int kSoftmaxRegisters = 200, kOtherRegisters = 96;
+constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 88;
 static_assert(128 * kBlocks * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreads * 168, "the shares of the registers that the block was launched with");
 constexpr float kLazy = 8.0f, kLift = -32.0f;  // in powers of two
 
@@ -121,6 +121,36 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return *reinterpret_cast<uint32_t *>(&v);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// pairs of floats in a register pair each
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float *a, float *b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -133,6 +163,14 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_ld_x4(uint32_t taddr, uint32_t (&r)[4]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -253,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t queries = ptx::smem_u32(smem), ring = queries + kBlocks * S::kBytes;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kControl);
   uint64_t *kv_full = bars, *kv_empty = kv_full + kStages, *v_ok = kv_empty + kStages, *q_full = v_ok + kStages, *q_empty = q_full + kBlocks;
-  uint64_t *s_full = q_empty + kBlocks, *p_full = s_full + kBlocks, *o_full = p_full + kBlocks, *item_full = o_full + kBlocks;
+  uint64_t *s_full = q_empty + kBlocks, *p_half = s_full + kBlocks, *p_full = p_half + kBlocks, *o_full = p_full + kBlocks, *item_full = o_full + kBlocks;
   uint64_t *item_empty = item_full + kItemSlots;
   uint64_t *drained = item_empty + kItemSlots;  // for products on their way when a wait ran out
   Item *items = reinterpret_cast<Item *>(drained + 1);
@@ -271,6 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(q_full + i, 1);
       ptx::mbar_init(q_empty + i, 1);
       ptx::mbar_init(s_full + i, 1);
+      ptx::mbar_init(p_half + i, 4);
       ptx::mbar_init(p_full + i, 4);
       ptx::mbar_init(o_full + i, 1);
     }
@@ -299,22 +338,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     *abort_flag = 1;
     if (a.error_flag != nullptr) atomicExch(a.error_flag, kPromptTimeout);
   };
-  // the next item's description as the load warp left it; `n`: how many there have been
-  auto next_item = [&](Item &it, int n) {
+  // whether there is another item, whose description the load warp has left in items[n % kItemSlots]; `n`: how many there have been
+  auto next_item = [&](int n) {
     const int slot = n % kItemSlots;
     if (!ptx::mbar_wait(item_full + slot, (n / kItemSlots) & 1, abort_flag)) {
       give_up();
       return false;
     }
-    it = items[slot];
-    return it.state != 0;
+    return items[slot].state != 0;
   };
-  auto next_item_of_warp = [&](Item &it, int n) {  // all lanes, which have the same answer
-    const bool got = next_item(it, n);
+  auto next_item_of_warp = [&](int n) {  // all lanes, which have the same answer
+    const bool got = next_item(n);
     __syncwarp();
-    if (!__all_sync(0xffffffffu, got)) return false;
+    return (bool)__all_sync(0xffffffffu, got);
+  };
+  auto leave_item = [&](int n) {  // the warp has read what it needs of the description
+    __syncwarp();
     if (lane == 0) ptx::mbar_arrive(item_empty + n % kItemSlots);
-    return true;
   };
 
   if (warp < kSoftmaxWarps) {
@@ -333,14 +373,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         out[i < ahead ? i : (long long)a.rows * width - behind + (i - ahead)] = make_uint4(0, 0, 0, 0);
     }
     unsigned tiles_done = 0, values_done = 0, items_done = 0;  // for the barriers' parities: of this block, of all, of this block
-    Item it;
     bool ok = true;
-    for (int n = 0; ok; ++n) {
-      if (!next_item_of_warp(it, n)) break;
-      const unsigned value0 = values_done;
-      values_done += it.tiles;
+    for (int n = 0; ok && next_item_of_warp(n); values_done += items[n % kItemSlots].tiles, leave_item(n), ++n) {
+      const Item &it = items[n % kItemSlots];  // stays in shared memory, for want of registers
       if (it.count <= block * a.tokens) continue;  // nothing for this block
-      const int t = block * a.tokens + token, position = it.first + min(t, it.count - 1);
+      const int position = it.first + min(block * a.tokens + token, it.count - 1);
       const Seen seen = seen_by(it, position, a.window, a.sinks);
       float m = -INFINITY, l = 0.0f;  // maximum in powers of two, sum
       for (int tile = 0; tile < it.tiles; ++tile) {
@@ -349,10 +386,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = false;
         }
         __syncwarp();
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         ptx::tc_fence_after();
         uint32_t s[4][32];
 #pragma unroll
@@ -376,11 +411,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         float top[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          top[i] = __uint_as_float(s[i][0]);
+          top[i] = fmaxf(__uint_as_float(s[i][0]), __uint_as_float(s[i][1]));
 #pragma unroll
-          for (int j = 1; j < 32; ++j) top[i] = fmaxf(top[i], __uint_as_float(s[i][j]));
+          for (int j = 2; j < 32; j += 2) top[i] = max3(top[i], __uint_as_float(s[i][j]), __uint_as_float(s[i][j + 1]));
         }
-        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+        const float high = max3(fmaxf(top[0], top[1]), top[2], top[3]) * c;
         const bool raise = high > m + kLazy;
         if (__any_sync(0xffffffffu, raise)) {
           const float f = raise ? exp2_approx(m - high) : 1.0f;  // from -inf: 0, and nothing to keep
@@ -388,45 +423,54 @@ __global__ void __launch_bounds__(kThreads, 1)
           l *= f;
           if (tile > 0) {
 #pragma unroll 1
-            for (int i = 0; i < D; i += 32) {
-              uint32_t o[32];
-              ptx::tmem_ld_32x32b_x32(tmem_o + i, o);
+            for (int i = 0; i < D; i += 16) {
+              uint32_t o[16];
+              tmem_ld_x16(tmem_o + i, o);
               ptx::tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-              tmem_st_x32(tmem_o + i, o);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st_x16(tmem_o + i, o);
             }
           }
         }
         // a row with no finite score so far has maximum -inf: its probabilities are 0, not exp(-inf + inf)
         const float base = (m == -INFINITY ? 0.0f : m) - kLift;
-        float sum[2] = {0.0f, 0.0f};
+        const uint64_t c2 = pair(c, c), base2 = pair(-base, -base);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t p[32];
+        for (int i = 0; i < 4; ++i) {
+          uint32_t p[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float x = exp2_approx(fmaf(__uint_as_float(s[2 * i + j / 16][j % 16 * 2]), c, -base));
-            const float y = exp2_approx(fmaf(__uint_as_float(s[2 * i + j / 16][j % 16 * 2 + 1]), c, -base));
-            sum[0] += x;
-            sum[1] += y;
+          for (int j = 0; j < 16; ++j) {
+            float x, y;
+            unpair(fma_pair(pair(__uint_as_float(s[i][2 * j]), __uint_as_float(s[i][2 * j + 1])), c2, base2), &x, &y);
+            x = exp2_approx(x);
+            y = exp2_approx(y);
+            sum[j & 1] = add_pair(sum[j & 1], pair(x, y));
             p[j] = pack_bf16(x, y);
           }
-          tmem_st_x32(tmem_s + 32 * i, p);
+          tmem_st_x16(tmem_s + 16 * i, p);
+          if (i == 1) {  // the product may begin with half of the keys
+            tmem_st_wait();
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(p_half + block);
+          }
         }
-        l += sum[0] + sum[1];
+        float sums[4];
+        unpair(sum[0], &sums[0], &sums[1]);
+        unpair(sum[1], &sums[2], &sums[3]);
+        l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         tmem_st_wait();
         if (masked) {
-          const unsigned value = value0 + tile;
+          const unsigned value = values_done + tile;
           if (!ptx::mbar_wait(v_ok + value % kStages, (value / kStages) & 1, abort_flag)) {
             give_up();
             ok = false;
           }
           __syncwarp();
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           if ((not_finite[value % kStages * kCheckWarps] | not_finite[value % kStages * kCheckWarps + 1]) != 0)
             multiply_visible<D>(tmem_s, tmem_o, ring + (2 * value + 1) % kStages * S::kBytes,
                                 Seen{seen.low - tile * kTile, seen.high - tile * kTile, seen.sinks - tile * kTile}, tile == 0);
@@ -436,6 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) ptx::mbar_arrive(p_full + block);
       }
       if (!ok) break;
+      const int t = block * a.tokens + token, tiles = it.tiles, state = it.state;
       const bool there = token < a.tokens && t < it.count && it.chunk * a.chunk_heads + head < a.group;
       if (it.tiles > 0) {
         if (!ptx::mbar_wait(o_full + block, items_done++ & 1, abort_flag)) {
@@ -443,7 +488,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = false;
         }
         __syncwarp();
-        if (!__all_sync(0xffffffffu, ok)) break;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         ptx::tc_fence_after();
       }
       __nv_bfloat16 *out = a.out + ((long long)(it.row0 + t) * a.heads + it.kv * a.group + it.chunk * a.chunk_heads + head) * D;
@@ -451,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int i = 0; i < D; i += 32) {
         uint32_t o[32];
-        if (it.tiles > 0) {
+        if (tiles > 0) {
           ptx::tmem_ld_32x32b_x32(tmem_o + i, o);
           ptx::tmem_ld_wait();
         }
@@ -461,8 +507,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             w[e] = pack_bf16(__uint_as_float(o[j + 2 * e]) * f, __uint_as_float(o[j + 2 * e + 1]) * f);
-            if (position < 0 || it.tiles == 0) w[e] = 0;
-            if (it.state == 2) w[e] = 0x7fff7fffu;
+            if (position < 0 || tiles == 0) w[e] = 0;
+            if (state == 2) w[e] = 0x7fff7fffu;
           }
           if (there) *reinterpret_cast<uint4 *>(out + i + j) = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -602,9 +648,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) give_up();
           return ok;
         };
-        Item it;
-        for (int n = 0; ok; ++n) {
-          if (!next_item(it, n)) break;
+        for (int n = 0; ok && next_item(n); ++n) {
+          const Item it = items[n % kItemSlots];
           ptx::mbar_arrive(item_empty + n % kItemSlots);
           if (it.tiles == 0) continue;
           const int active = it.count > a.tokens ? 2 : 1;
@@ -637,15 +682,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++values;
             if (more && !wait(kv_full + next % kStages, next / kStages)) break;
             for (int b = 0; b < active; ++b) {
-              if (!wait(p_full + b, probs[b]++)) break;
-              ptx::tc_fence_after();
-              if (!by_rows) {
-                const uint32_t from = ring + value % kStages * S::kBytes;
+              const uint32_t from = ring + value % kStages * S::kBytes;
+              for (int half = 0; half < 2; ++half) {
+                if (!wait((half == 0 ? p_half : p_full) + b, probs[b])) break;
+                ptx::tc_fence_after();
+                if (!by_rows) {
 #pragma unroll
-                for (int k = 0; k < kTile / 16; ++k)
-                  mma_ts(tmem + S::kOutCol + b * D, tmem + b * kTile + k * 8, ptx::make_smem_desc(from + k * 2048, 1024, S::kHalf, 2), kOutputs,
-                         tile > 0 || k > 0);
+                  for (int k = 0; k < kTile / 32; ++k)
+                    mma_ts(tmem + S::kOutCol + b * D, tmem + b * kTile + half * 32 + k * 8,
+                           ptx::make_smem_desc(from + half * (kTile / 2) * 128 + k * 2048, 1024, S::kHalf, 2), kOutputs, tile > 0 || half > 0 || k > 0);
+                }
               }
+              if (!ok) break;
+              ++probs[b];
               if (b + 1 == active) ptx::tc_commit<1>(kv_empty + value % kStages);
               if (more)
                 scores(b, next, tile + 2 == it.tiles);
@@ -666,10 +715,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
       const int part = warp - kCheckWarp;
       unsigned copies = 0, values = 0;
-      Item it;
       bool ok = true;
-      for (int n = 0; ok; ++n) {
-        if (!next_item_of_warp(it, n)) break;
+      for (int n = 0; ok && next_item_of_warp(n); ++n) {
+        const Item it = items[n % kItemSlots];
+        leave_item(n);
         for (int tile = 0; tile < it.tiles; ++tile, copies += 2, ++values) {
           const unsigned copy = copies + 1;
           ok = ptx::mbar_wait(kv_full + copy % kStages, (copy / kStages) & 1, abort_flag);
