@@ -1,5 +1,5 @@
 // Attention of ragged prompts: causal, with a sliding window and a few first keys that stay visible.  32768 tokens of 32 / 8 heads of
-// 128 under a window of 4096: 2.38 ms, 867 TFLOP/s; 200 tokens: 14.6 us.
+// 128 under a window of 4096: 2.05 ms, 1000 TFLOP/s, in long runs, where the card's power is the bound (1.75 ms in a short one); 200 tokens: 11.2 us.
 //
 //   out[i, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q[i, h] . k_j - max),   j <= p and (p - j < window or j < sinks),   p the position of query i
 //
@@ -39,7 +39,33 @@ constexpr int kThreads = 32 * (kCheckWarp + kCheckWarps);
 constexpr int kItemSlots = 2;
 constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 88;
 static_assert(128 * kBlocks * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreads * 168, "the shares of the registers that the block was launched with");
+constexpr int kFirst = 96;  // keys whose product does not wait for the others' probabilities
 constexpr float kLazy = 8.0f, kLift = -32.0f;  // in powers of two
+
+// As ptx::mbar_wait, but the thread sleeps up to some microseconds between looks (or until the phase ends): waiting warps took 3 % of the rate, long runs of which
+// are bound by the card's power.
+__device__ __forceinline__ bool look(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(ok)
+      : "r"(ptx::smem_u32(bar)), "r"(parity), "r"(4000)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+  if (look(bar, parity)) return true;
+  const long long start = clock64();
+  while (true) {
+    if (look(bar, parity)) return true;
+    if (*abort_flag != 0) return false;
+    if (clock64() - start > ptx::kWaitLimitCycles) return false;
+  }
+}
 
 template <int D>
 struct Sizes {
@@ -291,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t queries = ptx::smem_u32(smem), ring = queries + kBlocks * S::kBytes;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kControl);
   uint64_t *kv_full = bars, *kv_empty = kv_full + kStages, *v_ok = kv_empty + kStages, *q_full = v_ok + kStages, *q_empty = q_full + kBlocks;
-  uint64_t *s_full = q_empty + kBlocks, *p_half = s_full + kBlocks, *p_full = p_half + kBlocks, *o_full = p_full + kBlocks, *item_full = o_full + kBlocks;
+  uint64_t *s_full = q_empty + kBlocks, *p_first = s_full + kBlocks, *p_full = p_first + kBlocks, *o_full = p_full + kBlocks, *item_full = o_full + kBlocks;
   uint64_t *item_empty = item_full + kItemSlots;
   uint64_t *drained = item_empty + kItemSlots;  // for products on their way when a wait ran out
   Item *items = reinterpret_cast<Item *>(drained + 1);
@@ -309,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(q_full + i, 1);
       ptx::mbar_init(q_empty + i, 1);
       ptx::mbar_init(s_full + i, 1);
-      ptx::mbar_init(p_half + i, 4);
+      ptx::mbar_init(p_first + i, 4);
       ptx::mbar_init(p_full + i, 4);
       ptx::mbar_init(o_full + i, 1);
     }
@@ -341,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // whether there is another item, whose description the load warp has left in items[n % kItemSlots]; `n`: how many there have been
   auto next_item = [&](int n) {
     const int slot = n % kItemSlots;
-    if (!ptx::mbar_wait(item_full + slot, (n / kItemSlots) & 1, abort_flag)) {
+    if (!wait_for(item_full + slot, (n / kItemSlots) & 1, abort_flag)) {
       give_up();
       return false;
     }
@@ -381,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Seen seen = seen_by(it, position, a.window, a.sinks);
       float m = -INFINITY, l = 0.0f;  // maximum in powers of two, sum
       for (int tile = 0; tile < it.tiles; ++tile) {
-        if (!ptx::mbar_wait(s_full + block, tiles_done++ & 1, abort_flag)) {
+        if (!wait_for(s_full + block, tiles_done++ & 1, abort_flag)) {
           give_up();
           ok = false;
         }
@@ -450,11 +476,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             p[j] = pack_bf16(x, y);
           }
           tmem_st_x16(tmem_s + 16 * i, p);
-          if (i == 1) {  // the product may begin with half of the keys
+          if (i == kFirst / 32 - 1) {  // the product may begin with the keys so far
             tmem_st_wait();
             ptx::tc_fence_before();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(p_half + block);
+            if (lane == 0) ptx::mbar_arrive(p_first + block);
           }
         }
         float sums[4];
@@ -464,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st_wait();
         if (masked) {
           const unsigned value = values_done + tile;
-          if (!ptx::mbar_wait(v_ok + value % kStages, (value / kStages) & 1, abort_flag)) {
+          if (!wait_for(v_ok + value % kStages, (value / kStages) & 1, abort_flag)) {
             give_up();
             ok = false;
           }
@@ -483,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t = block * a.tokens + token, tiles = it.tiles, state = it.state;
       const bool there = token < a.tokens && t < it.count && it.chunk * a.chunk_heads + head < a.group;
       if (it.tiles > 0) {
-        if (!ptx::mbar_wait(o_full + block, items_done++ & 1, abort_flag)) {
+        if (!wait_for(o_full + block, items_done++ & 1, abort_flag)) {
           give_up();
           ok = false;
         }
@@ -502,15 +528,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::tmem_ld_wait();
         }
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          uint32_t w[4];
+        for (int j = 0; j < 32; j += 16) {
+          uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 8; ++e) {
             w[e] = pack_bf16(__uint_as_float(o[j + 2 * e]) * f, __uint_as_float(o[j + 2 * e + 1]) * f);
             if (position < 0 || tiles == 0) w[e] = 0;
             if (state == 2) w[e] = 0x7fff7fffu;
           }
-          if (there) *reinterpret_cast<uint4 *>(out + i + j) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (there)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + i + j), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                         "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
         }
         __syncwarp();
       }
@@ -578,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int slot = n % kItemSlots;
         if (lane == 0) {
-          if (ptx::mbar_wait(item_empty + slot, ((n / kItemSlots) & 1) ^ 1, abort_flag)) {
+          if (wait_for(item_empty + slot, ((n / kItemSlots) & 1) ^ 1, abort_flag)) {
             items[slot] = it;
             ptx::mbar_arrive(item_full + slot);
           } else {
@@ -588,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (ok && it.state != 0 && it.tiles > 0) {
             auto fill = [&](int tile, bool of_keys) {
               const int stage = copies % kStages;
-              if (!ptx::mbar_wait(kv_empty + stage, ((copies / kStages) & 1) ^ 1, abort_flag)) {
+              if (!wait_for(kv_empty + stage, ((copies / kStages) & 1) ^ 1, abort_flag)) {
                 give_up();
                 ok = false;
                 return;
@@ -610,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             for (int b = 0; b < kBlocks && ok; ++b) {
               if (it.count <= b * a.tokens) continue;
-              if (!ptx::mbar_wait(q_empty + b, (loads[b] & 1) ^ 1, abort_flag)) {
+              if (!wait_for(q_empty + b, (loads[b] & 1) ^ 1, abort_flag)) {
                 give_up();
                 ok = false;
                 break;
@@ -644,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         unsigned copies = 0, values = 0, loads[kBlocks] = {0, 0}, probs[kBlocks] = {0, 0};
         bool ok = true;
         auto wait = [&](uint64_t *bar, unsigned parity) {
-          ok = ok && ptx::mbar_wait(bar, parity & 1, abort_flag);
+          ok = ok && wait_for(bar, parity & 1, abort_flag);
           if (!ok) give_up();
           return ok;
         };
@@ -683,14 +712,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (more && !wait(kv_full + next % kStages, next / kStages)) break;
             for (int b = 0; b < active; ++b) {
               const uint32_t from = ring + value % kStages * S::kBytes;
-              for (int half = 0; half < 2; ++half) {
-                if (!wait((half == 0 ? p_half : p_full) + b, probs[b])) break;
+              for (int piece = 0; piece < 2; ++piece) {
+                if (!wait((piece == 0 ? p_first : p_full) + b, probs[b])) break;
                 ptx::tc_fence_after();
                 if (!by_rows) {
 #pragma unroll
-                  for (int k = 0; k < kTile / 32; ++k)
-                    mma_ts(tmem + S::kOutCol + b * D, tmem + b * kTile + half * 32 + k * 8,
-                           ptx::make_smem_desc(from + half * (kTile / 2) * 128 + k * 2048, 1024, S::kHalf, 2), kOutputs, tile > 0 || half > 0 || k > 0);
+                  for (int k = 0; k < kTile / 16; ++k)
+                    if ((k < kFirst / 16) == (piece == 0))
+                      mma_ts(tmem + S::kOutCol + b * D, tmem + b * kTile + k * 8, ptx::make_smem_desc(from + k * 2048, 1024, S::kHalf, 2), kOutputs,
+                             tile > 0 || k > 0);
                 }
               }
               if (!ok) break;
@@ -721,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         leave_item(n);
         for (int tile = 0; tile < it.tiles; ++tile, copies += 2, ++values) {
           const unsigned copy = copies + 1;
-          ok = ptx::mbar_wait(kv_full + copy % kStages, (copy / kStages) & 1, abort_flag);
+          ok = wait_for(kv_full + copy % kStages, (copy / kStages) & 1, abort_flag);
           if (!ok) give_up();
           __syncwarp();
           ok = __all_sync(0xffffffffu, ok);
