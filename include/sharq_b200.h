@@ -441,11 +441,14 @@ int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, in
  * h / (heads / kv_heads).  With fill != 0 rows of out ahead of the first sequence and behind the last become zeros, else they stay as they are.
  * Sums and softmax statistics are float; probabilities enter the product with the values as bf16.  Offsets (int32, on the device) that go back or leave
  * [0, rows] make their sequence empty, those of keys make its rows NaN, and store 0x407 in *error_flag (may be NULL; 0x408: a wait ran out, results
- * are undefined).  head_dim 64 or 128, heads a multiple of kv_heads, rows and k_rows at most 2^30; no workspace. */
+ * are undefined).  head_dim 64 or 128, heads a multiple of kv_heads, rows and k_rows at most 2^30.  workspace:
+ * sharq_prompt_attention_workspace_bytes() bytes of scratch (0: none, by these sizes alone; few queries with many keys are cut into parts), 32-byte
+ * aligned, not shared by calls that overlap. */
+size_t sharq_prompt_attention_workspace_bytes(int rows, int k_rows, int heads, int kv_heads, int head_dim, int sequences, int window, int sinks);
 int sharq_prompt_attention(const void *q_bf16, int64_t q_row, int64_t q_head, const void *k_bf16, int64_t k_row, int64_t k_head,
                            const void *v_bf16, int64_t v_row, int64_t v_head, int rows, int k_rows, int heads, int kv_heads, int head_dim,
                            const int *offsets, const int *k_offsets, int sequences, int window, int sinks, float scale, void *out_bf16,
-                           int fill, int *error_flag, void *stream);
+                           int fill, void *workspace, size_t workspace_bytes, int *error_flag, void *stream);
 
 /* Pages and places of a step's tokens, from lengths on the device.  Sequence i holds lengths[i] tokens in the first
  * ceil(lengths[i] / page_size) pages of its row of page_table [sequences, max_pages] (page_table_stride entries between rows); the free pages are

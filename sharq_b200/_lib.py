@@ -107,7 +107,8 @@ SIGNATURES = {
         c_int, [_P, c_int64, c_int64, c_int, _P, _P, c_float, c_int, c_int, _P, _P, c_size_t, _P, _P]),
     "sharq_prompt_attention": (
         c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, _P, _P, c_int, c_int,
-                c_int, c_float, _P, c_int, _P, _P]),
+                c_int, c_float, _P, c_int, _P, c_size_t, _P, _P]),
+    "sharq_prompt_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "sharq_plan_paged_step": (
         c_int, [_P, c_int64, c_int, c_int, c_int, c_int, _P, _P, _P, _P, c_int, _P, c_int, _P, _P, _P, _P, _P]),
     "sharq_adjust_logits": (c_int, [_P, c_int64, _P, c_int64, c_int, c_int, c_int, _P, _P, _P]),

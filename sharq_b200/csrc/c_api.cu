@@ -835,10 +835,28 @@ int sharq_paged_attention_windowed(const void *q_bf16, int64_t q_row, int64_t q_
                     "paged_attention");
 }
 
+static void prompt_window(int window, int sinks, sharq::PromptAttention *p) {  // 0: none
+  p->window = window == 0 || window > 1 << 30 ? 1 << 30 : window;
+  p->sinks = window == 0 ? 0 : sinks;
+}
+
+size_t sharq_prompt_attention_workspace_bytes(int rows, int k_rows, int heads, int kv_heads, int head_dim, int sequences, int window, int sinks) {
+  if (rows < 1 || k_rows < 1 || kv_heads < 1 || heads < 1 || heads % kv_heads != 0 || sequences < 1 || window < 0 || sinks < 0) return 0;
+  sharq::PromptAttention p = {};
+  p.rows = rows;
+  p.k_rows = k_rows;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.head_dim = head_dim;
+  p.seqs = sequences;
+  prompt_window(window, sinks, &p);
+  return sharq::prompt_attention_workspace_bytes(p);
+}
+
 int sharq_prompt_attention(const void *q_bf16, int64_t q_row, int64_t q_head, const void *k_bf16, int64_t k_row, int64_t k_head,
                            const void *v_bf16, int64_t v_row, int64_t v_head, int rows, int k_rows, int heads, int kv_heads, int head_dim,
                            const int *offsets, const int *k_offsets, int sequences, int window, int sinks, float scale, void *out_bf16,
-                           int fill, int *error_flag, void *stream) {
+                           int fill, void *workspace, size_t workspace_bytes, int *error_flag, void *stream) {
   SHARQ_REQUIRE(q_bf16 && k_bf16 && v_bf16 && offsets && out_bf16, "null buffer");
   SHARQ_REQUIRE(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128, got %d", head_dim);
   SHARQ_REQUIRE(rows >= 1 && rows <= 1 << 30 && k_rows >= 1 && k_rows <= 1 << 30, "rows and k_rows must be in [1, 2^30]");
@@ -850,6 +868,9 @@ int sharq_prompt_attention(const void *q_bf16, int64_t q_row, int64_t q_head, co
   for (const int64_t s : strides)
     SHARQ_REQUIRE(s > 0 && s % 8 == 0 && s < (int64_t)1 << 38, "the strides of q, k and v must be positive multiples of 8");
   SHARQ_REQUIRE(aligned16(q_bf16) && aligned16(k_bf16) && aligned16(v_bf16) && aligned16(out_bf16), "buffers must be 16-byte aligned");
+  const size_t need = sharq_prompt_attention_workspace_bytes(rows, k_rows, heads, kv_heads, head_dim, sequences, window, sinks);
+  SHARQ_REQUIRE(workspace_bytes >= need && (need == 0 || workspace) && (reinterpret_cast<uintptr_t>(workspace) & 31) == 0,
+                "workspace too small or not aligned to 32 bytes: need %zu bytes", need);
   sharq::PromptAttention p = {};
   p.q = q_bf16;
   p.k = k_bf16;
@@ -868,11 +889,11 @@ int sharq_prompt_attention(const void *q_bf16, int64_t q_row, int64_t q_head, co
   p.offsets = offsets;
   p.k_offsets = k_offsets;
   p.seqs = sequences;
-  p.window = window == 0 || window > 1 << 30 ? 1 << 30 : window;
-  p.sinks = window == 0 ? 0 : sinks;
+  prompt_window(window, sinks, &p);
   p.scale = scale;
   p.out = out_bf16;
   p.fill = fill != 0;
+  p.workspace = workspace;
   p.error_flag = error_flag;
   return check_cuda(sharq::run_prompt_attention(p, as_stream(stream)), "prompt_attention");
 }

@@ -96,8 +96,10 @@ struct PromptAttention {
   float scale;
   void *out;
   bool fill;
+  void *workspace;
   int *error_flag;
 };
+size_t prompt_attention_workspace_bytes(const PromptAttention &p);  // from the sizes alone
 cudaError_t run_prompt_attention(const PromptAttention &p, cudaStream_t stream);
 
 // Leave for `bytes` of shared memory, asked for once per kernel and device (ready: a static array per kernel).

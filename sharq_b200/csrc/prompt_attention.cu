@@ -22,6 +22,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "decode_ops.cuh"
@@ -87,15 +88,22 @@ struct Args {
   int window, sinks;  // window: 2^30 for none
   float scale_log2;   // scale * log2(e)
   bool fill;          // rows of no sequence become zeros
+  bool wide;          // out begins at a multiple of 32 bytes
+  bool split;         // items are cut where the CTAs' equal stretches of the list end
+  float *parts;       // split: [2 * CTAs][kBlocks][kTile][head_dim] sums of probabilities times values, then [2 * CTAs][kBlocks][kTile] of their [maximum, sum]
+  int4 *joins;        // split: [CTAs][2] of the item that begins in a CTA's stretch and goes on: {row0, count, first, column}, {parts (0: none), ...}
   int *error_flag;
 };
+constexpr int kItemCost = 3;      // of an item in the list, in tiles, for its queries and its result
+constexpr int kStretchLeast = 8;  // units of a CTA
 
 // What a CTA works on: `count` tokens from row `row0` on, the first at position `first`, of heads kv and chunk.  Their keys are a list of `s_pad` first ones
-// and those from position `base` on, of which there are `total` in all, in `tiles` tiles.
+// and those from position `base` on, of which there are `total` in all, in `tiles` tiles; the CTA takes those from `begin` to `end`.
 struct Item {
   int state;  // 0: no more items, 1: an item, 2: one whose keys are not known (its rows come out as NaN)
   int row0, count, first, kv, chunk;
   int k_row0, base, s_pad, total, tiles;
+  int begin, end, place;  // place: of the part that it leaves, -1 where it has all tiles
 };
 
 __device__ __forceinline__ void set_keys(Item &it, int keys, int window, int sinks) {
@@ -168,6 +176,12 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
   uint64_t v;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
   return v;
+}
+
+__device__ __forceinline__ void st_global32(void *to, const uint32_t *w) {  // 32 bytes at a multiple of 32
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+               "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -400,13 +414,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     unsigned tiles_done = 0, values_done = 0, items_done = 0;  // for the barriers' parities: of this block, of all, of this block
     bool ok = true;
-    for (int n = 0; ok && next_item_of_warp(n); values_done += items[n % kItemSlots].tiles, leave_item(n), ++n) {
+    for (int n = 0; ok && next_item_of_warp(n); values_done += items[n % kItemSlots].end - items[n % kItemSlots].begin, leave_item(n), ++n) {
       const Item &it = items[n % kItemSlots];  // stays in shared memory, for want of registers
       if (it.count <= block * a.tokens) continue;  // nothing for this block
       const int position = it.first + min(block * a.tokens + token, it.count - 1);
       const Seen seen = seen_by(it, position, a.window, a.sinks);
       float m = -INFINITY, l = 0.0f;  // maximum in powers of two, sum
-      for (int tile = 0; tile < it.tiles; ++tile) {
+      for (int tile = it.begin; tile < it.end; ++tile) {
         if (!wait_for(s_full + block, tiles_done++ & 1, abort_flag)) {
           give_up();
           ok = false;
@@ -447,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float f = raise ? exp2_approx(m - high) : 1.0f;  // from -inf: 0, and nothing to keep
           if (raise) m = high;
           l *= f;
-          if (tile > 0) {
+          if (tile > it.begin) {
 #pragma unroll 1
             for (int i = 0; i < D; i += 16) {
               uint32_t o[16];
@@ -489,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         tmem_st_wait();
         if (masked) {
-          const unsigned value = values_done + tile;
+          const unsigned value = values_done + tile - it.begin;
           if (!wait_for(v_ok + value % kStages, (value / kStages) & 1, abort_flag)) {
             give_up();
             ok = false;
@@ -499,16 +513,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           if ((not_finite[value % kStages * kCheckWarps] | not_finite[value % kStages * kCheckWarps + 1]) != 0)
             multiply_visible<D>(tmem_s, tmem_o, ring + (2 * value + 1) % kStages * S::kBytes,
-                                Seen{seen.low - tile * kTile, seen.high - tile * kTile, seen.sinks - tile * kTile}, tile == 0);
+                                Seen{seen.low - tile * kTile, seen.high - tile * kTile, seen.sinks - tile * kTile}, tile == it.begin);
         }
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(p_full + block);
       }
       if (!ok) break;
-      const int t = block * a.tokens + token, tiles = it.tiles, state = it.state;
+      const int t = block * a.tokens + token, tiles = it.end - it.begin, state = it.state;
       const bool there = token < a.tokens && t < it.count && it.chunk * a.chunk_heads + head < a.group;
-      if (it.tiles > 0) {
+      if (tiles > 0) {
         if (!wait_for(o_full + block, items_done++ & 1, abort_flag)) {
           give_up();
           ok = false;
@@ -517,6 +531,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ptx::tc_fence_after();
+      }
+      if (it.place >= 0) {  // a part, to be joined with those of other CTAs
+        const long long at = ((long long)it.place * kBlocks + block) * kTile + row;
+        float *part = a.parts + at * D;
+#pragma unroll 1
+        for (int i = 0; i < D; i += 32) {
+          uint32_t o[32];
+          ptx::tmem_ld_32x32b_x32(tmem_o + i, o);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) st_global32(part + i + j, &o[j]);
+        }
+        reinterpret_cast<float2 *>(a.parts + 2LL * gridDim.x * kBlocks * kTile * D)[at] = make_float2(m, l);
+        ptx::tc_fence_before();
+        continue;
       }
       __nv_bfloat16 *out = a.out + ((long long)(it.row0 + t) * a.heads + it.kv * a.group + it.chunk * a.chunk_heads + head) * D;
       const float f = 1.0f / l;
@@ -536,10 +565,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (position < 0 || tiles == 0) w[e] = 0;
             if (state == 2) w[e] = 0x7fff7fffu;
           }
-          if (there)
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + i + j), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-                         "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                         : "memory");
+          if (there && a.wide) {
+            st_global32(out + i + j, w);
+          } else if (there) {
+            *reinterpret_cast<uint4 *>(out + i + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4 *>(out + i + j + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
         }
         __syncwarp();
       }
@@ -548,63 +579,142 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     if (warp == kLoadWarp) {
-      // blocks of two times `tokens` tokens, of all sequences
-      const int span = kBlocks * a.tokens;
-      int blocks = 0, reached = 0;
+      // blocks of two times `tokens` tokens, of all sequences, times heads: the list of items
+      const int span = kBlocks * a.tokens, columns = a.kv_heads * a.chunks;
       bool bad = false;
+      // the block `index` of rows [from, to) with keys [k0, k1)
+      auto describe = [&](Item &it, int from, int to, int k0, int k1, int index) {
+        const bool known = k0 >= 0 && k0 <= k1 && k1 <= a.k_rows;
+        it.state = known ? 1 : 2;
+        it.row0 = from + index * span;
+        it.count = min(span, to - it.row0);
+        it.k_row0 = k0;
+        it.first = (k1 - k0) - (to - from) + index * span;
+        set_keys(it, k1 - k0, a.window, a.sinks);
+        if (!known) it.tiles = 0;
+        it.begin = 0;
+        it.end = it.tiles;
+        it.place = -1;
+      };
+      auto keys_of = [&](int seq0, const Bounds &b) {  // of the lane's sequence
+        const bool given = a.k_offsets != nullptr && seq0 + lane < a.seqs;
+        return given ? make_int2(a.k_offsets[seq0 + lane], a.k_offsets[seq0 + lane + 1]) : make_int2(b.row0, b.row1);
+      };
+      int blocks = 0, reached = 0;
       for (int b0 = 0; b0 < a.seqs; b0 += 32) {
         const Bounds b = bounds_of(a, b0, lane, &reached);
         bad |= b.bad;
         blocks += (b.row1 - b.row0 + span - 1) / span;
       }
       blocks = __reduce_add_sync(0xffffffffu, blocks);
-      const int columns = a.kv_heads * a.chunks;
+      // Whole items: CTAs take turns.  The last block of a sequence first: it sees most.
+      long long turn = blockIdx.x;
+      auto next_whole = [&](Item &it) {
+        it.state = 0;
+        const long long at = turn;
+        turn += gridDim.x;
+        if (at >= (long long)blocks * columns) return;
+        const int block = (int)(at / columns), column = (int)(at - (long long)block * columns);
+        it.kv = column / a.chunks;
+        it.chunk = column - it.kv * a.chunks;
+        int before = 0;
+        reached = 0;
+        for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+          const Bounds b = bounds_of(a, b0, lane, &reached);
+          int ends = (b.row1 - b.row0 + span - 1) / span;
+#pragma unroll
+          for (int off = 1; off < 32; off <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, ends, off);
+            if (lane >= off) ends += up;
+          }
+          const unsigned over = __ballot_sync(0xffffffffu, before + ends > block);
+          if (over != 0) {
+            const int in = __ffs(over) - 1;
+            const int2 k = keys_of(b0, b);
+            describe(it, __shfl_sync(0xffffffffu, b.row0, in), __shfl_sync(0xffffffffu, b.row1, in), __shfl_sync(0xffffffffu, k.x, in),
+                     __shfl_sync(0xffffffffu, k.y, in), before + __shfl_sync(0xffffffffu, ends, in) - 1 - block);
+            return;
+          }
+          before += __shfl_sync(0xffffffffu, ends, 31);
+        }
+      };
+      // Split: the list in units, kItemCost and an item's tiles each.  Finds the item that unit u belongs to -> where it begins; or, u < 0, the list's length.
+      auto find = [&](Item &it, long long u) {
+        long long before = 0;
+        reached = 0;
+        for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+          const Bounds b = bounds_of(a, b0, lane, &reached);
+          const int2 k = keys_of(b0, b);
+          for (int in = 0; in < min(32, a.seqs - b0); ++in) {
+            const int from = __shfl_sync(0xffffffffu, b.row0, in), to = __shfl_sync(0xffffffffu, b.row1, in);
+            const int k0 = __shfl_sync(0xffffffffu, k.x, in), k1 = __shfl_sync(0xffffffffu, k.y, in), count = (to - from + span - 1) / span;
+            for (int i0 = 0; i0 < count; i0 += 32) {
+              long long units = 0;
+              if (i0 + lane < count) {
+                describe(it, from, to, k0, k1, i0 + lane);
+                units = (long long)(kItemCost + max(it.tiles, 1)) * columns;
+              }
+              long long ends = units;
+#pragma unroll
+              for (int off = 1; off < 32; off <<= 1) {
+                const long long up = __shfl_up_sync(0xffffffffu, ends, off);
+                if (lane >= off) ends += up;
+              }
+              const unsigned over = __ballot_sync(0xffffffffu, u >= 0 && before + ends > u);
+              if (over != 0) {
+                const int of = __ffs(over) - 1;
+                const long long start = before + __shfl_sync(0xffffffffu, ends - units, of);
+                describe(it, from, to, k0, k1, i0 + of);
+                const int cost = kItemCost + max(it.tiles, 1), column = (int)((u - start) / cost);
+                it.kv = column / a.chunks;
+                it.chunk = column - it.kv * a.chunks;
+                return start + (long long)column * cost;
+              }
+              before += __shfl_sync(0xffffffffu, ends, 31);
+            }
+          }
+        }
+        return before;
+      };
+      long long unit = 0, unit_end = 0, per = 0;
+      if (a.split) {
+        Item it;
+        const long long total = find(it, -1);
+        per = max((long long)kStretchLeast, (total + gridDim.x - 1) / gridDim.x);
+        unit = min(total, blockIdx.x * per);
+        unit_end = min(total, unit + per);
+        if (lane < 2) a.joins[2 * blockIdx.x + lane] = make_int4(0, 0, 0, 0);
+        __syncwarp();
+      }
+      auto next_part = [&](Item &it) {
+        while (unit < unit_end) {
+          const long long start = find(it, unit);
+          const int tiles = max(it.tiles, 1), skip = (int)(unit - start), left = (int)(unit_end - unit);
+          const int begin = max(0, skip - kItemCost), end = min(tiles, skip + left - kItemCost);
+          unit = start + kItemCost + tiles;
+          if (begin >= end) continue;
+          if (begin > 0 || end < tiles) {
+            it.begin = begin;
+            it.end = end;
+            it.place = 2 * blockIdx.x + (begin == 0 ? 1 : 0);
+            if (begin == 0 && lane == 0) {
+              a.joins[2 * blockIdx.x] = make_int4(it.row0, it.count, it.first, it.kv * a.chunks + it.chunk);
+              a.joins[2 * blockIdx.x + 1] = make_int4(1 + (int)((tiles - end + per - 1) / per), 0, 0, 0);
+            }
+          }
+          return;
+        }
+        it.state = 0;
+      };
       unsigned copies = 0, loads[kBlocks] = {0, 0};
       bool ok = true;
       for (int n = 0; ok; ++n) {
-        const long long at = (long long)blockIdx.x + (long long)n * gridDim.x;
         Item it;
-        it.state = at < (long long)blocks * columns ? 1 : 0;
-        if (it.state != 0) {
-          const int block = (int)(at / columns), column = (int)(at - (long long)block * columns);
-          it.kv = column / a.chunks;
-          it.chunk = column - it.kv * a.chunks;
-          int before = 0;
-          reached = 0;
-          for (int b0 = 0; b0 < a.seqs; b0 += 32) {
-            const Bounds b = bounds_of(a, b0, lane, &reached);
-            int ends = (b.row1 - b.row0 + span - 1) / span;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-              const int up = __shfl_up_sync(0xffffffffu, ends, off);
-              if (lane >= off) ends += up;
-            }
-            const unsigned over = __ballot_sync(0xffffffffu, before + ends > block);
-            if (over != 0) {
-              const int in = __ffs(over) - 1, seq = b0 + in;
-              const int from = __shfl_sync(0xffffffffu, b.row0, in), to = __shfl_sync(0xffffffffu, b.row1, in);
-              const int index = before + __shfl_sync(0xffffffffu, ends, in) - 1 - block;  // the last block first: it sees most
-              it.row0 = from + index * span;
-              it.count = min(span, to - it.row0);
-              int k0 = from, k1 = to;
-              if (a.k_offsets != nullptr) {
-                k0 = a.k_offsets[seq];
-                k1 = a.k_offsets[seq + 1];
-              }
-              const bool known = k0 >= 0 && k0 <= k1 && k1 <= a.k_rows;
-              it.k_row0 = k0;
-              it.first = (k1 - k0) - (to - from) + index * span;
-              set_keys(it, k1 - k0, a.window, a.sinks);
-              if (!known) {
-                bad = true;
-                it.state = 2;
-                it.tiles = 0;
-              }
-              break;
-            }
-            before += __shfl_sync(0xffffffffu, ends, 31);
-          }
-        }
+        if (a.split)
+          next_part(it);
+        else
+          next_whole(it);
+        bad |= it.state == 2;
         const int slot = n % kItemSlots;
         if (lane == 0) {
           if (wait_for(item_empty + slot, ((n / kItemSlots) & 1) ^ 1, abort_flag)) {
@@ -614,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             give_up();
             ok = false;
           }
-          if (ok && it.state != 0 && it.tiles > 0) {
+          if (ok && it.state != 0 && it.end > it.begin) {
             auto fill = [&](int tile, bool of_keys) {
               const int stage = copies % kStages;
               if (!wait_for(kv_empty + stage, ((copies / kStages) & 1) ^ 1, abort_flag)) {
@@ -649,10 +759,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int half = 0; half < S::kHalves; ++half)
                 copy_4d(queries + b * S::kBytes + half * S::kHalf, &map_q, it.kv * a.group + it.chunk * a.chunk_heads, it.row0 + b * a.tokens, half,
                         q_full + b);
-              if (b == 0) fill(0, true);
+              if (b == 0) fill(it.begin, true);
             }
-            for (int tile = 0; tile < it.tiles && ok; ++tile) {
-              if (tile > 0) fill(tile, true);
+            for (int tile = it.begin; tile < it.end && ok; ++tile) {
+              if (tile > it.begin) fill(tile, true);
               if (ok) fill(tile, false);
             }
           }
@@ -680,7 +790,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int n = 0; ok && next_item(n); ++n) {
           const Item it = items[n % kItemSlots];
           ptx::mbar_arrive(item_empty + n % kItemSlots);
-          if (it.tiles == 0) continue;
+          const int tiles = it.end - it.begin;
+          if (tiles == 0) continue;
           const int active = it.count > a.tokens ? 2 : 1;
           auto scores = [&](int b, unsigned copy, bool last) {  // S of block b and the tile that is copy `copy`
             const uint32_t keys = ring + copy % kStages * S::kBytes;
@@ -697,14 +808,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!wait(q_full + b, loads[b]++)) break;
             if (b == 0 && !wait(kv_full + copies % kStages, copies / kStages)) break;
             ptx::tc_fence_after();
-            scores(b, copies, it.tiles == 1);
+            scores(b, copies, tiles == 1);
           }
           if (!ok) break;
           ptx::tc_commit<1>(kv_empty + copies % kStages);
           ++copies;
-          for (int tile = 0; tile < it.tiles && ok; ++tile) {
+          for (int tile = 0; tile < tiles && ok; ++tile) {
             const unsigned value = copies, next = copies + 1;
-            const bool more = tile + 1 < it.tiles;
+            const bool more = tile + 1 < tiles;
             if (!wait(kv_full + value % kStages, value / kStages)) break;
             if (!wait(v_ok + values % kStages, values / kStages)) break;
             const bool by_rows = (not_finite[values % kStages * kCheckWarps] | not_finite[values % kStages * kCheckWarps + 1]) != 0;
@@ -727,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               ++probs[b];
               if (b + 1 == active) ptx::tc_commit<1>(kv_empty + value % kStages);
               if (more)
-                scores(b, next, tile + 2 == it.tiles);
+                scores(b, next, tile + 2 == tiles);
               else
                 ptx::tc_commit<1>(o_full + b);
             }
@@ -749,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int n = 0; ok && next_item_of_warp(n); ++n) {
         const Item it = items[n % kItemSlots];
         leave_item(n);
-        for (int tile = 0; tile < it.tiles; ++tile, copies += 2, ++values) {
+        for (int tile = it.begin; tile < it.end; ++tile, copies += 2, ++values) {
           const unsigned copy = copies + 1;
           ok = wait_for(kv_full + copy % kStages, (copy / kStages) & 1, abort_flag);
           if (!ok) give_up();
@@ -786,6 +897,55 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Joins the parts of the items that begin in one CTA's stretch and end in a later one's, in the order of the list: the result does not depend on timing.  A warp
+// takes a row.
+constexpr int kJoinWarps = 8, kJoinSlices = 8;
+
+template <int D>
+__global__ void __launch_bounds__(32 * kJoinWarps) prompt_attention_join_kernel(const __grid_constant__ Args a, int ctas) {
+  ptx::grid_dependency_wait();
+  const int4 item = a.joins[2 * blockIdx.x];
+  const int parts = min(a.joins[2 * blockIdx.x + 1].x, ctas - (int)blockIdx.x), lane = threadIdx.x & 31;
+  if (parts < 2) return;
+  const int kv = item.w / a.chunks, chunk = item.w - kv * a.chunks;
+  const float2 *ml = reinterpret_cast<const float2 *>(a.parts + 2LL * ctas * kBlocks * kTile * D);
+  for (int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); row < kBlocks * kTile; row += kJoinSlices * kJoinWarps) {
+    const int block = row / kTile, token = row % kTile / a.chunk_heads, head = row % kTile % a.chunk_heads, t = block * a.tokens + token;
+    if (token >= a.tokens || t >= item.y || chunk * a.chunk_heads + head >= a.group) continue;
+    float top = -INFINITY, sum = 0.0f, acc[D / 32];
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) acc[e] = 0.0f;
+    for (int i = 0; i < parts; ++i) {
+      const long long at = (2LL * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kBlocks * kTile + row;
+      const float2 of = ml[at];
+      const float *x = a.parts + at * D + lane * (D / 32);
+      // NaN in a maximum makes all NaN; -inf: nothing there, and nothing to keep
+      const float high = of.x > top ? of.x : of.x != of.x ? of.x : top;
+      const float f_old = top == high ? 1.0f : exp2_approx(top - high), f = of.x == high ? 1.0f : exp2_approx(of.x - high);
+      top = high;
+      sum = sum * f_old + of.y * f;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) acc[e] = acc[e] * f_old + x[e] * f;
+    }
+    __nv_bfloat16 *out = a.out + ((long long)(item.x + t) * a.heads + kv * a.group + chunk * a.chunk_heads + head) * D + lane * (D / 32);
+    const float f = 1.0f / sum;
+#pragma unroll
+    for (int e = 0; e < D / 32; e += 2)
+      *reinterpret_cast<uint32_t *>(out + e) = item.z + t < 0 ? 0 : pack_bf16(acc[e] * f, acc[e + 1] * f);
+  }
+}
+
+// Whether items are cut: where there are few, of many tiles each, from sizes of tensors alone.  @SPLITRULE@
+bool is_split(const PromptAttention &p, const Args &a, int sms) {
+  const long long span = kBlocks * a.tokens, items = (p.rows / span + p.seqs) * a.kv_heads * a.chunks;
+  const long long keys = std::min<long long>(p.k_rows / p.seqs, (long long)a.window + a.sinks + span);
+  return items < 4LL * sms && p.seqs <= 128 && keys >= 8 * kTile;
+}
+
+size_t split_bytes(int head_dim, int ctas) {
+  return 2 * (size_t)ctas * kBlocks * kTile * (head_dim + 2) * sizeof(float) + 2 * (size_t)ctas * sizeof(int4);
+}
+
 bool encode(CUtensorMap *map, const void *base, int rows, int heads, int halves, long long row_stride, long long head_stride, bool heads_first,
             int box_rows, int box_heads, int box_halves) {
   // [128 bytes][heads][rows][halves] for the queries, [128 bytes][rows][halves][heads] for keys and values; strides in elements
@@ -800,40 +960,7 @@ bool encode(CUtensorMap *map, const void *base, int rows, int heads, int halves,
   return make_tensor_map(map, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int D>
-cudaError_t launch(const PromptAttention &p, const Args &a, int sms, cudaStream_t stream) {
-  using S = Sizes<D>;
-  CUtensorMap q, k, v, k8, v8;
-  if (!encode(&q, p.q, p.rows, p.heads, S::kHalves, p.q_row, p.q_head, true, a.tokens, a.chunk_heads, 1) ||
-      !encode(&k, p.k, p.k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, kTile, 1, S::kHalves) ||
-      !encode(&v, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, kTile, 1, S::kHalves) ||
-      !encode(&k8, p.k, p.k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, 8, 1, 1) ||
-      !encode(&v8, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, 8, 1, 1))
-    return cudaErrorInvalidValue;
-  static bool ready[64] = {};
-  const cudaError_t err = allow_smem(prompt_attention_kernel<D>, S::kTotal, ready);
-  if (err != cudaSuccess) return err;
-  const long long most = ((long long)p.rows / (kBlocks * a.tokens) + p.seqs) * a.kv_heads * a.chunks;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)(most < sms ? most : sms));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = S::kTotal;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, prompt_attention_kernel<D>, q, k, v, k8, v8, a);
-}
-
-}  // namespace
-
-cudaError_t run_prompt_attention(const PromptAttention &p, cudaStream_t stream) {
-  int dev = 0, sms = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (err != cudaSuccess) return err;
+Args args_of(const PromptAttention &p) {
   Args a = {};
   a.offsets = p.offsets;
   a.k_offsets = p.k_offsets;
@@ -851,8 +978,64 @@ cudaError_t run_prompt_attention(const PromptAttention &p, cudaStream_t stream) 
   a.sinks = p.sinks;
   a.scale_log2 = p.scale * 1.4426950408889634f;
   a.fill = p.fill;
+  a.wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
   a.error_flag = p.error_flag;
-  return p.head_dim == 128 ? launch<128>(p, a, sms, stream) : launch<64>(p, a, sms, stream);
+  return a;
+}
+
+template <int D>
+cudaError_t launch(const PromptAttention &p, Args a, int sms, cudaStream_t stream) {
+  using S = Sizes<D>;
+  CUtensorMap q, k, v, k8, v8;
+  if (!encode(&q, p.q, p.rows, p.heads, S::kHalves, p.q_row, p.q_head, true, a.tokens, a.chunk_heads, 1) ||
+      !encode(&k, p.k, p.k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, kTile, 1, S::kHalves) ||
+      !encode(&v, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, kTile, 1, S::kHalves) ||
+      !encode(&k8, p.k, p.k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, 8, 1, 1) ||
+      !encode(&v8, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, 8, 1, 1))
+    return cudaErrorInvalidValue;
+  static bool ready[64] = {};
+  cudaError_t err = allow_smem(prompt_attention_kernel<D>, S::kTotal, ready);
+  if (err != cudaSuccess) return err;
+  const long long most = ((long long)p.rows / (kBlocks * a.tokens) + p.seqs) * a.kv_heads * a.chunks;
+  a.split = is_split(p, a, sms);
+  const int ctas = !a.split && most < sms ? (int)most : sms;
+  if (a.split) {
+    a.parts = static_cast<float *>(p.workspace);
+    a.joins = reinterpret_cast<int4 *>(a.parts + 2LL * ctas * kBlocks * kTile * (D + 2));
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kTotal;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  err = cudaLaunchKernelEx(&cfg, prompt_attention_kernel<D>, q, k, v, k8, v8, a);
+  if (err != cudaSuccess || !a.split) return err;
+  cfg.gridDim = dim3((unsigned)ctas, kJoinSlices);
+  cfg.blockDim = dim3(32 * kJoinWarps);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, prompt_attention_join_kernel<D>, a, ctas);
+}
+
+int sm_count() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return sms;
+}
+
+}  // namespace
+
+size_t prompt_attention_workspace_bytes(const PromptAttention &p) {
+  const int sms = sm_count();
+  return is_split(p, args_of(p), sms) ? split_bytes(p.head_dim, sms) : 0;
+}
+
+cudaError_t run_prompt_attention(const PromptAttention &p, cudaStream_t stream) {
+  return p.head_dim == 128 ? launch<128>(p, args_of(p), sm_count(), stream) : launch<64>(p, args_of(p), sm_count(), stream);
 }
 
 }  // namespace sharq

@@ -128,6 +128,69 @@ def test_heads_of_a_group(group):
     ops.check_device_errors()
 
 
+SPLIT = [([1], [5000], 8, 2, 128), ([70, 3], [3000, 9000], 8, 2, 64), ([2000], [2000], 4, 1, 128), ([1, 1, 130, 40, 0, 7], [4097, 1, 2222, 9001, 50, 5], 7, 1, 128),
+         ([600, 300], [6600, 1300], 8, 8, 64), ([33], [20000], 2, 2, 128), ([5, 900], [3, 4000], 16, 1, 64)]
+
+
+@pytest.mark.parametrize("lengths,keys,heads,kv_heads,dim", SPLIT)
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1500, 5), (1100, 300)])
+def test_few_queries_with_many_keys(lengths, keys, heads, kv_heads, dim, window, sinks):
+    """Cut into parts that CTAs share."""
+    from sharq_b200 import _lib
+
+    assert _lib.lib().sharq_prompt_attention_workspace_bytes(sum(lengths), sum(keys), heads, kv_heads, dim, len(lengths), window or 0, sinks) > 0
+    q, k, v = inputs(lengths, keys, heads, kv_heads, dim, 7, behind=3)
+    got = ops.prompt_attention(q, k, v, ends(lengths), window=window, sinks=sinks, k_offsets=ends(keys))
+    check(got, q, k, v, lengths, keys, window, sinks)
+    assert (got[sum(lengths):] == 0).all()
+    assert torch.equal(got, ops.prompt_attention(q, k, v, ends(lengths), window=window, sinks=sinks, k_offsets=ends(keys)))
+    ops.check_device_errors()
+
+
+def test_parts_with_values_that_are_not_finite_and_bad_offsets():
+    lengths, keys = [40, 30, 50], [3000, 4000, 2500]
+    q, k, v = inputs(lengths, keys, 4, 2, 128, 3)
+    v[2990, 1, 5], v[3001, 0, 9], v[7100, 1, 3] = math.inf, math.nan, -math.inf
+    got = ops.prompt_attention(q, k, v, ends(lengths), k_offsets=ends(keys))
+    check(got, q, k, v, lengths, keys)
+    q[45, 2, 3] = math.nan
+    got = ops.prompt_attention(q, k, v, ends(lengths), k_offsets=ends(keys))
+    assert got[45, 2].isnan().all()
+    at = ends(keys)
+    at[1] = 9501
+    got = ops.prompt_attention(q, k, v, ends(lengths), k_offsets=at)
+    with pytest.raises(RuntimeError, match="offsets"):
+        ops.check_device_errors()
+    assert got[:70].isnan().all() and not got[70:, :2].isnan().any()
+
+
+def test_parts_in_a_graph_whose_lengths_change():
+    q, k, v = inputs([300], [9000], 8, 2, 128, 4)
+    at, keys = ends([200, 100]), ends([5000, 4000])
+    ops.prompt_attention(q, k, v, at, k_offsets=keys)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.prompt_attention(q, k, v, at, k_offsets=keys)
+    for lengths, m in (([299, 1], [300, 8700]), ([0, 300], [10, 8990]), ([100, 50], [9000, 0]), ([150, 150], [4500, 4500])):
+        at.copy_(ends(lengths))
+        keys.copy_(ends(m))
+        graph.replay()
+        check(got, q, k, v, lengths, m)
+    ops.check_device_errors()
+
+
+def test_an_output_at_any_multiple_of_16_bytes():
+    lengths = [130, 70]
+    q, k, v = inputs(lengths, lengths, 4, 2, 64, 5)
+    want = ops.prompt_attention(q, k, v, ends(lengths))
+    for shift in (8, 16, 24):
+        out = torch.full((200 * 256 + 64,), 3.0, dtype=torch.bfloat16, device="cuda")
+        ops.prompt_attention(q, k, v, ends(lengths), out=out[shift:shift + 200 * 256].view(200, 4, 64))
+        assert torch.equal(out[shift:shift + 200 * 256].view(200, 4, 64), want) and (out[:shift] == 3).all() and (out[shift + 200 * 256:] == 3).all()
+    with pytest.raises(RuntimeError, match="16-byte"):
+        ops.prompt_attention(q, k, v, ends(lengths), out=out[4:4 + 200 * 256].view(200, 4, 64))
+
+
 def test_many_sequences():
     g = torch.Generator().manual_seed(3)
     lengths = (torch.rand(700, generator=g) ** 4 * 90).int().tolist()
