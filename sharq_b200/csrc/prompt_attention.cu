@@ -23,6 +23,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 #include "decode_ops.cuh"
@@ -912,20 +913,24 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prompt_attention_join_kernel(
   for (int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); row < kBlocks * kTile; row += kJoinSlices * kJoinWarps) {
     const int block = row / kTile, token = row % kTile / a.chunk_heads, head = row % kTile % a.chunk_heads, t = block * a.tokens + token;
     if (token >= a.tokens || t >= item.y || chunk * a.chunk_heads + head >= a.group) continue;
-    float top = -INFINITY, sum = 0.0f, acc[D / 32];
+    auto place = [&](int i) { return (2LL * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kBlocks * kTile + row; };
+    // the maximum first, so that the parts are read without waiting for one another (one that is not a number has such a sum, too)
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, ml[place(i)].x);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    float sum = 0.0f, acc[D / 32];
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) acc[e] = 0.0f;
+#pragma unroll 4
     for (int i = 0; i < parts; ++i) {
-      const long long at = (2LL * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kBlocks * kTile + row;
+      const long long at = place(i);
       const float2 of = ml[at];
       const float *x = a.parts + at * D + lane * (D / 32);
-      // NaN in a maximum makes all NaN; -inf: nothing there, and nothing to keep
-      const float high = of.x > top ? of.x : of.x != of.x ? of.x : top;
-      const float f_old = top == high ? 1.0f : exp2_approx(top - high), f = of.x == high ? 1.0f : exp2_approx(of.x - high);
-      top = high;
-      sum = sum * f_old + of.y * f;
+      const float f = of.x == top ? 1.0f : exp2_approx(of.x - top);  // also where all are -inf: sums of nothing
+      sum += of.y * f;
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) acc[e] = acc[e] * f_old + x[e] * f;
+      for (int e = 0; e < D / 32; ++e) acc[e] += x[e] * f;
     }
     __nv_bfloat16 *out = a.out + ((long long)(item.x + t) * a.heads + kv * a.group + chunk * a.chunk_heads + head) * D + lane * (D / 32);
     const float f = 1.0f / sum;
@@ -935,11 +940,15 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prompt_attention_join_kernel(
   }
 }
 
-// Whether items are cut: where there are few, of many tiles each, from sizes of tensors alone.  @SPLITRULE@
+// Whether items are cut, from sizes of tensors alone: where what it costs (the parts' way to memory and back and the second launch, as much as some 20 tiles of 128 or 10
+// of 64) is less than what CTAs wait for the one with the most tiles, as far as the average sequence tells.  Whole / cut, us, 32 / 8 heads of 128: 64 queries behind 8000
+// keys 126 / 46, 512 behind 30000 455 / 243; four pieces of 500 behind 1000 149 / 160, a prompt of 2048 56 / 59; 8 heads of 64, 4095 behind 6000 137 / 121.
 bool is_split(const PromptAttention &p, const Args &a, int sms) {
-  const long long span = kBlocks * a.tokens, items = (p.rows / span + p.seqs) * a.kv_heads * a.chunks;
-  const long long keys = std::min<long long>(p.k_rows / p.seqs, (long long)a.window + a.sinks + span);
-  return items < 4LL * sms && p.seqs <= 128 && keys >= 8 * kTile;
+  const double span = kBlocks * a.tokens, items = (std::floor(p.rows / span) + p.seqs) * a.kv_heads * a.chunks, turns = items / sms;
+  const double keys = (double)p.k_rows / p.seqs, ahead = std::max(0.0, keys - (double)p.rows / p.seqs), seen = (double)a.window + a.sinks;
+  const double most = std::min(keys, seen + span) / kTile, average = std::min(ahead + 0.5 * (keys - ahead), seen) / kTile + 0.5;
+  const double whole = turns <= 1 ? most : std::max(most, (turns + 0.5) * average), cut = turns * average + (p.head_dim == 128 ? 20 : 10);
+  return p.seqs <= 128 && whole > cut;
 }
 
 size_t split_bytes(int head_dim, int ctas) {
