@@ -179,11 +179,12 @@ __global__ void __launch_bounds__(kThreads, 2) logit_rules_kernel(const __grid_c
     if (!stays(at)) return;
     double bias = (double)value;
     if ((twice[at >> 5] >> (at & 31) & 1) != 0) {  // one of several: the first of them adds all up, in their order
+      auto is = [&](int k) { return (unsigned)a.bias_ids[k] - (unsigned)first == (unsigned)at; };
       int k = bias0;
-      while (a.bias_ids[k] - first != at) ++k;
+      while (!is(k)) ++k;
       if (k != j) return;
       for (++k; k < bias1; ++k)
-        if (a.bias_ids[k] - first == at) bias += (double)a.bias_values[k];
+        if (is(k)) bias += (double)a.bias_values[k];
     }
     out[at] = rounded<T>(penalised(widened<T>(x), words[at], penalty) + bias);
   };

@@ -555,7 +555,7 @@ def _attention(qkv: torch.Tensor, b: int, s: int, heads: int, kv_heads: int, d: 
                                        sinks=sinks).view(b * s, heads * d)
         q, k = (x.view(b, s, -1, d).transpose(1, 2) for x in got)
         v = qkv[:, (heads + kv_heads) * d:].view(b, s, kv_heads, d).transpose(1, 2)
-    if window > 0 and fused and qkv.is_cuda:
+    if window > 0 and fused and qkv.is_cuda and d in (64, 128):
         offsets = torch.arange(0, b * s + 1, s, dtype=torch.int32, device=qkv.device)
         q, k, v = (x.transpose(1, 2).flatten(0, 1) for x in (q, k, v))  # views: rows one behind the other
         return ops.prompt_attention(q, k, v, offsets, window=window, sinks=sinks).view(b * s, heads * d)

@@ -127,7 +127,8 @@ class PagedKVCache:
     def free(self, sequence: int) -> None:
         """Gives the pages of a sequence back; it is empty then, and another prompt may take its place (SharqDecoder.prefill with sequences)."""
         if self.on_device:
-            ended = torch.zeros(self.sequences, dtype=torch.int32, device=self.table.device).index_fill_(0, torch.tensor([sequence], device=self.table.device), 1)
+            ended = torch.zeros(self.sequences, dtype=torch.int32, device=self.table.device)
+            ended[range(self.sequences)[sequence]] = 1  # a number outside is an IndexError here, too
             self.plan(torch.zeros_like(ended), 0, ended.bool())
             return
         self._free += reversed(self._held[sequence])

@@ -32,6 +32,8 @@ class LogitRules:
     def append_(self, token_ids: torch.Tensor) -> None:
         """One more token [rows] of every history.  Where there is no room the last place is overwritten and the length, which adjust_logits
         reports then, goes on."""
+        if self.tokens is None or self.tokens.shape[1] == 0:
+            raise ValueError("there is no history to append to")
         at = self.lengths.long().clamp(0, self.tokens.shape[1] - 1)
         self.tokens.scatter_(1, at[:, None], token_ids.to(self.tokens.dtype)[:, None])
         self.lengths += 1
