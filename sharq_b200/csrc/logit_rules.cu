@@ -197,10 +197,13 @@ __global__ void __launch_bounds__(kThreads, 2) logit_rules_kernel(const __grid_c
 
 template <typename T, typename Id, int kVec>
 cudaError_t launch(LogitRules a, cudaStream_t stream) {
+  static int counts[64] = {};  // SMs of a device
   int dev = 0, sms = 0;
   cudaError_t err = cudaGetDevice(&dev);
-  if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (err == cudaSuccess && dev < 64) sms = counts[dev];
+  if (err == cudaSuccess && sms == 0) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (err != cudaSuccess) return err;
+  if (dev < 64) counts[dev] = sms;
   // Equal slices of a row, as many as its tokens need, or as give every SM a CTA, but of 1024 tokens at least
   const int most = (a.vocab + 1023) / 1024, enough = (a.vocab + kSliceMost - 1) / kSliceMost, wanted = (sms + a.rows - 1) / a.rows;
   const int slices = wanted > most ? most : wanted > enough ? wanted : enough;

@@ -86,6 +86,7 @@ struct Args {
   __nv_bfloat16 *out;
   int rows, k_rows, seqs;
   int heads, kv_heads, group, chunks, chunk_heads, tokens;  // chunk_heads: query heads of a block; tokens: of a block
+  int span;           // tokens of an item: of one block or two
   int window, sinks;  // window: 2^30 for none
   float scale_log2;   // scale * log2(e)
   bool fill;          // rows of no sequence become zeros
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     if (warp == kLoadWarp) {
       // blocks of two times `tokens` tokens, of all sequences, times heads: the list of items
-      const int span = kBlocks * a.tokens, columns = a.kv_heads * a.chunks;
+      const int span = a.span, columns = a.kv_heads * a.chunks;
       bool bad = false;
       // the block `index` of rows [from, to) with keys [k0, k1)
       auto describe = [&](Item &it, int from, int to, int k0, int k1, int index) {
@@ -944,7 +945,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prompt_attention_join_kernel(
 // of 64) is less than what CTAs wait for the one with the most tiles, as far as the average sequence tells.  Whole / cut, us, 32 / 8 heads of 128: 64 queries behind 8000
 // keys 126 / 46, 512 behind 30000 455 / 243; four pieces of 500 behind 1000 149 / 160, a prompt of 2048 56 / 59; 8 heads of 64, 4095 behind 6000 137 / 121.
 bool is_split(const PromptAttention &p, const Args &a, int sms) {
-  const double span = kBlocks * a.tokens, items = (std::floor(p.rows / span) + p.seqs) * a.kv_heads * a.chunks, turns = items / sms;
+  const double span = a.span, items = (std::floor(p.rows / span) + p.seqs) * a.kv_heads * a.chunks, turns = items / sms;
   const double keys = (double)p.k_rows / p.seqs, ahead = std::max(0.0, keys - (double)p.rows / p.seqs), seen = (double)a.window + a.sinks;
   const double most = std::min(keys, seen + span) / kTile, average = std::min(ahead + 0.5 * (keys - ahead), seen) / kTile + 0.5;
   const double whole = turns <= 1 ? most : std::max(most, (turns + 0.5) * average), cut = turns * average + (p.head_dim == 128 ? 20 : 10);
@@ -969,7 +970,7 @@ bool encode(CUtensorMap *map, const void *base, int rows, int heads, int halves,
   return make_tensor_map(map, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-Args args_of(const PromptAttention &p) {
+Args args_of(const PromptAttention &p, int sms) {
   Args a = {};
   a.offsets = p.offsets;
   a.k_offsets = p.k_offsets;
@@ -983,6 +984,9 @@ Args args_of(const PromptAttention &p) {
   a.chunks = (a.group + kTile - 1) / kTile;
   a.chunk_heads = (a.group + a.chunks - 1) / a.chunks;
   a.tokens = kTile / a.chunk_heads;
+  // One block where there are SMs for each: its exponentials share theirs with no other's (200 tokens of 32 / 8 heads 9.9 us instead of 11.3).
+  const long long singles = ((long long)p.rows / a.tokens + p.seqs) * a.kv_heads * a.chunks;
+  a.span = singles <= sms ? a.tokens : kBlocks * a.tokens;
   a.window = p.window;
   a.sinks = p.sinks;
   a.scale_log2 = p.scale * 1.4426950408889634f;
@@ -998,14 +1002,18 @@ cudaError_t launch(const PromptAttention &p, Args a, int sms, cudaStream_t strea
   CUtensorMap q, k, v, k8, v8;
   if (!encode(&q, p.q, p.rows, p.heads, S::kHalves, p.q_row, p.q_head, true, a.tokens, a.chunk_heads, 1) ||
       !encode(&k, p.k, p.k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, kTile, 1, S::kHalves) ||
-      !encode(&v, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, kTile, 1, S::kHalves) ||
-      !encode(&k8, p.k, p.k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, 8, 1, 1) ||
-      !encode(&v8, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, 8, 1, 1))
+      !encode(&v, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, kTile, 1, S::kHalves))
+    return cudaErrorInvalidValue;
+  // copies of 8 keys join the first ones and the window's; without first ones there are none
+  if (p.sinks == 0)
+    k8 = k, v8 = v;
+  else if (!encode(&k8, p.k, p.k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, 8, 1, 1) ||
+           !encode(&v8, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, 8, 1, 1))
     return cudaErrorInvalidValue;
   static bool ready[64] = {};
   cudaError_t err = allow_smem(prompt_attention_kernel<D>, S::kTotal, ready);
   if (err != cudaSuccess) return err;
-  const long long most = ((long long)p.rows / (kBlocks * a.tokens) + p.seqs) * a.kv_heads * a.chunks;
+  const long long most = ((long long)p.rows / a.span + p.seqs) * a.kv_heads * a.chunks;
   a.split = is_split(p, a, sms);
   const int ctas = !a.split && most < sms ? (int)most : sms;
   if (a.split) {
@@ -1031,8 +1039,12 @@ cudaError_t launch(const PromptAttention &p, Args a, int sms, cudaStream_t strea
 }
 
 int sm_count() {
+  static int counts[64] = {};
   int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 148;
+  if (dev < 64 && counts[dev] > 0) return counts[dev];
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  if (dev < 64) counts[dev] = sms;
   return sms;
 }
 
@@ -1040,11 +1052,12 @@ int sm_count() {
 
 size_t prompt_attention_workspace_bytes(const PromptAttention &p) {
   const int sms = sm_count();
-  return is_split(p, args_of(p), sms) ? split_bytes(p.head_dim, sms) : 0;
+  return is_split(p, args_of(p, sms), sms) ? split_bytes(p.head_dim, sms) : 0;
 }
 
 cudaError_t run_prompt_attention(const PromptAttention &p, cudaStream_t stream) {
-  return p.head_dim == 128 ? launch<128>(p, args_of(p), sm_count(), stream) : launch<64>(p, args_of(p), sm_count(), stream);
+  const int sms = sm_count();
+  return p.head_dim == 128 ? launch<128>(p, args_of(p, sms), sms, stream) : launch<64>(p, args_of(p, sms), sms, stream);
 }
 
 }  // namespace sharq
