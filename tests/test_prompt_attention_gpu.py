@@ -135,17 +135,22 @@ SPLIT = [([1], [5000], 8, 2, 128), ([70, 3], [3000, 9000], 8, 2, 64), ([3500], [
 @pytest.mark.parametrize("lengths,keys,heads,kv_heads,dim", SPLIT)
 @pytest.mark.parametrize("window,sinks", [(None, 0), (3000, 5), (2700, 300)])
 def test_few_queries_with_many_keys(lengths, keys, heads, kv_heads, dim, window, sinks):
-    """Cut into parts that CTAs share."""
-    from sharq_b200 import _lib
-
-    parts = _lib.lib().sharq_prompt_attention_workspace_bytes(sum(lengths), sum(keys), heads, kv_heads, dim, len(lengths), window or 0, sinks) > 0
-    assert parts or window
+    """Most of them cut into parts that CTAs share."""
     q, k, v = inputs(lengths, keys, heads, kv_heads, dim, 7, behind=3)
     got = ops.prompt_attention(q, k, v, ends(lengths), window=window, sinks=sinks, k_offsets=ends(keys))
     check(got, q, k, v, lengths, keys, window, sinks)
     assert (got[sum(lengths):] == 0).all()
     assert torch.equal(got, ops.prompt_attention(q, k, v, ends(lengths), window=window, sinks=sinks, k_offsets=ends(keys)))
     ops.check_device_errors()
+
+
+def test_which_are_cut():
+    from sharq_b200 import _lib
+
+    size = _lib.lib().sharq_prompt_attention_workspace_bytes
+    cut = [size(sum(n), sum(m), heads, kv_heads, dim, len(n), 0, 0) > 0 for n, m, heads, kv_heads, dim in SPLIT]
+    assert cut == [True, True, False, True, True, True, False]
+    assert size(120, 9500, 4, 2, 128, 3, 0, 0) > 0 and size(300, 9000, 8, 2, 128, 2, 0, 0) > 0  # of the two tests below
 
 
 def test_parts_with_values_that_are_not_finite_and_bad_offsets():
