@@ -8,6 +8,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContextLight.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -48,6 +49,18 @@ inline void *stream_of(const Tensor &t) { return c10::cuda::getCurrentCUDAStream
 
 inline Tensor empty_like_on(const Tensor &ref, at::IntArrayRef sizes, at::ScalarType type) {
   return at::empty(sizes, ref.options().dtype(type).layout(at::kStrided).requires_grad(false));
+}
+
+// ... made without the dispatcher, which takes a microsecond of the six that a small call takes on the host.  The device must be the current one.
+inline Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) {
+  int64_t n = 1;
+  for (const int64_t s : sizes) n *= s;
+  const size_t bytes = (size_t)n * c10::elementSize(type);
+  c10::Allocator *from = c10::cuda::CUDACachingAllocator::get();
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(c10::Storage::use_byte_size_t(), bytes, from->allocate(bytes), from, true),
+                                                      c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
 }
 
 inline bool is_plain(const Tensor &t, at::ScalarType type) { return t.is_cuda() && t.scalar_type() == type && t.is_contiguous(); }
@@ -518,13 +531,13 @@ Tensor paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_c
     need(is_plain(*out, at::kBFloat16) && out->device() == dev && out->sizes() == q.sizes(),
          "out must be a contiguous CUDA bfloat16 tensor shaped like q");
   c10::cuda::OptionalCUDAGuard guard(dev);
-  Tensor o = out ? *out : empty_like_on(q, {seqs, heads, d}, at::kBFloat16);
+  Tensor o = out ? *out : fresh({seqs, heads, d}, at::kBFloat16);
   if (seqs == 0) return o;
   sharq_paged_cache used = c;
   used.sequences = (int)seqs;
   const int64_t ws_bytes = (int64_t)sharq_paged_attention_windowed_workspace_bytes((int)heads, &used, w, first);
   Tensor ws;
-  if (ws_bytes > 0) ws = empty_like_on(q, {ws_bytes}, at::kByte);
+  if (ws_bytes > 0) ws = fresh({ws_bytes}, at::kByte);
   check(sharq_paged_attention_windowed(ptr(q), seqs > 1 ? q.stride(0) : 0, heads > 1 ? q.stride(1) : 0, (int)heads, &used,
                                        static_cast<const int *>(ptr(lengths)), (float)(scale ? *scale : 1.0 / std::sqrt((double)d)), w, first, ptr(o),
                                        ws_bytes > 0 ? ptr(ws) : nullptr, (size_t)ws_bytes, flag_of(flag), stream_of(q)));
@@ -591,14 +604,14 @@ Tensor prompt_attention(const Tensor &q, const Tensor &k, const Tensor &v, const
         fail(std::string("strides of ") + "qkv"[i] + " must be positive multiples of 8");
     }
   c10::cuda::OptionalCUDAGuard guard(dev);
-  Tensor o = out ? *out : empty_like_on(q, {rows, heads, d}, at::kBFloat16);
+  Tensor o = out ? *out : fresh({rows, heads, d}, at::kBFloat16);
   if (rows == 0) return o;
   // without any key there is nothing to read: the queries stand for keys that no sequence has
   const Tensor &keys = k_rows > 0 ? k : q, &values = k_rows > 0 ? v : q;
   const int first = (int)std::min<int64_t>(sinks, INT32_MAX), most = (int)std::max<int64_t>(k_rows, 1);
   const int64_t ws_bytes = (int64_t)sharq_prompt_attention_workspace_bytes((int)rows, most, (int)heads, (int)kv_heads, (int)d, (int)offsets.size(0) - 1, w, first);
   Tensor ws;
-  if (ws_bytes > 0) ws = empty_like_on(q, {ws_bytes}, at::kByte);
+  if (ws_bytes > 0) ws = fresh({ws_bytes}, at::kByte);
   check(sharq_prompt_attention(ptr(q), strides[0][0], strides[0][1], ptr(keys), strides[1][0], strides[1][1], ptr(values), strides[2][0], strides[2][1],
                                (int)rows, most, (int)heads, (int)kv_heads, (int)d, static_cast<const int *>(ptr(offsets)),
                                k_offsets ? static_cast<const int *>(ptr(*k_offsets)) : nullptr, (int)offsets.size(0) - 1, w,
@@ -631,7 +644,7 @@ std::vector<Tensor> plan_paged_step(const Tensor &table, const Tensor &lengths, 
   c10::cuda::OptionalCUDAGuard guard(dev);
   // the parts begin at multiples of 16 bytes, and are made without the dispatcher
   const int64_t at_rows = (n + 4) & ~int64_t(3), padded = (rows + 3) & ~int64_t(3);
-  const Tensor out = empty_like_on(table, {at_rows + 2 * padded}, at::kInt);
+  const Tensor out = fresh({at_rows + 2 * padded}, at::kInt);
   int *at = static_cast<int *>(ptr(out));
   auto part = [&](int64_t offset, int64_t size) {
     Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(out.storage()), out.key_set(), c10::scalarTypeToTypeMeta(at::kInt));
@@ -717,7 +730,7 @@ Tensor adjust_logits(const Tensor &logits, const OptionalTensor &tokens, const O
     need(rows <= 1 || out->stride(0) == logits.stride(0), "out must be logits or not overlap them");
   }
   c10::cuda::OptionalCUDAGuard guard(dev);
-  Tensor o = out ? *out : empty_like_on(logits, {rows, vocab}, logits.scalar_type());
+  Tensor o = out ? *out : fresh({rows, vocab}, logits.scalar_type());
   if (rows == 0) return o;
   check(sharq_adjust_logits(ptr(logits), rows > 1 ? logits.stride(0) : vocab, ptr(o), rows > 1 ? o.stride(0) : vocab, (int)rows, (int)vocab,
                             logits.scalar_type() == at::kBFloat16, &r, flag_of(flag), stream_of(logits)));
