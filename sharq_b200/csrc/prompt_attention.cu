@@ -1,5 +1,5 @@
 // Attention of ragged prompts: causal, with a sliding window and a few first keys that stay visible.  32768 tokens of 32 / 8 heads of
-// 128 under a window of 4096: 2.05 ms, 1000 TFLOP/s, in long runs, where the card's power is the bound (1.75 ms in a short one); 200 tokens: 11.2 us.
+// 128 under a window of 4096: 2.04 ms, 1010 TFLOP/s, in long runs, where the card's power is the bound (1.75 ms in a short one); 200 tokens: 11.1 us.
 //
 //   out[i, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q[i, h] . k_j - max),   j <= p and (p - j < window or j < sinks),   p the position of query i
 //
@@ -16,6 +16,12 @@
 // more than 2^kLazy, for the raise is a pass over O.  Probabilities carry a factor of 2^-32, so that no sum of finite values overflows, and
 // enter the product as bf16, as in the library attention of prompts without a window: off by 2^-9 each, which leaves a result about as near as its own
 // rounding to bf16.  (As two bf16 numbers, as the decode step has them, the second product would be a third more work for the tensor cores.)
+// The second product begins when three quarters of a tile's probabilities are there.  All 128 scores of a row stay in registers, for reading tensor memory
+// again took longer than the exponentials (2726 us instead of then 2085; 32 at a time with the maximum beside the exponentials 2179; a row in two threads,
+// which have to meet twice, 2824).  Exponentials by a polynomial on the units that multiply, for an eighth to a half of them, 2124 to 2473: a warp's instructions
+// follow one another too slowly for more of them to pay, and each takes power.
+//
+// Items go in turns over the CTAs, or, few ones with many tiles, in equal stretches of the list of all tiles, whose ends cut items into parts that a second kernel joins.
 //
 // A masked key has probability 0, which a value that is not finite (another sequence's, or memory that nothing has written) would turn to NaN.  Two
 // warps look for such values in every tile where something is masked; a tile that has one is multiplied row by row, visible keys only, in plain float.
@@ -246,7 +252,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       : "memory");
 }
 
-// 128 bytes of a head x ... of a [128 bytes][rows or heads][...] array; see encode()
+// a box of a map that encode() made, from the beginning of its 128-byte rows on
 __device__ __forceinline__ void copy_4d(uint32_t dst, const CUtensorMap *m, int c1, int c2, int c3, uint64_t *bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),

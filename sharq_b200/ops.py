@@ -15,6 +15,8 @@ Extra ops that the reference does not have (all optional for a drop-in):
   scaled_sparse_residual_quantize_x   prepare with the host-side amax/divide folded in
   rope_append_paged, paged_attention, weight_only_linear   the operators of a decode step: rotary embedding with the append to
                                  a paged key/value cache, attention over it, few unquantised rows times a 4-bit weight
+  prompt_attention, plan_paged_step, adjust_logits   what a server's step has beside those: attention of ragged prompts (sliding window, first keys),
+                                 pages and places of its tokens, penalties, biases and masks on logits
 """
 from __future__ import annotations
 
