@@ -414,7 +414,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool negative = a.scale_log2 < 0.0f;
     const float c = fmaxf(fabsf(a.scale_log2), 1.2e-38f);  // not 0: masked scores are -inf, and stay so
     if (a.fill) {  // rows of no sequence, a share of them per thread
-      const int begin = min(max(a.offsets[0], 0), a.rows), end = min(max(a.offsets[a.seqs], 0), a.rows);
+      int begin = a.rows, end = 0;  // what sequences may have, also where some offsets are wrong
+      for (int i = lane; i <= a.seqs; i += 32) {
+        const int at = a.offsets[i];
+        if (at >= 0 && at <= a.rows) begin = min(begin, at), end = max(end, at);
+      }
+      begin = __reduce_min_sync(0xffffffffu, begin);
+      end = __reduce_max_sync(0xffffffffu, end);
       const long long width = (long long)a.heads * D / 8, ahead = begin * width, behind = (long long)max(a.rows - max(end, begin), 0) * width;
       uint4 *out = reinterpret_cast<uint4 *>(a.out);
       for (long long i = (long long)blockIdx.x * (32 * kSoftmaxWarps) + threadIdx.x; i < ahead + behind; i += (long long)gridDim.x * (32 * kSoftmaxWarps))

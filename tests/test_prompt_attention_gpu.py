@@ -312,6 +312,20 @@ def test_offsets_that_cannot_be():
     ops.check_device_errors()
 
 
+@pytest.mark.parametrize("bad,whole", [([0, 100, 60], (0, 100)), ([2 ** 31 - 1, 0, 50], (0, 50)), ([-7, 40, 130], (40, 130)), ([30, 130, -1], (30, 130))])
+def test_rows_of_a_good_sequence_beside_bad_offsets(bad, whole):
+    """They are neither zeros, as rows of no sequence, nor another sequence's."""
+    n = whole[1] - whole[0]
+    q, k, v = inputs([150], [150], 4, 2, 128, 15)
+    rows = slice(*whole)
+    want = ops.prompt_attention(*(x[rows].contiguous() for x in (q, k, v)), ends([n]), window=40, sinks=2)
+    for _ in range(5):
+        got = ops.prompt_attention(q, k, v, torch.tensor(bad, dtype=torch.int32, device="cuda"), window=40, sinks=2)
+        assert torch.equal(got[rows], want) and (got[max(whole[1], *(x for x in bad if x <= 150)):] == 0).all()
+        with pytest.raises(RuntimeError, match="offsets"):
+            ops.check_device_errors()
+
+
 def test_offsets_beyond_32_bits():
     """Elements of the activations beyond 2^31, and rows far into a sequence."""
     heads, dim, n = 160, 128, 110000
