@@ -623,6 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       blocks = __reduce_add_sync(0xffffffffu, blocks);
       // Whole items: CTAs take turns.  The last block of a sequence first: it sees most.
       long long turn = blockIdx.x;
+      int b_now = 0, before_now = 0, reached_now = 0;  // of the 32 sequences that the last item was found among: later ones lie there or behind
       auto next_whole = [&](Item &it) {
         it.state = 0;
         const long long at = turn;
@@ -631,9 +632,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int block = (int)(at / columns), column = (int)(at - (long long)block * columns);
         it.kv = column / a.chunks;
         it.chunk = column - it.kv * a.chunks;
-        int before = 0;
-        reached = 0;
-        for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+        int before = before_now;
+        reached = reached_now;
+        for (int b0 = b_now; b0 < a.seqs; b0 += 32) {
+          const int ahead = reached;
           const Bounds b = bounds_of(a, b0, lane, &reached);
           int ends = (b.row1 - b.row0 + span - 1) / span;
 #pragma unroll
@@ -643,6 +645,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const unsigned over = __ballot_sync(0xffffffffu, before + ends > block);
           if (over != 0) {
+            b_now = b0;
+            before_now = before;
+            reached_now = ahead;
             const int in = __ffs(over) - 1;
             const int2 k = keys_of(b0, b);
             describe(it, __shfl_sync(0xffffffffu, b.row0, in), __shfl_sync(0xffffffffu, b.row1, in), __shfl_sync(0xffffffffu, k.x, in),

@@ -343,6 +343,31 @@ def test_offsets_beyond_32_bits():
     ops.check_device_errors()
 
 
+def test_two_calls_at_once():
+    """On streams of their own, beside one another and beside a product that uses tensor memory too."""
+    lengths = [[700, 90, 1200], [40] * 60]
+    sets = [inputs(n, n, 8, 2, 128, 20 + i) for i, n in enumerate(lengths)]
+    at = [ends(n) for n in lengths]
+    want = [ops.prompt_attention(*x, at[i], window=300, sinks=4) for i, x in enumerate(sets)]
+    w = torch.randn(1024, 512, device="cuda").to(torch.bfloat16)
+    qw, sfs, sfd, scale = ops.scaled_quantize_w32_shared(w)
+    x = torch.randn(300, 512, device="cuda").to(torch.bfloat16)
+    product = ops.sharq_linear_forward(x, qw, sfs, sfd, float(scale))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = [[], [], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.prompt_attention(*sets[i], at[i], window=300, sinks=4))
+        with torch.cuda.stream(streams[2]):
+            got[2].append(ops.sharq_linear_forward(x, qw, sfs, sfd, float(scale)))
+    torch.cuda.synchronize()
+    for a, b in zip(got, (*want, product)):
+        assert all(torch.equal(y, b) for y in a)
+    ops.check_device_errors()
+
+
 def test_captured_and_on_another_stream():
     lengths = [100, 300]
     q, k, v = inputs(lengths, lengths, 4, 2, 128, 14)
