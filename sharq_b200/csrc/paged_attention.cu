@@ -30,6 +30,10 @@
 // two f16 numbers, 21 bits (with one, values that nearly cancel came out several steps off; it costs nothing for 128 sequences of 33 to 8192 tokens, 1 % for
 // 8 x 2048 tokens of 8 heads, 7 % for 20 x 2000).  For bf16 caches they carry a factor of 2^-32, so that no sum of finite values overflows; 2^-94 of the
 // maximum and less is 0.
+//
+// With a window a sequence's tiles are those with a token that is seen, so everything above goes on over a shorter list (an instance of its own: a call without a
+// window runs the code it ran); hidden tokens in the tiles at the window's ends get the score -inf and values of 0.  Window 4096 of 100000 tokens of 8 heads: 12.5 us,
+// as 4096 tokens without one; 96 sequences of up to 12000 in e4m3, window 2048: 58 to 61 us, 0.78 to 0.74 of the rate of a copy.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

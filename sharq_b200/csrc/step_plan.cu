@@ -1,4 +1,4 @@
-// Pages and places of a step's tokens from the sequences' lengths, in one launch.  16 sequences of one token: 4.1 us (a call takes 6.8 on the
+// Pages and places of a step's tokens from the sequences' lengths, in one launch.  16 sequences of one token: 4.1 us (a call takes 6.4 on the
 // host); 1000 sequences, 60 prompts: 11.7 us.
 //
 //   need_i = ceil((length_i + count_i) / P) - ceil(length_i / P),   row r belongs to the i with offsets_i <= r < offsets_i + count_i
