@@ -493,8 +493,9 @@ int sharq_adjust_logits(const void *logits, int64_t logits_stride, void *out, in
                         const sharq_logit_rules *rules, int *error_flag, void *stream);
 
 /* Test/tuning hook: how many SM clock cycles a cross-GPU wait of the all-reduce and transition
- * kernels may take before the kernel gives up, stores its error code and returns (0 restores the
- * defaults of two to ten seconds).  Applies to launches made after the call. */
+ * kernels, or a wait inside the attention of prompts, may take before the kernel gives up, stores its error
+ * code and returns (0 restores the defaults of two to ten seconds, and of one second, which is the most for the
+ * attention of prompts).  Applies to launches made after the call. */
 int sharq_set_wait_limit_cycles(long long cycles);
 
 /* Test/tuning hook: force the GEMM kernel variant (0 = automatic; 128 or 256 = single-CTA kernel

@@ -592,6 +592,7 @@ int sharq_set_wait_limit_cycles(long long cycles) {
   SHARQ_REQUIRE(cycles >= 0, "cycles must be >= 0 (0 restores the defaults)");
   sharq::set_allreduce_wait_limit(cycles);
   sharq::set_sp_transition_wait_limit(cycles);
+  sharq::set_prompt_attention_wait_limit(cycles);
   return 0;
 }
 

@@ -101,6 +101,8 @@ struct PromptAttention {
 };
 size_t prompt_attention_workspace_bytes(const PromptAttention &p);  // from the sizes alone
 cudaError_t run_prompt_attention(const PromptAttention &p, cudaStream_t stream);
+// Clock cycles that a wait inside it may take, of launches from now on; 0: the default, which no other setting exceeds.
+void set_prompt_attention_wait_limit(long long cycles);
 
 // Leave for `bytes` of shared memory, asked for once per kernel and device (ready: a static array per kernel).
 template <typename Kernel>

@@ -65,13 +65,14 @@ __device__ __forceinline__ bool look(uint64_t *bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+// sooner: by how many cycles a wait ends ahead of the usual limit.
+__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, volatile int *abort_flag, long long sooner) {
   if (look(bar, parity)) return true;
   const long long start = clock64();
   while (true) {
     if (look(bar, parity)) return true;
     if (*abort_flag != 0) return false;
-    if (clock64() - start > ptx::kWaitLimitCycles) return false;
+    if (clock64() - start > ptx::kWaitLimitCycles - sooner) return false;
   }
 }
 
@@ -100,6 +101,7 @@ struct Args {
   bool split;         // items are cut where the CTAs' equal stretches of the list end
   float *parts;       // split: [2 * CTAs][kBlocks][kTile][head_dim] sums of probabilities times values, then [2 * CTAs][kBlocks][kTile] of their [maximum, sum]
   int4 *joins;        // split: [CTAs][2] of the item that begins in a CTA's stretch and goes on: {row0, count, first, column}, {parts (0: none), ...}
+  long long sooner;   // see wait_for
   int *error_flag;
 };
 constexpr int kItemCost = 3;      // of an item in the list, in tiles, for its queries and its result
@@ -346,6 +348,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int *not_finite = reinterpret_cast<volatile int *>(items + kItemSlots);  // [kStages][kCheckWarps]
   volatile int *abort_flag = not_finite + kStages * kCheckWarps;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(const_cast<int *>(abort_flag) + 1);
+  unsigned *issued = tmem_slot + 1;  // copies of tiles, and of each block's queries: left here by the load warp when it has ended
+  bool multiplies = false;           // the thread that issues products
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -389,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // whether there is another item, whose description the load warp has left in items[n % kItemSlots]; `n`: how many there have been
   auto next_item = [&](int n) {
     const int slot = n % kItemSlots;
-    if (!wait_for(item_full + slot, (n / kItemSlots) & 1, abort_flag)) {
+    if (!wait_for(item_full + slot, (n / kItemSlots) & 1, abort_flag, a.sooner)) {
       give_up();
       return false;
     }
@@ -435,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Seen seen = seen_by(it, position, a.window, a.sinks);
       float m = -INFINITY, l = 0.0f;  // maximum in powers of two, sum
       for (int tile = it.begin; tile < it.end; ++tile) {
-        if (!wait_for(s_full + block, tiles_done++ & 1, abort_flag)) {
+        if (!wait_for(s_full + block, tiles_done++ & 1, abort_flag, a.sooner)) {
           give_up();
           ok = false;
         }
@@ -518,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st_wait();
         if (masked) {
           const unsigned value = values_done + tile - it.begin;
-          if (!wait_for(v_ok + value % kStages, (value / kStages) & 1, abort_flag)) {
+          if (!wait_for(v_ok + value % kStages, (value / kStages) & 1, abort_flag, a.sooner)) {
             give_up();
             ok = false;
           }
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t = block * a.tokens + token, tiles = it.end - it.begin, state = it.state;
       const bool there = token < a.tokens && t < it.count && it.chunk * a.chunk_heads + head < a.group;
       if (tiles > 0) {
-        if (!wait_for(o_full + block, items_done++ & 1, abort_flag)) {
+        if (!wait_for(o_full + block, items_done++ & 1, abort_flag, a.sooner)) {
           give_up();
           ok = false;
         }
@@ -736,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bad |= it.state == 2;
         const int slot = n % kItemSlots;
         if (lane == 0) {
-          if (wait_for(item_empty + slot, ((n / kItemSlots) & 1) ^ 1, abort_flag)) {
+          if (wait_for(item_empty + slot, ((n / kItemSlots) & 1) ^ 1, abort_flag, a.sooner)) {
             items[slot] = it;
             ptx::mbar_arrive(item_full + slot);
           } else {
@@ -746,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (ok && it.state != 0 && it.end > it.begin) {
             auto fill = [&](int tile, bool of_keys) {
               const int stage = copies % kStages;
-              if (!wait_for(kv_empty + stage, ((copies / kStages) & 1) ^ 1, abort_flag)) {
+              if (!wait_for(kv_empty + stage, ((copies / kStages) & 1) ^ 1, abort_flag, a.sooner)) {
                 give_up();
                 ok = false;
                 return;
@@ -768,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             for (int b = 0; b < kBlocks && ok; ++b) {
               if (it.count <= b * a.tokens) continue;
-              if (!wait_for(q_empty + b, (loads[b] & 1) ^ 1, abort_flag)) {
+              if (!wait_for(q_empty + b, (loads[b] & 1) ^ 1, abort_flag, a.sooner)) {
                 give_up();
                 ok = false;
                 break;
@@ -791,18 +795,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (it.state == 0) break;
       }
       if (__any_sync(0xffffffffu, bad) && lane == 0 && a.error_flag != nullptr) atomicCAS(a.error_flag, 0, kBadOffsets);
-      if (!ok && lane == 0) {  // what is on its way must land before this memory is another CTA's
-        for (unsigned i = copies > kStages ? copies - kStages : 0; i < copies; ++i) ptx::mbar_drain(kv_full + i % kStages, (i / kStages) & 1);
-        for (int b = 0; b < kBlocks; ++b)
-          if (loads[b] > 0) ptx::mbar_drain(q_full + b, (loads[b] - 1) & 1);
-      }
+      if (lane == 0) issued[0] = copies, issued[1] = loads[0], issued[2] = loads[1];
     } else if (warp == kMmaWarp) {
-      if (ptx::elect_one()) {
+      multiplies = ptx::elect_one();
+      if (multiplies) {
         constexpr uint32_t kScores = make_idesc_bf16<kTile, false>(), kOutputs = make_idesc_bf16<D, true>();
         unsigned copies = 0, values = 0, loads[kBlocks] = {0, 0}, probs[kBlocks] = {0, 0};
         bool ok = true;
         auto wait = [&](uint64_t *bar, unsigned parity) {
-          ok = ok && wait_for(bar, parity & 1, abort_flag);
+          ok = ok && wait_for(bar, parity & 1, abort_flag, a.sooner);
           if (!ok) give_up();
           return ok;
         };
@@ -866,10 +867,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             copies += more ? 2 : 1;
           }
         }
-        if (!ok) {  // the products that were issued must have ended before their memory is another CTA's
-          ptx::tc_commit<1>(drained);
-          ptx::mbar_drain(drained, 0);
-        }
       }
       __syncwarp();
     } else {
@@ -881,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         leave_item(n);
         for (int tile = it.begin; tile < it.end; ++tile, copies += 2, ++values) {
           const unsigned copy = copies + 1;
-          ok = wait_for(kv_full + copy % kStages, (copy / kStages) & 1, abort_flag);
+          ok = wait_for(kv_full + copy % kStages, (copy / kStages) & 1, abort_flag, a.sooner);
           if (!ok) give_up();
           __syncwarp();
           ok = __all_sync(0xffffffffu, ok);
@@ -910,6 +907,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   ptx::tc_fence_before();
   __syncthreads();
+  if (*abort_flag != 0) {
+    // A wait ran out, in whichever warp: the others may have ended in good order and left copies and products on their way.  These land and end before
+    // the memory is another CTA's.
+    if (warp == kLoadWarp && lane == 0) {
+      const unsigned copies = issued[0];
+      for (unsigned i = copies > kStages ? copies - kStages : 0; i < copies; ++i) ptx::mbar_drain(kv_full + i % kStages, (i / kStages) & 1);
+      for (int b = 0; b < kBlocks; ++b)
+        if (issued[1 + b] > 0) ptx::mbar_drain(q_full + b, (issued[1 + b] - 1) & 1);
+    }
+    if (multiplies) {
+      ptx::tc_commit<1>(drained);
+      ptx::mbar_drain(drained, 0);
+    }
+    __syncwarp();
+  }
   if (warp == kMmaWarp) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc<1>(tmem, 512);
@@ -987,8 +999,11 @@ bool encode(CUtensorMap *map, const void *base, int rows, int heads, int halves,
   return make_tensor_map(map, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+long long g_sooner = 0;  // host-side setting, see set_prompt_attention_wait_limit
+
 Args args_of(const PromptAttention &p, int sms) {
   Args a = {};
+  a.sooner = g_sooner;
   a.offsets = p.offsets;
   a.k_offsets = p.k_offsets;
   a.out = static_cast<__nv_bfloat16 *>(p.out);
@@ -1066,6 +1081,8 @@ int sm_count() {
 }
 
 }  // namespace
+
+void set_prompt_attention_wait_limit(long long cycles) { g_sooner = cycles > 0 ? std::max(0LL, ptx::kWaitLimitCycles - cycles) : 0; }
 
 size_t prompt_attention_workspace_bytes(const PromptAttention &p) {
   const int sms = sm_count();
