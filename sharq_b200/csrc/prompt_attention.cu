@@ -417,18 +417,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem_s = lanes + block * kTile, tmem_o = lanes + S::kOutCol + block * D;
     const bool negative = a.scale_log2 < 0.0f;
     const float c = fmaxf(fabsf(a.scale_log2), 1.2e-38f);  // not 0: masked scores are -inf, and stay so
-    if (a.fill) {  // rows of no sequence, a share of them per thread
-      int begin = a.rows, end = 0;  // what sequences may have, also where some offsets are wrong
-      for (int i = lane; i <= a.seqs; i += 32) {
-        const int at = a.offsets[i];
-        if (at >= 0 && at <= a.rows) begin = min(begin, at), end = max(end, at);
+    if (a.fill) {  // rows of no sequence become zeros, a share of them per thread
+      const long long width = (long long)a.heads * D / 8;
+      auto clear = [&](int from, int to) {
+        uint4 *out = reinterpret_cast<uint4 *>(a.out);
+        for (long long i = from * width + (long long)blockIdx.x * (32 * kSoftmaxWarps) + threadIdx.x; i < to * width; i += (long long)gridDim.x * (32 * kSoftmaxWarps))
+          out[i] = make_uint4(0, 0, 0, 0);
+      };
+      bool wrong = false;
+      for (int i = lane; i <= a.seqs; i += 32) wrong |= a.offsets[i] < (i > 0 ? a.offsets[i - 1] : 0) || a.offsets[i] > a.rows;
+      if (!__any_sync(0xffffffffu, wrong)) {
+        clear(0, a.offsets[0]);
+        clear(a.offsets[a.seqs], a.rows);
+      } else {  // also those between the sequences that have rows, which lie in ascending order
+        int reached = 0, covered = 0;
+        for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+          const Bounds b = bounds_of(a, b0, lane, &reached);
+          for (unsigned left = __ballot_sync(0xffffffffu, b.row1 > b.row0); left != 0; left &= left - 1) {
+            const int in = __ffs(left) - 1, row0 = __shfl_sync(0xffffffffu, b.row0, in);
+            clear(covered, row0);
+            __syncwarp();
+            covered = __shfl_sync(0xffffffffu, b.row1, in);
+          }
+        }
+        clear(covered, a.rows);
       }
-      begin = __reduce_min_sync(0xffffffffu, begin);
-      end = __reduce_max_sync(0xffffffffu, end);
-      const long long width = (long long)a.heads * D / 8, ahead = begin * width, behind = (long long)max(a.rows - max(end, begin), 0) * width;
-      uint4 *out = reinterpret_cast<uint4 *>(a.out);
-      for (long long i = (long long)blockIdx.x * (32 * kSoftmaxWarps) + threadIdx.x; i < ahead + behind; i += (long long)gridDim.x * (32 * kSoftmaxWarps))
-        out[i < ahead ? i : (long long)a.rows * width - behind + (i - ahead)] = make_uint4(0, 0, 0, 0);
+      __syncwarp();
     }
     unsigned tiles_done = 0, values_done = 0, items_done = 0;  // for the barriers' parities: of this block, of all, of this block
     bool ok = true;
