@@ -860,7 +860,8 @@ int sharq_prompt_attention(const void *q_bf16, int64_t q_row, int64_t q_head, co
                            int fill, void *workspace, size_t workspace_bytes, int *error_flag, void *stream) {
   SHARQ_REQUIRE(q_bf16 && k_bf16 && v_bf16 && offsets && out_bf16, "null buffer");
   SHARQ_REQUIRE(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128, got %d", head_dim);
-  SHARQ_REQUIRE(rows >= 1 && rows <= 1 << 30 && k_rows >= 1 && k_rows <= 1 << 30, "rows and k_rows must be in [1, 2^30]");
+  SHARQ_REQUIRE(rows >= 1 && rows <= 1 << 30 && k_rows >= (k_offsets ? 0 : 1) && k_rows <= 1 << 30,
+                "rows and k_rows must be in [1, 2^30], or k_rows 0 with k_offsets");
   SHARQ_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads <= 65536, "heads must be a positive multiple of kv_heads, at most 65536");
   SHARQ_REQUIRE(sequences > 0 && sequences <= 1 << 28, "sequences must be in [1, 2^28]");
   SHARQ_REQUIRE(window >= 0 && sinks >= 0, "window and sinks must not be negative");

@@ -1046,15 +1046,16 @@ template <int D>
 cudaError_t launch(const PromptAttention &p, Args a, int sms, cudaStream_t stream) {
   using S = Sizes<D>;
   CUtensorMap q, k, v, k8, v8;
+  const int k_rows = std::max(p.k_rows, 1);  // a map has a row; where there is none no sequence has keys, and nothing is read
   if (!encode(&q, p.q, p.rows, p.heads, S::kHalves, p.q_row, p.q_head, true, a.tokens, a.chunk_heads, 1) ||
-      !encode(&k, p.k, p.k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, kTile, 1, S::kHalves) ||
-      !encode(&v, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, kTile, 1, S::kHalves))
+      !encode(&k, p.k, k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, kTile, 1, S::kHalves) ||
+      !encode(&v, p.v, k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, kTile, 1, S::kHalves))
     return cudaErrorInvalidValue;
   // copies of 8 keys join the first ones and the window's; without first ones there are none
   if (p.sinks == 0)
     k8 = k, v8 = v;
-  else if (!encode(&k8, p.k, p.k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, 8, 1, 1) ||
-           !encode(&v8, p.v, p.k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, 8, 1, 1))
+  else if (!encode(&k8, p.k, k_rows, p.kv_heads, S::kHalves, p.k_row, p.k_head, false, 8, 1, 1) ||
+           !encode(&v8, p.v, k_rows, p.kv_heads, S::kHalves, p.v_row, p.v_head, false, 8, 1, 1))
     return cudaErrorInvalidValue;
   static bool ready[64] = {};
   cudaError_t err = allow_smem(prompt_attention_kernel<D>, S::kTotal, ready);

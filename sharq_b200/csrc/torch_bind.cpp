@@ -606,14 +606,14 @@ Tensor prompt_attention(const Tensor &q, const Tensor &k, const Tensor &v, const
   c10::cuda::OptionalCUDAGuard guard(dev);
   Tensor o = out ? *out : fresh({rows, heads, d}, at::kBFloat16);
   if (rows == 0) return o;
-  // without any key there is nothing to read: the queries stand for keys that no sequence has
+  // without any key nothing is read, but the addresses must be some: those of the queries
   const Tensor &keys = k_rows > 0 ? k : q, &values = k_rows > 0 ? v : q;
-  const int first = (int)std::min<int64_t>(sinks, INT32_MAX), most = (int)std::max<int64_t>(k_rows, 1);
-  const int64_t ws_bytes = (int64_t)sharq_prompt_attention_workspace_bytes((int)rows, most, (int)heads, (int)kv_heads, (int)d, (int)offsets.size(0) - 1, w, first);
+  const int first = (int)std::min<int64_t>(sinks, INT32_MAX);
+  const int64_t ws_bytes = (int64_t)sharq_prompt_attention_workspace_bytes((int)rows, (int)k_rows, (int)heads, (int)kv_heads, (int)d, (int)offsets.size(0) - 1, w, first);
   Tensor ws;
   if (ws_bytes > 0) ws = fresh({ws_bytes}, at::kByte);
   check(sharq_prompt_attention(ptr(q), strides[0][0], strides[0][1], ptr(keys), strides[1][0], strides[1][1], ptr(values), strides[2][0], strides[2][1],
-                               (int)rows, most, (int)heads, (int)kv_heads, (int)d, static_cast<const int *>(ptr(offsets)),
+                               (int)rows, (int)k_rows, (int)heads, (int)kv_heads, (int)d, static_cast<const int *>(ptr(offsets)),
                                k_offsets ? static_cast<const int *>(ptr(*k_offsets)) : nullptr, (int)offsets.size(0) - 1, w,
                                first, (float)(scale ? *scale : 1.0 / std::sqrt((double)d)), ptr(o), !out, ws_bytes > 0 ? ptr(ws) : nullptr,
                                (size_t)ws_bytes, flag_of(flag), stream_of(q)));

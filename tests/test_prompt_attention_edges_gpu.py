@@ -63,6 +63,18 @@ def test_rows_of_no_sequence_beside_parts():
     assert (got[100:] == 0).all()
 
 
+def test_keys_that_are_not_there():
+    """Without any key, offsets of keys that claim one cannot be: NaN, and reported; a sequence of no keys beside it has zeros."""
+    q = inputs([7], [7], 4, 2, 64, 1)[0]
+    none = torch.zeros(0, 2, 64, dtype=torch.bfloat16, device="cuda")
+    got = ops.prompt_attention(q, none, none, i32([0, 2, 5, 7]), k_offsets=i32([0, 0, 1, 1]))
+    with pytest.raises(RuntimeError, match="offsets"):
+        ops.check_device_errors()
+    assert (got[:2] == 0).all() and got[2:].isnan().all()  # the third one's keys begin behind the last row too
+    assert (ops.prompt_attention(q, none, none, i32([0, 2, 5]), k_offsets=i32([0, 0, 0])) == 0).all()
+    ops.check_device_errors()
+
+
 @pytest.mark.parametrize("dim,group", [(128, 4), (64, 1)])
 @pytest.mark.parametrize("keys", [200, 5000])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
