@@ -438,7 +438,8 @@ int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, in
  * its queries: the i-th of n queries has position p = keys - n + i, and sees the key at position j where
  *   j <= p and (p - j < window or j < sinks)          (window 0: every j <= p)
  * out = sum_j softmax_j(scale * q . k[j]) v[j] over those; a query that sees none gives zeros.  Query head h reads key/value head
- * h / (heads / kv_heads).  With fill != 0 rows of out ahead of the first sequence and behind the last become zeros, else they stay as they are.
+ * h / (heads / kv_heads).  With fill != 0 rows of out that belong to no sequence become zeros, else they stay as they are.  out may be q
+ * where the heads of q are dense (q_head == head_dim, q_row == heads * head_dim), and must not overlap q, k or v otherwise.
  * Sums and softmax statistics are float; probabilities enter the product with the values as bf16.  Offsets (int32, on the device) that go back or leave
  * [0, rows] make their sequence empty, those of keys make its rows NaN, and store 0x407 in *error_flag (may be NULL; 0x408: a wait ran out, results
  * are undefined).  head_dim 64 or 128, heads a multiple of kv_heads, rows and k_rows at most 2^30; with k_offsets k_rows may be 0 (k and v are not read then,

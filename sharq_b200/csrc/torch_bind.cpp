@@ -603,6 +603,16 @@ Tensor prompt_attention(const Tensor &q, const Tensor &k, const Tensor &v, const
       if (strides[i][j] <= 0 || strides[i][j] % 8 != 0)
         fail(std::string("strides of ") + "qkv"[i] + " must be positive multiples of 8");
     }
+  if (out) {  // over the queries, element for element, each block has read its own when it writes; anywhere else the order would matter
+    const char *begin = static_cast<const char *>(ptr(*out)), *end = begin + out->nbytes();
+    for (int i = 0; i < 3; ++i) {
+      const Tensor &t = *held[i];
+      if (t.numel() == 0 || out->numel() == 0 || (i == 0 && ptr(t) == begin && t.is_contiguous())) continue;
+      const char *from = static_cast<const char *>(ptr(t));
+      const int64_t span = ((t.size(0) - 1) * strides[i][0] + (t.size(1) - 1) * strides[i][1] + d) * t.element_size();
+      need(from + span <= begin || end <= from, "out must be q or not overlap q, k and v");
+    }
+  }
   c10::cuda::OptionalCUDAGuard guard(dev);
   Tensor o = out ? *out : fresh({rows, heads, d}, at::kBFloat16);
   if (rows == 0) return o;

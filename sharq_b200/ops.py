@@ -254,8 +254,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     [rows, heads, head_dim].  Sequence s has the rows offsets[s] to offsets[s + 1] (int32, on the device).  With window a query at position p sees
     the keys at p - window + 1 to p and the first `sinks`, else all up to p.  k_offsets: the rows of k and v that a sequence has, of which the last
     belong to its queries (a later piece of a prompt); a query ahead of all of its keys gives zeros.  scale: default head_dim ** -0.5.  Float32
-    sums and statistics, probabilities in bf16 for the product with the values, one rounding of the result.  Rows of no sequence are zeros, or with out stay
-    as they are.  Offsets that go back or beyond the rows are reported by check_device_errors: such a sequence has no rows, one with such
+    sums and statistics, probabilities in bf16 for the product with the values, one rounding of the result.  Rows of no sequence are zeros, or with out (which may be
+    q itself, if that is contiguous, and overlaps q, k and v nowhere else) stay as they are.  Offsets that go back or beyond the rows are reported by check_device_errors: such a sequence has no rows, one with such
     k_offsets NaN.  The same bits from call to call."""
     return _lib.native().prompt_attention(q, k, v, offsets, window, sinks, scale, k_offsets, out, _error_flag(q.device))
 

@@ -75,6 +75,29 @@ def test_keys_that_are_not_there():
     ops.check_device_errors()
 
 
+def test_an_output_over_inputs():
+    """Over the queries themselves, element for element, it is as good as any; anywhere else over what is read it is refused."""
+    lengths = [90, 200, 10]
+    for heads, kv_heads, keys in ((4, 2, None), (2, 2, [3000, 4000, 2000])):
+        q, k, v = inputs(lengths, keys or lengths, heads, kv_heads, 128, 6)
+        more = dict(window=30, sinks=2) if keys is None else dict(k_offsets=ends(keys))
+        want = ops.prompt_attention(q, k, v, ends(lengths), **more)
+        for _ in range(5):
+            over = q.clone()
+            assert ops.prompt_attention(over, k, v, ends(lengths), out=over, **more) is over
+            assert torch.equal(over, want)
+    q, k, v = inputs(lengths, lengths, 2, 2, 64, 7)
+    buffer = torch.zeros(4 * 300 * 128, dtype=torch.bfloat16, device="cuda")
+    at = lambda n: buffer[n * 128:(n + 300) * 128].view(300, 2, 64)  # noqa: E731
+    for changes in (dict(k=at(0)), dict(v=at(0)), dict(k=at(299)), dict(v=at(299)), dict(q=at(1)), dict(q=at(299)),
+                    dict(q=buffer[:300 * 256].view(300, 4, 64)[:, :2])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.prompt_attention(**{**dict(q=q, k=k, v=v, offsets=ends(lengths)), **changes}, out=at(0))
+    # side by side is not over one another
+    ops.prompt_attention(at(0), at(300), at(600), ends(lengths), out=at(900))
+    ops.check_device_errors()
+
+
 @pytest.mark.parametrize("dim,group", [(128, 4), (64, 1)])
 @pytest.mark.parametrize("keys", [200, 5000])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
