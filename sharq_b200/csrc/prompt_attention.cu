@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = tmem + ((uint32_t)(warp % 4) << 21);  // 32 lanes of tensor memory per warp
     const uint32_t tmem_s = lanes + block * kTile, tmem_o = lanes + S::kOutCol + block * D;
     const bool negative = a.scale_log2 < 0.0f;
-    const float c = fmaxf(fabsf(a.scale_log2), 1.2e-38f);  // not 0: masked scores are -inf, and stay so
+    const float c = fabsf(a.scale_log2) < 1.2e-38f ? 1.2e-38f : fabsf(a.scale_log2);  // not 0: masked scores are -inf, and stay so; NaN is NaN
     if (a.fill) {  // rows of no sequence become zeros, a share of them per thread
       const long long width = (long long)a.heads * D / 8;
       auto clear = [&](int from, int to) {

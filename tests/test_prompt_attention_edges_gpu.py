@@ -98,6 +98,12 @@ def test_an_output_over_inputs():
     ops.check_device_errors()
 
 
+@pytest.mark.parametrize("keys", [300, 5000])
+def test_a_scale_that_is_nan(keys):
+    q, k, v = inputs([300], [keys], 4, 2, 128, 8)
+    assert ops.prompt_attention(q, k, v, ends([300]), scale=math.nan, k_offsets=ends([keys])).isnan().all()
+
+
 @pytest.mark.parametrize("dim,group", [(128, 4), (64, 1)])
 @pytest.mark.parametrize("keys", [200, 5000])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
