@@ -442,7 +442,7 @@ int sharq_weight_only_linear(const void *x_bf16, int64_t x_row, int m, int n, in
  * where the heads of q are dense (q_head == head_dim, q_row == heads * head_dim), and must not overlap q, k or v otherwise.
  * Sums and softmax statistics are float; probabilities enter the product with the values as bf16.  Offsets (int32, on the device) that go back or leave
  * [0, rows] make their sequence empty, those of keys make its rows NaN, and store 0x407 in *error_flag (may be NULL; 0x408: a wait ran out, results
- * are undefined).  head_dim 64 or 128, heads a multiple of kv_heads, rows and k_rows at most 2^30; with k_offsets k_rows may be 0 (k and v are not read then,
+ * are undefined).  head_dim 64 or 128, heads a multiple of kv_heads, rows and k_rows at most 2^30, sequences at most 2^24; with k_offsets k_rows may be 0 (k and v are not read then,
  * but must be addresses).  workspace:
  * sharq_prompt_attention_workspace_bytes() bytes of scratch (0: none, by these sizes alone; few queries with many keys are cut into parts), 32-byte
  * aligned, not shared by calls that overlap. */

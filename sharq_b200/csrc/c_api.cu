@@ -863,7 +863,8 @@ int sharq_prompt_attention(const void *q_bf16, int64_t q_row, int64_t q_head, co
   SHARQ_REQUIRE(rows >= 1 && rows <= 1 << 30 && k_rows >= (k_offsets ? 0 : 1) && k_rows <= 1 << 30,
                 "rows and k_rows must be in [1, 2^30], or k_rows 0 with k_offsets");
   SHARQ_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads <= 65536, "heads must be a positive multiple of kv_heads, at most 65536");
-  SHARQ_REQUIRE(sequences > 0 && sequences <= 1 << 28, "sequences must be in [1, 2^28]");
+  // every CTA walks through all offsets, 24 ns a sequence, while its other warps wait, for a second at most
+  SHARQ_REQUIRE(sequences > 0 && sequences <= 1 << 24, "sequences must be in [1, 2^24]");
   SHARQ_REQUIRE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
   SHARQ_REQUIRE(k_offsets || k_rows == rows, "without k_offsets there is a key for every query");
   const int64_t strides[6] = {q_row, q_head, k_row, k_head, v_row, v_head};

@@ -586,7 +586,7 @@ Tensor prompt_attention(const Tensor &q, const Tensor &k, const Tensor &v, const
        "q must have head_dim elements per head and a multiple of the heads of k");
   if (d != 64 && d != 128) fail("head_dim must be 64 or 128, got " + std::to_string(d));
   need(rows <= 1 << 30 && k_rows <= 1 << 30 && heads <= 65536, "too many rows or heads");
-  need(offsets.dim() == 1 && offsets.size(0) >= 2 && offsets.size(0) <= 1 << 28, "offsets must have an entry for every sequence and one more");
+  need(offsets.dim() == 1 && offsets.size(0) >= 2 && offsets.size(0) <= (1 << 24) + 1, "offsets must have an entry for every sequence, at most 2^24, and one more");
   check_indices(offsets, offsets.size(0), dev, "offsets");
   if (k_offsets)
     check_indices(*k_offsets, offsets.size(0), dev, "k_offsets");
