@@ -478,7 +478,8 @@ int sharq_plan_paged_step(int *page_table, int64_t page_table_stride, int sequen
  *   x = -inf                                               where bit (token % 32) of mask[r * mask_stride + token / 32] is not set
  * in double, rounded once; a logit that nothing concerns stays as it is.  Each of tokens with lengths, the penalties, the biases and the mask
  * may be NULL.  Strides in elements (words for the mask, which has ceil(vocab / 32) in a row).  What lies outside its range (a length, an offset, a token of vocab or more,
- * the token of a bias) is passed over and stores 0x406 in *error_flag (may be NULL).  rows <= 65535. */
+ * the token of a bias) is passed over and stores 0x406 in *error_flag (may be NULL); prompt_lengths[r] below 0 counts as 0, above lengths[r] as that.
+ * rows <= 65535, width and biases <= 2^30. */
 typedef struct sharq_logit_rules {
   const void *tokens;
   int64_t tokens_stride;

@@ -924,7 +924,10 @@ int sharq_adjust_logits(const void *logits, int64_t logits_stride, void *out, in
   SHARQ_REQUIRE(rules->lengths ? rules->tokens || rules->width == 0 : !rules->tokens, "tokens and lengths go together");
   SHARQ_REQUIRE(rules->lengths || !(rules->prompt_lengths || rules->repetition || rules->presence || rules->frequency),
                 "prompt_lengths and the penalties need tokens");
-  SHARQ_REQUIRE(!rules->lengths || (rules->width >= 0 && (rows == 1 || rules->tokens_stride >= 0)), "the width of tokens must be >= 0");
+  // (indices of a thread run up to some thousands beyond both)
+  SHARQ_REQUIRE(!rules->lengths || (rules->width >= 0 && rules->width <= 1 << 30 && (rows == 1 || rules->tokens_stride >= 0)),
+                "the width of tokens must be in [0, 2^30]");
+  SHARQ_REQUIRE(rules->biases <= 1 << 30, "biases must be at most 2^30");
   SHARQ_REQUIRE(rules->biases >= 0 && (rules->bias_offsets || rules->biases == 0) && (rules->biases == 0 || (rules->bias_ids && rules->bias_values)),
                 "biases go with bias_offsets, bias_ids and bias_values");
   SHARQ_REQUIRE(!rules->mask || rows == 1 || rules->mask_stride >= 0, "the stride of the mask must be >= 0");

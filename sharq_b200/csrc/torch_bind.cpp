@@ -686,8 +686,8 @@ Tensor adjust_logits(const Tensor &logits, const OptionalTensor &tokens, const O
   need(tokens.has_value() == lengths.has_value(), "tokens and lengths go together");
   if (tokens) {
     need(tokens->is_cuda() && tokens->device() == dev && (tokens->scalar_type() == at::kInt || tokens->scalar_type() == at::kLong) &&
-             tokens->dim() == 2 && tokens->size(0) == rows && tokens->size(1) <= INT32_MAX && (tokens->size(1) <= 1 || tokens->stride(1) == 1),
-         "tokens must be a CUDA int32 or int64 matrix with a row per row of logits and unit column stride, on their device");
+             tokens->dim() == 2 && tokens->size(0) == rows && tokens->size(1) <= 1 << 30 && (tokens->size(1) <= 1 || tokens->stride(1) == 1),
+         "tokens must be a CUDA int32 or int64 matrix of at most 2^30 columns, with a row per row of logits and unit column stride, on their device");
     check_indices(*lengths, rows, dev, "lengths");
     r.tokens = ptr(*tokens);
     r.tokens_stride = rows > 1 ? tokens->stride(0) : 0;
@@ -712,7 +712,7 @@ Tensor adjust_logits(const Tensor &logits, const OptionalTensor &tokens, const O
     need(bias->size() == 3, "bias must be (offsets, ids, values)");
     const Tensor &ids = (*bias)[1], &values = (*bias)[2];
     check_indices((*bias)[0], rows + 1, dev, "offsets of the biases");
-    need(ids.dim() == 1 && ids.size(0) <= INT32_MAX, "ids of the biases must be a vector");
+    need(ids.dim() == 1 && ids.size(0) <= 1 << 30, "ids of the biases must be a vector of at most 2^30");
     check_indices(ids, ids.size(0), dev, "ids of the biases");
     need(is_plain(values, at::kFloat) && values.device() == dev && values.sizes() == ids.sizes(),
          "values of the biases must be a contiguous CUDA float32 vector with one entry per id");
