@@ -1,4 +1,4 @@
-// Penalties for repeated tokens, biases and masks on logits, in one launch.  256 rows of 152064 with histories of up to 6000 tokens: 77.6 us, 4.1 TB/s; one
+// Penalties for repeated tokens, biases and masks on logits, in one launch.  256 rows of 152064 with histories of up to 6000 tokens: 78.5 us, 4.1 TB/s; one
 // row of 128256: 3.4 us (a call takes 5.6 on the host).
 //
 //   x' = x > 0 ? x / r : x r   (tokens of the history),   x' - f n - p [n > 0]   (n: how often the answer so far has the token),   + biases,   -inf where masked
@@ -55,13 +55,46 @@ __device__ __forceinline__ double widened(T x) {
 
 constexpr int kThreads = 512, kSliceMost = 16384;
 
+// Tokens with several biases, a lane each: the warp goes through the list for 32 neighbours at a time, and each lane adds up its token's in their order.  The list
+// is read as often as there are such neighbours, 32 times per warp at most, however many biases a token has.  several: of the 32 neighbours that
+// begin at 32 * (warp + 16 * lane), those that are such tokens and are not masked.
+template <typename T>
+__device__ __forceinline__ void add_several(const int *ids, const float *values, int biases, int first, unsigned several, const unsigned *words, const T *in, T *out,
+                                            double repetition, double presence, double frequency) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (unsigned left = __ballot_sync(0xffffffffu, several != 0); left != 0; left &= left - 1) {
+    const int from = __ffs(left) - 1, word = warp + from * (kThreads / 32);
+    const unsigned these = __shfl_sync(0xffffffffu, several, from);
+    double bias = -0.0;  // which changes no number that it is added to
+    for (int j0 = 0; j0 < biases; j0 += 32) {
+      const unsigned at = j0 + lane < biases ? (unsigned)ids[j0 + lane] - (unsigned)first : ~0u;
+      const bool mine = (int)(at >> 5) == word && (these >> (at & 31) & 1) != 0;
+      unsigned hits = __ballot_sync(0xffffffffu, mine);
+      if (hits == 0) continue;
+      const float value = mine ? values[j0 + lane] : 0.0f;
+      for (; hits != 0; hits &= hits - 1) {
+        const int of = __ffs(hits) - 1;
+        const unsigned whose = __shfl_sync(0xffffffffu, at, of) & 31;
+        const float x = __shfl_sync(0xffffffffu, value, of);
+        if (whose == (unsigned)lane) bias += (double)x;
+      }
+      __syncwarp();
+    }
+    if ((these >> lane & 1) != 0) {
+      const int at = word * 32 + lane;
+      out[at] = rounded<T>(penalised(widened<T>(in[at]), words[at], {repetition, presence, frequency}) + bias);
+    }
+    __syncwarp();
+  }
+}
+
 // T: type of the logits; Id: of the history's tokens; kVec: logits of a 16-byte access, or 1
 template <typename T, typename Id, int kVec>
 __global__ void __launch_bounds__(kThreads, 2) logit_rules_kernel(const __grid_constant__ LogitRules a) {
   constexpr int kPer = kSliceMost / (kThreads * kVec);  // accesses of a thread
   // for every token of the slice how often the history has it, and two bits: it has a bias, it has several; then the history's tokens, each once, in any order
   extern __shared__ __align__(16) unsigned words[];
-  __shared__ int listed;
+  __shared__ int listed, repeated;  // repeated: some token has several biases
   unsigned *biased = words + a.slice, *twice = biased + a.slice / 32, *kept = twice + a.slice / 32;  // kept: the mask
   unsigned short *list = reinterpret_cast<unsigned short *>(kept + a.slice / 32);
   const int row = blockIdx.y, tid = threadIdx.x;
@@ -104,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 2) logit_rules_kernel(const __grid_c
   }
 
   for (int i = tid * 4; i < a.slice + a.slice / 16; i += kThreads * 4) *reinterpret_cast<uint4 *>(words + i) = make_uint4(0, 0, 0, 0);
-  if (tid == 0) listed = 0;
+  if (tid == 0) listed = repeated = 0;
   __syncthreads();
   const Id *tokens = static_cast<const Id *>(a.tokens) + row * a.tokens_stride;
   auto place = [&](Id id, int *at) {  // in the slice
@@ -134,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 2) logit_rules_kernel(const __grid_c
   }
   auto mark = [&](int at) {
     const unsigned bit = 1u << (at & 31);
-    if ((atomicOr(biased + (at >> 5), bit) & bit) != 0) atomicOr(twice + (at >> 5), bit);
+    if ((atomicOr(biased + (at >> 5), bit) & bit) != 0) atomicOr(twice + (at >> 5), bit), repeated = 1;
   };
   for (int j = bias0 + tid; j < bias1; j += kThreads) {
     const long long at = (long long)a.bias_ids[j] - first;
@@ -167,30 +200,29 @@ __global__ void __launch_bounds__(kThreads, 2) logit_rules_kernel(const __grid_c
   }
   __syncthreads();
 
-  // those that something concerns, from the logits as they were, over what has just been written
+  // those that something concerns, from the logits as they were, over what has just been written (few turns of these loops: unrolled, 79.1 us)
   const Penalty penalty = {repetition, presence, frequency};
   auto stays = [&](int at) { return (kept[at >> 5] >> (at & 31) & 1) != 0; };
   const int concerned = listed;
+#pragma unroll 1
   for (int j = tid; j < concerned; j += kThreads) {
     const int at = list[j];
     if ((biased[at >> 5] >> (at & 31) & 1) == 0 && stays(at)) out[at] = rounded<T>(penalised(widened<T>(in[at]), words[at], penalty));
   }
-  auto add = [&](int j, int at, T x, float value) {  // bias j
-    if (!stays(at)) return;
-    double bias = (double)value;
-    if ((twice[at >> 5] >> (at & 31) & 1) != 0) {  // one of several: the first of them adds all up, in their order
-      auto is = [&](int k) { return (unsigned)a.bias_ids[k] - (unsigned)first == (unsigned)at; };
-      int k = bias0;
-      while (!is(k)) ++k;
-      if (k != j) return;
-      for (++k; k < bias1; ++k)
-        if (is(k)) bias += (double)a.bias_values[k];
-    }
-    out[at] = rounded<T>(penalised(widened<T>(x), words[at], penalty) + bias);
+  // a token with one bias, by the bias's thread
+  auto add = [&](int at, T x, float value) {
+    if (stays(at) && (twice[at >> 5] >> (at & 31) & 1) == 0) out[at] = rounded<T>(penalised(widened<T>(x), words[at], penalty) + (double)value);
   };
+#pragma unroll 1
   for (int j = bias0 + tid; j < bias1; j += kThreads) {
     const long long at = (long long)a.bias_ids[j] - first;
-    if (at >= 0 && at < size) add(j, (int)at, in[at], a.bias_values[j]);
+    if (at >= 0 && at < size) add((int)at, in[at], a.bias_values[j]);
+  }
+  if (repeated != 0) {
+    static_assert(kThreads >= kSliceMost / 32, "32 neighbours per thread, of which its warp looks after all");
+    const int word = (tid >> 5) + (tid & 31) * (kThreads / 32);
+    const unsigned several = word < a.slice / 32 ? twice[word] & kept[word] : 0;
+    add_several<T>(a.bias_ids + bias0, a.bias_values + bias0, bias1 - bias0, first, several, words, in, out, penalty.repetition, penalty.presence, penalty.frequency);
   }
   if (bad && a.error_flag != nullptr) atomicCAS(a.error_flag, 0, kBadLogitRules);
 }
