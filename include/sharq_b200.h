@@ -464,10 +464,15 @@ int sharq_prompt_attention(const void *q_bf16, int64_t q_row, int64_t q_head, co
  * of the `rows` rows are a row's place for sharq_rope_append_paged: position -1 in the rows of a sequence that got nothing, and -1 with
  * sequence 0 behind the last.
  * No sequence grows beyond max_tokens (0: what its row of the table holds).  A length, count, sum of counts above `rows` or number of free pages that cannot be makes the sequences that it concerns get nothing and stores 0x405 in
- * *error_flag (may be NULL).  rows and free_pages_size at most 2^30; no workspace; calls on one cache must not overlap. */
+ * *error_flag (may be NULL); length -1 with count 0 is passed over.  rows and free_pages_size at most 2^30; no workspace; calls on one cache must not overlap. */
 int sharq_plan_paged_step(int *page_table, int64_t page_table_stride, int sequences, int max_pages, int page_size, int max_tokens, int *lengths,
                           const int *counts, const unsigned char *released, int *free_pages, int free_pages_size, int *free_count,
                           int rows, int *offsets, int *positions, int *row_sequences, int *error_flag, void *stream);
+
+/* The same; a sequence for which the pages do not suffice stores 0x409 in *error_flag too. */
+int sharq_plan_paged_step_strict(int *page_table, int64_t page_table_stride, int sequences, int max_pages, int page_size, int max_tokens,
+                                 int *lengths, const int *counts, const unsigned char *released, int *free_pages, int free_pages_size,
+                                 int *free_count, int rows, int *offsets, int *positions, int *row_sequences, int *error_flag, void *stream);
 
 /* Penalties for repeated tokens, biases and masks on logits [rows, vocab] (float, or bf16 with bf16 != 0), into out of the same type, which may be
  * the logits themselves but must not overlap them otherwise.  tokens [rows, width] (int32, or int64 with wide_tokens != 0) is the history of

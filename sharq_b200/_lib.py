@@ -111,6 +111,8 @@ SIGNATURES = {
     "sharq_prompt_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "sharq_plan_paged_step": (
         c_int, [_P, c_int64, c_int, c_int, c_int, c_int, _P, _P, _P, _P, c_int, _P, c_int, _P, _P, _P, _P, _P]),
+    "sharq_plan_paged_step_strict": (
+        c_int, [_P, c_int64, c_int, c_int, c_int, c_int, _P, _P, _P, _P, c_int, _P, c_int, _P, _P, _P, _P, _P]),
     "sharq_adjust_logits": (c_int, [_P, c_int64, _P, c_int64, c_int, c_int, c_int, _P, _P, _P]),
     "sharq_noalloc_max_rows": (c_int, []),
     "sharq_noalloc_last_error": (c_char_p, []),

@@ -901,9 +901,9 @@ int sharq_prompt_attention(const void *q_bf16, int64_t q_row, int64_t q_head, co
   return check_cuda(sharq::run_prompt_attention(p, as_stream(stream)), "prompt_attention");
 }
 
-int sharq_plan_paged_step(int *page_table, int64_t page_table_stride, int sequences, int max_pages, int page_size, int max_tokens, int *lengths,
-                          const int *counts, const unsigned char *released, int *free_pages, int free_pages_size, int *free_count,
-                          int rows, int *offsets, int *positions, int *row_sequences, int *error_flag, void *stream) {
+static int plan_paged_step(int *page_table, int64_t page_table_stride, int sequences, int max_pages, int page_size, int max_tokens, int *lengths,
+                           const int *counts, const unsigned char *released, int *free_pages, int free_pages_size, int *free_count,
+                           int rows, int *offsets, int *positions, int *row_sequences, int *error_flag, bool strict, void *stream) {
   SHARQ_REQUIRE(page_table && lengths && counts && free_count && offsets, "null buffer");
   SHARQ_REQUIRE(sequences > 0 && max_pages > 0 && page_size > 0, "sequences, max_pages and page_size must be positive");
   SHARQ_REQUIRE(max_tokens >= 0, "max_tokens must not be negative");
@@ -912,8 +912,22 @@ int sharq_plan_paged_step(int *page_table, int64_t page_table_stride, int sequen
   SHARQ_REQUIRE(free_pages_size <= 1 << 30, "free_pages_size must be at most 2^30");
   SHARQ_REQUIRE(rows >= 0 && rows <= 1 << 30 && (rows == 0 || (positions && row_sequences)), "rows must be in [0, 2^30], with a place for each");
   const sharq::StepPlan p = {page_table, page_table_stride, sequences, max_pages, page_size, max_tokens, lengths, counts, released, free_pages,
-                             free_pages_size, free_count, rows, offsets, positions, row_sequences, error_flag};
+                             free_pages_size, free_count, rows, offsets, positions, row_sequences, error_flag, strict};
   return check_cuda(sharq::run_step_plan(p, as_stream(stream)), "plan_paged_step");
+}
+
+int sharq_plan_paged_step(int *page_table, int64_t page_table_stride, int sequences, int max_pages, int page_size, int max_tokens, int *lengths,
+                          const int *counts, const unsigned char *released, int *free_pages, int free_pages_size, int *free_count,
+                          int rows, int *offsets, int *positions, int *row_sequences, int *error_flag, void *stream) {
+  return plan_paged_step(page_table, page_table_stride, sequences, max_pages, page_size, max_tokens, lengths, counts, released, free_pages,
+                         free_pages_size, free_count, rows, offsets, positions, row_sequences, error_flag, false, stream);
+}
+
+int sharq_plan_paged_step_strict(int *page_table, int64_t page_table_stride, int sequences, int max_pages, int page_size, int max_tokens, int *lengths,
+                                 const int *counts, const unsigned char *released, int *free_pages, int free_pages_size, int *free_count,
+                                 int rows, int *offsets, int *positions, int *row_sequences, int *error_flag, void *stream) {
+  return plan_paged_step(page_table, page_table_stride, sequences, max_pages, page_size, max_tokens, lengths, counts, released, free_pages,
+                         free_pages_size, free_count, rows, offsets, positions, row_sequences, error_flag, true, stream);
 }
 
 int sharq_adjust_logits(const void *logits, int64_t logits_stride, void *out, int64_t out_stride, int rows, int vocab, int bf16,

@@ -16,6 +16,7 @@ constexpr int kBadStepPlan = 0x405;     // error code: a length, count or number
 constexpr int kBadLogitRules = 0x406;   // error code: a token, length or offset outside its range
 constexpr int kBadOffsets = 0x407;      // error code: offsets of prompts that go back, or beyond the rows
 constexpr int kPromptTimeout = 0x408;   // error code: a wait inside the attention of prompts ran out
+constexpr int kPagesShort = 0x409;      // error code: pages that did not suffice for a step's tokens
 
 // A position of a sequence in the cache; also what the kernels check before every access.
 struct PagedCache {
@@ -62,6 +63,7 @@ struct StepPlan {
   int rows;
   int *offsets, *positions, *row_sequences;
   int *error_flag;
+  bool strict;  // pages that do not suffice are an error
 };
 cudaError_t run_step_plan(const StepPlan &plan, cudaStream_t stream);
 

@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(kPlanThreadsMost) step_plan_kernel(const __gri
   }
 
   int need_before = 0, rows_before = 0;
+  bool wanting = false;  // pages, for some sequence
   for (int i0 = 0; i0 < p.sequences; i0 += threads) {
     const int i = i0 + tid;
     int length = 0, count = 0, held = 0, need = 0;
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(kPlanThreadsMost) step_plan_kernel(const __gri
       count = p.counts[i];
       if (p.released != nullptr && p.released[i] != 0) length = 0, keeps = false;
       fits = length >= 0 && count >= 0 && length <= most && count <= most - length;
-      if (!fits) bad = true;
+      if (!fits && (length != -1 || count != 0)) bad = true;  // -1 may stand for a sequence that takes none, as long as none is asked for
       count = max(count, 0);
       if (fits) {
         held = pages_of(length, p.page_size);
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(kPlanThreadsMost) step_plan_kernel(const __gri
     const int row_end = plus(rows_before, ends.b), need_end = plus(need_before, ends.a);
     const bool given = fits && !no_stack && (need == 0 || need_end <= free_now) && row_end <= p.rows;
     if (fits && row_end > p.rows) bad = true;
+    if (fits && !no_stack && need > 0 && need_end > free_now) wanting = true;
     need_ends[tid] = ends.a;
     row_ends[tid] = ends.b;
     held_of[tid] = held;
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(kPlanThreadsMost) step_plan_kernel(const __gri
     p.offsets[0] = 0;
     if (!no_stack) *p.free_count = free_now - taken;
   }
-  if (bad && p.error_flag != nullptr) atomicCAS(p.error_flag, 0, kBadStepPlan);
+  if ((bad || (wanting && p.strict)) && p.error_flag != nullptr) atomicCAS(p.error_flag, 0, bad ? kBadStepPlan : kPagesShort);
 }
 
 }  // namespace

@@ -633,7 +633,7 @@ Tensor prompt_attention(const Tensor &q, const Tensor &k, const Tensor &v, const
 // -> offsets [sequences + 1], positions [rows], sequences [rows], views of one allocation
 std::vector<Tensor> plan_paged_step(const Tensor &table, const Tensor &lengths, const Tensor &counts, const Tensor &free_pages,
                                     const Tensor &free_count, int64_t page_size, int64_t rows, const std::optional<Tensor> &released,
-                                    const std::optional<int64_t> &max_tokens, const Tensor &flag) {
+                                    const std::optional<int64_t> &max_tokens, const Tensor &flag, bool strict) {
   need(table.is_cuda() && table.scalar_type() == at::kInt && table.dim() == 2 && table.numel() > 0 && (table.size(1) <= 1 || table.stride(1) == 1),
        "page_table must be a CUDA int32 matrix [sequences, pages] with unit column stride");
   const at::Device dev = table.device();
@@ -662,11 +662,12 @@ std::vector<Tensor> plan_paged_step(const Tensor &table, const Tensor &lengths, 
     t.unsafeGetTensorImpl()->set_sizes_contiguous({size});
     return t;
   };
-  check(sharq_plan_paged_step(static_cast<int *>(ptr(table)), n > 1 ? table.stride(0) : table.size(1), (int)n, (int)table.size(1), (int)page_size,
-                              max_tokens ? (int)std::min<int64_t>(*max_tokens, INT32_MAX) : 0, static_cast<int *>(ptr(lengths)), static_cast<const int *>(ptr(counts)),
-                              released ? static_cast<const unsigned char *>(ptr(*released)) : nullptr, static_cast<int *>(ptr(free_pages)),
-                              (int)free_pages.size(0), static_cast<int *>(ptr(free_count)), (int)rows, at, at + at_rows, at + at_rows + padded,
-                              flag_of(flag), stream_of(table)));
+  const auto plan = strict ? sharq_plan_paged_step_strict : sharq_plan_paged_step;
+  check(plan(static_cast<int *>(ptr(table)), n > 1 ? table.stride(0) : table.size(1), (int)n, (int)table.size(1), (int)page_size,
+             max_tokens ? (int)std::min<int64_t>(*max_tokens, INT32_MAX) : 0, static_cast<int *>(ptr(lengths)), static_cast<const int *>(ptr(counts)),
+             released ? static_cast<const unsigned char *>(ptr(*released)) : nullptr, static_cast<int *>(ptr(free_pages)),
+             (int)free_pages.size(0), static_cast<int *>(ptr(free_count)), (int)rows, at, at + at_rows, at + at_rows + padded,
+             flag_of(flag), stream_of(table)));
   return {part(0, n + 1), part(at_rows, rows), part(at_rows + padded, rows)};
 }
 

@@ -27,6 +27,7 @@ Weights are random (N(0, 0.02)): there are no checkpoints in this environment.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -637,9 +638,10 @@ class SharqDecoder(torch.nn.Module):
         """token_ids [B, S] -> logits of the last position [B, vocab] (float32), with rules as they change them.
         reference=True runs the unquantised bf16 layers (needs keep_reference=True).  cache: holds the prompts afterwards (decode), as its
         sequences, which are B and empty, or as those listed in sequences, which are B and empty, whatever the others hold.  In a cache that hands
-        its pages out on the device a prompt takes the place of what its sequence held, and a sequence for which the pages do not suffice stays empty."""
+        its pages out on the device a prompt takes the place of what its sequence held.  Where the pages do not suffice for one, its logits are NaN, ops.check_device_errors
+        reports it, and its sequence (device_lengths -1) takes no tokens of decode until it gets a prompt or is freed."""
         b, s = token_ids.shape
-        kvs = [None] * len(self.layers)
+        kvs, refused = [None] * len(self.layers), None
         if cache is None and sequences is not None:
             raise ValueError("sequences are those of a cache")
         if cache is not None:
@@ -648,6 +650,7 @@ class SharqDecoder(torch.nn.Module):
                 if b != len(which) or s > cache.max_tokens:
                     raise ValueError("prefill takes a sequence of the cache for every prompt, of at most max_tokens")
                 positions, rows = cache.step_places(which, s, restart=True)
+                refused = positions.view(b, s)[:, :1] < 0
                 kvs = [cache.layer(i, positions, rows, None) for i in range(len(self.layers))]
             elif b != len(which) or any(cache.lengths[i] for i in which):
                 raise ValueError("prefill takes an empty cache with a sequence for every prompt" if sequences is None else
@@ -688,6 +691,8 @@ class SharqDecoder(torch.nn.Module):
             last = x[:, -1, :].float()
         if cache is not None and not cache.on_device:
             cache.advance(counts)
+        if refused is not None:
+            last = last.masked_fill(refused, math.nan)
         return self._logits(last, rules)
 
     def new_cache(self, sequences: int, max_tokens: int, page_size: int = 64, pages: int = None, dtype: torch.dtype = torch.bfloat16,
@@ -705,7 +710,8 @@ class SharqDecoder(torch.nn.Module):
         """One more token of every sequence of the cache (an empty one begins with it), or of those listed in sequences, in that order:
         token_ids [B] -> logits of the next one [B, vocab] (float32).  weight_only: the linears take the activations unquantised (at most 16 sequences).  reference: as in prefill.  rules: change the logits; their rows are
         those of token_ids.  With a cache that hands its pages out on the device, and all its sequences, the call can be captured in a CUDA graph whose replays go
-        on from token to token; a sequence for which the pages do not suffice keeps its length, and one that has max_tokens, which is reported."""
+        on from token to token; a sequence for which the pages do not suffice keeps its length, and so does one that has max_tokens or waits for its prompt: ops.check_device_errors
+        reports them, and their logits mean nothing."""
         which = cache.chosen(sequences)
         b = int(token_ids.shape[0])
         if token_ids.dim() != 1 or b != len(which):

@@ -70,14 +70,18 @@ class PagedKVCache:
 
     def plan(self, counts: torch.Tensor, rows: int, released: Optional[torch.Tensor] = None):
         """counts[i] (int32, on the device) more tokens for every sequence i, which with released (bool) gives back what it holds first ->
-        (offsets, positions, sequences) of the `rows` rows of the step, see ops.plan_paged_step."""
+        (offsets, positions, sequences) of the `rows` rows of the step, see ops.plan_paged_step.  Where the pages do not suffice, which reserve() raises,
+        check_device_errors does."""
         if not self.on_device:
             raise RuntimeError("the pages of this cache are handed out on the host: reserve() and advance()")
+        if released is not None:  # what waited for its prompt (length -1) holds nothing
+            self.device_lengths.masked_fill_(released.bool() & (self.device_lengths == -1), 0)
         return ops.plan_paged_step(self.table, self.device_lengths, counts, self.free_pages, self.free_count, self.page_size, rows, released,
-                                   self.max_tokens)
+                                   self.max_tokens, strict=True)
 
     def step_places(self, which: Sequence[int], tokens: int, restart: bool = False):
-        """plan() of `tokens` new tokens of every sequence in `which` -> (positions, sequences), int32, in the order of `which`.  restart: they begin anew."""
+        """plan() of `tokens` new tokens of every sequence in `which` -> (positions, sequences), int32, in the order of `which`.  restart: they begin anew, and
+        those for which the pages do not suffice are left with length -1: no token is taken for them until they begin anew once more, or are freed."""
         device, everyone = self.table.device, list(which) == list(range(self.sequences))
         if everyone:
             chosen = torch.ones(self.sequences, dtype=torch.int32, device=device)
@@ -85,6 +89,8 @@ class PagedKVCache:
             at = torch.tensor(list(which), device=device)
             chosen = torch.zeros(self.sequences, dtype=torch.int32, device=device).index_fill_(0, at, 1)
         offsets, positions, sequences = self.plan(chosen * tokens, len(which) * tokens, chosen.bool() if restart else None)
+        if restart and tokens > 0:
+            self.device_lengths.masked_fill_(chosen.bool() & (self.device_lengths == 0), -1)
         if list(which) != sorted(which):
             row = (offsets[at][:, None] + torch.arange(tokens, device=device)).reshape(-1)
             positions, sequences = positions[row], sequences[row]

@@ -37,6 +37,7 @@ _BAD_CACHE_INDEX = 0x402  # kBadCacheIndex of csrc/decode_ops.cuh
 _ATTENTION_TIMEOUT, _WEIGHT_ONLY_TIMEOUT = 0x403, 0x404  # kAttentionTimeout, kWeightOnlyTimeout of csrc/decode_ops.cuh
 _BAD_STEP_PLAN, _BAD_LOGIT_RULES = 0x405, 0x406  # kBadStepPlan, kBadLogitRules of csrc/decode_ops.cuh
 _BAD_OFFSETS, _PROMPT_TIMEOUT = 0x407, 0x408  # kBadOffsets, kPromptTimeout of csrc/decode_ops.cuh
+_PAGES_SHORT = 0x409  # kPagesShort of csrc/decode_ops.cuh
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -94,6 +95,8 @@ def check_device_errors(device=None) -> None:
                 raise RuntimeError(f"sharq_b200 prompt_attention: offsets went back or beyond the rows on cuda:{idx}")
             if code == _PROMPT_TIMEOUT:
                 raise RuntimeError(f"sharq_b200 prompt_attention: a wait ran out on cuda:{idx}; outputs are undefined")
+            if code == _PAGES_SHORT:
+                raise RuntimeError(f"sharq_b200 plan_paged_step: the free pages did not suffice for all of a step's tokens on cuda:{idx}")
             if code in (_ATTENTION_TIMEOUT, _WEIGHT_ONLY_TIMEOUT):
                 name = "paged_attention" if code == _ATTENTION_TIMEOUT else "weight_only_linear"
                 raise RuntimeError(f"sharq_b200 {name}: a wait for a copy ran out on cuda:{idx}; outputs are undefined")
@@ -261,15 +264,17 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
 
 def plan_paged_step(page_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
-                    page_size: int, rows: int, released: Optional[torch.Tensor] = None, max_tokens: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                    page_size: int, rows: int, released: Optional[torch.Tensor] = None, max_tokens: Optional[int] = None,
+                    strict: bool = False) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Pages and places of a step's tokens, handed out on the device in one launch: sequence i, which holds lengths[i] tokens in the pages of its row
     of page_table [sequences, pages], gets counts[i] more -> (offsets [sequences + 1], positions [rows], sequences [rows]), the places that
     rope_append_paged takes, sequence after sequence.  All int32.  page_table, lengths, free_pages (a stack, of which the first
     free_count[0] are free) and free_count [1] change in place.  Sequences with released (bool) give their pages back first and are empty.  Where the
     pages do not suffice for a sequence and those ahead of it, it gets nothing: its length stays and its rows have position -1, as rows behind the
-    last have.  No sequence grows beyond max_tokens, or what its row of page_table holds.  A length, count, sum of counts above `rows` or free_count that cannot be is reported by check_device_errors, and its sequences get nothing."""
+    last have; with strict check_device_errors reports it.  No sequence grows beyond max_tokens, or what its row of page_table holds.  A length, count, sum of counts
+    above `rows` or free_count that cannot be is reported by check_device_errors, and its sequences get nothing; length -1 with count 0 is passed over."""
     return _lib.native().plan_paged_step(page_table, lengths, counts, free_pages, free_count, page_size, rows, released, max_tokens,
-                                         _error_flag(page_table.device))
+                                         _error_flag(page_table.device), strict)
 
 
 def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,

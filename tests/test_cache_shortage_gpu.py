@@ -1,0 +1,75 @@
+"""Caches that hand their pages out on the device, where the pages do not suffice."""
+import pytest
+import torch
+
+from sharq_b200 import ops
+from tests.test_decode_gpu import small, tokens
+
+pytestmark = pytest.mark.gpu
+
+
+def model_of(**kw):
+    from sharq_b200.decoder import SharqDecoder
+
+    cfg = small(**kw)
+    return SharqDecoder(cfg, torch.device("cuda"), mode="BF16", seed=3), cfg
+
+
+@pytest.mark.parametrize("window", [0, 20])
+def test_a_prompt_without_pages_is_reported_and_nothing_follows_it(window):
+    model, cfg = model_of(window=window, sinks=4 if window else 0)
+    ids = tokens(cfg, 3, 33)
+    cache = model.new_cache(3, 64, page_size=16, pages=5, on_device=True)
+    logits = model.prefill(ids, cache=cache)  # three pages each: the first one's, and no others
+    with pytest.raises(RuntimeError, match="pages"):
+        ops.check_device_errors()
+    assert logits[0].isfinite().all() and logits[1:].isnan().all()
+    for _ in range(2):  # two pages are free, but a token without its prompt does not take one
+        model.decode(ids[:, 0], cache)
+        with pytest.raises(RuntimeError, match="plan_paged_step"):
+            ops.check_device_errors()
+    assert cache.device_lengths.tolist() == [35, -1, -1] and int(cache.free_count) == 2
+    # where there is room the prompt takes its place after all, and steps go on from it
+    cache.free(0)
+    other = model.new_cache(3, 64, page_size=16, on_device=True)
+    for c in (cache, other):
+        c.first = model.prefill(ids[1:2], cache=c, sequences=[1])
+        c.second = model.decode(ids[[1], 4], c, sequences=[1])
+    assert torch.equal(cache.first, other.first) and (cache.second - other.second).norm() <= 0.08 * other.second.norm()
+    cache.free(2)
+    assert cache.device_lengths.tolist() == [0, 34, 0] and int(cache.free_count) == 2
+    model.decode(ids[[2], 0], cache, sequences=[2])  # a sequence that is empty and waits for nothing begins with a token
+    assert cache.device_lengths.tolist() == [0, 34, 1]
+    ops.check_device_errors()
+
+
+def test_tokens_without_pages_are_reported():
+    model, cfg = model_of()
+    ids = tokens(cfg, 2, 20)
+    cache = model.new_cache(2, 64, page_size=16, pages=3, on_device=True)
+    model.prefill(ids[:, :15], cache=cache)
+    model.decode(ids[:, 15], cache)
+    ops.check_device_errors()
+    assert model.decode(ids[:, 16], cache).isfinite().all()
+    with pytest.raises(RuntimeError, match="pages"):
+        ops.check_device_errors()
+    assert cache.device_lengths.tolist() == [17, 16]
+    cache.free(0)
+    model.decode(ids[[1], 16], cache, sequences=[1])  # the same token again, now that there is a page
+    assert cache.device_lengths.tolist() == [0, 17]
+    ops.check_device_errors()
+
+
+def test_plans_report_a_shortage_where_they_are_asked_to():
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for strict in (False, True):
+        for counts, free, short in (([1, 1, 1], 2, True), ([0, 1, 0], 0, True), ([1, 0, 1], 2, False), ([0, 0, 0], 0, False)):
+            lengths, left = dev([16, 16, 32]), dev([free])
+            got = ops.plan_paged_step(torch.zeros(3, 4, dtype=torch.int32, device="cuda"), lengths, dev(counts), dev(list(range(9))), left, 16, 3, strict=strict)
+            if short and strict:
+                with pytest.raises(RuntimeError, match="pages"):
+                    ops.check_device_errors()
+            ops.check_device_errors()
+            taken = [n for n in (torch.tensor(counts).cumsum(0)).tolist()]
+            assert lengths.tolist() == [n + (c if t <= free else 0) for n, c, t in zip([16, 16, 32], counts, taken)]
+            assert len(got) == 3
