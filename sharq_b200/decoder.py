@@ -644,6 +644,8 @@ class SharqDecoder(torch.nn.Module):
         kvs, refused = [None] * len(self.layers), None
         if cache is None and sequences is not None:
             raise ValueError("sequences are those of a cache")
+        if rules is not None:
+            rules.check_rows(b)
         if cache is not None:
             which = cache.chosen(sequences)
             if cache.on_device:
@@ -718,6 +720,8 @@ class SharqDecoder(torch.nn.Module):
             raise ValueError("decode takes one token for every sequence of the cache" + ("" if sequences is None else " that is listed"))
         if weight_only and b > 16:
             raise ValueError(f"weight_only takes at most 16 sequences, got {b}")
+        if rules is not None:
+            rules.check_rows(b)
         if cache.on_device:
             positions, rows = cache.step_places(which, 1)
             return self.decode_step(token_ids, cache, positions, positions + 1, reference, weight_only, None if sequences is None else rows.long(),

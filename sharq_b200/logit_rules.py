@@ -24,6 +24,15 @@ class LogitRules:
     bias: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None  # offsets int32 [rows + 1], ids int32, values float32
     mask: Optional[torch.Tensor] = None            # int32 [rows, ceil(vocab / 32)], a bit per token
 
+    def check_rows(self, rows: int) -> None:
+        """Refuses rules of another number of rows, ahead of a step that would have changed its cache when adjust_logits refuses them."""
+        held = {name: getattr(self, name) for name in ("tokens", "lengths", "prompt_lengths", "repetition", "presence", "frequency", "mask")}
+        for name, t in held.items():
+            if t is not None and t.shape[:1] != (rows,):
+                raise ValueError(f"{name} of the rules must have a row for each of the {rows} rows of logits, not shape {tuple(t.shape)}")
+        if self.bias is not None and self.bias[0].shape != (rows + 1,):
+            raise ValueError(f"the biases' offsets must be {rows + 1} for {rows} rows of logits, not shape {tuple(self.bias[0].shape)}")
+
     def apply_(self, logits: torch.Tensor) -> torch.Tensor:
         """The logits [rows, vocab], changed in place."""
         return ops.adjust_logits(logits, self.tokens, self.lengths, self.prompt_lengths, self.repetition, self.presence, self.frequency, self.bias,

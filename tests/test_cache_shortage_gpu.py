@@ -1,4 +1,4 @@
-"""Caches that hand their pages out on the device, where the pages do not suffice."""
+"""Caches that hand their pages out on the device, where the pages do not suffice or an argument is refused."""
 import pytest
 import torch
 
@@ -73,3 +73,23 @@ def test_plans_report_a_shortage_where_they_are_asked_to():
             taken = [n for n in (torch.tensor(counts).cumsum(0)).tolist()]
             assert lengths.tolist() == [n + (c if t <= free else 0) for n, c, t in zip([16, 16, 32], counts, taken)]
             assert len(got) == 3
+
+
+def test_rules_of_other_rows_are_refused_before_anything_changes():
+    from sharq_b200.logit_rules import LogitRules
+
+    model, cfg = model_of()
+    ids = tokens(cfg, 2, 9)
+    rules = LogitRules(tokens=ids.clone(), lengths=torch.full((2,), 9, dtype=torch.int32, device="cuda"))
+    for on_device in (False, True):
+        cache = model.new_cache(2, 64, page_size=16, on_device=on_device)
+        with pytest.raises((ValueError, RuntimeError)):
+            model.prefill(ids[:1], cache=cache, sequences=[1], rules=rules)
+        assert cache.device_lengths.tolist() == [0, 0]
+        model.prefill(ids, cache=cache, rules=rules)
+        with pytest.raises((ValueError, RuntimeError)):
+            model.decode(ids[1:, 0], cache, sequences=[1], rules=rules)
+        assert cache.device_lengths.tolist() == [9, 9]
+        model.decode(ids[:, 0], cache, rules=rules)
+        assert cache.device_lengths.tolist() == [10, 10]
+    ops.check_device_errors()
