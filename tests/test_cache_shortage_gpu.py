@@ -93,3 +93,32 @@ def test_rules_of_other_rows_are_refused_before_anything_changes():
         model.decode(ids[:, 0], cache, rules=rules)
         assert cache.device_lengths.tolist() == [10, 10]
     ops.check_device_errors()
+
+
+def test_steps_of_a_full_cache_report_the_plan_and_nothing_else():
+    """Steps go on, captured ones too, with some sequences left out; neither the append nor the attention has anything to say about them."""
+    model, cfg = model_of(window=20, sinks=3)
+    ids = tokens(cfg, 4, 30)
+    cache = model.new_cache(4, 48, page_size=16, pages=9, on_device=True)
+    model.prefill(ids[:, :30], cache=cache)
+    ops.check_device_errors()
+    token = ids[:, 0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        model.decode(token, cache)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        logits = model.decode(token, cache)
+    codes = []
+    for _ in range(20):
+        graph.replay()
+        codes.append(int(ops._ERROR_FLAGS[0]))
+        ops._ERROR_FLAGS[0].zero_()
+        assert logits.isfinite().all()
+    # 31 tokens each; all grow to 32, then the first one alone, which gets the last page, up to max_tokens
+    assert cache.device_lengths.tolist() == [48, 32, 32, 32] and int(cache.free_count) == 0
+    # no error, then pages that do not suffice, and from 48 on either that or a length that cannot be, whichever comes first
+    assert codes[:17] == [0] + [0x409] * 16 and set(codes[17:]) <= {0x405, 0x409}
+    ops.check_device_errors()
