@@ -417,8 +417,8 @@ int sharq_paged_attention(const void *q_bf16, int64_t q_row, int64_t q_head, int
                           const int *lengths, float scale, void *out_bf16, void *workspace, size_t workspace_bytes, int *error_flag,
                           void *stream);
 
-/* ... of the last `window` tokens of a sequence and its first `sinks`, those that it has (window 0: of all).  Pages with no token that is seen are not
- * read, and their entries in the table may be anything. */
+/* ... of the last `window` tokens of a sequence and its first `sinks`, those that it has (window 0: of all).  Pages with no token that is seen are
+ * read only beside one in the same tile, say nothing, and their entries in the table may be anything. */
 size_t sharq_paged_attention_windowed_workspace_bytes(int heads, const sharq_paged_cache *cache, int window, int sinks);
 int sharq_paged_attention_windowed(const void *q_bf16, int64_t q_row, int64_t q_head, int heads, const sharq_paged_cache *cache,
                                    const int *lengths, float scale, int window, int sinks, void *out_bf16, void *workspace,

@@ -1,5 +1,5 @@
 // Attention of ragged prompts: causal, with a sliding window and a few first keys that stay visible.  32768 tokens of 32 / 8 heads of
-// 128 under a window of 4096: 2.04 ms, 1010 TFLOP/s, in long runs, where the card's power is the bound (1.75 ms in a short one); 200 tokens: 11.1 us.
+// 128 under a window of 4096: 2.04 ms, 1010 TFLOP/s, in long runs, where the card's power is the bound (1.75 ms in a short one); 200 tokens: 11.3 us.
 //
 //   out[i, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q[i, h] . k_j - max),   j <= p and (p - j < window or j < sinks),   p the position of query i
 //
@@ -14,8 +14,9 @@
 //
 // Warps 0-3 and 4-7 hold a row per thread: maximum, exponentials and sum need no other thread.  The maximum is raised only where a score exceeds it by
 // more than 2^kLazy, for the raise is a pass over O.  Probabilities carry a factor of 2^-32, so that no sum of finite values overflows, and
-// enter the product as bf16, as in the library attention of prompts without a window: off by 2^-9 each, which leaves a result about as near as its own
-// rounding to bf16.  (As two bf16 numbers, as the decode step has them, the second product would be a third more work for the tensor cores.)
+// enter the product as bf16, as in the library attention of prompts without a window: off by up to 2^-8 each, which leaves a result about as near as its own
+// rounding to bf16.  (As two bf16 numbers, as the decode step has them, the second product would be a third more work for the tensor cores.)  The factor takes five bits
+// of the exponent's argument, 2^-18 of a probability, and the exponential is the hardware's, to 2 units in the last place of a float: both are far below that.
 // The second product begins when three quarters of a tile's probabilities are there.  All 128 scores of a row stay in registers, for reading tensor memory
 // again took longer than the exponentials (2726 us instead of then 2085; 32 at a time with the maximum beside the exponentials 2179; a row in two threads,
 // which have to meet twice, 2824).  Exponentials by a polynomial on the units that multiply, for an eighth to a half of them, 2124 to 2473: a warp's instructions

@@ -245,7 +245,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     of every sequence, the new one among them, applied to the values.  Length 0 gives zeros.  A length beyond the page table or a page
     outside the cache makes that sequence's rows NaN and is reported by check_device_errors.  A sequence may stand in several
     rows with lengths of their own (drafted tokens).  The same bits from call to call.  With window only the last `window` tokens of a sequence and its
-    first `sinks` are seen; pages without any of those are not read, and their entries in the table may be anything."""
+    first `sinks` are seen; pages without any of those are read only beside one in the same tile, say nothing, and their entries in the table may be anything."""
     return _lib.native().paged_attention(q, k_cache, v_cache, page_table, lengths, scale, k_scale, v_scale, out, _error_flag(q.device), window,
                                          sinks)
 
