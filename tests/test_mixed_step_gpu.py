@@ -1,4 +1,4 @@
-"""A server's step with prompts and single tokens in it, by the operators in the order that the integration guide gives."""
+"""A server's step with prompts and single tokens in it: the operators in the order in which a server calls them, each against its definition."""
 import pytest
 import torch
 
